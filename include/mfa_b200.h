@@ -122,6 +122,33 @@ MFA_API int mfa_bwd(const void* q, const void* k, const void* v, const void* out
                     int32_t causal, int32_t dtype, int32_t layout, void* stream);
 
 /*
+ * Attention with a sliding window and sink tokens, and k / v heads shared by groups of query
+ * heads: query i sees key j if j <= i and (j > i - window or j < sinks); query head h reads k / v
+ * head h / (heads / kv_heads). q and out have `heads` heads, k and v `kv_heads` (a divisor of
+ * heads); d = 32, 64 or 128, any n, window >= 1 (at n or more: causal attention), sinks >= 0.
+ * lse (may be NULL): the row log-sum-exp over the visible keys, fp32 [B*H, N]. Key blocks that
+ * no row of a query block sees are neither read nor computed. k and v must be finite also where
+ * they are masked, as for mfa_fwd. No counterpart in the reference.
+ */
+MFA_API int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
+                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
+                           int64_t window, int64_t sinks, float scale, int32_t dtype,
+                           int32_t layout, void* stream);
+
+/*
+ * Backward of mfa_fwd_window (D = 64; others: MFA_ERR_HEAD_DIM "The backward pass supports only
+ * D=64"): dq, dk, dv from q, k, v, out, lse, dout. dk and dv of a shared head are the sum over its
+ * query heads, in a fixed order. Takes 8 bytes per query row and up to a few hundred 64 KB
+ * partial sums (of key blocks that many queries see) from the library's stream-ordered pool. No
+ * counterpart in the reference.
+ */
+MFA_API int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
+                           const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
+                           int64_t window, int64_t sinks, float scale, int32_t dtype,
+                           int32_t layout, void* stream);
+
+/*
  * Device scratch, in bytes, that one call of mfa_fwd (or mfa_fwd_f16 / mfa_fwd_lse, and with d
  * = 64 and fp16 mfa_fwd_f16_noalloc) takes on the current device for these extents: 0 when
  * whole query blocks fill the SMs evenly, else the split plan's partial-result slots (2 x

@@ -175,6 +175,88 @@ std::vector<torch::Tensor> flash_attn_backward(torch::Tensor q, torch::Tensor k,
   return {dq, dk, dv};
 }
 
+// q [B, H, N, D] and k, v [B, Hkv, N, D] of the windowed attention.
+void check_window_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  TORCH_CHECK(k.is_cuda(), "k must be a CUDA tensor");
+  TORCH_CHECK(v.is_cuda(), "v must be a CUDA tensor");
+  TORCH_CHECK(q.scalar_type() == torch::kFloat16 || q.scalar_type() == torch::kBFloat16,
+              "q must be float16 or bfloat16");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type(), "k must have the same dtype as q");
+  TORCH_CHECK(v.scalar_type() == q.scalar_type(), "v must have the same dtype as q");
+  TORCH_CHECK(k.device() == q.device(), "k must be on the same device as q");
+  TORCH_CHECK(v.device() == q.device(), "v must be on the same device as q");
+  TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
+  TORCH_CHECK(k.is_contiguous(), "k must be contiguous");
+  TORCH_CHECK(v.is_contiguous(), "v must be contiguous");
+  TORCH_CHECK(q.dim() == 4, "q must have shape [B, H, N, D]");
+  TORCH_CHECK(k.dim() == 4 && k.size(0) == q.size(0) && k.size(2) == q.size(2) &&
+                  k.size(3) == q.size(3),
+              "k must have shape [B, Hkv, N, D] with q's B, N and D");
+  TORCH_CHECK(v.sizes() == k.sizes(), "v must have the same shape as k");
+}
+
+int dtype_of(const torch::Tensor& x) {
+  return x.scalar_type() == torch::kBFloat16 ? MFA_DTYPE_BF16 : MFA_DTYPE_FP16;
+}
+
+void* current_stream() {
+  return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream());
+}
+
+// Windowed attention: (out, lse), lse undefined unless asked for.
+std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Tensor k,
+                                                     torch::Tensor v, int64_t window,
+                                                     int64_t sinks, bool with_lse) {
+  check_window_inputs(q, k, v);
+  const c10::cuda::CUDAGuard device_guard(q.device());
+  auto out = torch::empty_like(q);
+  torch::Tensor lse;
+  if (with_lse)
+    lse = torch::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(torch::kFloat32));
+  const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
+  const int rc = mfa_fwd_window(
+      q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+      with_lse ? lse.data_ptr<float>() : nullptr, q.size(0), q.size(1), k.size(1), q.size(2),
+      static_cast<int32_t>(q.size(3)), window, sinks, scale, dtype_of(q), MFA_LAYOUT_BHND,
+      current_stream());
+  if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
+  if (with_lse) return {out, lse};
+  return {out};
+}
+
+// Its backward: dq, dk, dv.
+std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Tensor k,
+                                                      torch::Tensor v, torch::Tensor out,
+                                                      torch::Tensor lse, torch::Tensor dout,
+                                                      int64_t window, int64_t sinks) {
+  check_window_inputs(q, k, v);
+  TORCH_CHECK(out.is_cuda() && out.device() == q.device() && dout.is_cuda() &&
+                  dout.device() == q.device() && lse.is_cuda() && lse.device() == q.device(),
+              "out, lse and dout must be on q's device");
+  TORCH_CHECK(out.sizes() == q.sizes() && dout.sizes() == q.sizes(),
+              "out and dout must have the same shape as q");
+  TORCH_CHECK(out.scalar_type() == q.scalar_type() && dout.scalar_type() == q.scalar_type(),
+              "out and dout must have q's dtype");
+  TORCH_CHECK(out.is_contiguous() && dout.is_contiguous() && lse.is_contiguous(),
+              "out, lse and dout must be contiguous");
+  TORCH_CHECK(lse.scalar_type() == torch::kFloat32, "lse must be float32");
+  TORCH_CHECK(lse.numel() == q.size(0) * q.size(1) * q.size(2),
+              "lse must have one value per query row");
+  const c10::cuda::CUDAGuard device_guard(q.device());
+  auto dq = torch::empty_like(q);
+  auto dk = torch::empty_like(k);
+  auto dv = torch::empty_like(v);
+  const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
+  const int rc = mfa_bwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                dout.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(),
+                                dk.data_ptr(), dv.data_ptr(), q.size(0), q.size(1), k.size(1),
+                                q.size(2), static_cast<int32_t>(q.size(3)), window, sinks, scale,
+                                dtype_of(q), MFA_LAYOUT_BHND, current_stream());
+  if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
+  return {dq, dk, dv};
+}
+
 // Same as forward, writing into a caller-provided contiguous tensor of q's shape and dtype
 // (used by the pipelined host-buffer path to fill slices of one device buffer).
 void flash_attn_forward_into(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out,
@@ -361,5 +443,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Forward of the query rows [q_begin, q_end) of every head into out");
   m.def("forward_pinned", &flash_attn_forward_pinned,
         "Pipelined forward on host tensors [rows, N, D] cut into pieces at `bounds`");
+  m.def("forward_window", &flash_attn_forward_window,
+        "Forward with a sliding window and sink tokens: [out] or, with_lse, [out, lse]");
+  m.def("backward_window", &flash_attn_backward_window,
+        "Backward of forward_window: (dq, dk, dv) (D = 64)");
   m.def("version", []() { return std::string(mfa_version()); });
 }

@@ -27,6 +27,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "mfa_common.cuh"
 #include "mfa_exp2.cuh"
@@ -54,10 +55,29 @@ struct BwdParams {
   int ctas;
   int by_length;  // causal only: deal units out by length (below), else strided
   int reverse;    // CTA cta0 + c deals as CTA ctas - 1 - c (the second pass of a mixed launch)
+  // Window variant only (see BwdWindowCursor)
+  int window, sinks, sink_blocks;
+  int group;         // query heads per k / v head
+  int units;         // units of this pass, pieces counted
+  int chunk_sink;    // dK/dV: steps of a piece, and pieces, of a sink block's unit ...
+  int pieces_sink;
+  int chunk_rest;    // ... and of any other block's
+  int pieces_rest;
+  int* claimed;      // units handed out so far
+  float* partials;   // dK/dV: [slot][dK, dV][128][64] of the units in pieces
 };
 
-template <bool kDKV_, bool kCausal_, bool kBF16_>
+template <class Cfg>
+struct BwdCursor;
+template <class Cfg>
+struct BwdWindowCursor;
+
+template <bool kDKV_, bool kCausal_, bool kBF16_, bool kWindow_ = false>
 struct BwdConfig {
+  // sliding window with sink tokens and grouped k / v heads, as the forward's window variant
+  static constexpr bool kWindow = kWindow_;
+  static_assert(!kWindow_ || kCausal_, "the window variant is causal");
+  using Cursor = std::conditional_t<kWindow_, BwdWindowCursor<BwdConfig>, BwdCursor<BwdConfig>>;
   static constexpr bool kDKV = kDKV_;  // dK/dV pass (k, v resident) or dQ pass (q, dO resident)
   static constexpr bool kCausal = kCausal_;
   static constexpr bool kBF16 = kBF16_;
@@ -98,10 +118,15 @@ struct BwdConfig {
   static constexpr int kBarAccDone = kBarOpFull + 1;        // TS MMAs of a step completed
   static constexpr int kBarStage = kBarAccDone + 1;         // output staging written (16 warps)
   static constexpr int kBarDrain = kBarStage + 1;  // [2]: one per MMA issuer
-  static constexpr int kNumBars = kBarDrain + 2;
+  // window variant: the ring of claimed units (index published / read by every other role)
+  static constexpr int kClaims = 4;
+  static constexpr int kBarClaimFull = kBarDrain + 2;  // [kClaims]
+  static constexpr int kBarClaimEmpty = kBarClaimFull + (kWindow ? kClaims : 0);
+  static constexpr int kNumBars = kBarClaimEmpty + (kWindow ? kClaims : 0);
+  static constexpr int kClaimReaders = kSoftmaxWarps + 3;  // two MMA warps and the store thread
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kAbortOff = kTmemSlotOff + 4;
-  static constexpr int kSmemBytes = kAbortOff + 4 + 1024;
+  static constexpr int kSmemBytes = kAbortOff + 4 + (kWindow ? 4 * kClaims : 0) + 1024;
 
   static constexpr int kTmemCols = 512;
   static constexpr int kColS = 0;
@@ -112,6 +137,14 @@ struct BwdConfig {
   static constexpr int kColAcc1 = 448;               // dK/dV pass: dK
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
+
+// Window variant: where a CTA's roles find the units that its load thread has claimed.
+struct BwdClaims {
+  volatile int* ring;
+  uint32_t bars;
+  const Watchdog* wd;
+};
+enum class BwdRole { kLoad, kLane, kWarp };  // the load thread, one other thread, a whole warp
 
 // Units are (batch * head, 128-row block) pairs, u = bh * blocks + block.
 // dQ pass: unit = query block b, steps = key blocks [0, b + 1) with the causal mask, else all.
@@ -156,7 +189,7 @@ struct BwdCursor {
     const int blk = Cfg::kDKV ? wave : p.blocks - 1 - wave;
     return head * p.blocks + blk;
   }
-  __device__ void init(const BwdParams& p) {
+  __device__ void init(const BwdParams& p, const BwdClaims&, BwdRole) {
     seg = 0;
     u = unit_at(p, 0);
     if (u >= 0) {
@@ -178,16 +211,169 @@ struct BwdCursor {
       }
     }
   }
+  __device__ void next_unit(const BwdParams& p) {
+    j = j1 - 1;
+    step(p);
+  }
+  __device__ int row_block(const BwdParams& p) const { return u % p.blocks; }
+  __device__ int head_row(const BwdParams& p) const { return u / p.blocks; }
+  __device__ HeadBatch resident(const BwdParams& p) const {
+    const int bh = u / p.blocks;
+    return {bh % p.heads, bh / p.heads};
+  }
+  __device__ HeadBatch streamed(const BwdParams& p) const { return resident(p); }
+  __device__ int block() const { return j; }
+  __device__ size_t vec_row(const BwdParams& p) const { return static_cast<size_t>(u / p.blocks); }
+  __device__ bool in_pieces() const { return false; }
+  __device__ int slot() const { return 0; }
 };
 
-__device__ __forceinline__ HeadBatch bwd_head_batch(const BwdParams& p, int u) {
-  const int bh = u / p.blocks;
-  return {bh % p.heads, bh / p.heads};
-}
+// Units of the window variant, with k / v heads shared by `group` query heads:
+// dQ pass: unit = (query head, query block), steps = the key blocks that hold sinks before the
+// window, then the window's blocks up to the diagonal.
+// dK/dV pass: unit = (k / v head, key block), steps = for each of the group's query heads the
+// query blocks from the diagonal to the last one that sees a key of the block (for a block
+// with sinks, to the end of the sequence). The sum over the group stays in TMEM, so shared
+// heads need no atomics. A unit of more steps than its chunk is cut into pieces of that many
+// steps, whose sums go to `partials` for mfa_bwd_reduce_kernel: the units of sink blocks run
+// over the whole sequence and would otherwise outlast all the others.
+// Units differ in length, so each CTA claims its next one from a counter when it has issued
+// the last loads of the current one; long units come first (sink blocks, then key blocks from
+// the first; query blocks from the last). Which CTA takes a unit changes no result. The load
+// thread claims, and passes the index to the other roles through a ring of kClaims entries.
+template <class Cfg>
+struct BwdWindowCursor {
+  const BwdClaims* c;
+  BwdRole role;
+  int seg;        // units started by this CTA so far - 1
+  int blk, row;   // resident block, its batch * head row (k / v heads in the dK/dV pass)
+  int j;          // streamed block, from...
+  int j0, j1;     // ... [j0, j1); dQ: steps, the first `sinks` of them before the window
+  int sinks, skip;
+  int g;          // dK/dV: query head of the group
+  int left;       // steps after this one; -1: no unit
+  int steps;      // steps of the unit
+  int piece;      // dK/dV: its slot in `partials`, or -1
+  int ahead;      // load thread: the index claimed ahead
+
+  // Steps of key block b in the dK/dV pass, for one query head.
+  __device__ static int span(const BwdParams& p, int b) {
+    if (b < p.sink_blocks) return p.blocks - b;
+    const int last = b + ((126 + p.window) >> 7);  // block of query 128 b + 127 + window - 1
+    return (last < p.blocks - 1 ? last : p.blocks - 1) - b + 1;
+  }
+  // The unit with index i; false if it is a piece past its unit's end.
+  __device__ bool set(const BwdParams& p, int i) {
+    piece = -1;
+    if (Cfg::kDKV) {
+      const int head_sinks = p.bh * p.pieces_sink;
+      const int sink_units = p.sink_blocks * head_sinks;
+      const bool sink = i < sink_units;
+      const int pieces = sink ? p.pieces_sink : p.pieces_rest;
+      const int per_block = p.bh * pieces;
+      const int k = sink ? i : i - sink_units;
+      const int part = k % per_block / p.bh;
+      blk = k / per_block + (sink ? 0 : p.sink_blocks);
+      row = k % p.bh;
+      j0 = blk;
+      j1 = blk + span(p, blk);
+      const int chunk = sink ? p.chunk_sink : p.chunk_rest;
+      const int total = (j1 - j0) * p.group;
+      const int s0 = part * chunk;
+      if (s0 >= total) return false;
+      steps = total - s0 < chunk ? total - s0 : chunk;
+      if (steps < total) piece = i;
+      g = s0 / (j1 - j0);
+      j = j0 + s0 % (j1 - j0);
+      sinks = skip = 0;
+    } else {
+      blk = p.blocks - 1 - i / p.bh;
+      row = i % p.bh;
+      const int oldest = blk * Cfg::kRows - p.window + 1;
+      const int w0 = oldest > 0 ? oldest >> 7 : 0;
+      sinks = p.sink_blocks < w0 ? p.sink_blocks : w0;
+      skip = w0 - sinks;
+      j = j0 = g = 0;
+      steps = j1 = blk + 1 - skip;
+    }
+    left = steps - 1;
+    return true;
+  }
+  __device__ void claim(const BwdParams& p) {
+    volatile int* ring = c->ring;
+    const int slot = seg % Cfg::kClaims;
+    const uint32_t phase = static_cast<uint32_t>(seg / Cfg::kClaims) & 1u;
+    const uint32_t full = c->bars + 8u * static_cast<uint32_t>(Cfg::kBarClaimFull + slot);
+    const uint32_t empty = c->bars + 8u * static_cast<uint32_t>(Cfg::kBarClaimEmpty + slot);
+    left = -1;
+    if (role == BwdRole::kLoad) {
+      int i = ahead;
+      while (i < p.units && !set(p, i)) i = atomicAdd(p.claimed, 1);
+      const bool any = i < p.units;
+      if (!any) left = -1;
+      if (any) ahead = atomicAdd(p.claimed, 1);
+      if (!wait_single(empty, phase ^ 1u, *c->wd, kSiteLoadQEmpty)) {
+        left = -1;
+        return;
+      }
+      ring[slot] = any ? i : -1;
+      mbar_arrive(full);
+      return;
+    }
+    const bool ok = role == BwdRole::kWarp ? wait_warp(full, phase, *c->wd, kSiteMmaQ)
+                                           : wait_single(full, phase, *c->wd, kSiteMmaQ);
+    if (!ok) return;
+    const int i = ring[slot];
+    if (role == BwdRole::kWarp) __syncwarp();
+    if (role == BwdRole::kLane || (threadIdx.x & 31) == 0) mbar_arrive(empty);
+    if (i >= 0) set(p, i);
+  }
+  __device__ void init(const BwdParams& p, const BwdClaims& claims, BwdRole r) {
+    c = &claims;
+    role = r;
+    seg = 0;
+    if (role == BwdRole::kLoad) ahead = atomicAdd(p.claimed, 1);
+    claim(p);
+  }
+  __device__ bool valid() const { return left >= 0; }
+  __device__ bool first_step() const { return left == steps - 1; }
+  // The next step of this unit; false after the last one.
+  __device__ bool advance() {
+    if (left == 0) return false;
+    --left;
+    if (++j >= j1) {
+      j = j0;
+      ++g;
+    }
+    return true;
+  }
+  __device__ void next_unit(const BwdParams& p) {
+    ++seg;
+    claim(p);
+  }
+  __device__ void step(const BwdParams& p) {
+    if (!advance()) next_unit(p);
+  }
+  __device__ int row_block(const BwdParams&) const { return blk; }
+  __device__ int head_row(const BwdParams&) const { return row; }
+  __device__ HeadBatch resident(const BwdParams& p) const {
+    return {row % p.heads, row / p.heads};  // heads: of the resident tensors
+  }
+  __device__ HeadBatch streamed(const BwdParams& p) const {
+    const HeadBatch r = resident(p);
+    return {Cfg::kDKV ? r.h * p.group + g : r.h / p.group, r.b};
+  }
+  __device__ int block() const { return Cfg::kDKV || j < sinks ? j : j + skip; }
+  __device__ size_t vec_row(const BwdParams& p) const {  // query row of the L2 / D slices
+    return static_cast<size_t>(row) * p.group + g;
+  }
+  __device__ bool in_pieces() const { return piece >= 0; }
+  __device__ int slot() const { return piece; }
+};
 
 template <class Cfg>
 __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem, uint32_t bars,
-                                              const Watchdog& wd) {
+                                              const Watchdog& wd, const BwdClaims& claims) {
   constexpr int ST = Cfg::STAGES;
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
   const uint32_t sbase = smem_addr(smem);
@@ -196,19 +382,19 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
   tma_prefetch_desc(&p.tm_s0);
   tma_prefetch_desc(&p.tm_s1);
   const uint64_t keep = l2_policy_evict_last();  // streamed blocks are re-read by other units
-  BwdCursor<Cfg> cur;
-  cur.init(p);
+  typename Cfg::Cursor cur;
+  cur.init(p, claims, BwdRole::kLoad);
   int g = 0;
   int res_loaded = 0, str_issued = 0;
   while (cur.valid()) {
-    const HeadBatch hb = bwd_head_batch(p, cur.u);
     if (cur.first_step()) {
+      const HeadBatch hb = cur.resident(p);
       const int s = cur.seg, b = s & 1;
       if (!wait_single(bar(Cfg::kBarResEmpty + b), (static_cast<uint32_t>(s >> 1) & 1u) ^ 1u, wd,
                        kSiteLoadQEmpty))
         break;
       mbar_arrive_expect_tx(bar(Cfg::kBarResFull + b), 2 * Cfg::kTileBytes);
-      const int row = (cur.u % p.blocks) * Cfg::kRows;
+      const int row = cur.row_block(p) * Cfg::kRows;
       const uint32_t dst = sbase + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
       tma_load_4d(dst, &p.tm_x, bar(Cfg::kBarResFull + b), 0, row, hb.h, hb.b);
       tma_load_4d(dst + Cfg::kTileBytes, &p.tm_y, bar(Cfg::kBarResFull + b), 0, row, hb.h, hb.b);
@@ -220,14 +406,15 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
       break;
     mbar_arrive_expect_tx(bar(Cfg::kBarStrFull + st),
                           2 * Cfg::kTileBytes + (Cfg::kDKV ? Cfg::kVecBytes : 0));
-    const int row = cur.j * Cfg::kCols;
+    const HeadBatch hb = cur.streamed(p);
+    const int row = cur.block() * Cfg::kCols;
     const uint32_t dst = sbase + Cfg::kStrOff + st * 2 * Cfg::kTileBytes;
     tma_load_4d_hint(dst, &p.tm_s0, bar(Cfg::kBarStrFull + st), 0, row, hb.h, hb.b, keep);
     tma_load_4d_hint(dst + Cfg::kTileBytes, &p.tm_s1, bar(Cfg::kBarStrFull + st), 0, row, hb.h,
                      hb.b, keep);
     if (Cfg::kDKV) {
       // L2 and D of the 128 streamed queries (padded arrays: 512-byte aligned slices)
-      const size_t off = static_cast<size_t>(cur.u / p.blocks) * p.blocks * Cfg::kCols + row;
+      const size_t off = cur.vec_row(p) * p.blocks * Cfg::kCols + row;
       const uint32_t vdst = sbase + Cfg::kVecOff + st * Cfg::kVecBytes;
       bulk_load(vdst, p.lse2 + off, Cfg::kCols * 4, bar(Cfg::kBarStrFull + st));
       bulk_load(vdst + Cfg::kCols * 4, p.di + off, Cfg::kCols * 4, bar(Cfg::kBarStrFull + st));
@@ -255,7 +442,8 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
 // empty barrier counts one commit from each.
 template <class Cfg, bool kAcc>
 __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, uint32_t bars,
-                                             uint32_t tmem, const Watchdog& wd) {
+                                             uint32_t tmem, const Watchdog& wd,
+                                             const BwdClaims& claims) {
   constexpr int ST = Cfg::STAGES;
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
   const uint32_t sbase = smem_addr(smem);
@@ -269,15 +457,14 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
   const bool leader = elect_one();
   bool issued_any = false;
 
-  BwdCursor<Cfg> cs, cp;
-  cs.init(p);
-  cp.init(p);
+  typename Cfg::Cursor cur;
+  cur.init(p, claims, BwdRole::kWarp);
   int gs = 0, gp = 0;
   // S and dP of step gs once the softmax warps have read those of step gs - 1.
   auto issue_ss = [&]() -> bool {
-    const int b = cs.seg & 1;
-    if (cs.first_step()) {
-      if (!wait_warp(bar(Cfg::kBarResFull + b), static_cast<uint32_t>(cs.seg >> 1) & 1u, wd,
+    const int b = cur.seg & 1;
+    if (cur.first_step()) {
+      if (!wait_warp(bar(Cfg::kBarResFull + b), static_cast<uint32_t>(cur.seg >> 1) & 1u, wd,
                      kSiteMmaQ))
         return false;
     }
@@ -306,15 +493,15 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
     __syncwarp();
     issued_any = true;
     ++gs;
-    cs.step(p);
+    cur.step(p);
     return true;
   };
 
   if (!kAcc) {
-    while (cs.valid())
+    while (cur.valid())
       if (!issue_ss()) goto unwind;
   }
-  while (kAcc && cp.valid()) {
+  while (kAcc && cur.valid()) {
     {
       const int st = gp % ST;
       // the stage's tiles are this thread's operands too
@@ -325,7 +512,7 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
         goto unwind;
       tc_fence_after();
       if (leader) {
-        const bool fresh = cp.first_step();
+        const bool fresh = cur.first_step();
         const uint32_t s0 = str_mn_lo + st * 2 * kTile, s1 = s0 + kTile;
         if (Cfg::kDKV) {
 #pragma unroll
@@ -348,7 +535,7 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
       __syncwarp();
       issued_any = true;
       ++gp;
-      cp.step(p);
+      cur.step(p);
     }
   }
   // Every commit of this pass has arrived before the role returns (the barriers may be
@@ -415,6 +602,21 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
             if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
       }
     }
+    if constexpr (Cfg::kWindow) {
+      // keys older than the window, but for the sinks
+      const int key0 = j * Cfg::kCols;
+      if (key0 <= row0 + 15 - p.window && key0 + Cfg::kCols > p.sinks) {
+        const int t0 = row0 + gq - p.window - key0;  // too old when k <= t0 (+8 for e >= 2)
+        const int s0 = p.sinks - key0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = 8 * i + q2 + (e & 1);
+            if (k <= t0 + 8 * (e >> 1) && k >= s0) sr[4 * i + e] = __float_as_uint(-INFINITY);
+          }
+      }
+    }
   } else if (Cfg::kCausal && j == blk) {
     // diagonal block: queries (columns) before the key row score -inf
     const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k < t0 (+8 for e >= 2)
@@ -423,6 +625,18 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (8 * i + q2 + (e & 1) < t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
+  }
+  if constexpr (Cfg::kDKV && Cfg::kWindow) {
+    // queries (columns) for which the key row, unless a sink, is older than the window
+    if ((j + 1) * Cfg::kCols > row0 + p.window && row0 + 16 > p.sinks) {
+      const int t0 = row0 + gq + p.window - j * Cfg::kCols;  // too old when c >= t0 (+8 ...)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (8 * i + q2 + (e & 1) >= t0 + 8 * (e >> 1) && row0 + gq + 8 * (e >> 1) >= p.sinks)
+            sr[4 * i + e] = __float_as_uint(-INFINITY);
+    }
   }
 
   const uint64_t c2 = f2_splat(p.scale_log2);
@@ -481,7 +695,8 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
 
 template <class Cfg>
 __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* smem, uint32_t bars,
-                                                 uint32_t tmem, const Watchdog& wd) {
+                                                 uint32_t tmem, const Watchdog& wd,
+                                                 const BwdClaims& claims) {
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -496,11 +711,11 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
   const uint32_t tOp0 = tmem + lb + Cfg::kColOp0 + 32 * half;
   const uint32_t tOp1 = tmem + lb + Cfg::kColOp1 + 32 * half;
   int g = 0;
-  BwdCursor<Cfg> cur;
-  cur.init(p);
+  typename Cfg::Cursor cur;
+  cur.init(p, claims, BwdRole::kWarp);
   while (cur.valid()) {
-    const int blk = cur.u % p.blocks;
-    const int bh = cur.u / p.blocks;
+    const int blk = cur.row_block(p);
+    const int bh = cur.head_row(p);
     const int row0 = blk * Cfg::kRows + slice;  // first resident row of this warp
     float lrow[2] = {0.f, 0.f}, drow[2] = {0.f, 0.f};
     if (!Cfg::kDKV) {
@@ -511,11 +726,21 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
         drow[r] = p.di[idx];
       }
     }
-    const int j0 = cur.j0, j1 = cur.j1, b = cur.seg & 1;
-    for (int j = j0; j < j1; ++j, ++g) {
-      if (!bwd_step<Cfg>(p, smem, bars, tS, tDP, tOp0, tOp1, lane, half, g, blk, j, row0, lrow,
-                         drow, wd))
-        return;
+    const int b = cur.seg & 1;
+    if constexpr (Cfg::kWindow) {
+      do {
+        if (!bwd_step<Cfg>(p, smem, bars, tS, tDP, tOp0, tOp1, lane, half, g, blk, cur.block(),
+                           row0, lrow, drow, wd))
+          return;
+        ++g;
+      } while (cur.advance());
+    } else {
+      const int j0 = cur.j0, j1 = cur.j1;
+      for (int j = j0; j < j1; ++j, ++g) {
+        if (!bwd_step<Cfg>(p, smem, bars, tS, tDP, tOp0, tOp1, lane, half, g, blk, j, row0, lrow,
+                           drow, wd))
+          return;
+      }
     }
     // ---- unit epilogue: accumulators -> (scaled) fp16 / bf16 -> staging -> TMA
     if (!wait_warp(bar(Cfg::kBarAccDone), static_cast<uint32_t>(g - 1) & 1u, wd, kSiteSoftOFinal))
@@ -541,7 +766,26 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
         }
       }
     };
-    if (Cfg::kDKV) {
+    if (Cfg::kDKV && cur.in_pieces()) {
+      // a piece's sums, unscaled, for the reduce kernel
+      float* part = p.partials + static_cast<size_t>(cur.slot()) *
+                                     (2 * Cfg::kRows * Cfg::kHeadDim);
+      auto keep_acc = [&](uint32_t col, float* dst) {
+        uint32_t a[16];
+        tmem_ld_16x256b_sync(tmem + lb + col + 32 * half, a);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float* at = dst + (slice + gq + 8 * r) * Cfg::kHeadDim + 32 * half + 2 * q;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float2*>(at + 8 * i) =
+                make_float2(__uint_as_float(a[4 * i + 2 * r]),
+                            __uint_as_float(a[4 * i + 2 * r + 1]));
+        }
+      };
+      keep_acc(Cfg::kColAcc1, part);
+      keep_acc(Cfg::kColAcc0, part + Cfg::kRows * Cfg::kHeadDim);
+    } else if (Cfg::kDKV) {
       stage_acc(Cfg::kColAcc1, p.scale, res);                    // dK over the k tile
       stage_acc(Cfg::kColAcc0, 1.0f, res + Cfg::kTileBytes);     // dV over the v tile
     } else {
@@ -552,8 +796,7 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
     __syncwarp();
     // staging rows written: the store warp takes the unit from here (bwd_store_role)
     if (lane == 0) mbar_arrive(bar(Cfg::kBarStage));
-    cur.j = cur.j1 - 1;
-    cur.step(p);
+    cur.next_unit(p);
   }
 }
 
@@ -562,26 +805,27 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
 // the stores have read them; the softmax-side warps go straight on to the next unit.
 template <class Cfg>
 __device__ __forceinline__ void bwd_store_role(const BwdParams& p, uint8_t* smem, uint32_t bars,
-                                               const Watchdog& wd) {
+                                               const Watchdog& wd, const BwdClaims& claims) {
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
-  BwdCursor<Cfg> cur;
-  cur.init(p);
+  typename Cfg::Cursor cur;
+  cur.init(p, claims, BwdRole::kLane);
   int stores = 0;
   while (cur.valid()) {
     const int b = cur.seg & 1;
     if (!wait_single(bar(Cfg::kBarStage), static_cast<uint32_t>(stores) & 1u, wd, kSiteSoftStage))
       break;
     uint8_t* res = smem + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
-    const int r0 = (cur.u % p.blocks) * Cfg::kRows;
-    const HeadBatch hb = bwd_head_batch(p, cur.u);
-    tma_store_4d(&p.tm_o0, smem_addr(res), 0, r0, hb.h, hb.b);
-    if (Cfg::kDKV) tma_store_4d(&p.tm_o1, smem_addr(res + Cfg::kTileBytes), 0, r0, hb.h, hb.b);
-    tma_store_commit();
-    tma_store_wait_read();
+    if (!cur.in_pieces()) {
+      const int r0 = cur.row_block(p) * Cfg::kRows;
+      const HeadBatch hb = cur.resident(p);
+      tma_store_4d(&p.tm_o0, smem_addr(res), 0, r0, hb.h, hb.b);
+      if (Cfg::kDKV) tma_store_4d(&p.tm_o1, smem_addr(res + Cfg::kTileBytes), 0, r0, hb.h, hb.b);
+      tma_store_commit();
+      tma_store_wait_read();
+    }
     mbar_arrive(bar(Cfg::kBarResEmpty + b));
     ++stores;
-    cur.j = cur.j1 - 1;
-    cur.step(p);
+    cur.next_unit(p);
   }
   // unwinding or done: shared memory must outlive every store's read of it
   tma_store_wait_read();
@@ -605,6 +849,12 @@ __device__ __forceinline__ void bwd_init_bars(uint32_t bars) {
   mbar_init(bars + 8 * Cfg::kBarStage, Cfg::kSoftmaxWarps);
   mbar_init(bars + 8 * Cfg::kBarDrain, 1);
   mbar_init(bars + 8 * (Cfg::kBarDrain + 1), 1);
+  if constexpr (Cfg::kWindow) {
+    for (int i = 0; i < Cfg::kClaims; ++i) {
+      mbar_init(bars + 8 * (Cfg::kBarClaimFull + i), 1);
+      mbar_init(bars + 8 * (Cfg::kBarClaimEmpty + i), Cfg::kClaimReaders);
+    }
+  }
   mbar_init_fence();
 }
 
@@ -622,7 +872,8 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
   constexpr int kBarOff = CA::kBarOff > CB::kBarOff ? CA::kBarOff : CB::kBarOff;
   constexpr int kTmemSlotOff = kBarOff + CA::kNumBars * 8;
   constexpr int kAbortOff = kTmemSlotOff + 4;
-  static_assert(kAbortOff + 4 + 1024 <= (CA::kSmemBytes > CB::kSmemBytes ? CA::kSmemBytes
+  constexpr int kRingBytes = CA::kWindow ? 4 * CA::kClaims : 0;
+  static_assert(kAbortOff + 4 + kRingBytes + 1024 <= (CA::kSmemBytes > CB::kSmemBytes ? CA::kSmemBytes
                                                                          : CB::kSmemBytes),
                 "barriers inside the launch's shared memory");
   extern __shared__ uint8_t smem_raw[];
@@ -633,6 +884,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
   const uint32_t bars = smem_addr(smem + kBarOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kTmemSlotOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
+  volatile int* ring = reinterpret_cast<volatile int*>(smem + kAbortOff + 4);
   // Between the passes: true if the second pass runs (the same verdict in every thread:
   // nothing writes the flag between the two barriers).
   auto next_pass = [&]() -> bool {
@@ -661,9 +913,10 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     named_bar_arrive(1, CA::kThreads);
     setmaxnreg_dec<CA::kControlRegs>();
     const Watchdog wd{abort_flag, pa.status, pa.timeout_ns};
-    if (lane == 0) bwd_load_role<CA>(pa, smem, bars, wd);
+    const BwdClaims claims{ring, bars, &wd};
+    if (lane == 0) bwd_load_role<CA>(pa, smem, bars, wd, claims);
     if constexpr (kTwo) {
-      if (next_pass() && lane == 0) bwd_load_role<CB>(pb, smem, bars, wd);
+      if (next_pass() && lane == 0) bwd_load_role<CB>(pb, smem, bars, wd, claims);
     }
   } else {
     if (warp == 0) {
@@ -675,29 +928,30 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     tc_fence_after();
     tmem = *tmem_slot;
     const Watchdog wd{abort_flag, pa.status, pa.timeout_ns};
+    const BwdClaims claims{ring, bars, &wd};
     if (warp < CA::kSoftmaxWarps) {
       setmaxnreg_inc<CA::kSoftmaxRegs>();
-      bwd_softmax_role<CA>(pa, smem, bars, tmem, wd);
+      bwd_softmax_role<CA>(pa, smem, bars, tmem, wd, claims);
       if constexpr (kTwo) {
-        if (next_pass()) bwd_softmax_role<CB>(pb, smem, bars, tmem, wd);
+        if (next_pass()) bwd_softmax_role<CB>(pb, smem, bars, tmem, wd, claims);
       }
     } else {
       setmaxnreg_dec<CA::kControlRegs>();
       if (warp == CA::kMmaWarp) {
-        bwd_mma_role<CA, false>(pa, smem, bars, tmem, wd);
+        bwd_mma_role<CA, false>(pa, smem, bars, tmem, wd, claims);
       } else if (warp == CA::kAccWarp) {
-        bwd_mma_role<CA, true>(pa, smem, bars, tmem, wd);
+        bwd_mma_role<CA, true>(pa, smem, bars, tmem, wd, claims);
       } else if (warp == CA::kStoreWarp) {
-        if (lane == 0) bwd_store_role<CA>(pa, smem, bars, wd);
+        if (lane == 0) bwd_store_role<CA>(pa, smem, bars, wd, claims);
       }
       if constexpr (kTwo) {
         if (next_pass()) {
           if (warp == CB::kMmaWarp) {
-            bwd_mma_role<CB, false>(pb, smem, bars, tmem, wd);
+            bwd_mma_role<CB, false>(pb, smem, bars, tmem, wd, claims);
           } else if (warp == CB::kAccWarp) {
-            bwd_mma_role<CB, true>(pb, smem, bars, tmem, wd);
+            bwd_mma_role<CB, true>(pb, smem, bars, tmem, wd, claims);
           } else if (warp == CB::kStoreWarp) {
-            if (lane == 0) bwd_store_role<CB>(pb, smem, bars, wd);
+            if (lane == 0) bwd_store_role<CB>(pb, smem, bars, wd, claims);
           }
         }
       }
@@ -735,6 +989,58 @@ __global__ void __launch_bounds__(BwdConfig<true, kCausal, kBF16>::kThreads, 1)
   bwd_cta<BwdConfig<true, kCausal, kBF16>, BwdConfig<false, kCausal, kBF16>, true>(pkv, pq);
 }
 
+// Window variant: every CTA on both passes, dK/dV units first (they are the longer ones), each
+// unit claimed from the pass's counter.
+template <bool kBF16>
+__global__ void __launch_bounds__(BwdConfig<true, true, kBF16, true>::kThreads, 1)
+    mfa_bwd_window_kernel(const __grid_constant__ BwdParams pq,
+                          const __grid_constant__ BwdParams pkv) {
+  bwd_cta<BwdConfig<true, true, kBF16, true>, BwdConfig<false, true, kBF16, true>, true>(pkv, pq);
+}
+
+// dK and dV of the blocks whose units ran in pieces: the sum of the pieces in order, dK scaled.
+// One CTA per (block, k / v head row) pair that may have pieces, sink blocks first; 16 threads per
+// row, four columns each.
+template <bool kBF16>
+__global__ void __launch_bounds__(256) mfa_bwd_reduce_kernel(const BwdParams p, uint16_t* dk,
+                                                             uint16_t* dv, long long stride_b,
+                                                             long long stride_h,
+                                                             long long stride_n) {
+  constexpr int kTile = 128 * 64;
+  const int pair = static_cast<int>(blockIdx.x);
+  const int blk = pair / p.bh, row = pair % p.bh;
+  const bool sink = blk < p.sink_blocks;
+  const int span = BwdWindowCursor<BwdConfig<true, true, kBF16, true>>::span(p, blk);
+  const int chunk = sink ? p.chunk_sink : p.chunk_rest;
+  const int count = (span * p.group + chunk - 1) / chunk;
+  if (count < 2) return;
+  // unit index of the pair's piece 0; its pieces are p.bh apart
+  const long long first =
+      sink ? static_cast<long long>(blk) * p.bh * p.pieces_sink + row
+           : static_cast<long long>(p.sink_blocks) * p.bh * p.pieces_sink +
+                 static_cast<long long>(blk - p.sink_blocks) * p.bh * p.pieces_rest + row;
+  const long long base =
+      static_cast<long long>(row / p.heads) * stride_b + (row % p.heads) * stride_h;
+  const int col = 4 * (threadIdx.x & 15);
+  for (int r = threadIdx.x >> 4; r < 128 && blk * 128 + r < p.n; r += 16) {
+    float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+    for (int i = 0; i < count; ++i) {
+      const float* at = p.partials + (first + static_cast<long long>(i) * p.bh) * (2 * kTile) +
+                        r * 64 + col;
+      const float4 a = *reinterpret_cast<const float4*>(at);
+      const float4 b = *reinterpret_cast<const float4*>(at + kTile);
+      k.x += a.x, k.y += a.y, k.z += a.z, k.w += a.w;
+      v.x += b.x, v.y += b.y, v.z += b.z, v.w += b.w;
+    }
+    const long long off = base + static_cast<long long>(blk * 128 + r) * stride_n + col;
+    *reinterpret_cast<uint2*>(dk + off) =
+        make_uint2(pack_pair<kBF16>(k.x * p.scale, k.y * p.scale),
+                   pack_pair<kBF16>(k.z * p.scale, k.w * p.scale));
+    *reinterpret_cast<uint2*>(dv + off) =
+        make_uint2(pack_pair<kBF16>(v.x, v.y), pack_pair<kBF16>(v.z, v.w));
+  }
+}
+
 // One pass per launch (many units per SM), all CTAs on it; a kernel of its own, which measured
 // 2-5% faster than the two-pass kernel above run with all CTAs on one pass.
 template <bool kDKV, bool kCausal, bool kBF16>
@@ -760,7 +1066,10 @@ __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const 
                                                            const float* lse, float* lse2,
                                                            float* di, int bh, int n, int heads,
                                                            long long stride_b, long long stride_h,
-                                                           long long stride_n, int blocks) {
+                                                           long long stride_n, int blocks,
+                                                           int* counters = nullptr) {
+  // window variant: the two passes' unit counters start at zero
+  if (counters != nullptr && blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
   const long long rows = static_cast<long long>(bh) * blocks * 128;  // a multiple of 4
   const int sub = threadIdx.x & 7;
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);

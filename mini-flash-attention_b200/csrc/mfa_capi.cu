@@ -19,6 +19,7 @@
 #include "../../include/mfa_b200.h"
 #include "mfa_bwd_kernel.cuh"
 #include "mfa_fwd_kernel.cuh"
+#include "mfa_host.h"
 
 namespace mfa {
 namespace {
@@ -420,21 +421,27 @@ int check_common(const void* q, const void* k, const void* v, void* out, int64_t
 // q, k, v and out must be memory that device `dev` addresses directly (its own device memory
 // or managed memory). A host, foreign or dangling pointer is refused here, before anything is
 // launched, instead of faulting the GPU inside the kernel.
+int check_device_pointer(const void* ptr, const char* name, int dev) {
+  cudaPointerAttributes a = {};
+  const cudaError_t e = cudaPointerGetAttributes(&a, ptr);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(MFA_ERR_INVALID_ARGUMENT, std::string(name) + " is not a CUDA pointer");
+  }
+  const bool ok = (a.type == cudaMemoryTypeDevice && a.device == dev) ||
+                  a.type == cudaMemoryTypeManaged;
+  if (!ok)
+    return fail(MFA_ERR_INVALID_ARGUMENT,
+                std::string(name) + " must point to memory of the current device");
+  return MFA_OK;
+}
+
 int check_device_pointers(const void* q, const void* k, const void* v, const void* out, int dev) {
   const void* ptrs[4] = {q, k, v, out};
   const char* names[4] = {"q", "k", "v", "out"};
   for (int i = 0; i < 4; ++i) {
-    cudaPointerAttributes a = {};
-    const cudaError_t e = cudaPointerGetAttributes(&a, ptrs[i]);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      return fail(MFA_ERR_INVALID_ARGUMENT, std::string(names[i]) + " is not a CUDA pointer");
-    }
-    const bool ok = (a.type == cudaMemoryTypeDevice && a.device == dev) ||
-                    a.type == cudaMemoryTypeManaged;
-    if (!ok)
-      return fail(MFA_ERR_INVALID_ARGUMENT,
-                  std::string(names[i]) + " must point to memory of the current device");
+    const int rc = check_device_pointer(ptrs[i], names[i], dev);
+    if (rc != MFA_OK) return rc;
   }
   return MFA_OK;
 }
@@ -556,6 +563,64 @@ __global__ void __launch_bounds__(32, 1) watchdog_selftest_kernel(unsigned long 
 }
 
 }  // namespace
+}  // namespace mfa
+
+// What the other translation units of the library share with this one (mfa_host.h).
+namespace mfa {
+namespace host {
+
+int fail(int code, const std::string& msg) { return mfa::fail(code, msg); }
+int fail_cuda(cudaError_t e, const char* what) { return mfa::fail_cuda(e, what); }
+
+int open_device(Device* out) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaGetDevice");
+  const int rc = prepare_device(dev);
+  if (rc != MFA_OK) return rc;
+  const DeviceState& ds = g_devices[dev];
+  *out = {dev, ds.num_sms, ds.status_ptr, ds.pool, g_watchdog_ns};
+  return MFA_OK;
+}
+
+int check_pointer(const void* p, const char* name, int dev) {
+  return check_device_pointer(p, name, dev);
+}
+
+int encode_heads(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
+                 int64_t d, int layout, bool bf16) {
+  return encode_tensor(map, base, batch, heads, n, d, layout, bf16);
+}
+
+int encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+               const uint64_t* stride_bytes, const uint32_t* box, bool bf16) {
+  std::string why;
+  auto encode = tensor_map_encoder(&why);
+  if (!encode) return fail(MFA_ERR_CUDA, why);
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], one[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    one[i] = 1;
+    if (i + 1 < rank) s[i] = stride_bytes[i];
+  }
+  const CUresult r = encode(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+      static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, b, one,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(MFA_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
+  return MFA_OK;
+}
+
+Strides strides_of(int layout, int64_t heads, int64_t n, int64_t d) {
+  const mfa::Strides s = layout_strides(layout, heads, n, d);
+  return {s.n, s.h, s.b};
+}
+
+}  // namespace host
 }  // namespace mfa
 
 using namespace mfa;

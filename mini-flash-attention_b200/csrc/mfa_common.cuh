@@ -36,6 +36,12 @@ struct FwdParams {
   // Optional (null: not written): natural-log row log-sum-exp of the scaled scores,
   // lse[bh * N + row] = ln(sum_k exp(scale * q.k)), for the backward pass.
   float* lse;
+  // Window variant: query i sees keys j <= i with j > i - window or j < sinks; the key blocks
+  // [0, sink_blocks) hold sinks; query head h reads k / v head h / kv_group.
+  int window;
+  int sinks;
+  int sink_blocks;
+  int kv_group;
 };
 
 // Status codes written to FwdParams::status by the watchdog: kStatusTimeoutBase + site. The

@@ -45,6 +45,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "mfa_common.cuh"
 #include "mfa_exp2.cuh"
@@ -53,8 +54,18 @@
 
 namespace mfa {
 
-template <int NQ_, int STAGES_, bool CAUSAL_, bool BF16_, int D_, bool LSE_ = false>
+template <bool kCausal>
+struct StepCursor;
+template <int kRowsPerUnit>
+struct WindowCursor;
+
+template <int NQ_, int STAGES_, bool CAUSAL_, bool BF16_, int D_, bool LSE_ = false,
+          bool WINDOW_ = false>
 struct FwdConfig {
+  // Sliding window with sink tokens, and k / v heads shared by groups of query heads (a
+  // causal variant: query i sees key j if j <= i and (j > i - window or j < sinks)).
+  static constexpr bool kWindow = WINDOW_;
+  static_assert(!WINDOW_ || (CAUSAL_ && LSE_), "the window variant is causal, lse optional");
   static constexpr bool kLSE = LSE_;  // also write the row log-sum-exp (FwdParams::lse)
   static constexpr int NQ = NQ_;
   static constexpr int STAGES = STAGES_;
@@ -62,6 +73,7 @@ struct FwdConfig {
   static constexpr bool kBF16 = BF16_;      // q, k, v, P and out in bf16 instead of fp16
   static constexpr int kRows = 128;       // query rows per tile (= MMA M)
   static constexpr int kRowsPerUnit = kRows * NQ;
+  using Cursor = std::conditional_t<WINDOW_, WindowCursor<kRows * NQ_>, StepCursor<CAUSAL_>>;
   static constexpr int kKeys = 128;       // keys per block (= S tile N)
   static constexpr int kHeadDim = D_;     // 32, 64 or 128
   static constexpr int kTileBytes = kRows * kHeadDim * 2;  // one 128-row tile of q, k or v
@@ -217,6 +229,71 @@ struct StepCursor {
   }
 };
 
+// Walks whole query blocks u = cta, cta + ctas, ... of the windowed attention, whose key blocks
+// are those that hold sinks and lie before the window, then those from the oldest key that the
+// block's first row sees to its last row: steps() of them, numbered j, key block block().
+// A query block qb whose window starts past key 0 has kRowsPerUnit / 128 + ceil((window - 1) /
+// 128) window blocks, the same for all of them, so the blocks are dealt out without a split.
+template <int kRowsPerUnit>
+struct WindowCursor {
+  int u;        // current query block, row-major over (head, query block)
+  int j;        // current step
+  int j0, j1;   // steps of u: [0, j1)
+  int rem;      // query blocks after this one
+  int seg_idx;  // index of the current query block in this CTA
+  int sinks;    // steps before the window
+  int skip;     // key blocks between them and the window
+
+  __device__ void start(const FwdParams& p) {
+    const int qb = p.sc.qb_of(u);
+    const int oldest = qb * kRowsPerUnit - p.window + 1;  // key of the block's first row
+    const int w0 = oldest > 0 ? oldest >> 7 : 0;
+    const int last = (qb + 1) * (kRowsPerUnit / 128) - 1;
+    sinks = p.sink_blocks < w0 ? p.sink_blocks : w0;
+    skip = w0 - sinks;
+    j = j0 = 0;
+    j1 = (last < p.sc.nkb ? last + 1 : p.sc.nkb) - skip;
+  }
+  __device__ void init(const FwdParams& p) {
+    const int units = p.sc.bh * p.sc.q_blocks;  // < 2^31 (checked by the launcher)
+    seg_idx = 0;
+    u = static_cast<int>(blockIdx.x);
+    rem = u < units ? (units - 1 - u) / static_cast<int>(gridDim.x) : 0;
+    if (u < units) {
+      start(p);
+    } else {
+      u = 0;
+      j = j0 = j1 = sinks = skip = 0;
+    }
+  }
+  __device__ bool valid() const { return j < j1; }
+  __device__ bool first_step() const { return j == 0; }
+  __device__ bool first_of_range() const { return seg_idx == 0; }
+  __device__ bool whole(const Schedule&) const { return true; }
+  __device__ int block() const { return j < sinks ? j : j + skip; }
+  __device__ void next_segment(const FwdParams& p) {
+    j = j1 - 1;
+    step(p);
+  }
+  __device__ void step(const FwdParams& p) {
+    if (++j >= j1 && rem > 0) {
+      u += static_cast<int>(gridDim.x);
+      --rem;
+      ++seg_idx;
+      start(p);
+    }
+  }
+};
+
+// Whether key block kb holds a key that some row of the 128-row tile at query row r0 sees (of a
+// tile past the last row, every block: nobody reads its result, and it keeps at least one).
+// A unit of two tiles takes one window block more than each of them needs: tile 0 does not see
+// the block of tile 1's diagonal, tile 1 not the oldest block of tile 0.
+__device__ __forceinline__ bool window_live(const FwdParams& p, int r0, int kb) {
+  if (r0 >= p.nq) return true;
+  return kb * 128 <= r0 + 127 && (kb * 128 + 127 > r0 - p.window || kb < p.sink_blocks);
+}
+
 // Head and batch index of unit u: its (batch * head) row is u / q_blocks, heads fastest.
 __device__ __forceinline__ HeadBatch head_batch(const FwdParams& p, int u) {
   const int bh = p.sc.head_of(u);
@@ -236,7 +313,7 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
   // K/V blocks are re-read by every query-block pass over the same head: keep them in L2.
   const uint64_t keep = l2_policy_evict_last();
 
-  StepCursor<Cfg::kCausal> cur;
+  typename Cfg::Cursor cur;
   cur.init(p);
   int g = 0;  // global step index of this CTA
   int q_loaded = 0, k_issued = 0, v_issued = 0;
@@ -262,13 +339,20 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
     }
     const int st = g % ST;
     const uint32_t ph = static_cast<uint32_t>(g / ST) & 1u;
+    int key0, kv_head;  // first key and head of this step's k and v block
+    if constexpr (Cfg::kWindow) {
+      key0 = cur.block() * Cfg::kKeys;
+      kv_head = hb.h / p.kv_group;
+    } else {
+      key0 = cur.j * Cfg::kKeys;
+      kv_head = hb.h;
+    }
     if (!wait_single(bar(Cfg::kBarKEmpty + st), ph ^ 1u, wd, kSiteLoadKEmpty)) break;
     mbar_arrive_expect_tx(bar(Cfg::kBarKFull + st), Cfg::kTileBytes);
 #pragma unroll
     for (int x = 0; x < Cfg::kBoxes; ++x) {
       tma_load_4d_hint(sbase + Cfg::kKOff + st * Cfg::kTileBytes + x * Cfg::kBoxBytes, &p.tm_k,
-                       bar(Cfg::kBarKFull + st), x * Cfg::kBoxCols, cur.j * Cfg::kKeys, hb.h,
-                       hb.b, keep);
+                       bar(Cfg::kBarKFull + st), x * Cfg::kBoxCols, key0, kv_head, hb.b, keep);
     }
     k_issued = g + 1;
     if (!wait_single(bar(Cfg::kBarVEmpty + st), ph ^ 1u, wd, kSiteLoadVEmpty)) break;
@@ -276,8 +360,7 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
 #pragma unroll
     for (int x = 0; x < Cfg::kBoxes; ++x) {
       tma_load_4d_hint(sbase + Cfg::kVOff + st * Cfg::kTileBytes + x * Cfg::kBoxBytes, &p.tm_v,
-                       bar(Cfg::kBarVFull + st), x * Cfg::kBoxCols, cur.j * Cfg::kKeys, hb.h,
-                       hb.b, keep);
+                       bar(Cfg::kBarVFull + st), x * Cfg::kBoxCols, key0, kv_head, hb.b, keep);
     }
     v_issued = g + 1;
     ++g;
@@ -336,10 +419,14 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
   const bool leader = elect_one();
   bool issued_any = false;
 
-  StepCursor<Cfg::kCausal> cs, cp;  // next S step, next P.V step
+  typename Cfg::Cursor cs, cp;  // next S step, next P.V step
   cs.init(p);
   cp.init(p);
   int gs = 0, gp = 0;
+  // Window variant: the tile's own steps so far (the blocks it sees; the ring is walked by all
+  // of the unit's), and whether its current unit has had a P.V product.
+  [[maybe_unused]] int ts = 0, tp = 0;
+  [[maybe_unused]] bool fresh_unit = true;
   // S_i[gs] = Q_i K_gs^T once softmax_i has pulled S_i[gs-1] into registers.
   auto issue_s = [&]() -> bool {
     const int b = cs.seg_idx & 1;
@@ -352,10 +439,14 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
     if (!wait_warp(bar(Cfg::kBarKFull + st), static_cast<uint32_t>(gs / ST) & 1u, wd, kSiteMmaK))
       return false;
     const uint32_t kd = k_lo + st * kTileStep;
-    {
+    bool live = true;
+    if constexpr (Cfg::kWindow)
+      live = window_live(p, p.sc.qb_of(cs.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows, cs.block());
+    if (live) {
       const int i = tile;
-      if (gs > 0) {
-        if (!wait_warp(bar(Cfg::kBarSFree + i), static_cast<uint32_t>(gs - 1) & 1u, wd,
+      const int n_s = Cfg::kWindow ? ts : gs;  // S products of this tile before this one
+      if (n_s > 0) {
+        if (!wait_warp(bar(Cfg::kBarSFree + i), static_cast<uint32_t>(n_s - 1) & 1u, wd,
                        kSiteMmaSFree))
           return false;
       }
@@ -372,6 +463,7 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       }
       __syncwarp();
       issued_any = true;
+      ++ts;
     }
     if (leader) mma_commit(bar(Cfg::kBarKEmpty + st));
     __syncwarp();
@@ -391,11 +483,19 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       if (!wait_warp(bar(Cfg::kBarVFull + st), static_cast<uint32_t>(gp / ST) & 1u, wd, kSiteMmaV))
         goto unwind;
       const uint32_t vd = v_lo + st * kTileStep;
-      const bool fresh = cp.first_step();  // first block of a unit: overwrite O
-      {
+      bool fresh = cp.first_step();  // first block of a unit: overwrite O
+      bool live = true;
+      if constexpr (Cfg::kWindow) {
+        live = window_live(p, p.sc.qb_of(cp.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows,
+                           cp.block());
+        if (fresh) fresh_unit = true;
+        fresh = fresh_unit;  // the first block that the tile sees
+        if (live) fresh_unit = false;
+      }
+      if (live) {
         const int i = tile;
-        if (!wait_warp(bar(Cfg::kBarPFull + i), static_cast<uint32_t>(gp) & 1u, wd,
-                       kSiteMmaPFull))
+        if (!wait_warp(bar(Cfg::kBarPFull + i),
+                       static_cast<uint32_t>(Cfg::kWindow ? tp : gp) & 1u, wd, kSiteMmaPFull))
           goto unwind;
         tc_fence_after();
         if (leader) {
@@ -410,6 +510,7 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
         }
         __syncwarp();
         issued_any = true;
+        ++tp;
       }
       if (leader) mma_commit(bar(Cfg::kBarVEmpty + st));
       __syncwarp();
@@ -476,6 +577,23 @@ __device__ __forceinline__ bool softmax_step(const FwdParams& p, uint32_t bars, 
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
+      }
+    }
+    if constexpr (Cfg::kWindow) {
+      // Keys older than the window score -inf, but for the sinks. A block is tested when its
+      // first key is too old for the slice's last row and it holds other keys than sinks.
+      if (key0 <= row0 + 15 - p.window && key0 + Cfg::kKeys > p.sinks) {
+        const int t0 = row0 + (lane >> 2) - p.window - key0;  // row g: too old when c <= t0
+        const int s0 = p.sinks - key0;                        // a sink when c < s0
+        const int q2 = 2 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = 8 * i + q2 + (e & 1);
+            if (c <= t0 + 8 * (e >> 1) && c >= s0) sr[4 * i + e] = __float_as_uint(-INFINITY);
+          }
+        }
       }
     }
   }
@@ -601,7 +719,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
 
   int g = 0;  // global step index (phase of the per-step barriers)
   [[maybe_unused]] int stores = 0;  // whole units stored (staging phase; no store warp)
-  StepCursor<Cfg::kCausal> cur;
+  typename Cfg::Cursor cur;
   cur.init(p);
   while (cur.valid()) {
     float m_run[2] = {-INFINITY, -INFINITY};  // running max of s*scale*log2(e), per row
@@ -609,10 +727,23 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     const int row0 =  // first query row of this warp's slice (causal masking only)
         Cfg::kCausal ? p.q0 + p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows + slice
                      : 0;
-    for (int j = cur.j0; j < cur.j1; ++j, ++g) {
-      if (!softmax_step<Cfg>(p, bars, tS, tP, tO, tile, lane, g, j, row0, j == cur.j0, m_run,
-                             l_run, wd))
-        return;
+    if constexpr (Cfg::kWindow) {
+      bool first = true;
+      for (; cur.j < cur.j1; ++cur.j) {
+        const int kb = cur.block();
+        if (!window_live(p, row0 - slice, kb)) continue;
+        if (!softmax_step<Cfg>(p, bars, tS, tP, tO, tile, lane, g, kb, row0, first, m_run, l_run,
+                               wd))
+          return;
+        first = false;
+        ++g;
+      }
+    } else {
+      for (int j = cur.j0; j < cur.j1; ++j, ++g) {
+        if (!softmax_step<Cfg>(p, bars, tS, tP, tO, tile, lane, g, j, row0, j == cur.j0, m_run,
+                               l_run, wd))
+          return;
+      }
     }
     // ---- unit epilogue (g - 1 is the unit's last step)
     if (!wait_warp(bar(Cfg::kBarODone + tile), static_cast<uint32_t>(g - 1) & 1u, wd,
@@ -630,7 +761,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     tc_fence_before();
     const int b = cur.seg_idx & 1;
     if (cur.whole(p.sc)) {
-      if (Cfg::kLSE && q == 0) {
+      if (Cfg::kLSE && q == 0 && (!Cfg::kWindow || p.lse != nullptr)) {
         // log-sum-exp = ln 2 * (m + log2 l), m in scaled log2 units
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -718,7 +849,7 @@ template <class Cfg>
 __device__ __forceinline__ void store_role(const FwdParams& p, uint8_t* smem, uint32_t bars,
                                            const Watchdog& wd) {
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
-  StepCursor<Cfg::kCausal> cur;
+  typename Cfg::Cursor cur;
   cur.init(p);
   int stores = 0;  // whole units stored so far (phase of the staging barriers)
   while (cur.valid()) {
@@ -755,10 +886,11 @@ __device__ __forceinline__ void store_role(const FwdParams& p, uint8_t* smem, ui
   tma_store_wait_read();
 }
 
-template <int NQ, int STAGES, bool CAUSAL, bool BF16, int D, bool LSE>
-__global__ void __launch_bounds__(FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE>::kThreads, 1)
+template <int NQ, int STAGES, bool CAUSAL, bool BF16, int D, bool LSE, bool WINDOW = false>
+__global__ void __launch_bounds__(FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WINDOW>::kThreads,
+                                  1)
     mfa_fwd_kernel(const __grid_constant__ FwdParams p) {
-  using Cfg = FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE>;
+  using Cfg = FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WINDOW>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));

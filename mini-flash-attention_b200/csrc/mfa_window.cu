@@ -1,0 +1,353 @@
+// C-ABI launchers of the windowed attention (sliding window with sink tokens, grouped k / v heads):
+// forward and backward. Query i sees key j if j <= i and (j > i - window or j < sinks); query head
+// h reads k / v head h / (heads / kv_heads). The kernels are the window variants of the forward and
+// backward kernels (mfa_fwd_kernel.cuh, mfa_bwd_kernel.cuh).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+#include <string>
+
+#include "../../include/mfa_b200.h"
+#include "mfa_bwd_kernel.cuh"
+#include "mfa_fwd_kernel.cuh"
+#include "mfa_host.h"
+
+namespace mfa {
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+// The head dim's tile count and ring depth are the causal forward's.
+template <bool kBF16, int D>
+using Window = FwdConfig<D == 128 ? 1 : 2, D == 128 ? 2 : 3, true, kBF16, D, true, true>;
+
+template <class Cfg>
+auto* window_kernel() {
+  return &mfa_fwd_kernel<Cfg::NQ, Cfg::STAGES, true, Cfg::kBF16, Cfg::kHeadDim, true, true>;
+}
+
+template <bool kBF16>
+constexpr int window_bwd_smem() {
+  using CQ = BwdConfig<false, true, kBF16, true>;
+  using CK = BwdConfig<true, true, kBF16, true>;
+  return CQ::kSmemBytes > CK::kSmemBytes ? CQ::kSmemBytes : CK::kSmemBytes;
+}
+
+template <bool kBF16>
+cudaError_t set_attributes() {
+  const auto smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(window_kernel<Window<kBF16, 32>>(), smem,
+                                       Window<kBF16, 32>::kSmemBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(window_kernel<Window<kBF16, 64>>(), smem,
+                             Window<kBF16, 64>::kSmemBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(window_kernel<Window<kBF16, 128>>(), smem,
+                             Window<kBF16, 128>::kSmemBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(mfa_bwd_window_kernel<kBF16>, smem, window_bwd_smem<kBF16>());
+  return e;
+}
+
+int prepare(int dev) {
+  static std::once_flag once[kMaxDevices];
+  static cudaError_t error[kMaxDevices];
+  std::call_once(once[dev], [dev] {
+    error[dev] = set_attributes<false>();
+    if (error[dev] == cudaSuccess) error[dev] = set_attributes<true>();
+  });
+  return error[dev] == cudaSuccess ? MFA_OK : host::fail_cuda(error[dev], "window kernel set-up");
+}
+
+// The arguments of both directions, checked.
+struct Problem {
+  int64_t batch, heads, kv_heads, n, window, sinks;
+  int32_t d, dtype, layout;
+  float scale;
+};
+
+int check(Problem& w) {
+  if (w.batch < 0 || w.heads < 0 || w.kv_heads < 0 || w.n < 0)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "negative extent");
+  if (w.d != 32 && w.d != 64 && w.d != 128)
+    return host::fail(MFA_ERR_HEAD_DIM, "This kernel supports only D=32, D=64 and D=128");
+  if (w.dtype != MFA_DTYPE_FP16 && w.dtype != MFA_DTYPE_BF16)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "dtype must be MFA_DTYPE_FP16 or MFA_DTYPE_BF16");
+  if (w.layout != MFA_LAYOUT_BHND && w.layout != MFA_LAYOUT_BNHD)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT,
+                      "layout must be MFA_LAYOUT_BHND or MFA_LAYOUT_BNHD");
+  if (!(w.scale > 0.0f) || !std::isfinite(w.scale))
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+  if (w.window < 1) return host::fail(MFA_ERR_INVALID_ARGUMENT, "window must be at least 1");
+  if (w.sinks < 0) return host::fail(MFA_ERR_INVALID_ARGUMENT, "sinks must not be negative");
+  if (w.heads > 0 && (w.kv_heads == 0 || w.heads % w.kv_heads != 0))
+    return host::fail(MFA_ERR_INVALID_ARGUMENT,
+                      "the number of query heads must be a multiple of the k / v heads");
+  // blocks, units and steps are counted in 32 bits
+  if (w.n > 0x7fff0000LL) return host::fail(MFA_ERR_INVALID_ARGUMENT, "N is too large");
+  if (w.heads > 0 && w.batch > 0x7fffffffLL / w.heads)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "B * H is too large");
+  const int64_t blocks = (w.n + 127) / 128;
+  if (static_cast<double>(blocks) * static_cast<double>(w.batch * w.heads) > 0x3fff0000)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "B * H * N is too large");
+  // beyond the sequence both mean the same
+  if (w.window >= w.n) {
+    w.window = w.n > 0 ? w.n : 1;
+    w.sinks = 0;
+  }
+  if (w.sinks > w.n) w.sinks = w.n;
+  return MFA_OK;
+}
+
+int check_tensors(const void* const* ptrs, const char* const* names, int count, int dev) {
+  for (int i = 0; i < count; ++i) {
+    if (!ptrs[i]) return host::fail(MFA_ERR_INVALID_ARGUMENT, std::string("null ") + names[i]);
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15u)
+      return host::fail(MFA_ERR_INVALID_ARGUMENT,
+                        std::string(names[i]) + " must be 16-byte aligned");
+    const int rc = dev < 0 ? MFA_OK : host::check_pointer(ptrs[i], names[i], dev);
+    if (rc != MFA_OK) return rc;
+  }
+  return MFA_OK;
+}
+
+template <class Cfg>
+int launch_forward(const void* q, const void* k, const void* v, void* out, float* lse,
+                   const Problem& w, const host::Device& dev, cudaStream_t stream) {
+  FwdParams p = {};
+  const bool bf16 = Cfg::kBF16;
+  int rc = host::encode_heads(&p.tm_q, q, w.batch, w.heads, w.n, w.d, w.layout, bf16);
+  if (rc == MFA_OK)
+    rc = host::encode_heads(&p.tm_k, k, w.batch, w.kv_heads, w.n, w.d, w.layout, bf16);
+  if (rc == MFA_OK)
+    rc = host::encode_heads(&p.tm_v, v, w.batch, w.kv_heads, w.n, w.d, w.layout, bf16);
+  if (rc == MFA_OK)
+    rc = host::encode_heads(&p.tm_o, out, w.batch, w.heads, w.n, w.d, w.layout, bf16);
+  if (rc != MFA_OK) return rc;
+  p.n = p.nq = static_cast<int>(w.n);
+  p.heads = static_cast<int>(w.heads);
+  p.sc = make_schedule(w.batch * w.heads, w.n, w.n, Cfg::kRowsPerUnit, Cfg::kKeys, true);
+  p.scale_log2 = w.scale * 1.4426950408889634f;
+  p.timeout_ns = dev.timeout_ns;
+  p.status = dev.status;
+  p.lse = lse;
+  p.window = static_cast<int>(w.window);
+  p.sinks = static_cast<int>(w.sinks);
+  p.sink_blocks = static_cast<int>((w.sinks + 127) / 128);
+  p.kv_group = static_cast<int>(w.heads / w.kv_heads);
+  const int64_t units = static_cast<int64_t>(p.sc.q_blocks) * p.sc.bh;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(units < dev.sms ? units : dev.sms));
+  cfg.blockDim = dim3(Cfg::kThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, window_kernel<Cfg>(), p);
+  return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "window forward launch");
+}
+
+// How the dK/dV pass cuts its units into pieces (BwdWindowCursor). `span_steps` is the number of
+// (key block, query block) pairs of one head that hold a visible (key, query) pair: both passes
+// walk every one of them, the dK/dV pass at about 1.05 times a dQ step's cost.
+struct Pieces {
+  int chunk_sink, pieces_sink, chunk_rest, pieces_rest;
+};
+
+Pieces plan_pieces(int64_t blocks, int64_t sink_blocks, int64_t span, int64_t span_steps,
+                   int64_t kv_rows, int64_t group, int64_t sms) {
+  const double share = 2.05 * static_cast<double>(span_steps) *
+                       static_cast<double>(kv_rows * group) / static_cast<double>(sms);
+  // A unit of `len` steps stays whole while it is not the longest thing a CTA does: up to
+  // three quarters of a CTA's share of the work (units are claimed longest first). Longer ones
+  // are cut to a third of it, but to no less than 16 steps: writing a piece's 64 KB of sums and
+  // reading them back costs as much as about three steps.
+  const auto cut = [&](int64_t len, int& chunk, int& pieces) {
+    int64_t c = len;
+    if (static_cast<double>(len) > 0.75 * share) {
+      c = static_cast<int64_t>(std::ceil(share / 3));
+      if (c < 16) c = 16;
+      if (c > len) c = len;
+    }
+    pieces = static_cast<int>((len + c - 1) / c);
+    chunk = static_cast<int>((len + pieces - 1) / pieces);
+  };
+  Pieces out;
+  cut(blocks * group, out.chunk_sink, out.pieces_sink);
+  cut(span * group, out.chunk_rest, out.pieces_rest);
+  return out;
+}
+
+template <bool kBF16>
+int launch_backward(const void* q, const void* k, const void* v, const void* out,
+                    const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                    const Problem& w, const host::Device& dev, cudaStream_t stream) {
+  const int64_t blocks = (w.n + 127) / 128, bh = w.batch * w.heads, bhk = w.batch * w.kv_heads;
+  const int64_t group = w.heads / w.kv_heads, sb = (w.sinks + 127) / 128;
+  // (key block, query block) pairs of one head: `reach` later query blocks see a key block
+  // that holds no sinks, all later ones one that does
+  const int64_t reach = (126 + w.window) >> 7;
+  const int64_t span = reach + 1 < blocks ? reach + 1 : blocks;
+  const int64_t rest = blocks - sb, short_ones = reach < rest ? reach : rest;
+  const int64_t span_steps = sb * blocks - sb * (sb - 1) / 2 + (rest - short_ones) * span +
+                             short_ones * (short_ones + 1) / 2;
+  const Pieces pc = plan_pieces(blocks, sb, span, span_steps, bhk, group, dev.sms);
+  const int64_t sink_units = bhk * sb * pc.pieces_sink;
+  const int64_t kv_units = sink_units + bhk * rest * pc.pieces_rest, q_units = bh * blocks;
+  if (kv_units > 0x3fff0000LL || blocks * group > 0x3fff0000LL)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "B * H * N is too large");
+  const int64_t slots = pc.pieces_rest > 1 ? kv_units : pc.pieces_sink > 1 ? sink_units : 0;
+
+  // L2 and D of every row, the two counters, the pieces' sums (256-byte aligned)
+  const size_t rows = static_cast<size_t>(q_units) * 128;
+  const size_t floats = 2 * rows + 64 + static_cast<size_t>(slots) * 2 * 128 * 64;
+  float* ws = nullptr;
+  cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), floats * sizeof(float),
+                                          dev.pool, stream);
+  if (e != cudaSuccess) return host::fail_cuda(e, "cudaMallocFromPoolAsync (backward workspace)");
+  float* lse2 = ws;
+  float* di = ws + rows;
+  int* counters = reinterpret_cast<int*>(ws + 2 * rows);
+
+  BwdParams pkv = {};
+  pkv.n = static_cast<int>(w.n);
+  pkv.blocks = static_cast<int>(blocks);
+  pkv.scale = w.scale;
+  pkv.scale_log2 = w.scale * 1.4426950408889634f;
+  pkv.lse2 = lse2;
+  pkv.di = di;
+  pkv.timeout_ns = dev.timeout_ns;
+  pkv.status = dev.status;
+  pkv.window = static_cast<int>(w.window);
+  pkv.sinks = static_cast<int>(w.sinks);
+  pkv.sink_blocks = static_cast<int>(sb);
+  pkv.group = static_cast<int>(group);
+  pkv.chunk_sink = pc.chunk_sink;
+  pkv.pieces_sink = pc.pieces_sink;
+  pkv.chunk_rest = pc.chunk_rest;
+  pkv.pieces_rest = pc.pieces_rest;
+  pkv.partials = ws + 2 * rows + 64;
+  BwdParams pq = pkv;
+  pkv.heads = static_cast<int>(w.kv_heads);
+  pkv.bh = static_cast<int>(bhk);
+  pkv.units = static_cast<int>(kv_units);
+  pkv.claimed = counters;
+  pq.heads = static_cast<int>(w.heads);
+  pq.bh = static_cast<int>(bh);
+  pq.units = static_cast<int>(q_units);
+  pq.claimed = counters + 1;
+
+  struct Map {
+    CUtensorMap* to;
+    const void* base;
+    int64_t heads;
+  };
+  // dQ: q, dO resident; k, v streamed. dK, dV: k, v resident; q, dO streamed.
+  const Map maps[] = {{&pq.tm_x, q, w.heads},        {&pq.tm_y, dout, w.heads},
+                      {&pq.tm_s0, k, w.kv_heads},    {&pq.tm_s1, v, w.kv_heads},
+                      {&pq.tm_o0, dq, w.heads},      {&pkv.tm_o0, dk, w.kv_heads},
+                      {&pkv.tm_o1, dv, w.kv_heads}};
+  int rc = MFA_OK;
+  for (const Map& m : maps) {
+    rc = host::encode_heads(m.to, m.base, w.batch, m.heads, w.n, 64, w.layout, kBF16);
+    if (rc != MFA_OK) break;
+  }
+  pq.tm_o1 = pq.tm_o0;
+  pkv.tm_x = pq.tm_s0;
+  pkv.tm_y = pq.tm_s1;
+  pkv.tm_s0 = pq.tm_x;
+  pkv.tm_s1 = pq.tm_y;
+  if (rc == MFA_OK) {
+    const host::Strides st = host::strides_of(w.layout, w.heads, w.n, 64);
+    const int64_t need = (static_cast<int64_t>(rows) / 4 + 7) / 8;
+    const int64_t most = static_cast<int64_t>(dev.sms) * 16;
+    mfa_bwd_prep_kernel<kBF16><<<static_cast<unsigned>(need < most ? need : most), 256, 0, stream>>>(
+        out, dout, lse, lse2, di, static_cast<int>(bh), static_cast<int>(w.n),
+        static_cast<int>(w.heads), st.b, st.h, st.n, static_cast<int>(blocks), counters);
+    const int64_t units = kv_units > q_units ? kv_units : q_units;
+    const unsigned ctas = static_cast<unsigned>(units < dev.sms ? units : dev.sms);
+    e = cudaGetLastError();
+    if (e == cudaSuccess)
+      mfa_bwd_window_kernel<kBF16><<<ctas, BwdConfig<true, true, kBF16, true>::kThreads,
+                                     window_bwd_smem<kBF16>(), stream>>>(pq, pkv);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e == cudaSuccess && slots > 0) {
+      const host::Strides kv = host::strides_of(w.layout, w.kv_heads, w.n, 64);
+      const int64_t pairs = bhk * (pc.pieces_rest > 1 ? blocks : sb);
+      mfa_bwd_reduce_kernel<kBF16><<<static_cast<unsigned>(pairs), 256, 0, stream>>>(
+          pkv, static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), kv.b, kv.h, kv.n);
+      e = cudaGetLastError();
+    }
+  }
+  const cudaError_t ef = cudaFreeAsync(ws, stream);
+  if (rc != MFA_OK) return rc;
+  if (e == cudaSuccess) e = ef;
+  return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "window backward launch");
+}
+
+template <bool kBF16>
+int forward_d(const void* q, const void* k, const void* v, void* out, float* lse,
+              const Problem& w, const host::Device& dev, cudaStream_t s) {
+  if (w.d == 32) return launch_forward<Window<kBF16, 32>>(q, k, v, out, lse, w, dev, s);
+  if (w.d == 64) return launch_forward<Window<kBF16, 64>>(q, k, v, out, lse, w, dev, s);
+  return launch_forward<Window<kBF16, 128>>(q, k, v, out, lse, w, dev, s);
+}
+
+}  // namespace
+}  // namespace mfa
+
+using namespace mfa;
+
+extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
+                              int32_t d, int64_t window, int64_t sinks, float scale,
+                              int32_t dtype, int32_t layout, void* stream) {
+  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale};
+  int rc = check(w);
+  if (rc != MFA_OK || batch * heads == 0 || n == 0) return rc;
+  const void* ptrs[] = {q, k, v, out};
+  const char* names[] = {"q", "k", "v", "out"};
+  if ((rc = check_tensors(ptrs, names, 4, -1)) != MFA_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(lse) & 3u)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
+  host::Device dev;
+  if ((rc = host::open_device(&dev)) != MFA_OK || (rc = prepare(dev.index)) != MFA_OK) return rc;
+  if ((rc = check_tensors(ptrs, names, 4, dev.index)) != MFA_OK) return rc;
+  if (lse && (rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == MFA_DTYPE_BF16 ? forward_d<true>(q, k, v, out, lse, w, dev, s)
+                                 : forward_d<false>(q, k, v, out, lse, w, dev, s);
+}
+
+extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
+                              const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
+                              int32_t d, int64_t window, int64_t sinks, float scale,
+                              int32_t dtype, int32_t layout, void* stream) {
+  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale};
+  int rc = check(w);
+  if (rc != MFA_OK) return rc;
+  if (d != 64)
+    return host::fail(MFA_ERR_HEAD_DIM, "The backward pass supports only D=64");
+  if (batch * heads == 0 || n == 0) return MFA_OK;
+  const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv};
+  const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv"};
+  if ((rc = check_tensors(ptrs, names, 8, -1)) != MFA_OK) return rc;
+  if (!lse) return host::fail(MFA_ERR_INVALID_ARGUMENT, "null lse pointer");
+  if (reinterpret_cast<uintptr_t>(lse) & 3u)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
+  host::Device dev;
+  if ((rc = host::open_device(&dev)) != MFA_OK || (rc = prepare(dev.index)) != MFA_OK) return rc;
+  if ((rc = check_tensors(ptrs, names, 8, dev.index)) != MFA_OK) return rc;
+  if ((rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == MFA_DTYPE_BF16
+             ? launch_backward<true>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s)
+             : launch_backward<false>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s);
+}

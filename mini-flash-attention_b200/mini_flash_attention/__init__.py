@@ -12,9 +12,14 @@ the calls raise.
 ``forward_pinned`` runs the same forward on host tensors, overlapping the host<->device
 copies of batch*head slices with the kernels. ``forward_rows`` computes a range of query rows
 of every head (the per-GPU call when fewer batch*head rows than GPUs are sharded by query rows).
+``forward_window`` is attention with a sliding window and sink tokens, k / v heads shared by groups
+of query heads; ``forward_window_lse`` and ``backward_window`` are its training halves and
+``window_attention`` the differentiable form.
 """
-from ._cuda import (attention, backward, forward, forward_bnhd, forward_lse, forward_pinned,
-                    forward_rows, forward_wmma)
+from ._cuda import (attention, backward, backward_window, forward, forward_bnhd, forward_lse,
+                    forward_pinned, forward_rows, forward_window, forward_window_lse,
+                    forward_wmma, window_attention)
 
 __all__ = ["forward", "forward_wmma", "forward_bnhd", "forward_pinned", "forward_rows",
-           "forward_lse", "backward", "attention"]
+           "forward_lse", "backward", "attention", "forward_window", "forward_window_lse",
+           "backward_window", "window_attention"]

@@ -33,8 +33,9 @@ EXT_NAME = "mfa_b200_C"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + ["-O3", "-lineinfo", "-std=c++17", "-Xptxas", "-v"]
 
-LIB_SOURCES = [CSRC / "mfa_capi.cu"]
-LIB_DEPS = LIB_SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "mfa_b200.h"]
+LIB_SOURCES = [CSRC / "mfa_capi.cu", CSRC / "mfa_window.cu"]
+LIB_DEPS = (LIB_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
+            + [INCLUDE / "mfa_b200.h"])
 BINDING_SOURCES = [CSRC / "mfa_binding.cpp"]
 
 
@@ -62,17 +63,26 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         return out
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     tmp = BUILD_DIR / (LIB_NAME + ".tmp")
-    cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", f"-I{INCLUDE}",
-           "-Xlinker", f"-soname={LIB_NAME}",
-           *[str(s) for s in LIB_SOURCES], "-o", str(tmp)]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
-        sys.stdout.write(res.stdout)
-        sys.stderr.write(res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}): {' '.join(cmd)}")
-    (BUILD_DIR / "ptxas_lib.txt").write_text(res.stderr)
+    # one compiler process per translation unit, then the link
+    objects = [BUILD_DIR / (s.stem + ".o") for s in LIB_SOURCES]
+    compiles = [[_nvcc(), *NVCC_FLAGS, "-Xcompiler", "-fPIC", "-Xcompiler",
+                 "-fvisibility=hidden", f"-I{INCLUDE}", "-c", str(s), "-o", str(o)]
+                for s, o in zip(LIB_SOURCES, objects)]
+    link = [_nvcc(), *ARCH_FLAGS, "-shared", "-Xlinker", f"-soname={LIB_NAME}",
+            *[str(o) for o in objects], "-o", str(tmp)]
+    log = ""
+    for step in (compiles, [link]):
+        procs = [(cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE,
+                                        text=True)) for cmd in step]
+        done = [(cmd, proc, *proc.communicate()) for cmd, proc in procs]
+        for cmd, proc, stdout, stderr in done:
+            if verbose or proc.returncode != 0:
+                sys.stdout.write(stdout)
+                sys.stderr.write(stderr)
+            if proc.returncode != 0:
+                raise RuntimeError(f"nvcc failed ({proc.returncode}): {' '.join(cmd)}")
+            log += stderr
+    (BUILD_DIR / "ptxas_lib.txt").write_text(log)
     os.replace(tmp, out)
     return out
 

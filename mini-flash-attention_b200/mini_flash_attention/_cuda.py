@@ -77,6 +77,57 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _Attention.apply(q, k, v, causal)
 
 
+def forward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
+                   sinks: int = 0) -> torch.Tensor:
+    """Attention in which a token sees the ``window`` newest tokens up to itself and the ``sinks``
+    first ones of its sequence: query i sees key j if j <= i and (j > i - window or j < sinks).
+    q is [B, H, N, D]; k and v are [B, Hkv, N, D], Hkv a divisor of H (query head h reads k / v
+    head h // (H // Hkv)). fp16 or bf16, D = 32, 64 or 128, any N, scale 1/sqrt(D). Blocks of
+    keys that no query of a block sees are skipped. A batch padded behind its sequences needs no
+    mask: no token sees a later one (the padding has to be finite)."""
+    return _load_extension().forward_window(q, k, v, int(window), int(sinks), False)[0]
+
+
+def forward_window_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
+                       sinks: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """forward_window plus the row log-sum-exp over the visible keys as fp32 [B, H, N]."""
+    out, lse = _load_extension().forward_window(q, k, v, int(window), int(sinks), True)
+    return out, lse
+
+
+def backward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                    lse: torch.Tensor, dout: torch.Tensor, window: int,
+                    sinks: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients (dq, dk, dv) of forward_window for the output gradient dout, given its out and
+    lse (forward_window_lse); dk and dv of a shared head are summed over its query heads. D = 64,
+    fp16 or bf16."""
+    dq, dk, dv = _load_extension().backward_window(q, k, v, out, lse, dout.contiguous(),
+                                                   int(window), int(sinks))
+    return dq, dk, dv
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks):
+        out, lse = forward_window_lse(q, k, v, window, sinks)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.window, ctx.sinks = window, sinks
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        dq, dk, dv = backward_window(q, k, v, out, lse, dout, ctx.window, ctx.sinks)
+        return dq, dk, dv, None, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
+                     sinks: int = 0) -> torch.Tensor:
+    """Differentiable forward_window (D = 64 for gradients)."""
+    return _WindowAttention.apply(q, k, v, window, sinks)
+
+
 def forward_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_begin: int, q_end: int,
                  out: torch.Tensor | None = None, causal: bool = False) -> torch.Tensor:
     """Forward of the query rows [q_begin, q_end) of every head, each against all N keys (with

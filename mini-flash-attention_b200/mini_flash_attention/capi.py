@@ -19,6 +19,8 @@ EXPORTED_SYMBOLS = (
     "mfa_fwd_rows",
     "mfa_fwd_lse",
     "mfa_bwd",
+    "mfa_fwd_window",
+    "mfa_bwd_window",
     "mfa_fwd_workspace_bytes",
     "mfa_last_error_string",
     "mfa_device_status",
@@ -81,6 +83,13 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
                                                     ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                                     ctypes.c_void_p]
     lib.mfa_bwd.restype = ctypes.c_int
+    window_args = [ctypes.c_int64] * 4 + [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
+                                          ctypes.c_float, ctypes.c_int32, ctypes.c_int32,
+                                          ctypes.c_void_p]
+    lib.mfa_fwd_window.argtypes = [ctypes.c_void_p] * 5 + window_args
+    lib.mfa_fwd_window.restype = ctypes.c_int
+    lib.mfa_bwd_window.argtypes = [ctypes.c_void_p] * 9 + window_args
+    lib.mfa_bwd_window.restype = ctypes.c_int
     lib.mfa_last_error_string.argtypes = []
     lib.mfa_last_error_string.restype = ctypes.c_char_p
     lib.mfa_device_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_int]
@@ -149,6 +158,24 @@ def bwd(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_ptr: in
     """Launch mfa_bwd; raises MfaError."""
     _check(load().mfa_bwd(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, dq_ptr, dk_ptr, dv_ptr,
                           batch, heads, n, d, scale, int(causal), dtype, layout, stream))
+
+
+def fwd_window(q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, lse_ptr: int, batch: int,
+               heads: int, kv_heads: int, n: int, d: int, window: int, sinks: int, scale: float,
+               dtype: int = DTYPE_FP16, layout: int = LAYOUT_BHND, stream: int = 0) -> None:
+    """Launch mfa_fwd_window (lse_ptr 0: no log-sum-exp); raises MfaError."""
+    _check(load().mfa_fwd_window(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, batch, heads, kv_heads, n,
+                                 d, window, sinks, scale, dtype, layout, stream))
+
+
+def bwd_window(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_ptr: int,
+               dq_ptr: int, dk_ptr: int, dv_ptr: int, batch: int, heads: int, kv_heads: int,
+               n: int, d: int, window: int, sinks: int, scale: float, dtype: int = DTYPE_FP16,
+               layout: int = LAYOUT_BHND, stream: int = 0) -> None:
+    """Launch mfa_bwd_window; raises MfaError."""
+    _check(load().mfa_bwd_window(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, dq_ptr, dk_ptr,
+                                 dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale, dtype,
+                                 layout, stream))
 
 
 def fwd_workspace_bytes(batch: int, heads: int, n: int, d: int = 64,
