@@ -149,6 +149,75 @@ MFA_API int mfa_bwd_window(const void* q, const void* k, const void* v, const vo
                            int32_t layout, void* stream);
 
 /*
+ * Paged key / value cache. k_cache and v_cache are contiguous [pages, kv_heads, page_size, d]
+ * arrays of 16-bit elements; request r's token at position i is row i % page_size of page
+ * block_table[r][i / page_size] (int32 [batch, columns]); slot s is row s % page_size of page
+ * s / page_size. No counterpart in the reference, which has no cache.
+ *
+ * mfa_extend_block_tables makes room for added[r] tokens behind the cached[r] ones of every
+ * request (both int32 [batch]; negative counts as 0). Columns from ceil(cached / page_size) on are
+ * filled with the next entries of free_pages, request after request; slots[0..capacity) gets the
+ * slots of the new tokens, request after request, and -1 behind the last; starts[batch + 1] the
+ * requests' first indices in slots; *used the number of pages taken. A token whose page would be
+ * behind the row's last column or the last free page has the slot -1 (*used counts the pages past
+ * free_count, so used > free_count says that pages are missing). Tokens past `capacity` get pages
+ * but no slot. Entries of block_table in other columns are left as they are. page_size >= 1.
+ */
+MFA_API int mfa_extend_block_tables(int32_t* block_table, const int32_t* cached,
+                                    const int32_t* added, const int32_t* free_pages,
+                                    int32_t* slots, int32_t* starts, int32_t* used, int64_t batch,
+                                    int64_t columns, int64_t free_count, int64_t page_size,
+                                    int64_t capacity, void* stream);
+
+/*
+ * Copies token t's rows of k and v ([tokens, kv_heads, d]; token and head strides in elements,
+ * multiples of 8; d a multiple of 8) to slot slots[t]; tokens whose slot is outside the cache are
+ * skipped. A slot may occur once in a call: of two tokens with one slot either may stay, also
+ * in parts.
+ */
+MFA_API int mfa_append_kv(const void* k, const void* v, void* k_cache, void* v_cache,
+                          const int32_t* slots, int64_t tokens, int64_t kv_heads, int64_t d,
+                          int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                          int64_t v_head_stride, int64_t pages, int64_t page_size, void* stream);
+
+/*
+ * Attention of one query token per request over the cache: q and out are [batch, heads, d], d =
+ * 64 or 128, heads a multiple of kv_heads (at most 128 query heads a k / v head), page_size 16, 32,
+ * 64, 128 or 256. Request r has lengths[r] tokens (int32; clamped to [0, columns * page_size]), the
+ * query's own among them; visible are all of them, or with window > 0 those in the newest
+ * `window` positions and the first `sinks`. out is 0 for a request that sees nothing. Only pages
+ * with visible tokens are looked up and read, and what else their rows hold (NaN too) does not
+ * matter. A looked-up page outside the cache reads as zeros and sets the device status word
+ * (mfa_device_status) to 0x200. The workspace (256-byte aligned, mfa_paged_workspace_bytes) must
+ * not be shared by calls that may overlap; nothing in it has to be kept between calls.
+ */
+MFA_API int mfa_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                                const int32_t* block_table, const int32_t* lengths, void* out,
+                                void* workspace, uint64_t workspace_bytes, int64_t batch,
+                                int64_t heads, int64_t kv_heads, int32_t d, int64_t pages,
+                                int64_t page_size, int64_t columns, int64_t window, int64_t sinks,
+                                float scale, int32_t dtype, void* stream);
+
+/*
+ * The same for requests that share their first prefix_length tokens, in the pages prefix_pages
+ * (int32, ceil(prefix_length / page_size) of them) of the same cache; block_table and lengths
+ * tell each request's own tokens behind them. The prefix is read once for the whole batch.
+ */
+MFA_API int mfa_shared_prefix_attention(const void* q, const void* k_cache, const void* v_cache,
+                                        const int32_t* prefix_pages, int64_t prefix_length,
+                                        const int32_t* block_table, const int32_t* lengths,
+                                        void* out, void* workspace, uint64_t workspace_bytes,
+                                        int64_t batch, int64_t heads, int64_t kv_heads, int32_t d,
+                                        int64_t pages, int64_t page_size, int64_t columns,
+                                        float scale, int32_t dtype, void* stream);
+
+/* Workspace, in bytes, of mfa_paged_attention (prefix_length 0) or mfa_shared_prefix_attention on
+ * the current device; launches and allocates nothing. */
+MFA_API int mfa_paged_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int32_t d,
+                                      int64_t page_size, int64_t columns, int64_t prefix_length,
+                                      uint64_t* bytes);
+
+/*
  * Device scratch, in bytes, that one call of mfa_fwd (or mfa_fwd_f16 / mfa_fwd_lse, and with d
  * = 64 and fp16 mfa_fwd_f16_noalloc) takes on the current device for these extents: 0 when
  * whole query blocks fill the SMs evenly, else the split plan's partial-result slots (2 x
@@ -205,7 +274,8 @@ MFA_API const char* mfa_last_error_string(void);
 /*
  * Reads the device-side status word of `device` (synchronises that device first).
  * 0 = every kernel finished normally; 0x100 + site = a bounded mbarrier wait in some CTA
- * expired and that CTA unwound without writing its output tile. If `reset` is non-zero the
+ * expired and that CTA unwound without writing its output tile; 0x200 = a block table named a
+ * page outside its cache. If `reset` is non-zero the
  * word is cleared afterwards. No reference counterpart: the reference kernels have no
  * bounded waits.
  */

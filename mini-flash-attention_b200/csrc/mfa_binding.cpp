@@ -257,6 +257,154 @@ std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Te
   return {dq, dk, dv};
 }
 
+// ---------------------------------------------------------------- paged cache
+void check_index(const torch::Tensor& x, const char* name, const torch::Tensor& like) {
+  TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(x.device() == like.device(), name, " must be on the same device as ", "the others");
+  TORCH_CHECK(x.scalar_type() == torch::kInt32, name, " must be int32");
+  TORCH_CHECK(x.is_contiguous(), name, " must be contiguous");
+}
+
+// k_cache, v_cache [pages, Hkv, page_size, D] of one type and shape.
+void check_cache(const torch::Tensor& k_cache, const torch::Tensor& v_cache) {
+  TORCH_CHECK(k_cache.is_cuda(), "k_cache must be a CUDA tensor");
+  TORCH_CHECK(k_cache.scalar_type() == torch::kFloat16 ||
+                  k_cache.scalar_type() == torch::kBFloat16,
+              "k_cache must be float16 or bfloat16");
+  TORCH_CHECK(k_cache.dim() == 4, "k_cache must have shape [pages, Hkv, page_size, D]");
+  TORCH_CHECK(v_cache.device() == k_cache.device(), "v_cache must be on the same device as k_cache");
+  TORCH_CHECK(v_cache.scalar_type() == k_cache.scalar_type(),
+              "v_cache must have the same dtype as k_cache");
+  TORCH_CHECK(v_cache.sizes() == k_cache.sizes(), "v_cache must have the same shape as k_cache");
+  TORCH_CHECK(k_cache.is_contiguous() && v_cache.is_contiguous(),
+              "k_cache and v_cache must be contiguous");
+}
+
+// Pages and slots for new tokens: (slots, starts, used); block_table is extended in place.
+std::vector<torch::Tensor> extend_block_tables(torch::Tensor block_table, torch::Tensor cached,
+                                               torch::Tensor added, torch::Tensor free_pages,
+                                               int64_t page_size, int64_t capacity) {
+  check_index(block_table, "block_table", block_table);
+  check_index(cached, "cached", block_table);
+  check_index(added, "added", block_table);
+  check_index(free_pages, "free_pages", block_table);
+  TORCH_CHECK(block_table.dim() == 2, "block_table must have shape [B, columns]");
+  const int64_t batch = block_table.size(0);
+  TORCH_CHECK(cached.dim() == 1 && cached.size(0) == batch && added.dim() == 1 &&
+                  added.size(0) == batch,
+              "cached and added must have one value per request");
+  TORCH_CHECK(free_pages.dim() == 1, "free_pages must have one dimension");
+  TORCH_CHECK(capacity >= 0, "capacity must not be negative");
+  const c10::cuda::CUDAGuard device_guard(block_table.device());
+  auto slots = torch::empty({capacity}, block_table.options());
+  auto starts = torch::empty({batch + 1}, block_table.options());
+  auto used = torch::empty({1}, block_table.options());
+  const int rc = mfa_extend_block_tables(
+      block_table.data_ptr<int>(), cached.data_ptr<int>(), added.data_ptr<int>(),
+      free_pages.data_ptr<int>(), slots.data_ptr<int>(), starts.data_ptr<int>(),
+      used.data_ptr<int>(), batch, block_table.size(1), free_pages.size(0), page_size, capacity,
+      current_stream());
+  if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
+  return {slots, starts, used};
+}
+
+// Rows of k and v [T, Hkv, D] (any token and head strides) to their slots of the caches.
+void append_kv(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache,
+               torch::Tensor slots) {
+  check_cache(k_cache, v_cache);
+  check_index(slots, "slots", k_cache);
+  for (const auto* x : {&k, &v}) {
+    const char* name = x == &k ? "k" : "v";
+    TORCH_CHECK(x->is_cuda() && x->device() == k_cache.device(), name,
+                " must be on the same device as k_cache");
+    TORCH_CHECK(x->scalar_type() == k_cache.scalar_type(), name,
+                " must have the same dtype as k_cache");
+    TORCH_CHECK(x->dim() == 3 && x->size(1) == k_cache.size(1) && x->size(2) == k_cache.size(3),
+                name, " must have shape [T, Hkv, D] with the cache's Hkv and D");
+    TORCH_CHECK(x->size(2) <= 1 || x->stride(2) == 1, name, " must be contiguous in D");
+  }
+  TORCH_CHECK(k.size(0) == v.size(0) && slots.dim() == 1 && slots.size(0) == k.size(0),
+              "k, v and slots must have one entry per token");
+  // a dimension of one element may have any stride
+  auto stride = [](const torch::Tensor& x, int dim) {
+    return x.size(dim) == 1 ? int64_t{0} : x.stride(dim);
+  };
+  const c10::cuda::CUDAGuard device_guard(k_cache.device());
+  const int rc = mfa_append_kv(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                               slots.data_ptr<int>(), k.size(0), k.size(1), k.size(2),
+                               stride(k, 0), stride(k, 1), stride(v, 0), stride(v, 1),
+                               k_cache.size(0), k_cache.size(2), current_stream());
+  if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
+}
+
+// Attention of single tokens q [B, H, D] over the cache, behind the shared prefix if it has one.
+torch::Tensor attend_pages(const torch::Tensor& q, const torch::Tensor& k_cache,
+                           const torch::Tensor& v_cache, const torch::Tensor* prefix_pages,
+                           int64_t prefix_length, const torch::Tensor& block_table,
+                           const torch::Tensor& lengths, int64_t window, int64_t sinks) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  check_cache(k_cache, v_cache);
+  TORCH_CHECK(q.device() == k_cache.device(), "k_cache must be on the same device as q");
+  TORCH_CHECK(q.scalar_type() == k_cache.scalar_type(), "k_cache must have the same dtype as q");
+  TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == k_cache.size(3),
+              "q must have shape [B, H, D] with the cache's D");
+  check_index(block_table, "block_table", q);
+  check_index(lengths, "lengths", q);
+  const int64_t batch = q.size(0);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == batch,
+              "block_table must have shape [B, columns]");
+  TORCH_CHECK(lengths.dim() == 1 && lengths.size(0) == batch,
+              "lengths must have one value per request");
+  const int64_t page_size = k_cache.size(2);
+  if (prefix_pages) {
+    check_index(*prefix_pages, "prefix_pages", q);
+    TORCH_CHECK(prefix_length >= 0, "prefix_length must not be negative");
+    TORCH_CHECK(prefix_pages->dim() == 1 &&
+                    (page_size == 0 || prefix_length <= prefix_pages->size(0) * page_size),
+                "prefix_pages must hold prefix_length tokens");
+  }
+  const c10::cuda::CUDAGuard device_guard(q.device());
+  auto out = torch::empty_like(q);
+  uint64_t bytes = 0;
+  int rc = mfa_paged_workspace_bytes(batch, q.size(1), k_cache.size(1),
+                                     static_cast<int32_t>(q.size(2)), page_size,
+                                     block_table.size(1), prefix_length, &bytes);
+  if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
+  auto workspace = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
+  const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(2)));
+  const int32_t d = static_cast<int32_t>(q.size(2));
+  rc = prefix_pages
+           ? mfa_shared_prefix_attention(
+                 q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                 prefix_pages->data_ptr<int>(), prefix_length, block_table.data_ptr<int>(),
+                 lengths.data_ptr<int>(), out.data_ptr(), workspace.data_ptr(), bytes, batch,
+                 q.size(1), k_cache.size(1), d, k_cache.size(0), page_size, block_table.size(1),
+                 scale, dtype_of(q), current_stream())
+           : mfa_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                 block_table.data_ptr<int>(), lengths.data_ptr<int>(),
+                                 out.data_ptr(), workspace.data_ptr(), bytes, batch, q.size(1),
+                                 k_cache.size(1), d, k_cache.size(0), page_size,
+                                 block_table.size(1), window, sinks, scale, dtype_of(q),
+                                 current_stream());
+  if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
+  return out;
+}
+
+torch::Tensor paged_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+                              torch::Tensor block_table, torch::Tensor lengths, int64_t window,
+                              int64_t sinks) {
+  return attend_pages(q, k_cache, v_cache, nullptr, 0, block_table, lengths, window, sinks);
+}
+
+torch::Tensor shared_prefix_attention(torch::Tensor q, torch::Tensor k_cache,
+                                      torch::Tensor v_cache, torch::Tensor prefix_pages,
+                                      int64_t prefix_length, torch::Tensor block_table,
+                                      torch::Tensor lengths) {
+  return attend_pages(q, k_cache, v_cache, &prefix_pages, prefix_length, block_table, lengths, 0,
+                      0);
+}
+
 // Same as forward, writing into a caller-provided contiguous tensor of q's shape and dtype
 // (used by the pipelined host-buffer path to fill slices of one device buffer).
 void flash_attn_forward_into(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out,
@@ -447,5 +595,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Forward with a sliding window and sink tokens: [out] or, with_lse, [out, lse]");
   m.def("backward_window", &flash_attn_backward_window,
         "Backward of forward_window: (dq, dk, dv) (D = 64)");
+  m.def("extend_block_tables", &extend_block_tables,
+        "Pages and slots for new tokens of a paged cache: (slots, starts, used)");
+  m.def("append_kv", &append_kv, "Rows of k and v to their slots of a paged cache");
+  m.def("paged_attention", &paged_attention,
+        "Attention of single tokens over a paged cache, optionally a window with sinks");
+  m.def("shared_prefix_attention", &shared_prefix_attention,
+        "Attention of single tokens over a shared prefix and each request's own tokens");
   m.def("version", []() { return std::string(mfa_version()); });
 }

@@ -42,7 +42,16 @@ struct FwdParams {
   int sinks;
   int sink_blocks;
   int kv_group;
+  // Prefix variant: tm_q is {D, group, batch, kv_heads} with boxes of tile_batch requests (a
+  // query tile has tile_rows = tile_batch * group rows), tm_k and tm_v are {D, page_size,
+  // kv_heads, pages}; key i is in page prefix_pages[i >> page_shift].
+  int tile_batch, tile_rows;
+  const int* prefix_pages;
+  int page_shift, pages;
 };
+
+// Status word: a table named a page outside the cache (its rows read as zero).
+constexpr int kStatusBadPage = 0x200;
 
 // Status codes written to FwdParams::status by the watchdog: kStatusTimeoutBase + site. The
 // backward kernel reports its corresponding waits under the same codes: resident tiles as

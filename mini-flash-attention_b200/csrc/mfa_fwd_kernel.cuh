@@ -60,8 +60,13 @@ template <int kRowsPerUnit>
 struct WindowCursor;
 
 template <int NQ_, int STAGES_, bool CAUSAL_, bool BF16_, int D_, bool LSE_ = false,
-          bool WINDOW_ = false>
+          bool WINDOW_ = false, bool PREFIX_ = false>
 struct FwdConfig {
+  // Many requests' single queries against the one prefix that they share, in the pages of a
+  // cache: a head of the schedule is a k / v head, its query rows the group rows of every
+  // request, its keys the prefix. Every result goes to the workspace as a piece.
+  static constexpr bool kPrefix = PREFIX_;
+  static_assert(!PREFIX_ || (!CAUSAL_ && !LSE_ && !WINDOW_), "the prefix variant has no mask");
   // Sliding window with sink tokens, and k / v heads shared by groups of query heads (a
   // causal variant: query i sees key j if j <= i and (j > i - window or j < sinks)).
   static constexpr bool kWindow = WINDOW_;
@@ -383,6 +388,102 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
   }
 }
 
+// Load role of the prefix variant. A query tile is tile_batch requests' group rows (its rows
+// behind them are never written, and their results never read); a key block is one box for each
+// of its pages, of which those behind the prefix's end are left out. The page numbers of the
+// next block are read while this one's copies are issued.
+template <class Cfg>
+__device__ __forceinline__ void prefix_load_role(const FwdParams& p, uint8_t* smem, uint32_t bars,
+                                                 const Watchdog& wd) {
+  constexpr int ST = Cfg::STAGES;
+  constexpr int kMostPages = Cfg::kKeys / 16;
+  auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
+  const uint32_t sbase = smem_addr(smem);
+  tma_prefetch_desc(&p.tm_q);
+  tma_prefetch_desc(&p.tm_k);
+  tma_prefetch_desc(&p.tm_v);
+  const int box_shift = p.page_shift < 7 ? p.page_shift : 7;  // rows of a box
+  const int boxes = Cfg::kKeys >> box_shift;
+  const uint32_t box_bytes = static_cast<uint32_t>(Cfg::kRowBytes) << box_shift;
+  const uint32_t q_box_bytes = static_cast<uint32_t>(p.tile_rows * Cfg::kRowBytes);
+
+  typename Cfg::Cursor cur;
+  cur.init(p);
+  int pages[kMostPages];
+  auto read_pages = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < kMostPages; ++i) {
+      const int key = j * Cfg::kKeys + (i << box_shift);
+      pages[i] = i < boxes && key < p.n ? p.prefix_pages[key >> p.page_shift] : -1;
+    }
+  };
+  auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int key0, int head) {
+    const int left = (p.n - key0 + (1 << box_shift) - 1) >> box_shift;
+    const int here = left < boxes ? left : boxes;
+    mbar_arrive_expect_tx(full, Cfg::kBoxes * box_bytes * here);
+    const int row0 = key0 & ((1 << p.page_shift) - 1);
+#pragma unroll
+    for (int i = 0; i < kMostPages; ++i) {
+      if (i >= here) break;
+      // a page outside the cache: a place outside the map, which reads as zero
+      const bool bad = pages[i] < 0 || pages[i] >= p.pages;
+      if (bad) atomicCAS(p.status, 0, kStatusBadPage);
+#pragma unroll
+      for (int x = 0; x < Cfg::kBoxes; ++x)
+        tma_load_4d(dst + x * Cfg::kBoxBytes + i * box_bytes, map, full, x * Cfg::kBoxCols, row0,
+                    head, bad ? p.pages : pages[i]);
+    }
+  };
+  int g = 0, q_loaded = 0, k_issued = 0, v_issued = 0;
+  if (cur.valid()) read_pages(cur.j);
+  while (cur.valid()) {
+    const int head = p.sc.head_of(cur.u);
+    if (cur.first_step()) {
+      const int s = cur.seg_idx, b = s & 1;
+      if (!wait_single(bar(Cfg::kBarQEmpty + b), (static_cast<uint32_t>(s >> 1) & 1u) ^ 1u, wd,
+                       kSiteLoadQEmpty))
+        break;
+      mbar_arrive_expect_tx(bar(Cfg::kBarQFull + b), Cfg::NQ * Cfg::kBoxes * q_box_bytes);
+#pragma unroll
+      for (int i = 0; i < Cfg::NQ; ++i) {
+#pragma unroll
+        for (int x = 0; x < Cfg::kBoxes; ++x)
+          tma_load_4d(sbase + Cfg::kQOff + (b * Cfg::NQ + i) * Cfg::kTileBytes + x * Cfg::kBoxBytes,
+                      &p.tm_q, bar(Cfg::kBarQFull + b), x * Cfg::kBoxCols, 0,
+                      (p.sc.qb_of(cur.u) * Cfg::NQ + i) * p.tile_batch, head);
+      }
+      q_loaded = s + 1;
+    }
+    const int st = g % ST;
+    const uint32_t ph = static_cast<uint32_t>(g / ST) & 1u;
+    const int key0 = cur.j * Cfg::kKeys;
+    if (!wait_single(bar(Cfg::kBarKEmpty + st), ph ^ 1u, wd, kSiteLoadKEmpty)) break;
+    load(&p.tm_k, sbase + Cfg::kKOff + st * Cfg::kTileBytes, bar(Cfg::kBarKFull + st), key0, head);
+    k_issued = g + 1;
+    if (!wait_single(bar(Cfg::kBarVEmpty + st), ph ^ 1u, wd, kSiteLoadVEmpty)) break;
+    load(&p.tm_v, sbase + Cfg::kVOff + st * Cfg::kTileBytes, bar(Cfg::kBarVFull + st), key0, head);
+    v_issued = g + 1;
+    ++g;
+    cur.step(p);
+    if (cur.valid()) read_pages(cur.j);
+  }
+  if (*wd.abort) {
+    // Unwinding: wait for every copy this thread put in flight before shared memory goes away.
+    for (int b = 0; b < 2; ++b) {
+      int last = -1;
+      for (int s = b; s < q_loaded; s += 2) last = s;
+      if (last >= 0) drain_wait(bar(Cfg::kBarQFull + b), static_cast<uint32_t>(last >> 1) & 1u);
+    }
+    for (int st = 0; st < ST; ++st) {
+      int last_k = -1, last_v = -1;
+      for (int x = st; x < k_issued; x += ST) last_k = x;
+      for (int x = st; x < v_issued; x += ST) last_v = x;
+      if (last_k >= 0) drain_wait(bar(Cfg::kBarKFull + st), static_cast<uint32_t>(last_k / ST) & 1u);
+      if (last_v >= 0) drain_wait(bar(Cfg::kBarVFull + st), static_cast<uint32_t>(last_v / ST) & 1u);
+    }
+  }
+}
+
 // Executed by the whole MMA warp: waits and descriptor arithmetic stay warp-uniform (uniform
 // datapath, no per-MMA register moves); one elected lane issues tcgen05.mma / commit. Issue
 // cost per MMA matters here: a 128x64x16 P.V step is only 32 tensor-core cycles. S for step
@@ -483,6 +584,23 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       if (!wait_warp(bar(Cfg::kBarVFull + st), static_cast<uint32_t>(gp / ST) & 1u, wd, kSiteMmaV))
         goto unwind;
       const uint32_t vd = v_lo + st * kTileStep;
+      if constexpr (Cfg::kPrefix) {
+        // The prefix's last block: v rows behind its end, which the last page may hold and a
+        // page that was left out leaves as they were, become 0 (their P is 0, but 0 * NaN is
+        // not). Every issuer does so before its own products.
+        const int valid = p.n - cp.j * Cfg::kKeys;
+        if (valid < Cfg::kKeys) {
+          constexpr int kChunks = Cfg::kRowBytes / 16;
+          uint8_t* v_tile = smem + Cfg::kVOff + st * Cfg::kTileBytes;
+          for (int x = 0; x < Cfg::kBoxes; ++x)
+            for (int c = valid * kChunks + static_cast<int>(threadIdx.x & 31);
+                 c < Cfg::kKeys * kChunks; c += 32)
+              *reinterpret_cast<uint4*>(v_tile + x * Cfg::kBoxBytes + 16 * c) =
+                  make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
       bool fresh = cp.first_step();  // first block of a unit: overwrite O
       bool live = true;
       if constexpr (Cfg::kWindow) {
@@ -760,7 +878,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     tmem_ld_16x256b_sync(tO, o);
     tc_fence_before();
     const int b = cur.seg_idx & 1;
-    if (cur.whole(p.sc)) {
+    if (!Cfg::kPrefix && cur.whole(p.sc)) {
       if (Cfg::kLSE && q == 0 && (!Cfg::kWindow || p.lse != nullptr)) {
         // log-sum-exp = ln 2 * (m + log2 l), m in scaled log2 units
 #pragma unroll
@@ -818,9 +936,11 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     } else {
       // A piece of a query block: unnormalised O, the row max and the row sum go to this
       // CTA's workspace slot (first or last segment of its range) for the merge kernel.
-      float* ws = p.workspace +
-                  static_cast<size_t>(2 * blockIdx.x + (cur.first_of_range() ? 0 : 1)) *
-                      Cfg::kSlotFloats;
+      // Prefix variant: slot CTA + unit, which grows by one at least from one segment of the
+      // launch to the next, in the order of the steps.
+      const size_t slot = Cfg::kPrefix ? static_cast<size_t>(blockIdx.x) + cur.u
+                                       : 2 * blockIdx.x + (cur.first_of_range() ? 0 : 1);
+      float* ws = p.workspace + slot * Cfg::kSlotFloats;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int row = tile * Cfg::kRows + slice + gq + 8 * r;
@@ -853,7 +973,7 @@ __device__ __forceinline__ void store_role(const FwdParams& p, uint8_t* smem, ui
   cur.init(p);
   int stores = 0;  // whole units stored so far (phase of the staging barriers)
   while (cur.valid()) {
-    if (cur.whole(p.sc)) {
+    if (!Cfg::kPrefix && cur.whole(p.sc)) {
       const int b = cur.seg_idx & 1;
       const HeadBatch ob = head_batch(p, cur.u);
       bool ok = true;
@@ -886,11 +1006,12 @@ __device__ __forceinline__ void store_role(const FwdParams& p, uint8_t* smem, ui
   tma_store_wait_read();
 }
 
-template <int NQ, int STAGES, bool CAUSAL, bool BF16, int D, bool LSE, bool WINDOW = false>
-__global__ void __launch_bounds__(FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WINDOW>::kThreads,
-                                  1)
+template <int NQ, int STAGES, bool CAUSAL, bool BF16, int D, bool LSE, bool WINDOW = false,
+          bool PREFIX = false>
+__global__ void
+    __launch_bounds__(FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WINDOW, PREFIX>::kThreads, 1)
     mfa_fwd_kernel(const __grid_constant__ FwdParams p) {
-  using Cfg = FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WINDOW>;
+  using Cfg = FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WINDOW, PREFIX>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -940,7 +1061,12 @@ __global__ void __launch_bounds__(FwdConfig<NQ, STAGES, CAUSAL, BF16, D, LSE, WI
     if constexpr (Cfg::kRebalanceRegs) setmaxnreg_dec<Cfg::kControlRegs>();
     const Watchdog wd{abort_flag, p.status, p.timeout_ns};
     grid_dependency_wait();
-    if (lane == 0) load_role<Cfg>(p, smem, bars, wd);
+    if (lane == 0) {
+      if constexpr (Cfg::kPrefix)
+        prefix_load_role<Cfg>(p, smem, bars, wd);
+      else
+        load_role<Cfg>(p, smem, bars, wd);
+    }
   } else {
     if (warp == 0) {
       tmem_alloc(smem_addr(tmem_slot), Cfg::kTmemCols);

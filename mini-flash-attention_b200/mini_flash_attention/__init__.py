@@ -15,11 +15,16 @@ of every head (the per-GPU call when fewer batch*head rows than GPUs are sharded
 ``forward_window`` is attention with a sliding window and sink tokens, k / v heads shared by groups
 of query heads; ``forward_window_lse`` and ``backward_window`` are its training halves and
 ``window_attention`` the differentiable form.
+A paged key / value cache: ``extend_block_tables`` gives new tokens pages and slots on the GPU,
+``append_kv`` copies their k and v there, ``paged_attention`` is the attention of single tokens over
+it, and ``shared_prefix_attention`` the same behind a prefix that the whole batch shares.
 """
-from ._cuda import (attention, backward, backward_window, forward, forward_bnhd, forward_lse,
-                    forward_pinned, forward_rows, forward_window, forward_window_lse,
-                    forward_wmma, window_attention)
+from ._cuda import (append_kv, attention, backward, backward_window, extend_block_tables,
+                    forward, forward_bnhd, forward_lse, forward_pinned, forward_rows,
+                    forward_window, forward_window_lse, forward_wmma, paged_attention,
+                    shared_prefix_attention, window_attention)
 
 __all__ = ["forward", "forward_wmma", "forward_bnhd", "forward_pinned", "forward_rows",
            "forward_lse", "backward", "attention", "forward_window", "forward_window_lse",
-           "backward_window", "window_attention"]
+           "backward_window", "window_attention", "extend_block_tables", "append_kv",
+           "paged_attention", "shared_prefix_attention"]

@@ -33,7 +33,7 @@ EXT_NAME = "mfa_b200_C"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + ["-O3", "-lineinfo", "-std=c++17", "-Xptxas", "-v"]
 
-LIB_SOURCES = [CSRC / "mfa_capi.cu", CSRC / "mfa_window.cu"]
+LIB_SOURCES = [CSRC / "mfa_capi.cu", CSRC / "mfa_window.cu", CSRC / "mfa_paged.cu"]
 LIB_DEPS = (LIB_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
             + [INCLUDE / "mfa_b200.h"])
 BINDING_SOURCES = [CSRC / "mfa_binding.cpp"]

@@ -128,6 +128,63 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     return _WindowAttention.apply(q, k, v, window, sinks)
 
 
+def extend_block_tables(block_table: torch.Tensor, cached: torch.Tensor, added: torch.Tensor,
+                        free_pages: torch.Tensor, page_size: int,
+                        capacity: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages and slots for new tokens of a paged cache, without a word from the host.
+
+    Request r has cached[r] tokens, token i in row i % page_size of page block_table[r, i //
+    page_size], and gets added[r] more (int32 CUDA tensors, block_table [B, columns]). The pages
+    that it needs beyond its ceil(cached / page_size) are the next ones of ``free_pages``, request
+    after request; they are written into block_table in place, other entries stay. Returns
+
+    * slots, int32 [capacity]: page * page_size + row of every new token, request after request,
+      -1 behind the last one (``capacity`` is what the caller's k and v are padded to);
+    * starts, int32 [B + 1]: where each request's tokens start in slots;
+    * used, int32 [1]: how many of free_pages are taken. More than there are: pages were missing.
+
+    Tokens without a page (the list or the table's row ends) have the slot -1, too.
+    """
+    slots, starts, used = _load_extension().extend_block_tables(
+        block_table, cached, added, free_pages, int(page_size), int(capacity))
+    return slots, starts, used
+
+
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              slots: torch.Tensor) -> None:
+    """Copies the rows of k and v ([T, Hkv, D]; the token and head strides may be those of a fused
+    projection) to their slots (int32 [T], extend_block_tables) of the caches [pages, Hkv,
+    page_size, D], in place. Tokens whose slot is negative or past the cache are skipped; a slot
+    may occur only once."""
+    _load_extension().append_kv(k, v, k_cache, v_cache, slots)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, lengths: torch.Tensor, window: int = 0,
+                    sinks: int = 0) -> torch.Tensor:
+    """Attention of one token per request over a paged cache (the decoding form of
+    forward_window): q [B, H, D], caches [pages, Hkv, page_size, D], block_table int32 [B,
+    columns], lengths int32 [B], the query's own token among them. With ``window`` the ``window``
+    newest tokens and the ``sinks`` first are visible, otherwise all. fp16 or bf16, D = 64 or 128,
+    page sizes 16 to 256 (powers of two), H a multiple of Hkv (up to 128 heads a k / v head),
+    scale 1/sqrt(D). A request of length 0 gets 0. Lengths and table are read on the GPU: a
+    captured call may be replayed with others of the same shape. Pages without visible tokens are
+    not looked up, and rows that are not visible may hold anything."""
+    return _load_extension().paged_attention(q, k_cache, v_cache, block_table, lengths,
+                                             int(window), int(sinks))
+
+
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            prefix_pages: torch.Tensor, prefix_length: int,
+                            block_table: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
+    """paged_attention for a batch whose requests share their first ``prefix_length`` tokens,
+    stored once in the pages ``prefix_pages`` (int32) of the cache. block_table and lengths
+    describe what each request has of its own behind the prefix (a length of 0: nothing). The
+    prefix is read once and meets the queries of all requests in one matrix product."""
+    return _load_extension().shared_prefix_attention(q, k_cache, v_cache, prefix_pages,
+                                                     int(prefix_length), block_table, lengths)
+
+
 def forward_rows(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_begin: int, q_end: int,
                  out: torch.Tensor | None = None, causal: bool = False) -> torch.Tensor:
     """Forward of the query rows [q_begin, q_end) of every head, each against all N keys (with

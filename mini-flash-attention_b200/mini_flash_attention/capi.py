@@ -21,6 +21,11 @@ EXPORTED_SYMBOLS = (
     "mfa_bwd",
     "mfa_fwd_window",
     "mfa_bwd_window",
+    "mfa_extend_block_tables",
+    "mfa_append_kv",
+    "mfa_paged_attention",
+    "mfa_shared_prefix_attention",
+    "mfa_paged_workspace_bytes",
     "mfa_fwd_workspace_bytes",
     "mfa_last_error_string",
     "mfa_device_status",
@@ -37,6 +42,7 @@ MFA_ERR_CAUSAL = 4
 MFA_ERR_CUDA = 5
 MFA_ERR_DEVICE = 6
 STATUS_TIMEOUT_BASE = 0x100
+STATUS_BAD_PAGE = 0x200
 NOALLOC_SCRATCH_BYTES = 20971520  # MFA_NOALLOC_SCRATCH_BYTES
 DTYPE_FP16, DTYPE_BF16 = 0, 1
 LAYOUT_BHND, LAYOUT_BNHD = 0, 1
@@ -90,6 +96,18 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     lib.mfa_fwd_window.restype = ctypes.c_int
     lib.mfa_bwd_window.argtypes = [ctypes.c_void_p] * 9 + window_args
     lib.mfa_bwd_window.restype = ctypes.c_int
+    ptr, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+    lib.mfa_extend_block_tables.argtypes = [ptr] * 7 + [i64] * 5 + [ptr]
+    lib.mfa_append_kv.argtypes = [ptr] * 5 + [i64] * 9 + [ptr]
+    lib.mfa_paged_attention.argtypes = [ptr] * 7 + [ctypes.c_uint64] + [i64] * 3 + [
+        i32, *[i64] * 5, ctypes.c_float, i32, ptr]
+    lib.mfa_shared_prefix_attention.argtypes = [ptr] * 4 + [i64] + [ptr] * 4 + [
+        ctypes.c_uint64, *[i64] * 3, i32, *[i64] * 3, ctypes.c_float, i32, ptr]
+    lib.mfa_paged_workspace_bytes.argtypes = [i64] * 3 + [i32] + [i64] * 3 + [
+        ctypes.POINTER(ctypes.c_uint64)]
+    for name in ("mfa_extend_block_tables", "mfa_append_kv", "mfa_paged_attention",
+                 "mfa_shared_prefix_attention", "mfa_paged_workspace_bytes"):
+        getattr(lib, name).restype = ctypes.c_int
     lib.mfa_last_error_string.argtypes = []
     lib.mfa_last_error_string.restype = ctypes.c_char_p
     lib.mfa_device_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.c_int]
@@ -176,6 +194,57 @@ def bwd_window(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_
     _check(load().mfa_bwd_window(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, dq_ptr, dk_ptr,
                                  dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale, dtype,
                                  layout, stream))
+
+
+def extend_block_tables(table_ptr: int, cached_ptr: int, added_ptr: int, free_ptr: int,
+                        slots_ptr: int, starts_ptr: int, used_ptr: int, batch: int, columns: int,
+                        free_count: int, page_size: int, capacity: int, stream: int = 0) -> None:
+    """Launch mfa_extend_block_tables; raises MfaError."""
+    _check(load().mfa_extend_block_tables(table_ptr, cached_ptr, added_ptr, free_ptr, slots_ptr,
+                                          starts_ptr, used_ptr, batch, columns, free_count,
+                                          page_size, capacity, stream))
+
+
+def append_kv(k_ptr: int, v_ptr: int, k_cache_ptr: int, v_cache_ptr: int, slots_ptr: int,
+              tokens: int, kv_heads: int, d: int, k_strides: tuple[int, int],
+              v_strides: tuple[int, int], pages: int, page_size: int, stream: int = 0) -> None:
+    """Launch mfa_append_kv ((token, head) strides in elements); raises MfaError."""
+    _check(load().mfa_append_kv(k_ptr, v_ptr, k_cache_ptr, v_cache_ptr, slots_ptr, tokens,
+                                kv_heads, d, *k_strides, *v_strides, pages, page_size, stream))
+
+
+def paged_attention(q_ptr: int, k_cache_ptr: int, v_cache_ptr: int, table_ptr: int,
+                    lengths_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int,
+                    batch: int, heads: int, kv_heads: int, d: int, pages: int, page_size: int,
+                    columns: int, scale: float, window: int = 0, sinks: int = 0,
+                    dtype: int = DTYPE_FP16, stream: int = 0) -> None:
+    """Launch mfa_paged_attention; raises MfaError."""
+    _check(load().mfa_paged_attention(q_ptr, k_cache_ptr, v_cache_ptr, table_ptr, lengths_ptr,
+                                      out_ptr, workspace_ptr, workspace_bytes, batch, heads,
+                                      kv_heads, d, pages, page_size, columns, window, sinks,
+                                      scale, dtype, stream))
+
+
+def shared_prefix_attention(q_ptr: int, k_cache_ptr: int, v_cache_ptr: int, prefix_ptr: int,
+                            prefix_length: int, table_ptr: int, lengths_ptr: int, out_ptr: int,
+                            workspace_ptr: int, workspace_bytes: int, batch: int, heads: int,
+                            kv_heads: int, d: int, pages: int, page_size: int, columns: int,
+                            scale: float, dtype: int = DTYPE_FP16, stream: int = 0) -> None:
+    """Launch mfa_shared_prefix_attention; raises MfaError."""
+    _check(load().mfa_shared_prefix_attention(
+        q_ptr, k_cache_ptr, v_cache_ptr, prefix_ptr, prefix_length, table_ptr, lengths_ptr,
+        out_ptr, workspace_ptr, workspace_bytes, batch, heads, kv_heads, d, pages, page_size,
+        columns, scale, dtype, stream))
+
+
+def paged_workspace_bytes(batch: int, heads: int, kv_heads: int, d: int, page_size: int,
+                          columns: int, prefix_length: int = 0) -> int:
+    """Workspace bytes of paged_attention (or, with a prefix_length, shared_prefix_attention) on
+    the current device. Raises MfaError."""
+    out = ctypes.c_uint64(0)
+    _check(load().mfa_paged_workspace_bytes(batch, heads, kv_heads, d, page_size, columns,
+                                            prefix_length, ctypes.byref(out)))
+    return out.value
 
 
 def fwd_workspace_bytes(batch: int, heads: int, n: int, d: int = 64,
