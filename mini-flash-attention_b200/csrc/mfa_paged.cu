@@ -150,7 +150,8 @@ int check(Problem& w) {
   if (w.prefix > kMost) return invalid("the prefix is too long");
   if (w.heads == 0 || w.batch == 0) return MFA_OK;
   // steps of a launch are counted in 32 bits
-  const double tiles = static_cast<double>((w.columns * w.page_size + 63) / 64 + 1);
+  const double tiles =
+      static_cast<double>((w.columns * w.page_size + 63) / 64 + 1 + kPagedUnitSteps);
   if (tiles * static_cast<double>(w.units()) > 0x7fffff00 ||
       static_cast<double>(w.prefix / 128 + 1) * static_cast<double>(w.kv_heads * w.tiles()) >
           0x7fffff00)
@@ -160,6 +161,12 @@ int check(Problem& w) {
   if (w.window == 0) w.sinks = 0;
   if (w.sinks > most) w.sinks = most;
   return MFA_OK;
+}
+
+// Tiles of the longest request.
+int64_t most_tiles(const Problem& w) {
+  const int64_t tiles = (w.columns * w.page_size + 63) / 64;
+  return tiles > 0 ? tiles : 1;
 }
 
 // Parts of the workspace, in floats from its start (256-byte aligned parts).
@@ -173,7 +180,7 @@ Layout lay_out(const Problem& w, int64_t sms) {
   const auto whole = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   Layout l;
   // Two CTAs an SM, but no more than there can be steps.
-  const int64_t steps = w.units() * ((w.columns * w.page_size + 63) / 64 + (w.columns == 0));
+  const int64_t steps = w.units() * (most_tiles(w) + kPagedUnitSteps);
   l.ctas = steps < 2 * sms ? steps : 2 * sms;
   const bool shared = w.prefix > 0;
   const int64_t slots = shared ? l.ctas + w.units() : 2 * l.ctas;

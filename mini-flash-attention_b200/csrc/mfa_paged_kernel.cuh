@@ -76,24 +76,28 @@ struct PagedConfig {
   static constexpr int kBoxBytes = kKeys * 128;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStages = 98304 / (2 * kTileBytes);
-  static constexpr int kMergeCols = kD + 8;  // floats a row: lanes of 4 rows hit different banks
-  static constexpr int kMergeOff = kStages * 2 * kTileBytes;
-  static constexpr int kStatsOff = kMergeOff + kRows * kMergeCols * 4;  // [2][kWarps][kRows]
+  static constexpr int kQRowBytes = kD * 2 + 16;  // eight rows' 16-byte pieces hit all banks once
+  static constexpr int kQOff = kStages * 2 * kTileBytes;
+  // a round of the merge: eight rows by 64 columns of each warp
+  static constexpr int kMergeCols = 72;  // floats a row: float2s of four rows hit all banks once
+  static constexpr int kMergeOff = kQOff + kRows * kQRowBytes;
+  static constexpr int kStatsOff = kMergeOff + kWarps * 8 * kMergeCols * 4;  // [2][kWarps][kRows]
   static constexpr int kBarOff = kStatsOff + 2 * kWarps * kRows * 4;
-  static constexpr int kBarFull = 0, kBarEmpty = kStages;
-  static constexpr int kScanOff = kBarOff + 2 * kStages * 8;  // warp sums, start
+  static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarQFull = 2 * kStages,
+                       kBarQEmpty = 2 * kStages + 1;
+  static constexpr int kScanOff = kBarOff + (2 * kStages + 2) * 8;  // warp sums, start
   static constexpr int kAbortOff = kScanOff + 4 * (kWarps + 1 + 3);
   static constexpr int kSmemBytes = kAbortOff + 4 + 1024;
+  static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs an SM");
 };
 
 // Tiles of a request of n tokens: those that hold sinks before the window, then the window's.
 struct PagedSpan {
   int n, tiles, sinks, skip;
-  __device__ void set(const PagedParams& p, int request) {
+  __device__ void set(const PagedParams& p, int length) {
     const int most = p.columns << p.page_shift;  // < 2^31 (checked by the launcher)
-    n = p.lengths[request];
-    n = n < 0 ? 0 : n < most ? n : most;
-    const int last = n > 0 ? (n - 1) >> 6 : 0;  // an empty request has one step, which sees nothing
+    n = length < 0 ? 0 : length < most ? length : most;
+    const int last = n > 0 ? (n - 1) >> 6 : 0;  // an empty request has one tile, which sees nothing
     const int w0 = p.window > 0 && n > p.window ? (n - p.window) >> 6 : 0;
     const int sb = (p.sinks >> 6) + ((p.sinks & 63) != 0);
     sinks = sb < w0 ? sb : w0;
@@ -111,49 +115,80 @@ __device__ __forceinline__ int cta_of_step(long long s, long long total, int cta
   return static_cast<int>(((s + 1) * ctas - 1) / total);
 }
 
-// Where a CTA's share of the steps starts, found by all its threads.
+// A unit's first and last steps (query, merge, output) cost about as much as a tile of keys (with 4
+// rows and D = 64: 900 against 850 cycles), so shares count one step more than its tiles.
+constexpr int kPagedUnitSteps = 1;
+
+// A CTA's share of the steps, found by all its threads.
 struct PagedShare {
   int total;    // steps of the whole call
   int ctas;     // CTAs that get a share
   int begin, end;
   int request;  // of step `begin`
+  int length;   // its tokens
   int before;   // steps of the requests before it
 };
 
-// The walk over a CTA's share, by segments (the part of one unit that it holds).
+// The walk over a CTA's share, by segments (the tiles of one unit that it holds).
 struct PagedCursor {
   PagedSpan span;
   int request, unit_row;  // unit_row: k / v head * row_tiles + row tile
   int t;                  // next tile of the unit
   int left;               // steps left in the share
   int first;              // step of the unit's first tile
+  int ahead;              // length of the next request, read early
+
+  __device__ void read_ahead(const PagedParams& p) {
+    ahead = p.lengths[request + 1 < p.batch ? request + 1 : request];
+  }
   __device__ void init(const PagedParams& p, const PagedShare& sh) {
     left = sh.end - sh.begin;
-    if (left <= 0) return;
     request = sh.request;
-    span.set(p, request);
+    unit_row = t = first = 0;
+    if (left <= 0) return;
+    span.set(p, sh.length);
+    read_ahead(p);
     const int in = sh.begin - sh.before;
-    unit_row = in / span.tiles;
-    t = in - unit_row * span.tiles;
+    unit_row = in / (span.tiles + kPagedUnitSteps);
+    t = in - unit_row * (span.tiles + kPagedUnitSteps);
     first = sh.begin - t;
+    if (t >= span.tiles) next_unit(p);
   }
   __device__ int segment() const { return span.tiles - t < left ? span.tiles - t : left; }
-  __device__ void advance(const PagedParams& p, int steps) {
-    left -= steps;
-    t += steps;
-    if (t < span.tiles || left == 0) return;
-    first += span.tiles;
+  // Past the unit's last tile (t >= tiles).
+  __device__ void next_unit(const PagedParams& p) {
+    const int rest = span.tiles + kPagedUnitSteps - t;
+    left = left > rest ? left - rest : 0;
+    if (left == 0) return;
+    first += span.tiles + kPagedUnitSteps;
     t = 0;
     if (++unit_row == p.kv_heads * p.row_tiles) {
       unit_row = 0;
-      span.set(p, ++request);
+      ++request;
+      span.set(p, ahead);
+      read_ahead(p);
     }
+  }
+  __device__ void advance(const PagedParams& p, int tiles) {
+    left -= tiles;
+    t += tiles;
+    if (t == span.tiles && left > 0) next_unit(p);
+  }
+  // Query rows of the current unit.
+  __device__ int head(const PagedParams& p) const { return unit_row / p.row_tiles; }
+  __device__ int row0(const PagedParams& p) const { return unit_row % p.row_tiles * 16; }
+  __device__ int rows(const PagedParams& p) const {
+    const int r = p.group - row0(p);
+    return r < 16 ? r : 16;
+  }
+  __device__ size_t query(const PagedParams& p) const {  // its first row in q and out
+    return (static_cast<size_t>(request) * p.kv_heads + head(p)) * p.group + row0(p);
   }
 };
 
 template <class Cfg>
 __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* scan) {
-  // Each thread sums the tiles of a run of requests; the block's exclusive sums tell the one
+  // Each thread sums the steps of a run of requests; the block's exclusive sums tell the one
   // whose run holds the share's first step.
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + Cfg::kThreads - 1) / Cfg::kThreads;
@@ -162,8 +197,8 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   int mine = 0;
   PagedSpan span;
   for (int r = r0; r < r1; ++r) {
-    span.set(p, r);
-    mine += span.tiles;
+    span.set(p, p.lengths[r]);
+    mine += span.tiles + kPagedUnitSteps;
   }
   int upto = mine;
 #pragma unroll
@@ -173,16 +208,16 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   }
   if (lane == 31) scan[warp] = upto;
   __syncthreads();
-  int tiles = 0, before = upto - mine;
+  int steps = 0, before = upto - mine;
 #pragma unroll
   for (int w = 0; w <= Cfg::kWarps; ++w) {
     const int x = scan[w];
     if (w < warp) before += x;
-    tiles += x;
+    steps += x;
   }
   const int heads = p.kv_heads * p.row_tiles;
   PagedShare sh;
-  sh.total = tiles * heads;
+  sh.total = steps * heads;
   sh.ctas = static_cast<int>(gridDim.x) < sh.total ? static_cast<int>(gridDim.x) : sh.total;
   const int c = static_cast<int>(blockIdx.x);
   sh.begin = sh.end = 0;
@@ -192,21 +227,28 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   }
   if (before * heads <= sh.begin && sh.begin < (before + mine) * heads) {
     int r = r0;
-    for (span.set(p, r); (before + span.tiles) * heads <= sh.begin; span.set(p, r)) {
-      before += span.tiles;
-      ++r;
+    if (per > 1) {  // with one request a thread, the span is that request's
+      for (span.set(p, p.lengths[r]);
+           (before + span.tiles + kPagedUnitSteps) * heads <= sh.begin;
+           span.set(p, p.lengths[r])) {
+        before += span.tiles + kPagedUnitSteps;
+        ++r;
+      }
     }
     scan[Cfg::kWarps + 1] = r;
     scan[Cfg::kWarps + 2] = before * heads;
+    scan[Cfg::kWarps + 3] = span.n;
   }
   __syncthreads();
   sh.request = scan[Cfg::kWarps + 1];
   sh.before = scan[Cfg::kWarps + 2];
+  sh.length = scan[Cfg::kWarps + 3];
   return sh;
 }
 
-// Producer warp: the tiles of the share, a box for every page that holds a visible key. The page
-// numbers of the next tile are read while this one waits for its stage.
+// Producer warp: the query rows of each segment, then its tiles, a box for every page that holds
+// a visible key. Lane i looks up the page of box i of a batch of tiles (32 boxes at most, of one
+// segment); the next batch's are on their way while this one's copies are issued.
 template <class Cfg>
 __device__ __forceinline__ void paged_load_role(const PagedParams& p, const PagedShare& sh,
                                                 uint32_t smem, uint32_t bars,
@@ -214,58 +256,83 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
   const int lane = threadIdx.x & 31;
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
   const int box_shift = p.page_shift < 6 ? p.page_shift : 6;  // rows of a box
-  const int boxes = Cfg::kKeys >> box_shift;                  // pages of a tile (at most four)
+  const int tile_shift = 6 - box_shift;                       // boxes of a tile: 1, 2 or 4
   const uint32_t box_bytes = 128u << box_shift;
-  if (lane == 0) {
-    tma_prefetch_desc(&p.tm_k);
-    tma_prefetch_desc(&p.tm_v);
-  }
   PagedCursor cur;
   cur.init(p, sh);
-  // lane i: the page of box i of a tile, or -1 if nothing in it is visible
-  auto page_of = [&]() -> int {
-    if (lane >= boxes) return -1;
-    const int key0 = cur.span.tile(cur.t) * Cfg::kKeys + (lane << box_shift);
-    const int n = cur.span.n;
-    bool any = key0 < n;
-    if (p.window > 0)
-      any = any && (key0 + (1 << box_shift) > n - p.window || key0 < p.sinks);
-    if (!any) return -1;
-    const int page = p.block_table[static_cast<size_t>(cur.request) * p.columns +
-                                   (key0 >> p.page_shift)];
-    // an out-of-range page is out of the tensor map's range too: the copy fills zeros
-    return page < 0 || page >= p.pages ? p.pages : page;
+  struct Batch {
+    int count;     // tiles
+    int page;      // this lane's page, as the table has it
+    bool visible;  // whether a key of this lane's box is seen (its page was looked up)
   };
-  int page = cur.left > 0 ? page_of() : -1;
-  int g = 0;
-  while (cur.left > 0) {
-    const int now = page;
-    const int head = cur.unit_row / p.row_tiles;
-    const int row0 = cur.span.tile(cur.t) * Cfg::kKeys & ((1 << p.page_shift) - 1);
-    cur.advance(p, 1);
-    if (cur.left > 0) page = page_of();
-    const int st = g % Cfg::kStages;
-    const uint32_t ph = static_cast<uint32_t>(g / Cfg::kStages) & 1u;
-    if (!wait_warp(bar(Cfg::kBarEmpty + st), ph ^ 1u, wd, kSiteLoadKEmpty)) break;
-    const uint32_t have = __ballot_sync(0xffffffffu, now >= 0);
-    const bool bad = now == p.pages;
-    if (bad) atomicCAS(p.status, 0, kStatusBadPage);
-    if (lane == 0)
-      mbar_arrive_expect_tx(bar(Cfg::kBarFull + st),
-                            2 * Cfg::kBoxes * box_bytes * __popc(have));
-    __syncwarp();
-    const uint32_t k_dst = smem + st * 2 * Cfg::kTileBytes, v_dst = k_dst + Cfg::kTileBytes;
-    for (int i = 0; i < boxes; ++i) {
-      const int pg = __shfl_sync(0xffffffffu, now, i);
-      if (pg < 0 || lane != 0) continue;
-#pragma unroll
-      for (int x = 0; x < Cfg::kBoxes; ++x) {
-        const uint32_t off = x * Cfg::kBoxBytes + i * box_bytes;
-        tma_load_4d(k_dst + off, &p.tm_k, bar(Cfg::kBarFull + st), 64 * x, row0, head, pg);
-        tma_load_4d(v_dst + off, &p.tm_v, bar(Cfg::kBarFull + st), 64 * x, row0, head, pg);
-      }
+  auto look_up = [&](const PagedCursor& at) -> Batch {
+    Batch b;
+    const int most = 32 >> tile_shift, seg = at.segment();
+    b.count = seg < most ? seg : most;
+    const int i = lane >> tile_shift;
+    const int key0 = at.span.tile(at.t + i) * Cfg::kKeys +
+                     ((lane & ((1 << tile_shift) - 1)) << box_shift);
+    b.visible = i < b.count && key0 < at.span.n &&
+                (p.window == 0 || key0 + (1 << box_shift) > at.span.n - p.window ||
+                 key0 < p.sinks);
+    b.page = 0;
+    if (b.visible)
+      b.page = p.block_table[static_cast<size_t>(at.request) * p.columns + (key0 >> p.page_shift)];
+    return b;
+  };
+  Batch batch{0, 0, false};
+  if (cur.left > 0) batch = look_up(cur);
+  int g = 0, segs = 0;
+  bool fresh = true, ok = true;  // fresh: the batch starts a segment
+  while (cur.left > 0 && ok) {
+    PagedCursor next = cur;
+    next.advance(p, batch.count);
+    Batch later{0, 0, false};
+    if (next.left > 0) later = look_up(next);
+    const int head = cur.head(p);
+    if (fresh) {
+      if (!wait_warp(bar(Cfg::kBarQEmpty), (static_cast<uint32_t>(segs) & 1u) ^ 1u, wd,
+                     kSiteLoadQEmpty))
+        break;
+      const int rows = cur.rows(p);
+      if (lane == 0) mbar_arrive_expect_tx(bar(Cfg::kBarQFull), rows * Cfg::kD * 2);
+      __syncwarp();
+      if (lane < rows)
+        bulk_load(smem + Cfg::kQOff + lane * Cfg::kQRowBytes,
+                  p.q + (cur.query(p) + lane) * Cfg::kD, Cfg::kD * 2, bar(Cfg::kBarQFull));
+      ++segs;
     }
-    ++g;
+    // a page outside the cache: a place outside the map, which reads as zero
+    const bool bad = batch.visible && (batch.page < 0 || batch.page >= p.pages);
+    if (bad) atomicCAS(p.status, 0, kStatusBadPage);
+    const int page = bad ? p.pages : batch.page;
+    const uint32_t have = __ballot_sync(0xffffffffu, batch.visible);
+    for (int i = 0; i < batch.count; ++i) {
+      const int st = g % Cfg::kStages;
+      const uint32_t ph = static_cast<uint32_t>(g / Cfg::kStages) & 1u;
+      if (!(ok = wait_warp(bar(Cfg::kBarEmpty + st), ph ^ 1u, wd, kSiteLoadKEmpty))) break;
+      const uint32_t here = (have >> (i << tile_shift)) & ((1u << (1 << tile_shift)) - 1u);
+      if (lane == 0)
+        mbar_arrive_expect_tx(bar(Cfg::kBarFull + st),
+                              2 * Cfg::kBoxes * box_bytes * __popc(here));
+      __syncwarp();
+      const int row0 = (cur.span.tile(cur.t + i) * Cfg::kKeys) & ((1 << p.page_shift) - 1);
+      const uint32_t k_dst = smem + st * 2 * Cfg::kTileBytes, v_dst = k_dst + Cfg::kTileBytes;
+      for (int j = 0; j < 1 << tile_shift; ++j) {
+        const int pg = __shfl_sync(0xffffffffu, page, (i << tile_shift) + j);
+        if (!((here >> j) & 1u) || lane != 0) continue;
+#pragma unroll
+        for (int x = 0; x < Cfg::kBoxes; ++x) {
+          const uint32_t off = x * Cfg::kBoxBytes + j * box_bytes;
+          tma_load_4d(k_dst + off, &p.tm_k, bar(Cfg::kBarFull + st), 64 * x, row0, head, pg);
+          tma_load_4d(v_dst + off, &p.tm_v, bar(Cfg::kBarFull + st), 64 * x, row0, head, pg);
+        }
+      }
+      ++g;
+    }
+    fresh = next.t == 0;
+    cur = next;
+    batch = later;
   }
   if (*wd.abort && lane == 0) {
     // unwinding: shared memory must outlive the copies in flight
@@ -275,10 +342,11 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
       if (last >= 0)
         drain_wait(bar(Cfg::kBarFull + st), static_cast<uint32_t>(last / Cfg::kStages) & 1u);
     }
+    if (segs > 0) drain_wait(bar(Cfg::kBarQFull), static_cast<uint32_t>(segs - 1) & 1u);
   }
 }
 
-// The same keys' 8x8 blocks of 16-bit values, as they stand and transposed.
+// The 8x8 blocks of 16-bit values, as they stand and transposed.
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -308,7 +376,8 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
 }
 
 // Consumer warp. Fragments: lane 4 g + q holds rows g and g + 8 of the 16 query rows and, of
-// every 8 keys (scores) or 8 columns (out), the two at 2 q.
+// every 8 keys (scores) or 8 columns (out), the two at 2 q. With at most 8 rows the upper eight
+// (g + 8) take part in the products only, on what the query tile holds there, and are dropped.
 template <class Cfg>
 __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const PagedShare& sh,
                                                    uint8_t* smem_ptr, uint32_t bars,
@@ -324,39 +393,32 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
   float* stat_m = reinterpret_cast<float*>(smem_ptr + Cfg::kStatsOff);
   float* stat_l = stat_m + Cfg::kWarps * Cfg::kRows;
   const int slot_rows = p.group < Cfg::kRows ? p.group : Cfg::kRows;
-  const int heads = p.kv_heads * p.group;
 
   // ldmatrix row addresses inside a tile: this lane's key row and the 16-byte chunk, which the
   // 128-byte swizzle moves to chunk ^ (row % 8)
   const int mat = lane >> 3, mrow = lane & 7;
   const uint32_t k_row = (warp * 16 + (mat >> 1) * 8 + mrow) * 128;
   const uint32_t v_row = (warp * 16 + (mat & 1) * 8 + mrow) * 128;
+  const uint32_t q_row = smem + Cfg::kQOff + ((mat & 1) * 8 + mrow) * Cfg::kQRowBytes;
   auto chunk_off = [&](int chunk) -> uint32_t {
     return (chunk >> 3) * Cfg::kBoxBytes + (((chunk & 7) ^ mrow) << 4);
   };
 
   PagedCursor cur;
   cur.init(p, sh);
-  int g = 0;
+  int g = 0, segs = 0;
   bool ok = true, wrote = false;
   while (cur.left > 0) {
     const int seg = cur.segment();
-    const int kv_head = cur.unit_row / p.row_tiles;
-    const int tile_row0 = (cur.unit_row - kv_head * p.row_tiles) * Cfg::kRows;
-    const int rows = p.group - tile_row0 < Cfg::kRows ? p.group - tile_row0 : Cfg::kRows;
-    const size_t q_row0 =
-        static_cast<size_t>(cur.request) * heads + kv_head * p.group + tile_row0;
+    const int rows = cur.rows(p);
+    const bool upper = rows > 8;
     uint32_t qf[kKSteps][4];
+    if (ok) ok = wait_warp(bar(Cfg::kBarQFull), static_cast<uint32_t>(segs) & 1u, wd, kSiteMmaQ);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint32_t* src =
-          reinterpret_cast<const uint32_t*>(p.q + (q_row0 + gq + 8 * r) * D) + q;
-#pragma unroll
-      for (int kk = 0; kk < kKSteps; ++kk) {
-        qf[kk][r] = gq + 8 * r < rows ? src[8 * kk] : 0u;
-        qf[kk][2 + r] = gq + 8 * r < rows ? src[8 * kk + 4] : 0u;
-      }
-    }
+    for (int kk = 0; kk < kKSteps; ++kk) ldmatrix_x4(q_row + (2 * kk + (mat >> 1)) * 16, qf[kk]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(Cfg::kBarQEmpty));
+    ++segs;
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
@@ -405,9 +467,10 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
       for (int r = 0; r < 2; ++r)
         top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * c;
       if (__any_sync(0xffffffffu, top[0] > m[0] + kRescaleThreshold ||
-                                      top[1] > m[1] + kRescaleThreshold)) {
+                                      (upper && top[1] > m[1] + kRescaleThreshold))) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          if (r == 1 && !upper) break;
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
           const float next = fmaxf(m[r], top[r]);
@@ -421,9 +484,10 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
           }
         }
       }
-      uint32_t pf[4];  // P as the left operand: rows g, g + 8 by keys 2 q, then keys 2 q + 8
+      uint32_t pf[4] = {0u, 0u, 0u, 0u};  // P: rows g, g + 8 by keys 2 q, then by keys 2 q + 8
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
+        if (r == 1 && !upper) break;
         const float sub = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -444,7 +508,16 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
       if (lane == 0) mbar_arrive(bar(Cfg::kBarEmpty + st));
     }
 
-    // ---- the segment's end: the four warps' states to one, in warp 0
+    // ---- the segment's end: the four warps' states to one. In a round every warp leaves eight
+    // rows by 64 columns in shared memory, and the 128 threads rescale, add and write four
+    // columns of a row each.
+    const bool whole = cur.t == 0 && seg == cur.span.tiles;
+    const bool to_slot = p.pieces_only || !whole;
+    const int unit = cur.request * p.kv_heads * p.row_tiles + cur.unit_row;
+    const int slot = p.pieces_only ? static_cast<int>(blockIdx.x) + unit
+                                   : 2 * static_cast<int>(blockIdx.x) + (wrote ? 1 : 0);
+    float* slot_at = p.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
+    uint16_t* out_at = p.out + cur.query(p) * D;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -454,80 +527,53 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
         stat_l[warp * Cfg::kRows + gq + 8 * r] = l[r];
       }
     }
-    named_bar_sync(1, 32 * Cfg::kWarps);
-    float m_all[2], l_all[2];
+    const int mine = threadIdx.x >> 4, col4 = 4 * (threadIdx.x & 15);  // of a round's sums
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      m_all[r] = -INFINITY;
+      if (r == 1 && !upper) break;
 #pragma unroll
-      for (int w = 0; w < Cfg::kWarps; ++w)
-        m_all[r] = fmaxf(m_all[r], stat_m[w * Cfg::kRows + gq + 8 * r]);
-      const float sub = m_all[r] == -INFINITY ? 0.0f : m_all[r];
-      l_all[r] = 0.0f;
+      for (int x = 0; x < Cfg::kBoxes; ++x) {
+        if (r + x > 0) named_bar_sync(1, 32 * Cfg::kWarps);  // the round before has been read
 #pragma unroll
-      for (int w = 0; w < Cfg::kWarps; ++w)
-        l_all[r] += stat_l[w * Cfg::kRows + gq + 8 * r] *
-                    ex2_approx(stat_m[w * Cfg::kRows + gq + 8 * r] - sub);
-      const float f = ex2_approx(m[r] - sub);
+        for (int d = 0; d < 8; ++d)
+          *reinterpret_cast<float2*>(merge + (warp * 8 + gq) * Cfg::kMergeCols + 8 * d + 2 * q) =
+              make_float2(o[8 * x + d][2 * r], o[8 * x + d][2 * r + 1]);
+        named_bar_sync(1, 32 * Cfg::kWarps);
+        const int row = 8 * r + mine;
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d) {
-        o[d][2 * r] *= f;
-        o[d][2 * r + 1] *= f;
-      }
-    }
+        for (int w = 0; w < Cfg::kWarps; ++w) top = fmaxf(top, stat_m[w * Cfg::kRows + row]);
+        const float sub = top == -INFINITY ? 0.0f : top;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = Cfg::kWarps - 1; w > 0; --w) {
-      // warp w adds what the warps after it have left, and leaves the sum for warp w - 1
-      if (warp == w) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float* at = merge + (gq + 8 * r) * Cfg::kMergeCols + 2 * q;
-#pragma unroll
-          for (int d = 0; d < D / 8; ++d) {
-            float2* to = reinterpret_cast<float2*>(at + 8 * d);
-            float2 x = make_float2(o[d][2 * r], o[d][2 * r + 1]);
-            if (w < Cfg::kWarps - 1) {
-              const float2 y = *to;
-              x.x += y.x;
-              x.y += y.y;
+        for (int w = 0; w < Cfg::kWarps; ++w) {
+          const float f = ex2_approx(stat_m[w * Cfg::kRows + row] - sub);
+          const float4 y = *reinterpret_cast<const float4*>(
+              merge + (w * 8 + mine) * Cfg::kMergeCols + col4);
+          sum = fmaf(f, stat_l[w * Cfg::kRows + row], sum);
+          acc.x = fmaf(f, y.x, acc.x);
+          acc.y = fmaf(f, y.y, acc.y);
+          acc.z = fmaf(f, y.z, acc.z);
+          acc.w = fmaf(f, y.w, acc.w);
+        }
+        if (row < rows && ok) {
+          if (to_slot) {
+            *reinterpret_cast<float4*>(slot_at + row * D + 64 * x + col4) = acc;
+            if (x == 0 && col4 == 0) {
+              slot_at[slot_rows * D + row] = top;
+              slot_at[slot_rows * (D + 1) + row] = sum;
             }
-            *to = x;
+          } else {
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            *reinterpret_cast<uint2*>(out_at + row * D + 64 * x + col4) =
+                make_uint2(pack_pair<Cfg::kBF16>(acc.x * inv, acc.y * inv),
+                           pack_pair<Cfg::kBF16>(acc.z * inv, acc.w * inv));
           }
         }
       }
-      named_bar_sync(1, 32 * Cfg::kWarps);
     }
-    const bool whole = cur.t == 0 && seg == cur.span.tiles;
-    const bool to_slot = p.pieces_only || !whole;
-    const int unit = cur.request * p.kv_heads * p.row_tiles + cur.unit_row;
-    const int slot = p.pieces_only ? static_cast<int>(blockIdx.x) + unit
-                                   : 2 * static_cast<int>(blockIdx.x) + (wrote ? 1 : 0);
-    if (warp == 0 && ok) {
-      float* to = p.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = gq + 8 * r;
-        if (row >= rows) continue;
-        const float* from = merge + row * Cfg::kMergeCols + 2 * q;
-        const float inv = l_all[r] > 0.0f ? 1.0f / l_all[r] : 0.0f;
-#pragma unroll
-        for (int d = 0; d < D / 8; ++d) {
-          const float2 y = *reinterpret_cast<const float2*>(from + 8 * d);
-          const float a = o[d][2 * r] + y.x, b = o[d][2 * r + 1] + y.y;
-          if (to_slot)
-            *reinterpret_cast<float2*>(to + row * D + 8 * d + 2 * q) = make_float2(a, b);
-          else
-            *reinterpret_cast<uint32_t*>(p.out + (q_row0 + row) * D + 8 * d + 2 * q) =
-                pack_pair<Cfg::kBF16>(a * inv, b * inv);
-        }
-        if (to_slot && q == 0) {
-          to[slot_rows * D + row] = m_all[r];
-          to[slot_rows * (D + 1) + row] = l_all[r];
-        }
-      }
-    }
-    if (warp == 0 && lane == 0 && to_slot && cur.t == 0) {
-      // the unit starts here: its pieces run to the CTA of its last step (said also when
+    if (threadIdx.x == 0 && to_slot && cur.t == 0) {
+      // the unit starts here: its pieces run to the CTA of its last tile (said also when
       // unwinding: the combine kernel reads it in any case)
       const int last = cta_of_step(cur.first + cur.span.tiles - 1, sh.total, sh.ctas);
       PagedPieces out;
@@ -539,6 +585,8 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
     }
     if (!whole) wrote = true;
     cur.advance(p, seg);
+    // the sums are read before the next segment's statistics and rounds overwrite them
+    named_bar_sync(1, 32 * Cfg::kWarps);
   }
 }
 
@@ -554,16 +602,20 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, 2)
   // the combine kernel may be scheduled; it waits for this grid before it reads
   if (threadIdx.x == 0) grid_dependents_launch();
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
     *abort_flag = 0;
     for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(bars + 8 * (Cfg::kBarFull + s), 1);
       mbar_init(bars + 8 * (Cfg::kBarEmpty + s), Cfg::kWarps);
     }
+    mbar_init(bars + 8 * Cfg::kBarQFull, 1);
+    mbar_init(bars + 8 * Cfg::kBarQEmpty, Cfg::kWarps);
     mbar_init_fence();
   }
   grid_dependency_wait();  // nothing above touches global memory
   const PagedShare sh = paged_share<Cfg>(p, reinterpret_cast<int*>(smem + Cfg::kScanOff));
-  // no piece to combine, unless a consumer below says so (only warp 0's lane 0 writes it)
+  // no piece to combine, unless a consumer below says so (the same thread writes that)
   if (threadIdx.x == 0 && !p.pieces_only) p.pieces[blockIdx.x].count = 0;
   const Watchdog wd{abort_flag, p.status, p.timeout_ns};
   if (threadIdx.x < 32 * Cfg::kWarps)
@@ -593,60 +645,93 @@ struct CombineParams {
   PrefixPieces prefix;
 };
 
-// One CTA per entry of `pieces`; one float4 of a row a thread, all pieces in order.
+// One CTA per entry of `pieces`; one float4 of a row a thread. The pieces are read eight at a time
+// (one L2 round trip a batch) and folded in order.
 template <int D, bool kBF16, bool kPrefix>
 __global__ void __launch_bounds__(128) mfa_paged_combine_kernel(const CombineParams cp) {
+  constexpr int kBatch = 8;
   grid_dependency_wait();
   const PagedPieces pc = cp.pieces[blockIdx.x];
   if (pc.count == 0) return;
-  const int unit_rows16 = cp.kv_heads * cp.row_tiles;
-  const int request = pc.unit / unit_rows16, unit_row = pc.unit - request * unit_rows16;
+  const int units_a_request = cp.kv_heads * cp.row_tiles;
+  const int request = pc.unit / units_a_request, unit_row = pc.unit - request * units_a_request;
   const int kv_head = unit_row / cp.row_tiles;
   const int row0 = (unit_row - kv_head * cp.row_tiles) * 16;
   const int rows = cp.group - row0 < 16 ? cp.group - row0 : 16;
   const int slot_rows = cp.group < 16 ? cp.group : 16;
+  // The prefix's pieces first: CTAs c0 to c0 + prefix_count - 1 of its launch, row `in_unit` (plus
+  // this row) of their slots.
+  int prefix_count = 0, in_unit = 0;
+  long long prefix_slot = 0;
+  if (kPrefix) {
+    const PrefixPieces& pp = cp.prefix;
+    const int tile = request / pp.tile_batch, tiles_a_unit = pp.unit_rows >> 7;
+    const int qb = tile / tiles_a_unit;
+    in_unit = (tile - qb * tiles_a_unit) * 128 + (request - tile * pp.tile_batch) * cp.group + row0;
+    const long long u = static_cast<long long>(kv_head) * pp.q_blocks + qb;
+    const int c0 = cta_of_step(u * pp.steps, pp.total, pp.ctas);
+    prefix_count = cta_of_step((u + 1) * pp.steps - 1, pp.total, pp.ctas) - c0 + 1;
+    prefix_slot = c0 + u;
+  }
+  const int count = prefix_count + pc.count;
   for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {
     const int row = i / (D / 4), col = 4 * (i % (D / 4));
     float m = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float pm, float pl, const float4& x) {
-      const float next = fmaxf(m, pm);
-      const float sub = next == -INFINITY ? 0.0f : next;
-      const float f = ex2_approx(m - sub), w = ex2_approx(pm - sub);
-      l = l * f + pl * w;
-      acc.x = acc.x * f + x.x * w;
-      acc.y = acc.y * f + x.y * w;
-      acc.z = acc.z * f + x.z * w;
-      acc.w = acc.w * f + x.w * w;
-      m = next;
-    };
-    if (kPrefix) {
-      const PrefixPieces& pp = cp.prefix;
-      const int tile = request / pp.tile_batch;
-      const int in = (request - tile * pp.tile_batch) * cp.group + row0 + row;
-      const int tiles_a_unit = pp.unit_rows >> 7;
-      const int qb = tile / tiles_a_unit;
-      const int r = (tile - qb * tiles_a_unit) * 128 + in;
-      const long long u = static_cast<long long>(kv_head) * pp.q_blocks + qb;
-      const int c0 = cta_of_step(u * pp.steps, pp.total, pp.ctas);
-      const int c1 = cta_of_step((u + 1) * pp.steps - 1, pp.total, pp.ctas);
-      for (int c = c0; c <= c1; ++c) {
-        const float* at = pp.slots + (c + u) * (static_cast<long long>(pp.unit_rows) * (D + 2));
-        add(at[pp.unit_rows * D + r], at[pp.unit_rows * (D + 1) + r],
-            *reinterpret_cast<const float4*>(at + static_cast<size_t>(r) * D + col));
+    for (int k0 = 0; k0 < count; k0 += kBatch) {
+      float pm[kBatch], pl[kBatch];
+      float4 x[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int k = k0 + b;
+        pm[b] = -INFINITY;
+        pl[b] = 0.0f;
+        x[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k >= count) continue;
+        const float* at;
+        int r, stride;
+        if (kPrefix && k < prefix_count) {
+          r = in_unit + row;
+          stride = cp.prefix.unit_rows;
+          at = cp.prefix.slots + (prefix_slot + k) * (static_cast<long long>(stride) * (D + 2));
+        } else {
+          const int piece = k - prefix_count;
+          const int slot = piece == 0 ? pc.first
+                                      : cp.pieces_only ? pc.cta + piece + pc.unit
+                                                       : 2 * (pc.cta + piece);
+          r = row;
+          stride = slot_rows;
+          at = cp.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
+        }
+        pm[b] = at[stride * D + r];
+        pl[b] = at[stride * (D + 1) + r];
+        x[b] = *reinterpret_cast<const float4*>(at + static_cast<size_t>(r) * D + col);
       }
-    }
-    for (int k = 0; k < pc.count; ++k) {
-      const int slot = k == 0 ? pc.first
-                              : cp.pieces_only ? pc.cta + k + pc.unit : 2 * (pc.cta + k);
-      const float* at = cp.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
-      add(at[slot_rows * D + row], at[slot_rows * (D + 1) + row],
-          *reinterpret_cast<const float4*>(at + row * D + col));
+      float next = m;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) next = fmaxf(next, pm[b]);
+      const float sub = next == -INFINITY ? 0.0f : next;
+      const float f = ex2_approx(m - sub);
+      l *= f;
+      acc.x *= f;
+      acc.y *= f;
+      acc.z *= f;
+      acc.w *= f;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const float w = ex2_approx(pm[b] - sub);
+        l = fmaf(pl[b], w, l);
+        acc.x = fmaf(x[b].x, w, acc.x);
+        acc.y = fmaf(x[b].y, w, acc.y);
+        acc.z = fmaf(x[b].z, w, acc.z);
+        acc.w = fmaf(x[b].w, w, acc.w);
+      }
+      m = next;
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     uint16_t* to = cp.out +
-                   (static_cast<size_t>(request) * cp.kv_heads * cp.group + kv_head * cp.group +
-                    row0 + row) * D + col;
+                   ((static_cast<size_t>(request) * cp.kv_heads + kv_head) * cp.group + row0 + row) *
+                       D + col;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<kBF16>(acc.x * inv, acc.y * inv),
                                                pack_pair<kBF16>(acc.z * inv, acc.w * inv));
   }
