@@ -44,10 +44,12 @@ struct FwdParams {
   int kv_group;
   // Prefix variant: tm_q is {D, group, batch, kv_heads} with boxes of tile_batch requests (a
   // query tile has tile_rows = tile_batch * group rows), tm_k and tm_v are {D, page_size,
-  // kv_heads, pages}; key i is in page prefix_pages[i >> page_shift].
+  // kv_heads, pages}; key i is in page prefix_pages[i >> page_shift]; `splits` key
+  // ranges a unit.
   int tile_batch, tile_rows;
   const int* prefix_pages;
   int page_shift, pages;
+  int splits;
 };
 
 // Status word: a table named a page outside the cache (its rows read as zero).

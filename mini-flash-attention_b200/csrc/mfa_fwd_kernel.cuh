@@ -58,6 +58,7 @@ template <bool kCausal>
 struct StepCursor;
 template <int kRowsPerUnit>
 struct WindowCursor;
+struct PrefixCursor;
 
 template <int NQ_, int STAGES_, bool CAUSAL_, bool BF16_, int D_, bool LSE_ = false,
           bool WINDOW_ = false, bool PREFIX_ = false>
@@ -78,7 +79,9 @@ struct FwdConfig {
   static constexpr bool kBF16 = BF16_;      // q, k, v, P and out in bf16 instead of fp16
   static constexpr int kRows = 128;       // query rows per tile (= MMA M)
   static constexpr int kRowsPerUnit = kRows * NQ;
-  using Cursor = std::conditional_t<WINDOW_, WindowCursor<kRows * NQ_>, StepCursor<CAUSAL_>>;
+  using Cursor = std::conditional_t<
+      PREFIX_, PrefixCursor,
+      std::conditional_t<WINDOW_, WindowCursor<kRows * NQ_>, StepCursor<CAUSAL_>>>;
   static constexpr int kKeys = 128;       // keys per block (= S tile N)
   static constexpr int kHeadDim = D_;     // 32, 64 or 128
   static constexpr int kTileBytes = kRows * kHeadDim * 2;  // one 128-row tile of q, k or v
@@ -107,14 +110,26 @@ struct FwdConfig {
   // sub-partition); after the split: 512 x 104 + 128 x 64 = 640 x 96, and per sub-partition
   // 4 x 104 + 64 <= 512.
   static constexpr bool kRebalanceRegs = NQ == 2;
-  static constexpr int kThreads = kRebalanceRegs ? 32 * 20 : 32 * (kSoftmaxWarps + 2);
+  // Prefix variant: a warp of its own loads v (no output is stored, so with two tiles that is the
+  // store warp): with pages of 16 tokens a block is 16 copies a head-dim box, more than one
+  // thread issues in a step.
+  static constexpr int kVLoadWarp = kSoftmaxWarps + 2;
+  static constexpr int kThreads = kRebalanceRegs ? 32 * 20 : 32 * (kSoftmaxWarps + 2 + (PREFIX_ ? 1 : 0));
   static constexpr int kLaunchRegs = 96;
   static constexpr int kSoftmaxRegs = 104;
   static constexpr int kControlRegs = 64;
 
   // shared memory (offsets from a 1024-aligned base; swizzle atoms need 1024 / 512 alignment)
-  static constexpr int kQOff = 0;                              // two Q buffers of NQ tiles
-  static constexpr int kKOff = kQOff + 2 * NQ * kTileBytes;
+  static constexpr int kQOff = 0;                              // Q buffers of NQ tiles
+  // two Q buffers, so that the next unit's queries load early; one where a prefix wants the
+  // memory for a third stage of 64 KB
+  static constexpr int kQBuffers = PREFIX_ && D_ == 128 ? 1 : 2;
+  static constexpr int kKOff = kQOff + kQBuffers * NQ * kTileBytes;
+  // buffer of a CTA's s-th unit, and the phase of its barriers
+  __host__ __device__ static constexpr int q_buffer(int s) { return kQBuffers == 1 ? 0 : s & 1; }
+  __host__ __device__ static constexpr uint32_t q_phase(int s) {
+    return static_cast<uint32_t>(kQBuffers == 1 ? s : s >> 1) & 1u;
+  }
   static constexpr int kVOff = kKOff + STAGES * kTileBytes;
   static constexpr int kBarOff = kVOff + STAGES * kTileBytes;
   // barrier indices
@@ -299,6 +314,52 @@ __device__ __forceinline__ bool window_live(const FwdParams& p, int r0, int kb) 
   return kb * 128 <= r0 + 127 && (kb * 128 + 127 > r0 - p.window || kb < p.sink_blocks);
 }
 
+// Prefix variant: every unit's key blocks are cut into p.splits equal ranges; an item is a range
+// of a unit. Items are dealt out with the query blocks fastest, then the ranges, then the heads,
+// so that the CTAs that read the same keys do so at the same time and HBM gives them once, and
+// a CTA that has one item has one result. Equal shares of the steps, as StepCursor's, measured
+// 168 us against 144 at 128 requests x 4 rows behind 65536 tokens (8 heads of 128), 30 against 25
+// at 64 x 4 behind 16001, 21 against 16 at 32 x 4, and 87 against 89 at 250 x 8 rows behind 32768
+// (4 heads of 64), where two waves of items leave 3% of the SMs idle.
+struct PrefixCursor {
+  int item;
+  int u, j, j0, j1;  // as StepCursor's
+  int split;
+  int seg_idx;
+
+  __device__ void set(const FwdParams& p) {
+    const Schedule& sc = p.sc;
+    if (item >= sc.bh * sc.q_blocks * p.splits) {
+      u = j = j0 = j1 = split = 0;
+      return;
+    }
+    const int range = static_cast<int>(sc.qdiv(item));
+    const int head = range / p.splits;
+    split = range - head * p.splits;
+    u = head * sc.q_blocks + item - range * sc.q_blocks;
+    j = j0 = static_cast<int>(static_cast<long long>(split) * sc.nkb / p.splits);
+    j1 = static_cast<int>(static_cast<long long>(split + 1) * sc.nkb / p.splits);
+  }
+  __device__ void init(const FwdParams& p) {
+    item = static_cast<int>(blockIdx.x);
+    seg_idx = 0;
+    set(p);
+  }
+  __device__ bool valid() const { return j < j1; }
+  __device__ bool first_step() const { return j == j0; }
+  __device__ bool first_of_range() const { return seg_idx == 0; }
+  __device__ bool whole(const Schedule&) const { return false; }
+  __device__ int slot(const FwdParams& p) const { return u * p.splits + split; }
+  __device__ void next_segment(const FwdParams& p) {
+    item += static_cast<int>(gridDim.x);
+    ++seg_idx;
+    set(p);
+  }
+  __device__ void step(const FwdParams& p) {
+    if (++j >= j1) next_segment(p);
+  }
+};
+
 // Head and batch index of unit u: its (batch * head) row is u / q_blocks, heads fastest.
 __device__ __forceinline__ HeadBatch head_batch(const FwdParams& p, int u) {
   const int bh = p.sc.head_of(u);
@@ -388,98 +449,109 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
   }
 }
 
-// Load role of the prefix variant. A query tile is tile_batch requests' group rows (its rows
-// behind them are never written, and their results never read); a key block is one box for each
-// of its pages, of which those behind the prefix's end are left out. The page numbers of the
-// next block are read while this one's copies are issued.
-template <class Cfg>
+// Load role of the prefix variant, executed by two whole warps: queries and k (kValue false), or v.
+// A query tile is tile_batch requests' group rows (its rows behind them are never written, and
+// their results never read); a key block is one box for each of its pages, of which those behind
+// the prefix's end are left out. Lane i looks up box i of a batch of blocks (32 boxes); the next
+// batch's pages are on their way while this one's copies are issued.
+template <class Cfg, bool kValue>
 __device__ __forceinline__ void prefix_load_role(const FwdParams& p, uint8_t* smem, uint32_t bars,
                                                  const Watchdog& wd) {
   constexpr int ST = Cfg::STAGES;
-  constexpr int kMostPages = Cfg::kKeys / 16;
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
+  const int lane = threadIdx.x & 31;
   const uint32_t sbase = smem_addr(smem);
-  tma_prefetch_desc(&p.tm_q);
-  tma_prefetch_desc(&p.tm_k);
-  tma_prefetch_desc(&p.tm_v);
+  const CUtensorMap* map = kValue ? &p.tm_v : &p.tm_k;
+  constexpr int kFull = kValue ? Cfg::kBarVFull : Cfg::kBarKFull;
+  constexpr int kEmpty = kValue ? Cfg::kBarVEmpty : Cfg::kBarKEmpty;
+  constexpr int kOff = kValue ? Cfg::kVOff : Cfg::kKOff;
   const int box_shift = p.page_shift < 7 ? p.page_shift : 7;  // rows of a box
-  const int boxes = Cfg::kKeys >> box_shift;
+  const int block_shift = 7 - box_shift;                      // boxes of a block: 1 to 8
   const uint32_t box_bytes = static_cast<uint32_t>(Cfg::kRowBytes) << box_shift;
   const uint32_t q_box_bytes = static_cast<uint32_t>(p.tile_rows * Cfg::kRowBytes);
-
+  if (lane == 0) {
+    if (!kValue) tma_prefetch_desc(&p.tm_q);
+    tma_prefetch_desc(map);
+  }
+  auto look_up = [&](int block) -> int {  // this lane's page in the batch that starts at `block`
+    const long long key = static_cast<long long>(block) * Cfg::kKeys + (lane << box_shift);
+    return key < p.n ? p.prefix_pages[key >> p.page_shift] : 0;
+  };
   typename Cfg::Cursor cur;
   cur.init(p);
-  int pages[kMostPages];
-  auto read_pages = [&](int j) {
-#pragma unroll
-    for (int i = 0; i < kMostPages; ++i) {
-      const int key = j * Cfg::kKeys + (i << box_shift);
-      pages[i] = i < boxes && key < p.n ? p.prefix_pages[key >> p.page_shift] : -1;
-    }
-  };
-  auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int key0, int head) {
-    const int left = (p.n - key0 + (1 << box_shift) - 1) >> box_shift;
-    const int here = left < boxes ? left : boxes;
-    mbar_arrive_expect_tx(full, Cfg::kBoxes * box_bytes * here);
-    const int row0 = key0 & ((1 << p.page_shift) - 1);
-#pragma unroll
-    for (int i = 0; i < kMostPages; ++i) {
-      if (i >= here) break;
-      // a page outside the cache: a place outside the map, which reads as zero
-      const bool bad = pages[i] < 0 || pages[i] >= p.pages;
-      if (bad) atomicCAS(p.status, 0, kStatusBadPage);
-#pragma unroll
-      for (int x = 0; x < Cfg::kBoxes; ++x)
-        tma_load_4d(dst + x * Cfg::kBoxBytes + i * box_bytes, map, full, x * Cfg::kBoxCols, row0,
-                    head, bad ? p.pages : pages[i]);
-    }
-  };
-  int g = 0, q_loaded = 0, k_issued = 0, v_issued = 0;
-  if (cur.valid()) read_pages(cur.j);
-  while (cur.valid()) {
+  int g = 0, q_loaded = 0, issued = 0;
+  bool ok = true;
+  while (ok && cur.valid()) {
     const int head = p.sc.head_of(cur.u);
-    if (cur.first_step()) {
-      const int s = cur.seg_idx, b = s & 1;
-      if (!wait_single(bar(Cfg::kBarQEmpty + b), (static_cast<uint32_t>(s >> 1) & 1u) ^ 1u, wd,
-                       kSiteLoadQEmpty))
-        break;
-      mbar_arrive_expect_tx(bar(Cfg::kBarQFull + b), Cfg::NQ * Cfg::kBoxes * q_box_bytes);
+    int pages = look_up(cur.j0), later = 0, batch0 = cur.j0;
+    if (!kValue) {
+      const int s = cur.seg_idx, b = Cfg::q_buffer(s);
+      if (!wait_warp(bar(Cfg::kBarQEmpty + b), Cfg::q_phase(s) ^ 1u, wd, kSiteLoadQEmpty)) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar(Cfg::kBarQFull + b), Cfg::NQ * Cfg::kBoxes * q_box_bytes);
 #pragma unroll
-      for (int i = 0; i < Cfg::NQ; ++i) {
+        for (int i = 0; i < Cfg::NQ; ++i) {
 #pragma unroll
-        for (int x = 0; x < Cfg::kBoxes; ++x)
-          tma_load_4d(sbase + Cfg::kQOff + (b * Cfg::NQ + i) * Cfg::kTileBytes + x * Cfg::kBoxBytes,
-                      &p.tm_q, bar(Cfg::kBarQFull + b), x * Cfg::kBoxCols, 0,
-                      (p.sc.qb_of(cur.u) * Cfg::NQ + i) * p.tile_batch, head);
+          for (int x = 0; x < Cfg::kBoxes; ++x)
+            tma_load_4d(
+                sbase + Cfg::kQOff + (b * Cfg::NQ + i) * Cfg::kTileBytes + x * Cfg::kBoxBytes,
+                &p.tm_q, bar(Cfg::kBarQFull + b), x * Cfg::kBoxCols, 0,
+                (p.sc.qb_of(cur.u) * Cfg::NQ + i) * p.tile_batch, head);
+        }
       }
+      __syncwarp();
       q_loaded = s + 1;
     }
-    const int st = g % ST;
-    const uint32_t ph = static_cast<uint32_t>(g / ST) & 1u;
-    const int key0 = cur.j * Cfg::kKeys;
-    if (!wait_single(bar(Cfg::kBarKEmpty + st), ph ^ 1u, wd, kSiteLoadKEmpty)) break;
-    load(&p.tm_k, sbase + Cfg::kKOff + st * Cfg::kTileBytes, bar(Cfg::kBarKFull + st), key0, head);
-    k_issued = g + 1;
-    if (!wait_single(bar(Cfg::kBarVEmpty + st), ph ^ 1u, wd, kSiteLoadVEmpty)) break;
-    load(&p.tm_v, sbase + Cfg::kVOff + st * Cfg::kTileBytes, bar(Cfg::kBarVFull + st), key0, head);
-    v_issued = g + 1;
-    ++g;
-    cur.step(p);
-    if (cur.valid()) read_pages(cur.j);
+    for (int j = cur.j0; j < cur.j1; ++j) {
+      if (((j - batch0) << block_shift) == 32) {
+        batch0 = j;
+        pages = later;
+      }
+      if (j == batch0) {
+        // a page outside the cache: a place outside the map, which reads as zero
+        const bool bad = pages < 0 || pages >= p.pages;
+        if (bad) {
+          pages = p.pages;
+          atomicCAS(p.status, 0, kStatusBadPage);
+        }
+        later = look_up(batch0 + (32 >> block_shift));
+      }
+      const int st = g % ST;
+      if (!(ok = wait_warp(bar(kEmpty + st), (static_cast<uint32_t>(g / ST) & 1u) ^ 1u, wd,
+                           kValue ? kSiteLoadVEmpty : kSiteLoadKEmpty)))
+        break;
+      const int key0 = j * Cfg::kKeys;
+      const int left = (p.n - key0 + (1 << box_shift) - 1) >> box_shift;
+      const int here = left < 1 << block_shift ? left : 1 << block_shift;
+      const uint32_t full = bar(kFull + st), dst = sbase + kOff + st * Cfg::kTileBytes;
+      const int row0 = key0 & ((1 << p.page_shift) - 1);
+      if (lane == 0) mbar_arrive_expect_tx(full, Cfg::kBoxes * box_bytes * here);
+      __syncwarp();
+      for (int i = 0; i < here; ++i) {
+        const int page = __shfl_sync(0xffffffffu, pages, ((j - batch0) << block_shift) + i);
+        if (lane == 0) {
+#pragma unroll
+          for (int x = 0; x < Cfg::kBoxes; ++x)
+            tma_load_4d(dst + x * Cfg::kBoxBytes + i * box_bytes, map, full, x * Cfg::kBoxCols,
+                        row0, head, page);
+        }
+      }
+      __syncwarp();
+      issued = ++g;
+    }
+    cur.next_segment(p);
   }
-  if (*wd.abort) {
-    // Unwinding: wait for every copy this thread put in flight before shared memory goes away.
-    for (int b = 0; b < 2; ++b) {
+  if (*wd.abort && lane == 0) {
+    // Unwinding: wait for every copy of this warp in flight before shared memory goes away.
+    for (int b = 0; b < Cfg::kQBuffers; ++b) {
       int last = -1;
-      for (int s = b; s < q_loaded; s += 2) last = s;
-      if (last >= 0) drain_wait(bar(Cfg::kBarQFull + b), static_cast<uint32_t>(last >> 1) & 1u);
+      for (int s = b; s < q_loaded; s += Cfg::kQBuffers) last = s;
+      if (last >= 0) drain_wait(bar(Cfg::kBarQFull + b), Cfg::q_phase(last));
     }
     for (int st = 0; st < ST; ++st) {
-      int last_k = -1, last_v = -1;
-      for (int x = st; x < k_issued; x += ST) last_k = x;
-      for (int x = st; x < v_issued; x += ST) last_v = x;
-      if (last_k >= 0) drain_wait(bar(Cfg::kBarKFull + st), static_cast<uint32_t>(last_k / ST) & 1u);
-      if (last_v >= 0) drain_wait(bar(Cfg::kBarVFull + st), static_cast<uint32_t>(last_v / ST) & 1u);
+      int last = -1;
+      for (int x = st; x < issued; x += ST) last = x;
+      if (last >= 0) drain_wait(bar(kFull + st), static_cast<uint32_t>(last / ST) & 1u);
     }
   }
 }
@@ -530,10 +602,9 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
   [[maybe_unused]] bool fresh_unit = true;
   // S_i[gs] = Q_i K_gs^T once softmax_i has pulled S_i[gs-1] into registers.
   auto issue_s = [&]() -> bool {
-    const int b = cs.seg_idx & 1;
+    const int b = Cfg::q_buffer(cs.seg_idx);
     if (cs.first_step()) {
-      if (!wait_warp(bar(Cfg::kBarQFull + b), static_cast<uint32_t>(cs.seg_idx >> 1) & 1u, wd,
-                     kSiteMmaQ))
+      if (!wait_warp(bar(Cfg::kBarQFull + b), Cfg::q_phase(cs.seg_idx), wd, kSiteMmaQ))
         return false;
     }
     const int st = gs % ST;
@@ -577,7 +648,14 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
   while (cp.valid()) {
     // S of the next step goes in before P.V of this one, so the tensor core computes the
     // next scores while the softmax warps are still busy with this block.
-    if (cs.valid() && !issue_s()) goto unwind;
+    if constexpr (Cfg::kQBuffers == 1) {
+      // With one Q buffer, a unit's queries arrive only when the one before has been read to its
+      // end, this P.V among it: its first scores cannot go in ahead, and follow here.
+      if (cs.valid() && gs == gp && !issue_s()) goto unwind;
+      if (cs.valid() && gs == gp + 1 && !cs.first_step() && !issue_s()) goto unwind;
+    } else {
+      if (cs.valid() && !issue_s()) goto unwind;
+    }
     // ---- O_i += P_i[gp] V_gp once softmax_i has written P_i[gp] (and rescaled O_i if needed).
     {
       const int st = gp % ST;
@@ -877,7 +955,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     uint32_t o[Cfg::kHeadDim / 2];  // o[4i + e]: row gq + 8 (e / 2), d 8i + 2q + e % 2
     tmem_ld_16x256b_sync(tO, o);
     tc_fence_before();
-    const int b = cur.seg_idx & 1;
+    const int b = Cfg::q_buffer(cur.seg_idx);
     if (!Cfg::kPrefix && cur.whole(p.sc)) {
       if (Cfg::kLSE && q == 0 && (!Cfg::kWindow || p.lse != nullptr)) {
         // log-sum-exp = ln 2 * (m + log2 l), m in scaled log2 units
@@ -936,10 +1014,11 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     } else {
       // A piece of a query block: unnormalised O, the row max and the row sum go to this
       // CTA's workspace slot (first or last segment of its range) for the merge kernel.
-      // Prefix variant: slot CTA + unit, which grows by one at least from one segment of the
-      // launch to the next, in the order of the steps.
-      const size_t slot = Cfg::kPrefix ? static_cast<size_t>(blockIdx.x) + cur.u
-                                       : 2 * blockIdx.x + (cur.first_of_range() ? 0 : 1);
+      size_t slot;
+      if constexpr (Cfg::kPrefix)
+        slot = static_cast<size_t>(cur.slot(p));
+      else
+        slot = 2 * blockIdx.x + (cur.first_of_range() ? 0 : 1);
       float* ws = p.workspace + slot * Cfg::kSlotFloats;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -973,7 +1052,7 @@ __device__ __forceinline__ void store_role(const FwdParams& p, uint8_t* smem, ui
   cur.init(p);
   int stores = 0;  // whole units stored so far (phase of the staging barriers)
   while (cur.valid()) {
-    if (!Cfg::kPrefix && cur.whole(p.sc)) {
+    if (cur.whole(p.sc)) {
       const int b = cur.seg_idx & 1;
       const HeadBatch ob = head_batch(p, cur.u);
       bool ok = true;
@@ -1024,7 +1103,7 @@ __global__ void
 
   // The split-mode merge kernel may be scheduled now; it waits for this grid to complete
   // before reading anything this grid writes.
-  if (threadIdx.x == 0) grid_dependents_launch();
+  if (!Cfg::kPrefix && threadIdx.x == 0) grid_dependents_launch();
   // This grid is itself launched as a programmatic dependent of the stream's previous kernel:
   // the set-up below (barriers, TMEM) may overlap that kernel's tail; every warp then waits
   // for that kernel's completion before its role starts, i.e. before any global memory
@@ -1036,7 +1115,7 @@ __global__ void
   if (warp == Cfg::kLoadWarp) {
     if (lane == 0) {
       *abort_flag = 0;
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < 2; ++b) {  // (the prefix variant may use one)
         mbar_init(bars + 8 * (Cfg::kBarQFull + b), 1);
         mbar_init(bars + 8 * (Cfg::kBarQEmpty + b), Cfg::NQ);  // one arrive per tile epilogue
       }
@@ -1061,12 +1140,10 @@ __global__ void
     if constexpr (Cfg::kRebalanceRegs) setmaxnreg_dec<Cfg::kControlRegs>();
     const Watchdog wd{abort_flag, p.status, p.timeout_ns};
     grid_dependency_wait();
-    if (lane == 0) {
-      if constexpr (Cfg::kPrefix)
-        prefix_load_role<Cfg>(p, smem, bars, wd);
-      else
-        load_role<Cfg>(p, smem, bars, wd);
-    }
+    if constexpr (Cfg::kPrefix)
+      prefix_load_role<Cfg, false>(p, smem, bars, wd);
+    else if (lane == 0)
+      load_role<Cfg>(p, smem, bars, wd);
   } else {
     if (warp == 0) {
       tmem_alloc(smem_addr(tmem_slot), Cfg::kTmemCols);
@@ -1077,6 +1154,9 @@ __global__ void
     tc_fence_after();
     tmem = *tmem_slot;
     grid_dependency_wait();
+    // Prefix variant: the kernel behind it (the requests' own tokens) does not wait for this one,
+    // so it may only start once the stream's earlier work is done, which it relies on.
+    if (Cfg::kPrefix && threadIdx.x == 0) grid_dependents_launch();
     const Watchdog wd{abort_flag, p.status, p.timeout_ns};
     if (warp < Cfg::kSoftmaxWarps) {
       if constexpr (Cfg::kRebalanceRegs) setmaxnreg_inc<Cfg::kSoftmaxRegs>();
@@ -1085,6 +1165,8 @@ __global__ void
       if constexpr (Cfg::kRebalanceRegs) setmaxnreg_dec<Cfg::kControlRegs>();
       if (warp == Cfg::kMmaWarp || (Cfg::NQ == 2 && warp == Cfg::kMmaWarp2)) {
         mma_role<Cfg>(p, smem, bars, tmem, wd, warp == Cfg::kMmaWarp ? 0 : 1);
+      } else if (Cfg::kPrefix && warp == Cfg::kVLoadWarp) {
+        prefix_load_role<Cfg, true>(p, smem, bars, wd);
       } else if (Cfg::kStoreRole && warp == Cfg::kStoreWarp) {
         if (lane == 0) store_role<Cfg>(p, smem, bars, wd);
       }

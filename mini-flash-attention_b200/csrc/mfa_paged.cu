@@ -22,9 +22,10 @@ constexpr int64_t kMost = 0x7fffff00LL;  // 32-bit counters with room for a tile
 
 // The prefix variant of the forward kernel. D = 64 has two query tiles a CTA as the forward does,
 // or, when all rows fit one, one tile and a deeper ring (a prefix read for so few rows is bound
-// by HBM: 5 stages are 160 KB in flight on an SM); D = 128 one tile, as the forward.
+// by HBM: 5 stages are 160 KB in flight on an SM); D = 128 one tile, as the forward, and three
+// stages of 64 KB.
 template <bool kBF16, int D, int NQ>
-using Prefix = FwdConfig<NQ, D == 128 ? 2 : NQ == 1 ? 5 : 3, false, kBF16, D, false, false, true>;
+using Prefix = FwdConfig<NQ, D == 64 && NQ == 1 ? 5 : 3, false, kBF16, D, false, false, true>;
 
 template <class Cfg>
 auto* prefix_kernel() {
@@ -172,7 +173,7 @@ int64_t most_tiles(const Problem& w) {
 // Parts of the workspace, in floats from its start (256-byte aligned parts).
 struct Layout {
   int64_t ctas;         // of the paged kernel
-  int64_t prefix_ctas;  // of the prefix kernel
+  int64_t prefix_ctas, splits;  // of the prefix kernel
   int64_t slots, prefix_slots, pieces, bytes;
 };
 
@@ -188,14 +189,26 @@ Layout lay_out(const Problem& w, int64_t sms) {
   l.slots = 0;
   l.pieces = whole(slots * paged_slot_floats(static_cast<int>(w.slot_rows()), w.d));
   l.prefix_slots = l.pieces + whole(entries * static_cast<int64_t>(sizeof(PagedPieces)) / 4);
-  l.prefix_ctas = 0;
+  l.prefix_ctas = l.splits = 0;
   int64_t end = l.prefix_slots;
   if (shared) {
     const int nq = w.tiles_a_unit();
     const int64_t units = (w.tiles() + nq - 1) / nq * w.kv_heads;
-    const int64_t total = units * ((w.prefix + 127) / 128);
-    l.prefix_ctas = total < sms ? total : sms;
-    end += (l.prefix_ctas + units) * (128 * nq * (w.d + 2));
+    const int64_t blocks = (w.prefix + 127) / 128;
+    // As many ranges a unit as finish first: waves of items times their steps, each with about
+    // two steps' time more for its queries, first scores and result; and every range is one
+    // more piece for the combine kernel to read.
+    double best = 1e300;
+    for (int64_t s = 1; s <= blocks && (s == 1 || s * units <= 3 * sms); ++s) {
+      const int64_t waves = (units * s + sms - 1) / sms;
+      const double cost = static_cast<double>(waves * ((blocks + s - 1) / s + 2)) + 0.1 * s;
+      if (cost < best) {
+        best = cost;
+        l.splits = s;
+      }
+    }
+    l.prefix_ctas = units * l.splits < sms ? units * l.splits : sms;
+    end += units * l.splits * (128 * nq * (w.d + 2));
   }
   l.bytes = end * 4;
   return l;
@@ -239,8 +252,7 @@ int launch_prefix(const Arrays& x, const Problem& w, const Layout& l, const host
   p.n = static_cast<int>(w.prefix);
   p.heads = static_cast<int>(w.kv_heads);
   p.sc = make_schedule(w.kv_heads, w.tiles() * 128, w.prefix, Cfg::kRowsPerUnit, Cfg::kKeys, false);
-  p.split = 1;
-  set_ctas(p.sc, static_cast<int>(l.prefix_ctas));
+  p.splits = static_cast<int>(l.splits);
   p.scale_log2 = w.scale * 1.4426950408889634f;
   p.timeout_ns = dev.timeout_ns;
   p.status = dev.status;
@@ -250,8 +262,7 @@ int launch_prefix(const Arrays& x, const Problem& w, const Layout& l, const host
   p.prefix_pages = x.prefix_pages;
   p.page_shift = w.shift();
   p.pages = static_cast<int>(w.pages);
-  *pp = {p.workspace, p.sc.total(), p.sc.ctas, p.sc.nkb, p.sc.q_blocks, Cfg::kRowsPerUnit,
-         p.tile_batch};
+  *pp = {p.workspace, p.splits, p.sc.q_blocks, Cfg::kRowsPerUnit, p.tile_batch};
   const cudaError_t e = launch(prefix_kernel<Cfg>(), l.prefix_ctas, Cfg::kThreads, Cfg::kSmemBytes,
                                stream, p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "prefix attention launch");

@@ -613,7 +613,11 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, 2)
     mbar_init(bars + 8 * Cfg::kBarQEmpty, Cfg::kWarps);
     mbar_init_fence();
   }
-  grid_dependency_wait();  // nothing above touches global memory
+  // Nothing above touches global memory. Behind a prefix, the kernel before this one is the
+  // prefix's, whose results this one does not read, and it lets this one start only when all
+  // earlier work is done; so it waits for the prefix at its end instead (the combine kernel
+  // waits for this grid alone) and starts on every SM that the prefix has left.
+  if (!p.pieces_only) grid_dependency_wait();
   const PagedShare sh = paged_share<Cfg>(p, reinterpret_cast<int*>(smem + Cfg::kScanOff));
   // no piece to combine, unless a consumer below says so (the same thread writes that)
   if (threadIdx.x == 0 && !p.pieces_only) p.pieces[blockIdx.x].count = 0;
@@ -622,15 +626,14 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, 2)
     paged_consume_role<Cfg>(p, sh, smem, bars, wd);
   else
     paged_load_role<Cfg>(p, sh, smem_addr(smem), bars, wd);
+  if (p.pieces_only) grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------- combine
 // What a prefix that all requests share adds: slots of the forward kernel's prefix variant.
 struct PrefixPieces {
-  const float* slots;   // [slot][unit_rows] x (D sums, then maxima, then sums of p)
-  long long total;      // steps of the prefix launch
-  int ctas;
-  int steps;            // steps of one of its units
+  const float* slots;   // [unit][split][unit_rows] x (D sums, then maxima, then sums of p)
+  int splits;
   int q_blocks;         // units of a k / v head
   int unit_rows;        // rows of a unit, 128 a tile
   int tile_batch;       // requests of a 128-row tile
@@ -659,8 +662,7 @@ __global__ void __launch_bounds__(128) mfa_paged_combine_kernel(const CombinePar
   const int row0 = (unit_row - kv_head * cp.row_tiles) * 16;
   const int rows = cp.group - row0 < 16 ? cp.group - row0 : 16;
   const int slot_rows = cp.group < 16 ? cp.group : 16;
-  // The prefix's pieces first: CTAs c0 to c0 + prefix_count - 1 of its launch, row `in_unit` (plus
-  // this row) of their slots.
+  // The prefix's pieces first: row `in_unit` (plus this row) of their slots.
   int prefix_count = 0, in_unit = 0;
   long long prefix_slot = 0;
   if (kPrefix) {
@@ -669,9 +671,8 @@ __global__ void __launch_bounds__(128) mfa_paged_combine_kernel(const CombinePar
     const int qb = tile / tiles_a_unit;
     in_unit = (tile - qb * tiles_a_unit) * 128 + (request - tile * pp.tile_batch) * cp.group + row0;
     const long long u = static_cast<long long>(kv_head) * pp.q_blocks + qb;
-    const int c0 = cta_of_step(u * pp.steps, pp.total, pp.ctas);
-    prefix_count = cta_of_step((u + 1) * pp.steps - 1, pp.total, pp.ctas) - c0 + 1;
-    prefix_slot = c0 + u;
+    prefix_count = pp.splits;
+    prefix_slot = u * pp.splits;
   }
   const int count = prefix_count + pc.count;
   for (int i = threadIdx.x; i < rows * (D / 4); i += 128) {

@@ -36,7 +36,7 @@ class Cache:
             new = [torch.randn((len(positions), kv_heads, d), generator=g).to(dtype)
                    for _ in range(2)]
             k[rows, :, at % page], v[rows, :, at % page] = new
-            return [x.double() for x in new]
+            return [x.cuda().double() for x in new]
 
         self.shared = fill(self.prefix_pages, list(range(prefix)))
         at = shared
@@ -59,10 +59,11 @@ class Cache:
         return torch.tensor(self.prefix_pages, dtype=torch.int32, device="cuda")
 
     def reference(self, q):
-        """(value, bound) of the attention of q [B, H, D] (on the CPU)."""
-        u = half_step(self.dtype)
+        """(value, bound) of the attention of q [B, H, D]."""
+        u, q = half_step(self.dtype), q.cuda()
         floor = 2.0 ** -25 if self.dtype == torch.float16 else 0.0
-        value, bound = torch.zeros(q.shape, dtype=torch.float64), torch.full(q.shape, TINY).double()
+        value = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+        bound = torch.full_like(value, TINY)
         for r, (k, v) in enumerate(zip(self.keys, self.values)):
             k, v = (torch.cat((a, b)) for a, b in zip(self.shared, (k, v)))
             if not len(k):
@@ -85,7 +86,6 @@ def queries(batch, heads, d, dtype, seed=1):
 
 def check(out, value, bound):
     assert out.shape == value.shape
-    out = out.cpu()
     assert torch.isfinite(out).all()
     worst = ((out.double() - value).abs() - bound).max().item() if out.numel() else 0.0
     assert worst <= 0, f"{worst:.3g} over the bound"

@@ -126,6 +126,28 @@ def test_prefix_rows(batch, kv_heads, group, d):
     check(out, *cache.reference(q))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefix_several_units_a_cta(d):
+    # more query tiles than CTAs: a CTA goes over several units
+    lengths = [(5 * i) % 50 for i in range(320)]
+    cache = Cache(lengths, 4, d, 64, torch.bfloat16, prefix=1100)
+    q = queries(320, 4 * 31, d, torch.bfloat16)
+    k, v, table, own = cache.tensors()
+    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), 1100, table, own)
+    check(out, *cache.reference(q))
+
+
+@pytest.mark.parametrize("batch,d,page", [(40, 128, 128), (150, 128, 16), (150, 64, 256)])
+def test_prefix_past_the_l2(batch, d, page):
+    # a prefix of more bytes than stay in L2: the units of a head read the same keys at the same time
+    prefix = 32768 * 128 // d - 5
+    cache = Cache([i % 3 for i in range(batch)], 8, d, page, torch.float16, prefix=prefix)
+    q = queries(batch, 64, d, torch.float16)
+    k, v, table, own = cache.tensors()
+    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), prefix, table, own)
+    check(out, *cache.reference(q))
+
+
 def test_prefix_long_and_none():
     lengths = [5, 300]
     cache = Cache(lengths, 8, 64, 64, torch.float16, prefix=20000)
