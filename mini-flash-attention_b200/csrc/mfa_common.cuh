@@ -42,6 +42,7 @@ struct FwdParams {
   int sinks;
   int sink_blocks;
   int kv_group;
+  int whole_units;  // query blocks done whole; the others tile by tile (WindowCursor)
   // Prefix variant: tm_q is {D, group, batch, kv_heads} with boxes of tile_batch requests (a
   // query tile has tile_rows = tile_batch * group rows), tm_k and tm_v are {D, page_size,
   // kv_heads, pages}; key i is in page prefix_pages[i >> page_shift]; `splits` key

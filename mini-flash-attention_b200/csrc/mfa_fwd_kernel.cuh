@@ -249,70 +249,77 @@ struct StepCursor {
   }
 };
 
-// Walks whole query blocks u = cta, cta + ctas, ... of the windowed attention, whose key blocks
-// are those that hold sinks and lie before the window, then those from the oldest key that the
-// block's first row sees to its last row: steps() of them, numbered j, key block block().
-// A query block qb whose window starts past key 0 has kRowsPerUnit / 128 + ceil((window - 1) /
-// 128) window blocks, the same for all of them, so the blocks are dealt out without a split.
+// Walks query blocks cta, cta + ctas, ... of the windowed attention, whose key blocks are those
+// that hold sinks and lie before the window, then those from the oldest key that the block's first
+// row sees to its last row: steps numbered j, key block block(). A query block whose window starts
+// past key 0 has kRowsPerUnit / 128 + ceil((window - 1) / 128) window blocks, the same for all of
+// them, so the blocks are dealt out without a split. The items are p.whole_units query blocks, then
+// the others' two 128-row tiles one by one: where whole blocks would leave half of the CTAs or more
+// idle in the last wave, single tiles, which take a CTA 0.57 times as long (it has no other
+// tile's products to do meanwhile), end sooner.
 template <int kRowsPerUnit>
 struct WindowCursor {
-  int u;        // current query block, row-major over (head, query block)
+  int item;
+  int u;        // query block, row-major over (head, query block)
+  int row;      // first query row
+  int tiles;    // 128-row tiles
   int j;        // current step
-  int j0, j1;   // steps of u: [0, j1)
-  int rem;      // query blocks after this one
-  int seg_idx;  // index of the current query block in this CTA
+  int j0, j1;   // steps: [0, j1)
+  int seg_idx;  // index of the current item in this CTA
   int sinks;    // steps before the window
   int skip;     // key blocks between them and the window
 
   __device__ void start(const FwdParams& p) {
-    const int qb = p.sc.qb_of(u);
-    const int oldest = qb * kRowsPerUnit - p.window + 1;  // key of the block's first row
-    const int w0 = oldest > 0 ? oldest >> 7 : 0;
-    const int last = (qb + 1) * (kRowsPerUnit / 128) - 1;
-    sinks = p.sink_blocks < w0 ? p.sink_blocks : w0;
-    skip = w0 - sinks;
-    j = j0 = 0;
-    j1 = (last < p.sc.nkb ? last + 1 : p.sc.nkb) - skip;
+    const int units = p.sc.bh * p.sc.q_blocks;  // < 2^30 (checked by the launcher)
+    const int items = kRowsPerUnit == 128 ? units : 2 * units - p.whole_units;
+    u = j = j0 = j1 = sinks = skip = row = 0;
+    for (; item < items; item += static_cast<int>(gridDim.x)) {
+      const int single = item - p.whole_units;  // >= 0: a tile of its own
+      const bool one = kRowsPerUnit == 128 || single >= 0;
+      u = kRowsPerUnit > 128 && one ? p.whole_units + (single >> 1) : item;
+      row = p.sc.qb_of(u) * kRowsPerUnit + (kRowsPerUnit > 128 && one ? (single & 1) * 128 : 0);
+      if (row >= p.nq) continue;  // the second tile of a head's last block may be empty
+      tiles = one ? 1 : 2;
+      const int oldest = row - p.window + 1;
+      const int w0 = oldest > 0 ? oldest >> 7 : 0;
+      const int last = (row >> 7) + tiles - 1;
+      sinks = p.sink_blocks < w0 ? p.sink_blocks : w0;
+      skip = w0 - sinks;
+      j1 = (last < p.sc.nkb ? last + 1 : p.sc.nkb) - skip;
+      return;
+    }
   }
   __device__ void init(const FwdParams& p) {
-    const int units = p.sc.bh * p.sc.q_blocks;  // < 2^31 (checked by the launcher)
     seg_idx = 0;
-    u = static_cast<int>(blockIdx.x);
-    rem = u < units ? (units - 1 - u) / static_cast<int>(gridDim.x) : 0;
-    if (u < units) {
-      start(p);
-    } else {
-      u = 0;
-      j = j0 = j1 = sinks = skip = 0;
-    }
+    item = static_cast<int>(blockIdx.x);
+    start(p);
   }
   __device__ bool valid() const { return j < j1; }
   __device__ bool first_step() const { return j == 0; }
   __device__ bool first_of_range() const { return seg_idx == 0; }
   __device__ bool whole(const Schedule&) const { return true; }
   __device__ int block() const { return j < sinks ? j : j + skip; }
+  // First query row of a tile of the CTA, or -1 if the item does not have it.
+  __device__ int tile_row(int tile) const { return tile < tiles ? row + 128 * tile : -1; }
+  // Whether the tile sees a key of the current key block (of a tile past the last row, every
+  // block: nobody reads its result, and it keeps at least one). Two tiles take one window block
+  // more together than each of them needs: the first does not see the block of the second's
+  // diagonal, the second not the oldest block of the first.
+  __device__ bool live(const FwdParams& p, int tile) const {
+    const int r0 = tile_row(tile), kb = block();
+    if (r0 < 0) return false;
+    if (r0 >= p.nq) return true;
+    return kb * 128 <= r0 + 127 && (kb * 128 + 127 > r0 - p.window || kb < p.sink_blocks);
+  }
   __device__ void next_segment(const FwdParams& p) {
-    j = j1 - 1;
-    step(p);
+    item += static_cast<int>(gridDim.x);
+    ++seg_idx;
+    start(p);
   }
   __device__ void step(const FwdParams& p) {
-    if (++j >= j1 && rem > 0) {
-      u += static_cast<int>(gridDim.x);
-      --rem;
-      ++seg_idx;
-      start(p);
-    }
+    if (++j >= j1) next_segment(p);
   }
 };
-
-// Whether key block kb holds a key that some row of the 128-row tile at query row r0 sees (of a
-// tile past the last row, every block: nobody reads its result, and it keeps at least one).
-// A unit of two tiles takes one window block more than each of them needs: tile 0 does not see
-// the block of tile 1's diagonal, tile 1 not the oldest block of tile 0.
-__device__ __forceinline__ bool window_live(const FwdParams& p, int r0, int kb) {
-  if (r0 >= p.nq) return true;
-  return kb * 128 <= r0 + 127 && (kb * 128 + 127 > r0 - p.window || kb < p.sink_blocks);
-}
 
 // Prefix variant: every unit's key blocks are cut into p.splits equal ranges; an item is a range
 // of a unit. Items are dealt out with the query blocks fastest, then the ranges, then the heads,
@@ -366,6 +373,16 @@ __device__ __forceinline__ HeadBatch head_batch(const FwdParams& p, int u) {
   return {bh % p.heads, bh / p.heads};
 }
 
+// First query row of a tile of the current unit.
+template <class Cfg>
+__device__ __forceinline__ int tile_row0(const FwdParams& p, const typename Cfg::Cursor& cur,
+                                         int tile) {
+  if constexpr (Cfg::kWindow)
+    return cur.tile_row(tile);
+  else
+    return p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows;
+}
+
 template <class Cfg>
 __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uint32_t bars,
                                           const Watchdog& wd) {
@@ -391,14 +408,17 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
       if (!wait_single(bar(Cfg::kBarQEmpty + b), (static_cast<uint32_t>(s >> 1) & 1u) ^ 1u, wd,
                        kSiteLoadQEmpty))
         break;
-      mbar_arrive_expect_tx(bar(Cfg::kBarQFull + b), Cfg::NQ * Cfg::kTileBytes);
+      int tiles = Cfg::NQ;
+      if constexpr (Cfg::kWindow) tiles = cur.tiles;
+      mbar_arrive_expect_tx(bar(Cfg::kBarQFull + b), tiles * Cfg::kTileBytes);
 #pragma unroll
       for (int i = 0; i < Cfg::NQ; ++i) {
+        if (Cfg::kWindow && i >= tiles) break;
 #pragma unroll
         for (int x = 0; x < Cfg::kBoxes; ++x) {
           tma_load_4d(sbase + Cfg::kQOff + (b * Cfg::NQ + i) * Cfg::kTileBytes + x * Cfg::kBoxBytes,
                       &p.tm_q, bar(Cfg::kBarQFull + b), x * Cfg::kBoxCols,
-                      p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + i * Cfg::kRows, hb.h, hb.b);
+                      tile_row0<Cfg>(p, cur, i), hb.h, hb.b);
         }
       }
       q_loaded = s + 1;
@@ -612,8 +632,7 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       return false;
     const uint32_t kd = k_lo + st * kTileStep;
     bool live = true;
-    if constexpr (Cfg::kWindow)
-      live = window_live(p, p.sc.qb_of(cs.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows, cs.block());
+    if constexpr (Cfg::kWindow) live = cs.live(p, tile);
     if (live) {
       const int i = tile;
       const int n_s = Cfg::kWindow ? ts : gs;  // S products of this tile before this one
@@ -682,8 +701,7 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       bool fresh = cp.first_step();  // first block of a unit: overwrite O
       bool live = true;
       if constexpr (Cfg::kWindow) {
-        live = window_live(p, p.sc.qb_of(cp.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows,
-                           cp.block());
+        live = cp.live(p, tile);
         if (fresh) fresh_unit = true;
         fresh = fresh_unit;  // the first block that the tile sees
         if (live) fresh_unit = false;
@@ -921,15 +939,17 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
     float m_run[2] = {-INFINITY, -INFINITY};  // running max of s*scale*log2(e), per row
     float l_run[2] = {0.0f, 0.0f};            // this thread's partial row sums
     const int row0 =  // first query row of this warp's slice (causal masking only)
-        Cfg::kCausal ? p.q0 + p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows + slice
-                     : 0;
+        Cfg::kCausal ? p.q0 + tile_row0<Cfg>(p, cur, tile) + slice : 0;
     if constexpr (Cfg::kWindow) {
+      if (cur.tile_row(tile) < 0) {  // an item of one tile, the other one
+        cur.next_segment(p);
+        continue;
+      }
       bool first = true;
       for (; cur.j < cur.j1; ++cur.j) {
-        const int kb = cur.block();
-        if (!window_live(p, row0 - slice, kb)) continue;
-        if (!softmax_step<Cfg>(p, bars, tS, tP, tO, tile, lane, g, kb, row0, first, m_run, l_run,
-                               wd))
+        if (!cur.live(p, tile)) continue;
+        if (!softmax_step<Cfg>(p, bars, tS, tP, tO, tile, lane, g, cur.block(), row0, first, m_run,
+                               l_run, wd))
           return;
         first = false;
         ++g;
@@ -961,8 +981,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
         // log-sum-exp = ln 2 * (m + log2 l), m in scaled log2 units
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int qrow = p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows +
-                           slice + gq + 8 * r;
+          const int qrow = tile_row0<Cfg>(p, cur, tile) + slice + gq + 8 * r;
           if (qrow < p.nq)
             p.lse[static_cast<size_t>(p.sc.head_of(cur.u)) * p.n + qrow] =
                 (m_run[r] + log2f(l_row[r])) * 0.6931471805599453f;
@@ -997,7 +1016,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
           if (!wait_single(bar(Cfg::kBarStage + tile), static_cast<uint32_t>(stores) & 1u, wd,
                            kSiteSoftStage))
             return;
-          const int r0 = p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows;
+          const int r0 = tile_row0<Cfg>(p, cur, tile);
           if (r0 < p.nq) {
             const HeadBatch ob = head_batch(p, cur.u);
 #pragma unroll
@@ -1058,12 +1077,15 @@ __device__ __forceinline__ void store_role(const FwdParams& p, uint8_t* smem, ui
       bool ok = true;
 #pragma unroll
       for (int tile = 0; tile < Cfg::NQ; ++tile) {
+        // (items of one tile come last, so `stores` counts both tiles' stagings while there are
+        // two)
+        if (Cfg::kWindow && tile_row0<Cfg>(p, cur, tile) < 0) break;
         if (!wait_single(bar(Cfg::kBarStage + tile), static_cast<uint32_t>(stores) & 1u, wd,
                          kSiteSoftStage)) {
           ok = false;
           break;
         }
-        const int r0 = p.sc.qb_of(cur.u) * Cfg::kRowsPerUnit + tile * Cfg::kRows;
+        const int r0 = tile_row0<Cfg>(p, cur, tile);
         if (r0 < p.nq) {
           const uint32_t stage =
               smem_addr(smem + Cfg::kQOff + (b * Cfg::NQ + tile) * Cfg::kTileBytes);

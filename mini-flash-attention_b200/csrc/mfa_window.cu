@@ -138,9 +138,14 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
   p.sinks = static_cast<int>(w.sinks);
   p.sink_blocks = static_cast<int>((w.sinks + 127) / 128);
   p.kv_group = static_cast<int>(w.heads / w.kv_heads);
-  const int64_t units = static_cast<int64_t>(p.sc.q_blocks) * p.sc.bh;
+  // Query blocks of two tiles that would fill at most half of the SMs, or of the last wave, are
+  // done tile by tile.
+  const int64_t units = static_cast<int64_t>(p.sc.q_blocks) * p.sc.bh, over = units % dev.sms;
+  const int64_t whole = Cfg::NQ == 2 && 2 * over <= dev.sms ? units - over : units;
+  const int64_t items = 2 * units - whole;
+  p.whole_units = static_cast<int>(whole);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(units < dev.sms ? units : dev.sms));
+  cfg.gridDim = dim3(static_cast<unsigned>(items < dev.sms ? items : dev.sms));
   cfg.blockDim = dim3(Cfg::kThreads);
   cfg.dynamicSmemBytes = Cfg::kSmemBytes;
   cfg.stream = stream;
