@@ -580,62 +580,71 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
 
   const int q2 = 2 * (lane & 3) + 64 * half;  // first of this thread's columns in a block
   const int gq = lane >> 2;
-  if (!Cfg::kDKV) {
-    // keys past N (last key block) and, with the mask, keys after the query row
-    if (j == p.blocks - 1) {
-      const int valid = p.n - j * Cfg::kCols;
-      if (valid < Cfg::kCols) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (8 * i + q2 + (e & 1) >= valid) sr[4 * i + e] = __float_as_uint(-INFINITY);
-      }
-    }
-    if (Cfg::kCausal) {
-      const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k > t0 (+8 for e >= 2)
-      if (j * Cfg::kCols + Cfg::kCols - 1 > row0) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
-      }
-    }
-    if constexpr (Cfg::kWindow) {
-      // keys older than the window, but for the sinks
+  if constexpr (Cfg::kWindow) {
+    // This thread's 16 columns of a row are c0 + 8 i + e; see window_bits. (Keys past N are past
+    // every query; queries past N have L2 = +inf, so their P is 0.)
+    const int res0 = row0 + gq, str0 = j * Cfg::kCols + q2;  // first resident row, streamed column
+    if constexpr (!Cfg::kDKV) {
+      // resident queries, streamed keys: as in the forward kernel
       const int key0 = j * Cfg::kCols;
-      if (key0 <= row0 + 15 - p.window && key0 + Cfg::kCols > p.sinks) {
-        const int t0 = row0 + gq - p.window - key0;  // too old when k <= t0 (+8 for e >= 2)
-        const int s0 = p.sinks - key0;
+      if (key0 + Cfg::kCols - 1 > row0 ||
+          (key0 <= row0 + 15 - p.window && key0 + Cfg::kCols > p.sinks)) {
+        const uint32_t sink_bits = window_bits(p.sinks - 1 - str0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int r = 0; r < 2; ++r) {
+          const int t = res0 + 8 * r - str0;
+          const uint32_t seen = window_bits(t) & (~window_bits(t - p.window) | sink_bits);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = 8 * i + q2 + (e & 1);
-            if (k <= t0 + 8 * (e >> 1) && k >= s0) sr[4 * i + e] = __float_as_uint(-INFINITY);
-          }
+          for (int k = 0; k < 16; ++k)
+            if (!((seen >> k) & 1u)) sr[4 * (k >> 1) + 2 * r + (k & 1)] = __float_as_uint(-INFINITY);
+        }
+      }
+    } else {
+      // resident keys, streamed queries: those from the key on, up to window - 1 after it (for a
+      // sink, all)
+      if (j == blk || ((j + 1) * Cfg::kCols > row0 + p.window && row0 + 16 > p.sinks)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int t = res0 + 8 * r - str0;
+          uint32_t seen = ~window_bits(t - 1);
+          if (res0 + 8 * r >= p.sinks) seen &= window_bits(t + p.window - 1);
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (!((seen >> k) & 1u)) sr[4 * (k >> 1) + 2 * r + (k & 1)] = __float_as_uint(-INFINITY);
+        }
       }
     }
-  } else if (Cfg::kCausal && j == blk) {
-    // diagonal block: queries (columns) before the key row score -inf
-    const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k < t0 (+8 for e >= 2)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (8 * i + q2 + (e & 1) < t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
-  }
-  if constexpr (Cfg::kDKV && Cfg::kWindow) {
-    // queries (columns) for which the key row, unless a sink, is older than the window
-    if ((j + 1) * Cfg::kCols > row0 + p.window && row0 + 16 > p.sinks) {
-      const int t0 = row0 + gq + p.window - j * Cfg::kCols;  // too old when c >= t0 (+8 ...)
-#pragma unroll
+  } else {
+    if (!Cfg::kDKV) {
+      // keys past N (last key block) and, with the mask, keys after the query row
+      if (j == p.blocks - 1) {
+        const int valid = p.n - j * Cfg::kCols;
+        if (valid < Cfg::kCols) {
+  #pragma unroll
+          for (int i = 0; i < 8; ++i)
+  #pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (8 * i + q2 + (e & 1) >= valid) sr[4 * i + e] = __float_as_uint(-INFINITY);
+        }
+      }
+      if (Cfg::kCausal) {
+        const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k > t0 (+8 for e >= 2)
+        if (j * Cfg::kCols + Cfg::kCols - 1 > row0) {
+  #pragma unroll
+          for (int i = 0; i < 8; ++i)
+  #pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
+        }
+      }
+    } else if (Cfg::kCausal && j == blk) {
+      // diagonal block: queries (columns) before the key row score -inf
+      const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k < t0 (+8 for e >= 2)
+  #pragma unroll
       for (int i = 0; i < 8; ++i)
-#pragma unroll
+  #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (8 * i + q2 + (e & 1) >= t0 + 8 * (e >> 1) && row0 + gq + 8 * (e >> 1) >= p.sinks)
-            sr[4 * i + e] = __float_as_uint(-INFINITY);
+          if (8 * i + q2 + (e & 1) < t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
     }
   }
 

@@ -83,6 +83,14 @@ struct HeadBatch {
   int h, b;
 };
 
+// A thread's 32 columns of a row of a block are 8 i + 2 q + e; bit 2 i + e of the result tells
+// whether 8 i + e <= x, i.e. (x = c - 2 q) whether the column is at most c.
+__device__ __forceinline__ uint32_t window_bits(int x) {
+  const int rest = (x & 7) + 1;
+  const int count = 2 * (x >> 3) + (rest < 2 ? rest : 2);  // columns at most c
+  return x < 0 ? 0u : count >= 32 ? 0xffffffffu : (1u << count) - 1u;
+}
+
 struct Watchdog {
   volatile int* abort;
   int* status;

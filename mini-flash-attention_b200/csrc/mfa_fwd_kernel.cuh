@@ -766,47 +766,50 @@ __device__ __forceinline__ bool softmax_step(const FwdParams& p, uint32_t bars, 
   __syncwarp();
   if (lane == 0) mbar_arrive(bar(Cfg::kBarSFree + tile));
 
-  if (j == p.sc.nkb - 1) {
-    // last key block of the sequence: keys past N score -inf
-    const int valid = p.n - j * Cfg::kKeys;
-    if (valid < Cfg::kKeys) {
-      const int q2 = 2 * (lane & 3);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (8 * i + q2 + (e & 1) >= valid) sr[4 * i + e] = __float_as_uint(-INFINITY);
-      }
-    }
-  }
-  if constexpr (Cfg::kCausal) {
-    // Keys after the query row score -inf. row0 is the first query row of this warp's 16-row
-    // slice; only blocks that reach past it need the per-element test.
+  if constexpr (Cfg::kWindow) {
+    // Only blocks that reach past the slice's first row, or hold a key too old for its last row
+    // and other keys than sinks, have masked scores (keys past N are past every row).
     const int key0 = j * Cfg::kKeys;
-    if (key0 + Cfg::kKeys - 1 > row0) {
-      const int t0 = row0 + (lane >> 2) - key0;  // row g: column c is masked when c > t0
+    const bool late = key0 + Cfg::kKeys - 1 > row0;
+    const bool old = key0 <= row0 + 15 - p.window && key0 + Cfg::kKeys > p.sinks;
+    if (late || old) {
       const int q2 = 2 * (lane & 3);
+      const uint32_t sink_bits = window_bits(p.sinks - 1 - key0 - q2);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int r = 0; r < 2; ++r) {
+        const int t = row0 + (lane >> 2) + 8 * r - key0 - q2;  // the row's own key
+        const uint32_t seen = window_bits(t) & (~window_bits(t - p.window) | sink_bits);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
+        for (int k = 0; k < 32; ++k)
+          if (!((seen >> k) & 1u)) sr[4 * (k >> 1) + 2 * r + (k & 1)] = __float_as_uint(-INFINITY);
       }
     }
-    if constexpr (Cfg::kWindow) {
-      // Keys older than the window score -inf, but for the sinks. A block is tested when its
-      // first key is too old for the slice's last row and it holds other keys than sinks.
-      if (key0 <= row0 + 15 - p.window && key0 + Cfg::kKeys > p.sinks) {
-        const int t0 = row0 + (lane >> 2) - p.window - key0;  // row g: too old when c <= t0
-        const int s0 = p.sinks - key0;                        // a sink when c < s0
+  } else {
+    if (j == p.sc.nkb - 1) {
+      // last key block of the sequence: keys past N score -inf
+      const int valid = p.n - j * Cfg::kKeys;
+      if (valid < Cfg::kKeys) {
         const int q2 = 2 * (lane & 3);
-#pragma unroll
+  #pragma unroll
         for (int i = 0; i < 16; ++i) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = 8 * i + q2 + (e & 1);
-            if (c <= t0 + 8 * (e >> 1) && c >= s0) sr[4 * i + e] = __float_as_uint(-INFINITY);
-          }
+  #pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * i + q2 + (e & 1) >= valid) sr[4 * i + e] = __float_as_uint(-INFINITY);
+        }
+      }
+    }
+    if constexpr (Cfg::kCausal) {
+      // Keys after the query row score -inf. row0 is the first query row of this warp's 16-row
+      // slice; only blocks that reach past it need the per-element test.
+      const int key0 = j * Cfg::kKeys;
+      if (key0 + Cfg::kKeys - 1 > row0) {
+        const int t0 = row0 + (lane >> 2) - key0;  // row g: column c is masked when c > t0
+        const int q2 = 2 * (lane & 3);
+  #pragma unroll
+        for (int i = 0; i < 16; ++i) {
+  #pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
         }
       }
     }
