@@ -301,15 +301,17 @@ struct WindowCursor {
   __device__ int block() const { return j < sinks ? j : j + skip; }
   // First query row of a tile of the CTA, or -1 if the item does not have it.
   __device__ int tile_row(int tile) const { return tile < tiles ? row + 128 * tile : -1; }
-  // Whether the tile sees a key of the current key block (of a tile past the last row, every
-  // block: nobody reads its result, and it keeps at least one). Two tiles take one window block
-  // more together than each of them needs: the first does not see the block of the second's
-  // diagonal, the second not the oldest block of the first.
-  __device__ bool live(const FwdParams& p, int tile) const {
-    const int r0 = tile_row(tile), kb = block();
-    if (r0 < 0) return false;
-    if (r0 >= p.nq) return true;
-    return kb * 128 <= r0 + 127 && (kb * 128 + 127 > r0 - p.window || kb < p.sink_blocks);
+  // The step of which a tile sees no key, or -1. Two tiles have one window block more together
+  // than each of them needs: the first does not see the block of the second's diagonal, the
+  // second not the oldest block of the first unless it holds sinks. (A tile past the last row
+  // takes part in every step, and nobody reads its result.)
+  __device__ int dead_step(const FwdParams& p, int tile) const {
+    if (kRowsPerUnit == 128 || tiles == 1) return -1;
+    const int diagonal = row >> 7, last = j1 - 1 + skip;  // blocks: the first tile's, the last one
+    if (tile == 0) return last > diagonal ? j1 - 1 : -1;
+    const int oldest = sinks + skip;
+    const bool seen = oldest * 128 + 127 > row + 128 - p.window || oldest < p.sink_blocks;
+    return row + 128 < p.nq && !seen ? sinks : -1;
   }
   __device__ void next_segment(const FwdParams& p) {
     item += static_cast<int>(gridDim.x);
@@ -618,7 +620,7 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
   int gs = 0, gp = 0;
   // Window variant: the tile's own steps so far (the blocks it sees; the ring is walked by all
   // of the unit's), and whether its current unit has had a P.V product.
-  [[maybe_unused]] int ts = 0, tp = 0;
+  [[maybe_unused]] int ts = 0, tp = 0, s_dead = -1, p_dead = -1;
   [[maybe_unused]] bool fresh_unit = true;
   // S_i[gs] = Q_i K_gs^T once softmax_i has pulled S_i[gs-1] into registers.
   auto issue_s = [&]() -> bool {
@@ -632,7 +634,10 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       return false;
     const uint32_t kd = k_lo + st * kTileStep;
     bool live = true;
-    if constexpr (Cfg::kWindow) live = cs.live(p, tile);
+    if constexpr (Cfg::kWindow) {
+      if (cs.first_step()) s_dead = cs.dead_step(p, tile);
+      live = cs.tile_row(tile) >= 0 && cs.j != s_dead;
+    }
     if (live) {
       const int i = tile;
       const int n_s = Cfg::kWindow ? ts : gs;  // S products of this tile before this one
@@ -701,8 +706,11 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       bool fresh = cp.first_step();  // first block of a unit: overwrite O
       bool live = true;
       if constexpr (Cfg::kWindow) {
-        live = cp.live(p, tile);
-        if (fresh) fresh_unit = true;
+        if (fresh) {
+          fresh_unit = true;
+          p_dead = cp.dead_step(p, tile);
+        }
+        live = cp.tile_row(tile) >= 0 && cp.j != p_dead;
         fresh = fresh_unit;  // the first block that the tile sees
         if (live) fresh_unit = false;
       }
@@ -949,8 +957,9 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
         continue;
       }
       bool first = true;
+      const int dead = cur.dead_step(p, tile);
       for (; cur.j < cur.j1; ++cur.j) {
-        if (!cur.live(p, tile)) continue;
+        if (cur.j == dead) continue;
         if (!softmax_step<Cfg>(p, bars, tS, tP, tO, tile, lane, g, cur.block(), row0, first, m_run,
                                l_run, wd))
           return;
