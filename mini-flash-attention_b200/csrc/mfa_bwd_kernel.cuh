@@ -894,6 +894,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kTmemSlotOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
   volatile int* ring = reinterpret_cast<volatile int*>(smem + kAbortOff + 4);
+  if (CA::kWindow && threadIdx.x == 0) grid_dependents_launch();  // the reduce kernel, which waits
   // Between the passes: true if the second pass runs (the same verdict in every thread:
   // nothing writes the flag between the two barriers).
   auto next_pass = [&]() -> bool {
@@ -921,6 +922,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     __syncwarp();
     named_bar_arrive(1, CA::kThreads);
     setmaxnreg_dec<CA::kControlRegs>();
+    if constexpr (CA::kWindow) grid_dependency_wait();
     const Watchdog wd{abort_flag, pa.status, pa.timeout_ns};
     const BwdClaims claims{ring, bars, &wd};
     if (lane == 0) bwd_load_role<CA>(pa, smem, bars, wd, claims);
@@ -936,6 +938,9 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     named_bar_sync(1, CA::kThreads);
     tc_fence_after();
     tmem = *tmem_slot;
+    // window variant: a programmatic dependent of the row pass, as the forward kernel is of the
+    // stream's previous kernel
+    if constexpr (CA::kWindow) grid_dependency_wait();
     const Watchdog wd{abort_flag, pa.status, pa.timeout_ns};
     const BwdClaims claims{ring, bars, &wd};
     if (warp < CA::kSoftmaxWarps) {
@@ -1008,15 +1013,16 @@ __global__ void __launch_bounds__(BwdConfig<true, true, kBF16, true>::kThreads, 
 }
 
 // dK and dV of the blocks whose units ran in pieces: the sum of the pieces in order, dK scaled.
-// One CTA per (block, k / v head row) pair that may have pieces, sink blocks first; 16 threads per
-// row, four columns each.
+// One CTA per 16 rows of a (block, k / v head row) pair that may have pieces, sink blocks first; 16
+// threads per row, four columns each. The pieces are read four at a time (an L2 round trip each).
 template <bool kBF16>
 __global__ void __launch_bounds__(256) mfa_bwd_reduce_kernel(const BwdParams p, uint16_t* dk,
                                                              uint16_t* dv, long long stride_b,
                                                              long long stride_h,
                                                              long long stride_n) {
   constexpr int kTile = 128 * 64;
-  const int pair = static_cast<int>(blockIdx.x);
+  grid_dependency_wait();
+  const int pair = static_cast<int>(blockIdx.x) >> 3;
   const int blk = pair / p.bh, row = pair % p.bh;
   const bool sink = blk < p.sink_blocks;
   const int span = BwdWindowCursor<BwdConfig<true, true, kBF16, true>>::span(p, blk);
@@ -1031,8 +1037,10 @@ __global__ void __launch_bounds__(256) mfa_bwd_reduce_kernel(const BwdParams p, 
   const long long base =
       static_cast<long long>(row / p.heads) * stride_b + (row % p.heads) * stride_h;
   const int col = 4 * (threadIdx.x & 15);
-  for (int r = threadIdx.x >> 4; r < 128 && blk * 128 + r < p.n; r += 16) {
+  const int r = (static_cast<int>(blockIdx.x) & 7) * 16 + (threadIdx.x >> 4);
+  if (blk * 128 + r < p.n) {
     float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+#pragma unroll 4
     for (int i = 0; i < count; ++i) {
       const float* at = p.partials + (first + static_cast<long long>(i) * p.bh) * (2 * kTile) +
                         r * 64 + col;
@@ -1077,6 +1085,10 @@ __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const 
                                                            long long stride_b, long long stride_h,
                                                            long long stride_n, int blocks,
                                                            int* counters = nullptr) {
+  // window variant: a programmatic dependent, as is the kernel after it (neither does anything in
+  // a plain launch)
+  if (threadIdx.x == 0) grid_dependents_launch();
+  grid_dependency_wait();
   // window variant: the two passes' unit counters start at zero
   if (counters != nullptr && blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
   const long long rows = static_cast<long long>(bh) * blocks * 128;  // a multiple of 4

@@ -114,6 +114,24 @@ int check_tensors(const void* const* ptrs, const char* const* names, int count, 
   return MFA_OK;
 }
 
+// A programmatic dependent launch: the kernel waits for the stream's earlier work itself
+// (griddepcontrol.wait), and its set-up may overlap that work's end.
+template <class... Params, class... Args>
+cudaError_t launch(int64_t grid, int threads, int smem, cudaStream_t stream,
+                   void (*kernel)(Params...), const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <class Cfg>
 int launch_forward(const void* q, const void* k, const void* v, void* out, float* lse,
                    const Problem& w, const host::Device& dev, cudaStream_t stream) {
@@ -144,17 +162,8 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
   const int64_t whole = Cfg::NQ == 2 && 2 * over <= dev.sms ? units - over : units;
   const int64_t items = 2 * units - whole;
   p.whole_units = static_cast<int>(whole);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items < dev.sms ? items : dev.sms));
-  cfg.blockDim = dim3(Cfg::kThreads);
-  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, window_kernel<Cfg>(), p);
+  const cudaError_t e = launch(items < dev.sms ? items : dev.sms, Cfg::kThreads, Cfg::kSmemBytes,
+                               stream, window_kernel<Cfg>(), p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "window forward launch");
 }
 
@@ -272,22 +281,23 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
     const host::Strides st = host::strides_of(w.layout, w.heads, w.n, 64);
     const int64_t need = (static_cast<int64_t>(rows) / 4 + 7) / 8;
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
-    mfa_bwd_prep_kernel<kBF16><<<static_cast<unsigned>(need < most ? need : most), 256, 0, stream>>>(
-        out, dout, lse, lse2, di, static_cast<int>(bh), static_cast<int>(w.n),
-        static_cast<int>(w.heads), st.b, st.h, st.n, static_cast<int>(blocks), counters);
+    // the three kernels wait for the stream's earlier work themselves and may be set up while it ends
+    e = launch(need < most ? need : most, 256, 0, stream, &mfa_bwd_prep_kernel<kBF16>, out, dout,
+               lse, lse2, di, static_cast<int>(bh), static_cast<int>(w.n),
+               static_cast<int>(w.heads), static_cast<long long>(st.b),
+               static_cast<long long>(st.h), static_cast<long long>(st.n),
+               static_cast<int>(blocks), counters);
     const int64_t units = kv_units > q_units ? kv_units : q_units;
-    const unsigned ctas = static_cast<unsigned>(units < dev.sms ? units : dev.sms);
-    e = cudaGetLastError();
     if (e == cudaSuccess)
-      mfa_bwd_window_kernel<kBF16><<<ctas, BwdConfig<true, true, kBF16, true>::kThreads,
-                                     window_bwd_smem<kBF16>(), stream>>>(pq, pkv);
-    if (e == cudaSuccess) e = cudaGetLastError();
+      e = launch(units < dev.sms ? units : dev.sms, BwdConfig<true, true, kBF16, true>::kThreads,
+                 window_bwd_smem<kBF16>(), stream, &mfa_bwd_window_kernel<kBF16>, pq, pkv);
     if (e == cudaSuccess && slots > 0) {
       const host::Strides kv = host::strides_of(w.layout, w.kv_heads, w.n, 64);
       const int64_t pairs = bhk * (pc.pieces_rest > 1 ? blocks : sb);
-      mfa_bwd_reduce_kernel<kBF16><<<static_cast<unsigned>(pairs), 256, 0, stream>>>(
-          pkv, static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv), kv.b, kv.h, kv.n);
-      e = cudaGetLastError();
+      e = launch(8 * pairs, 256, 0, stream, &mfa_bwd_reduce_kernel<kBF16>, pkv,
+                 static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv),
+                 static_cast<long long>(kv.b), static_cast<long long>(kv.h),
+                 static_cast<long long>(kv.n));
     }
   }
   const cudaError_t ef = cudaFreeAsync(ws, stream);

@@ -106,26 +106,11 @@ def backward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
     return dq, dk, dv
 
 
-class _WindowAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks):
-        out, lse = forward_window_lse(q, k, v, window, sinks)
-        ctx.save_for_backward(q, k, v, out, lse)
-        ctx.window, ctx.sinks = window, sinks
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = backward_window(q, k, v, out, lse, dout, ctx.window, ctx.sinks)
-        return dq, dk, dv, None, None
-
-
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
                      sinks: int = 0) -> torch.Tensor:
-    """Differentiable forward_window (D = 64 for gradients)."""
-    return _WindowAttention.apply(q, k, v, window, sinks)
+    """Differentiable forward_window (D = 64 for gradients, which can be taken once: a gradient of a
+    gradient raises)."""
+    return _load_extension().window_attention(q, k, v, int(window), int(sinks))
 
 
 def extend_block_tables(block_table: torch.Tensor, cached: torch.Tensor, added: torch.Tensor,
