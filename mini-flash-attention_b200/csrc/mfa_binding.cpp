@@ -3,6 +3,7 @@
 // allocation, scale = 1/sqrt(D), device guard and current stream), calling the C ABI of
 // include/mfa_b200.h instead of C++ launchers.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -201,6 +202,12 @@ int dtype_of(const torch::Tensor& x) {
   return x.scalar_type() == torch::kBFloat16 ? MFA_DTYPE_BF16 : MFA_DTYPE_FP16;
 }
 
+// An uninitialised tensor of the current device, without the dispatcher's share of the call (about
+// a microsecond each, which a decoding step would notice).
+torch::Tensor new_empty(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 void* current_stream() {
   return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream());
 }
@@ -211,10 +218,10 @@ std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Ten
                                                      int64_t sinks, bool with_lse) {
   check_window_inputs(q, k, v);
   const c10::cuda::CUDAGuard device_guard(q.device());
-  auto out = torch::empty_like(q);
+  auto out = new_empty(q.sizes(), q.scalar_type(), q);
   torch::Tensor lse;
   if (with_lse)
-    lse = torch::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(torch::kFloat32));
+    lse = new_empty({q.size(0), q.size(1), q.size(2)}, torch::kFloat32, q);
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
   const int rc = mfa_fwd_window(
       q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
@@ -245,9 +252,9 @@ std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Te
   TORCH_CHECK(lse.numel() == q.size(0) * q.size(1) * q.size(2),
               "lse must have one value per query row");
   const c10::cuda::CUDAGuard device_guard(q.device());
-  auto dq = torch::empty_like(q);
-  auto dk = torch::empty_like(k);
-  auto dv = torch::empty_like(v);
+  auto dq = new_empty(q.sizes(), q.scalar_type(), q);
+  auto dk = new_empty(k.sizes(), k.scalar_type(), k);
+  auto dv = new_empty(v.sizes(), v.scalar_type(), v);
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
   const int rc = mfa_bwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                 dout.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(),
@@ -334,9 +341,9 @@ std::vector<torch::Tensor> extend_block_tables(torch::Tensor block_table, torch:
   TORCH_CHECK(free_pages.dim() == 1, "free_pages must have one dimension");
   TORCH_CHECK(capacity >= 0, "capacity must not be negative");
   const c10::cuda::CUDAGuard device_guard(block_table.device());
-  auto slots = torch::empty({capacity}, block_table.options());
-  auto starts = torch::empty({batch + 1}, block_table.options());
-  auto used = torch::empty({1}, block_table.options());
+  auto slots = new_empty({capacity}, torch::kInt32, block_table);
+  auto starts = new_empty({batch + 1}, torch::kInt32, block_table);
+  auto used = new_empty({1}, torch::kInt32, block_table);
   const int rc = mfa_extend_block_tables(
       block_table.data_ptr<int>(), cached.data_ptr<int>(), added.data_ptr<int>(),
       free_pages.data_ptr<int>(), slots.data_ptr<int>(), starts.data_ptr<int>(),
@@ -403,13 +410,13 @@ torch::Tensor attend_pages(const torch::Tensor& q, const torch::Tensor& k_cache,
                 "prefix_pages must hold prefix_length tokens");
   }
   const c10::cuda::CUDAGuard device_guard(q.device());
-  auto out = torch::empty_like(q);
+  auto out = new_empty(q.sizes(), q.scalar_type(), q);
   uint64_t bytes = 0;
   int rc = mfa_paged_workspace_bytes(batch, q.size(1), k_cache.size(1),
                                      static_cast<int32_t>(q.size(2)), page_size,
                                      block_table.size(1), prefix_length, &bytes);
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
-  auto workspace = torch::empty({static_cast<int64_t>(bytes)}, q.options().dtype(torch::kUInt8));
+  auto workspace = new_empty({static_cast<int64_t>(bytes)}, torch::kUInt8, q);
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(2)));
   const int32_t d = static_cast<int32_t>(q.size(2));
   rc = prefix_pages

@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(kExtendThreads) mfa_extend_kernel(const Extend
   const long long at = static_cast<long long>(blockIdx.x) * kN + tid;
   const long long step = static_cast<long long>(gridDim.x) * kN;
   const int page_size = p.page_size;
+  if (tid == 0) grid_dependents_launch();  // the copy may be set up, and waits
   grid_dependency_wait();
   long long tokens = 0, pages = 0;  // of the chunks before
   auto saturate = [](long long x) { return static_cast<int>(x < 0x7fffffff ? x : 0x7fffffff); };
@@ -146,28 +147,46 @@ struct AppendParams {
   Div31 by_chunks, by_heads, by_page;  // d / 8, kv_heads, page_size
 };
 
-// A copy: 16 bytes of k and of v a thread, neighbouring threads along a row.
+// A copy, bound by HBM: 16 bytes of k and of v a thread and item, neighbouring threads along a row,
+// four items' loads in flight at a time.
 __global__ void __launch_bounds__(256) mfa_append_kernel(const AppendParams p) {
+  constexpr int kBatch = 4;
+  if (threadIdx.x == 0) grid_dependents_launch();
   grid_dependency_wait();
   const int chunks = p.d / 8;
   const int t0 = static_cast<int>(blockIdx.x) * p.tokens_a_block;
   const int count = p.tokens - t0 < p.tokens_a_block ? p.tokens - t0 : p.tokens_a_block;
   const int items = count * p.kv_heads * chunks;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < items; i += 256) {
-    const int row = static_cast<int>(p.by_chunks(i));
-    const int in = static_cast<int>(p.by_heads(row));
-    const int c = i - row * chunks, h = row - in * p.kv_heads, t = t0 + in;
-    const int slot = p.slots[t];
-    if (slot < 0 || slot >= p.slot_count) continue;
-    const int page = static_cast<int>(p.by_page(slot));
-    const int at = slot - page * p.page_size;
-    const uint4 x = *reinterpret_cast<const uint4*>(p.k + t * p.k_token + h * p.k_head + 8 * c);
-    const uint4 y = *reinterpret_cast<const uint4*>(p.v + t * p.v_token + h * p.v_head + 8 * c);
-    const size_t to =
-        ((static_cast<size_t>(page) * p.kv_heads + h) * p.page_size + at) * p.d + 8 * c;
-    *reinterpret_cast<uint4*>(p.k_cache + to) = x;
-    *reinterpret_cast<uint4*>(p.v_cache + to) = y;
+  for (int i0 = threadIdx.x; i0 < items; i0 += 256 * kBatch) {
+    uint4 x[kBatch], y[kBatch];
+    long long to[kBatch];
+    int slot[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + 256 * b;
+      slot[b] = i < items ? p.slots[t0 + static_cast<int>(p.by_heads(p.by_chunks(i)))] : -1;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + 256 * b;
+      to[b] = -1;
+      if (slot[b] < 0 || slot[b] >= p.slot_count) continue;
+      const int row = static_cast<int>(p.by_chunks(i));
+      const int in = static_cast<int>(p.by_heads(row));
+      const int c = 8 * (i - row * chunks), h = row - in * p.kv_heads;
+      const long long t = t0 + in;
+      const int page = static_cast<int>(p.by_page(slot[b]));
+      x[b] = *reinterpret_cast<const uint4*>(p.k + t * p.k_token + h * p.k_head + c);
+      y[b] = *reinterpret_cast<const uint4*>(p.v + t * p.v_token + h * p.v_head + c);
+      to[b] = ((static_cast<long long>(page) * p.kv_heads + h) * p.page_size + slot[b] -
+               page * p.page_size) * p.d + c;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (to[b] < 0) continue;
+      *reinterpret_cast<uint4*>(p.k_cache + to[b]) = x[b];
+      *reinterpret_cast<uint4*>(p.v_cache + to[b]) = y[b];
+    }
   }
 }
 

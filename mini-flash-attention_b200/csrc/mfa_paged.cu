@@ -393,9 +393,9 @@ extern "C" int mfa_extend_block_tables(int32_t* block_table, const int32_t* cach
   p.capacity = static_cast<int>(capacity);
   p.starts = starts;
   p.used = used;
-  // about four tokens a thread, one CTA an SM at most (each scans all requests)
-  const int64_t need = (capacity + 4 * kExtendThreads - 1) / (4 * kExtendThreads);
-  const int64_t grid = need < 1 ? 1 : need < dev.sms ? need : dev.sms;
+  // a token a thread, two CTAs an SM at most (each scans all requests)
+  const int64_t need = (capacity + kExtendThreads - 1) / kExtendThreads;
+  const int64_t grid = need < 1 ? 1 : need < 2 * dev.sms ? need : 2 * dev.sms;
   const cudaError_t e = launch(&mfa_extend_kernel, grid, kExtendThreads, 0,
                                static_cast<cudaStream_t>(stream), p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "block table launch");

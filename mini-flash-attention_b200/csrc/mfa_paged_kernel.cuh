@@ -76,16 +76,14 @@ struct PagedConfig {
   static constexpr int kBoxBytes = kKeys * 128;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
   static constexpr int kStages = 98304 / (2 * kTileBytes);
-  static constexpr int kQRowBytes = kD * 2 + 16;  // eight rows' 16-byte pieces hit all banks once
-  static constexpr int kQOff = kStages * 2 * kTileBytes;
-  // a round of the merge: eight rows by 64 columns of each warp
+  // a round of the merge: eight rows by 64 columns of each warp, or four rows by 128
   static constexpr int kMergeCols = 72;  // floats a row: float2s of four rows hit all banks once
-  static constexpr int kMergeOff = kQOff + kRows * kQRowBytes;
+  static constexpr int kMergeCols4 = 136;
+  static constexpr int kMergeOff = kStages * 2 * kTileBytes;
   static constexpr int kStatsOff = kMergeOff + kWarps * 8 * kMergeCols * 4;  // [2][kWarps][kRows]
   static constexpr int kBarOff = kStatsOff + 2 * kWarps * kRows * 4;
-  static constexpr int kBarFull = 0, kBarEmpty = kStages, kBarQFull = 2 * kStages,
-                       kBarQEmpty = 2 * kStages + 1;
-  static constexpr int kScanOff = kBarOff + (2 * kStages + 2) * 8;  // warp sums, start
+  static constexpr int kBarFull = 0, kBarEmpty = kStages;
+  static constexpr int kScanOff = kBarOff + 2 * kStages * 8;  // warp sums, start
   static constexpr int kAbortOff = kScanOff + 4 * (kWarps + 1 + 3);
   static constexpr int kSmemBytes = kAbortOff + 4 + 1024;
   static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs an SM");
@@ -115,9 +113,11 @@ __device__ __forceinline__ int cta_of_step(long long s, long long total, int cta
   return static_cast<int>(((s + 1) * ctas - 1) / total);
 }
 
-// A unit's first and last steps (query, merge, output) cost about as much as a tile of keys (with 4
-// rows and D = 64: 900 against 850 cycles), so shares count one step more than its tiles.
-constexpr int kPagedUnitSteps = 1;
+// A unit's start and end (query, merge, output) cost about as much as two tiles of keys, so shares
+// count two steps more than its tiles: 18.3 us against 20.7 with one and 18.4 with three at 100
+// requests of 1 to 17 tiles (window 1024, D = 64); 137 to 138 us in all three at 64 requests of
+// up to 256.
+constexpr int kPagedUnitSteps = 2;
 
 // A CTA's share of the steps, found by all its threads.
 struct PagedShare {
@@ -246,8 +246,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   return sh;
 }
 
-// Producer warp: the query rows of each segment, then its tiles, a box for every page that holds
-// a visible key. Lane i looks up the page of box i of a batch of tiles (32 boxes at most, of one
+// Producer warp: the tiles of the share, a box for every page that holds a visible key. Lane i looks up the page of box i of a batch of tiles (32 boxes at most, of one
 // segment); the next batch's are on their way while this one's copies are issued.
 template <class Cfg>
 __device__ __forceinline__ void paged_load_role(const PagedParams& p, const PagedShare& sh,
@@ -282,26 +281,14 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
   };
   Batch batch{0, 0, false};
   if (cur.left > 0) batch = look_up(cur);
-  int g = 0, segs = 0;
-  bool fresh = true, ok = true;  // fresh: the batch starts a segment
+  int g = 0;
+  bool ok = true;
   while (cur.left > 0 && ok) {
     PagedCursor next = cur;
     next.advance(p, batch.count);
     Batch later{0, 0, false};
     if (next.left > 0) later = look_up(next);
     const int head = cur.head(p);
-    if (fresh) {
-      if (!wait_warp(bar(Cfg::kBarQEmpty), (static_cast<uint32_t>(segs) & 1u) ^ 1u, wd,
-                     kSiteLoadQEmpty))
-        break;
-      const int rows = cur.rows(p);
-      if (lane == 0) mbar_arrive_expect_tx(bar(Cfg::kBarQFull), rows * Cfg::kD * 2);
-      __syncwarp();
-      if (lane < rows)
-        bulk_load(smem + Cfg::kQOff + lane * Cfg::kQRowBytes,
-                  p.q + (cur.query(p) + lane) * Cfg::kD, Cfg::kD * 2, bar(Cfg::kBarQFull));
-      ++segs;
-    }
     // a page outside the cache: a place outside the map, which reads as zero
     const bool bad = batch.visible && (batch.page < 0 || batch.page >= p.pages);
     if (bad) atomicCAS(p.status, 0, kStatusBadPage);
@@ -330,7 +317,6 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
       }
       ++g;
     }
-    fresh = next.t == 0;
     cur = next;
     batch = later;
   }
@@ -342,7 +328,6 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
       if (last >= 0)
         drain_wait(bar(Cfg::kBarFull + st), static_cast<uint32_t>(last / Cfg::kStages) & 1u);
     }
-    if (segs > 0) drain_wait(bar(Cfg::kBarQFull), static_cast<uint32_t>(segs - 1) & 1u);
   }
 }
 
@@ -377,7 +362,7 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
 
 // Consumer warp. Fragments: lane 4 g + q holds rows g and g + 8 of the 16 query rows and, of
 // every 8 keys (scores) or 8 columns (out), the two at 2 q. With at most 8 rows the upper eight
-// (g + 8) take part in the products only, on what the query tile holds there, and are dropped.
+// (g + 8) take part in the products only, as zeros, and are dropped.
 template <class Cfg>
 __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const PagedShare& sh,
                                                    uint8_t* smem_ptr, uint32_t bars,
@@ -399,26 +384,46 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
   const int mat = lane >> 3, mrow = lane & 7;
   const uint32_t k_row = (warp * 16 + (mat >> 1) * 8 + mrow) * 128;
   const uint32_t v_row = (warp * 16 + (mat & 1) * 8 + mrow) * 128;
-  const uint32_t q_row = smem + Cfg::kQOff + ((mat & 1) * 8 + mrow) * Cfg::kQRowBytes;
   auto chunk_off = [&](int chunk) -> uint32_t {
     return (chunk >> 3) * Cfg::kBoxBytes + (((chunk & 7) ^ mrow) << 4);
   };
 
+  // Query fragments of a unit, straight from global memory; for every segment but the first they
+  // are asked for when the one before has done its last scores, and arrive during its merge.
+  uint32_t qf[kKSteps][4];
+  auto read_query = [&](const PagedCursor& at) {
+    const int rows = at.rows(p);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const uint32_t* src =
+          reinterpret_cast<const uint32_t*>(p.q + (at.query(p) + gq + 8 * r) * D) + q;
+      const bool here = gq + 8 * r < rows;
+#pragma unroll
+      for (int kk = 0; kk < kKSteps; ++kk) {
+        qf[kk][r] = here ? src[8 * kk] : 0u;
+        qf[kk][2 + r] = here ? src[8 * kk + 4] : 0u;
+      }
+    }
+  };
+
   PagedCursor cur;
   cur.init(p, sh);
-  int g = 0, segs = 0;
-  bool ok = true, wrote = false;
+  if (cur.left > 0) {
+    read_query(cur);
+    // The share's queries are one run of memory. Its first 128 lines are brought to L2: from HBM,
+    // busy with keys, a unit's queries would take longer than the merge that hides them.
+    const size_t row = cur.query(p) * D;
+    const size_t end = static_cast<size_t>(p.batch) * p.kv_heads * p.group * D;
+    const size_t mine = row + 64 * threadIdx.x;
+    if (mine < end)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + mine));
+  }
+  int g = 0;
+  bool ok = true, wrote = false, merged = false;
   while (cur.left > 0) {
     const int seg = cur.segment();
     const int rows = cur.rows(p);
     const bool upper = rows > 8;
-    uint32_t qf[kKSteps][4];
-    if (ok) ok = wait_warp(bar(Cfg::kBarQFull), static_cast<uint32_t>(segs) & 1u, wd, kSiteMmaQ);
-#pragma unroll
-    for (int kk = 0; kk < kKSteps; ++kk) ldmatrix_x4(q_row + (2 * kk + (mat >> 1)) * 16, qf[kk]);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar(Cfg::kBarQEmpty));
-    ++segs;
     float o[D / 8][4];
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
@@ -508,9 +513,13 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
       if (lane == 0) mbar_arrive(bar(Cfg::kBarEmpty + st));
     }
 
-    // ---- the segment's end: the four warps' states to one. In a round every warp leaves eight
-    // rows by 64 columns in shared memory, and the 128 threads rescale, add and write four
-    // columns of a row each.
+    // ---- the segment's end: the four warps' states to one. In a round every warp leaves its part
+    // of some rows and columns in shared memory, and the 128 threads rescale, add and write
+    // four columns of a row each.
+    if (merged) named_bar_sync(1, 32 * Cfg::kWarps);  // the last segment's have been read
+    PagedCursor next = cur;
+    next.advance(p, seg);
+    if (next.left > 0) read_query(next);
     const bool whole = cur.t == 0 && seg == cur.span.tiles;
     const bool to_slot = p.pieces_only || !whole;
     const int unit = cur.request * p.kv_heads * p.row_tiles + cur.unit_row;
@@ -527,48 +536,62 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
         stat_l[warp * Cfg::kRows + gq + 8 * r] = l[r];
       }
     }
-    const int mine = threadIdx.x >> 4, col4 = 4 * (threadIdx.x & 15);  // of a round's sums
+    // One thread's share of a round: four columns of a row, the warps' parts `part` floats apart.
+    auto add_up = [&](int row, int col, const float* from, int part) {
+      float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if (r == 1 && !upper) break;
+      for (int w = 0; w < Cfg::kWarps; ++w) top = fmaxf(top, stat_m[w * Cfg::kRows + row]);
+      const float sub = top == -INFINITY ? 0.0f : top;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int x = 0; x < Cfg::kBoxes; ++x) {
-        if (r + x > 0) named_bar_sync(1, 32 * Cfg::kWarps);  // the round before has been read
-#pragma unroll
-        for (int d = 0; d < 8; ++d)
-          *reinterpret_cast<float2*>(merge + (warp * 8 + gq) * Cfg::kMergeCols + 8 * d + 2 * q) =
-              make_float2(o[8 * x + d][2 * r], o[8 * x + d][2 * r + 1]);
-        named_bar_sync(1, 32 * Cfg::kWarps);
-        const int row = 8 * r + mine;
-        float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < Cfg::kWarps; ++w) top = fmaxf(top, stat_m[w * Cfg::kRows + row]);
-        const float sub = top == -INFINITY ? 0.0f : top;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < Cfg::kWarps; ++w) {
-          const float f = ex2_approx(stat_m[w * Cfg::kRows + row] - sub);
-          const float4 y = *reinterpret_cast<const float4*>(
-              merge + (w * 8 + mine) * Cfg::kMergeCols + col4);
-          sum = fmaf(f, stat_l[w * Cfg::kRows + row], sum);
-          acc.x = fmaf(f, y.x, acc.x);
-          acc.y = fmaf(f, y.y, acc.y);
-          acc.z = fmaf(f, y.z, acc.z);
-          acc.w = fmaf(f, y.w, acc.w);
+      for (int w = 0; w < Cfg::kWarps; ++w) {
+        const float f = ex2_approx(stat_m[w * Cfg::kRows + row] - sub);
+        const float4 y = *reinterpret_cast<const float4*>(from + w * part);
+        sum = fmaf(f, stat_l[w * Cfg::kRows + row], sum);
+        acc.x = fmaf(f, y.x, acc.x);
+        acc.y = fmaf(f, y.y, acc.y);
+        acc.z = fmaf(f, y.z, acc.z);
+        acc.w = fmaf(f, y.w, acc.w);
+      }
+      if (row >= rows || !ok) return;
+      if (to_slot) {
+        *reinterpret_cast<float4*>(slot_at + row * D + col) = acc;
+        if (col == 0) {
+          slot_at[slot_rows * D + row] = top;
+          slot_at[slot_rows * (D + 1) + row] = sum;
         }
-        if (row < rows && ok) {
-          if (to_slot) {
-            *reinterpret_cast<float4*>(slot_at + row * D + 64 * x + col4) = acc;
-            if (x == 0 && col4 == 0) {
-              slot_at[slot_rows * D + row] = top;
-              slot_at[slot_rows * (D + 1) + row] = sum;
-            }
-          } else {
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-            *reinterpret_cast<uint2*>(out_at + row * D + 64 * x + col4) =
-                make_uint2(pack_pair<Cfg::kBF16>(acc.x * inv, acc.y * inv),
-                           pack_pair<Cfg::kBF16>(acc.z * inv, acc.w * inv));
-          }
+      } else {
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        *reinterpret_cast<uint2*>(out_at + row * D + col) =
+            make_uint2(pack_pair<Cfg::kBF16>(acc.x * inv, acc.y * inv),
+                       pack_pair<Cfg::kBF16>(acc.z * inv, acc.w * inv));
+      }
+    };
+    if (D == 128 && rows <= 4) {
+      float* to = merge + (warp * 4 + gq) * Cfg::kMergeCols4 + 2 * q;
+      if (gq < 4) {
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+          *reinterpret_cast<float2*>(to + 8 * d) = make_float2(o[d][0], o[d][1]);
+      }
+      named_bar_sync(1, 32 * Cfg::kWarps);
+      const int row = threadIdx.x >> 5, col = 4 * (threadIdx.x & 31);
+      add_up(row, col, merge + row * Cfg::kMergeCols4 + col, 4 * Cfg::kMergeCols4);
+    } else {
+      const int row8 = threadIdx.x >> 4, col4 = 4 * (threadIdx.x & 15);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (r == 1 && !upper) break;
+#pragma unroll
+        for (int x = 0; x < Cfg::kBoxes; ++x) {
+          if (r + x > 0) named_bar_sync(1, 32 * Cfg::kWarps);  // the round before has been read
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            *reinterpret_cast<float2*>(merge + (warp * 8 + gq) * Cfg::kMergeCols + 8 * d + 2 * q) =
+                make_float2(o[8 * x + d][2 * r], o[8 * x + d][2 * r + 1]);
+          named_bar_sync(1, 32 * Cfg::kWarps);
+          add_up(8 * r + row8, 64 * x + col4, merge + row8 * Cfg::kMergeCols + col4,
+                 8 * Cfg::kMergeCols);
         }
       }
     }
@@ -584,9 +607,8 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
       p.pieces[p.pieces_only ? unit : static_cast<int>(blockIdx.x)] = out;
     }
     if (!whole) wrote = true;
-    cur.advance(p, seg);
-    // the sums are read before the next segment's statistics and rounds overwrite them
-    named_bar_sync(1, 32 * Cfg::kWarps);
+    cur = next;
+    merged = true;
   }
 }
 
@@ -609,8 +631,6 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, 2)
       mbar_init(bars + 8 * (Cfg::kBarFull + s), 1);
       mbar_init(bars + 8 * (Cfg::kBarEmpty + s), Cfg::kWarps);
     }
-    mbar_init(bars + 8 * Cfg::kBarQFull, 1);
-    mbar_init(bars + 8 * Cfg::kBarQEmpty, Cfg::kWarps);
     mbar_init_fence();
   }
   // Nothing above touches global memory. Behind a prefix, the kernel before this one is the
