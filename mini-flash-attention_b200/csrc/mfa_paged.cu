@@ -180,9 +180,11 @@ struct Layout {
 Layout lay_out(const Problem& w, int64_t sms) {
   const auto whole = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   Layout l;
-  // Two CTAs an SM, but no more than there can be steps.
+  // All that are resident at once, but no more than there can be steps.
   const int64_t steps = w.units() * (most_tiles(w) + kPagedUnitSteps);
-  l.ctas = steps < 2 * sms ? steps : 2 * sms;
+  const int64_t full =
+      sms * (w.d == 64 ? PagedConfig<64, false>::kCtas : PagedConfig<128, false>::kCtas);
+  l.ctas = steps < full ? steps : full;
   const bool shared = w.prefix > 0;
   const int64_t slots = shared ? l.ctas + w.units() : 2 * l.ctas;
   const int64_t entries = shared ? w.units() : l.ctas;

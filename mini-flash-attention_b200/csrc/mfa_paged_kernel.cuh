@@ -12,11 +12,10 @@
 // 390 operations a cycle are well inside what the warp-level tensor instruction gives; tcgen05
 // would pad the rows to 64 or 128 and bring the scores through tensor memory for nothing).
 //
-// Two CTAs per SM, each of four consumer warps and one producer warp, walk a common list of steps:
+// Two or three CTAs per SM, each of four consumer warps and one producer warp, walk a common list of steps:
 // a step is one 64-key tile of one unit, a unit one (request, k / v head, 16 query rows). The
 // lengths are known to the GPU only, so every CTA sums them and takes an equal share of the
-// steps. Tiles arrive by TMA, one box a page, in a ring of 96 KB (two CTAs: 192 KB in flight on
-// an SM). In a tile each warp takes 16 keys with a running maximum of its own; at the end of a
+// steps. Tiles arrive by TMA, one box a page, in a ring of stages. In a tile each warp takes 16 keys with a running maximum of its own; at the end of a
 // unit the four warps' states meet in shared memory. What a CTA's share cuts off goes to a slot
 // of the workspace as unnormalised 32-bit sums, which the combine kernel joins in CTA order.
 #pragma once
@@ -75,7 +74,11 @@ struct PagedConfig {
   static constexpr int kBoxes = kD / 64;
   static constexpr int kBoxBytes = kKeys * 128;
   static constexpr int kTileBytes = kBoxes * kBoxBytes;
-  static constexpr int kStages = 98304 / (2 * kTileBytes);
+  // CTAs of an SM, with 192 KB of stages together. (D = 64, two against three: 18.3 and 18.0 us at
+  // 100 requests of window 1024, 69.5 and 68.1 at 100 of up to 17 thousand tokens, 27.9 and 26.0
+  // with 16 rows; D = 128 has no registers for three.)
+  static constexpr int kCtas = kD == 64 ? 3 : 2;
+  static constexpr int kStages = 196608 / kCtas / (2 * kTileBytes);
   // a round of the merge: eight rows by 64 columns of each warp, or four rows by 128
   static constexpr int kMergeCols = 72;  // floats a row: float2s of four rows hit all banks once
   static constexpr int kMergeCols4 = 136;
@@ -86,7 +89,7 @@ struct PagedConfig {
   static constexpr int kScanOff = kBarOff + 2 * kStages * 8;  // warp sums, start
   static constexpr int kAbortOff = kScanOff + 4 * (kWarps + 1 + 3);
   static constexpr int kSmemBytes = kAbortOff + 4 + 1024;
-  static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs an SM");
+  static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 // Tiles of a request of n tokens: those that hold sinks before the window, then the window's.
@@ -132,11 +135,11 @@ struct PagedShare {
 // The walk over a CTA's share, by segments (the tiles of one unit that it holds).
 struct PagedCursor {
   PagedSpan span;
-  int request, unit_row;  // unit_row: k / v head * row_tiles + row tile
-  int t;                  // next tile of the unit
-  int left;               // steps left in the share
-  int first;              // step of the unit's first tile
-  int ahead;              // length of the next request, read early
+  int request, head, row0;  // k / v head and first query row (of the head's group) of the unit
+  int t;                    // next tile of the unit
+  int left;                 // steps left in the share
+  int first;                // step of the unit's first tile
+  int ahead;                // length of the next request, read early
 
   __device__ void read_ahead(const PagedParams& p) {
     ahead = p.lengths[request + 1 < p.batch ? request + 1 : request];
@@ -144,13 +147,15 @@ struct PagedCursor {
   __device__ void init(const PagedParams& p, const PagedShare& sh) {
     left = sh.end - sh.begin;
     request = sh.request;
-    unit_row = t = first = 0;
+    head = row0 = t = first = 0;
     if (left <= 0) return;
     span.set(p, sh.length);
     read_ahead(p);
     const int in = sh.begin - sh.before;
-    unit_row = in / (span.tiles + kPagedUnitSteps);
-    t = in - unit_row * (span.tiles + kPagedUnitSteps);
+    const int unit = in / (span.tiles + kPagedUnitSteps);  // of the request
+    t = in - unit * (span.tiles + kPagedUnitSteps);
+    head = unit / p.row_tiles;
+    row0 = 16 * (unit - head * p.row_tiles);
     first = sh.begin - t;
     if (t >= span.tiles) next_unit(p);
   }
@@ -162,12 +167,14 @@ struct PagedCursor {
     if (left == 0) return;
     first += span.tiles + kPagedUnitSteps;
     t = 0;
-    if (++unit_row == p.kv_heads * p.row_tiles) {
-      unit_row = 0;
-      ++request;
-      span.set(p, ahead);
-      read_ahead(p);
-    }
+    row0 += 16;
+    if (row0 < p.group) return;
+    row0 = 0;
+    if (++head < p.kv_heads) return;
+    head = 0;
+    ++request;
+    span.set(p, ahead);
+    read_ahead(p);
   }
   __device__ void advance(const PagedParams& p, int tiles) {
     left -= tiles;
@@ -175,14 +182,15 @@ struct PagedCursor {
     if (t == span.tiles && left > 0) next_unit(p);
   }
   // Query rows of the current unit.
-  __device__ int head(const PagedParams& p) const { return unit_row / p.row_tiles; }
-  __device__ int row0(const PagedParams& p) const { return unit_row % p.row_tiles * 16; }
   __device__ int rows(const PagedParams& p) const {
-    const int r = p.group - row0(p);
+    const int r = p.group - row0;
     return r < 16 ? r : 16;
   }
   __device__ size_t query(const PagedParams& p) const {  // its first row in q and out
-    return (static_cast<size_t>(request) * p.kv_heads + head(p)) * p.group + row0(p);
+    return (static_cast<size_t>(request) * p.kv_heads + head) * p.group + row0;
+  }
+  __device__ int unit(const PagedParams& p) const {
+    return (request * p.kv_heads + head) * p.row_tiles + (row0 >> 4);
   }
 };
 
@@ -288,7 +296,7 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
     next.advance(p, batch.count);
     Batch later{0, 0, false};
     if (next.left > 0) later = look_up(next);
-    const int head = cur.head(p);
+    const int head = cur.head;
     // a page outside the cache: a place outside the map, which reads as zero
     const bool bad = batch.visible && (batch.page < 0 || batch.page >= p.pages);
     if (bad) atomicCAS(p.status, 0, kStatusBadPage);
@@ -522,7 +530,7 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
     if (next.left > 0) read_query(next);
     const bool whole = cur.t == 0 && seg == cur.span.tiles;
     const bool to_slot = p.pieces_only || !whole;
-    const int unit = cur.request * p.kv_heads * p.row_tiles + cur.unit_row;
+    const int unit = cur.unit(p);
     const int slot = p.pieces_only ? static_cast<int>(blockIdx.x) + unit
                                    : 2 * static_cast<int>(blockIdx.x) + (wrote ? 1 : 0);
     float* slot_at = p.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
@@ -613,7 +621,7 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
 }
 
 template <int D, bool kBF16>
-__global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, 2)
+__global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D, kBF16>::kCtas)
     mfa_paged_kernel(const __grid_constant__ PagedParams p) {
   using Cfg = PagedConfig<D, kBF16>;
   extern __shared__ uint8_t smem_raw[];
