@@ -204,6 +204,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   const int r1 = r0 + per < p.batch ? r0 + per : p.batch;
   int mine = 0;
   PagedSpan span;
+#pragma unroll 4
   for (int r = r0; r < r1; ++r) {
     span.set(p, p.lengths[r]);
     mine += span.tiles + kPagedUnitSteps;

@@ -73,6 +73,13 @@ def test_decode_many_requests():
     check(decode(cache, q), *cache.reference(q))
 
 
+def test_decode_very_many_requests():
+    lengths = [(13 * i) % 90 for i in range(5000)]
+    cache = Cache(lengths, 1, 128, 16, torch.bfloat16)
+    q = queries(5000, 1, 128, torch.bfloat16)
+    check(decode(cache, q), *cache.reference(q))
+
+
 def test_decode_more_units_than_ctas():
     lengths = [100 + i for i in range(90)]
     cache = Cache(lengths, 4, 64, 32, torch.float16)

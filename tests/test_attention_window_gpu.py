@@ -167,6 +167,21 @@ def test_other_stream_and_captured_step():
             assert all(torch.equal(a, b) for a, b in zip(want, result))
 
 
+def test_captured_autograd_step():
+    # the whole step in a graph (as for any operator, no eager graph of the leaves may live then)
+    q, k, v, dout = inputs(1, 4, 2, 700, 64, torch.float16)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    want_out = mfa.window_attention(*leaves, 100, 3)
+    want = torch.autograd.grad(want_out, leaves, dout)
+    want_out = want_out.detach().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mfa.window_attention(*leaves, 100, 3)
+        got = torch.autograd.grad(out, leaves, dout)
+    graph.replay()
+    assert torch.equal(out, want_out) and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_capi_bnhd_layout():
     b, h, hk, n, window, sinks = 2, 4, 2, 333, 70, 5
     q, k, v, dout = inputs(b, h, hk, n, 64, torch.bfloat16)
