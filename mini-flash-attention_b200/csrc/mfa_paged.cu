@@ -40,9 +40,14 @@ cudaError_t set_prefix() {
 
 template <int D, bool kBF16>
 cudaError_t set_paged() {
-  return cudaFuncSetAttribute(mfa_paged_kernel<D, kBF16>,
-                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              PagedConfig<D, kBF16>::kSmemBytes);
+  constexpr int kSmem = PagedConfig<D, kBF16>::kSmemBytes;
+  constexpr auto kAttr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaFuncSetAttribute(mfa_paged_kernel<D, kBF16>, kAttr, kSmem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(mfa_paged_cluster_kernel<D, kBF16>, kAttr, kSmem);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(mfa_paged_cluster_kernel<D, kBF16>,
+                             cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
 }
 
 template <bool kBF16>
@@ -87,22 +92,27 @@ int check_pointers(const Pointer (&ptrs)[kCount], int dev) {
 }
 
 // A kernel that waits for the stream's earlier work itself (griddepcontrol.wait) and may be set up
-// while that work ends.
+// while that work ends; in clusters of `cluster` CTAs.
 template <class P>
 cudaError_t launch(void (*kernel)(P), int64_t grid, int threads, int smem, cudaStream_t stream,
-                   const P& params) {
+                   const P& params, int cluster = 1) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, params);
 }
+
+constexpr int64_t kInlinePrefixBytes = 16 << 20;
 
 // The arguments of the two attentions.
 struct Problem {
@@ -126,6 +136,19 @@ struct Problem {
   int64_t tile_batch() const { return 128 / group(); }
   int64_t tiles() const { return (batch + tile_batch() - 1) / tile_batch(); }
   int tiles_a_unit() const { return d == 128 || tiles() == 1 ? 1 : 2; }
+  // A prefix that costs less to read for every request (from L2) than the launches of its own
+  // kernel and of the joining of its pieces take: it becomes the first tiles of each request.
+  bool prefix_inline() const {
+    return static_cast<double>(batch) * static_cast<double>(prefix) *
+               static_cast<double>(kv_heads * d * 4) <= kInlinePrefixBytes;
+  }
+  bool prefix_apart() const { return prefix > 0 && !prefix_inline(); }
+  int64_t prefix_tiles() const { return prefix_apart() ? 0 : (prefix + 63) / 64; }
+  // Tiles of the longest request.
+  int64_t most_tiles() const {
+    const int64_t t = (columns * page_size + 63) / 64 + prefix_tiles();
+    return t > 0 ? t : 1;
+  }
 };
 
 int check(Problem& w) {
@@ -151,8 +174,7 @@ int check(Problem& w) {
   if (w.prefix > kMost) return invalid("the prefix is too long");
   if (w.heads == 0 || w.batch == 0) return MFA_OK;
   // steps of a launch are counted in 32 bits
-  const double tiles =
-      static_cast<double>((w.columns * w.page_size + 63) / 64 + 1 + kPagedUnitSteps);
+  const double tiles = static_cast<double>(w.most_tiles() + kPagedUnitSteps);
   if (tiles * static_cast<double>(w.units()) > 0x7fffff00 ||
       static_cast<double>(w.prefix / 128 + 1) * static_cast<double>(w.kv_heads * w.tiles()) >
           0x7fffff00)
@@ -164,14 +186,9 @@ int check(Problem& w) {
   return MFA_OK;
 }
 
-// Tiles of the longest request.
-int64_t most_tiles(const Problem& w) {
-  const int64_t tiles = (w.columns * w.page_size + 63) / 64;
-  return tiles > 0 ? tiles : 1;
-}
-
 // Parts of the workspace, in floats from its start (256-byte aligned parts).
 struct Layout {
+  int cluster;          // CTAs a unit of the cluster kernel; 0: the paged and combine kernels
   int64_t ctas;         // of the paged kernel
   int64_t prefix_ctas, splits;  // of the prefix kernel
   int64_t slots, prefix_slots, pieces, bytes;
@@ -179,19 +196,27 @@ struct Layout {
 
 Layout lay_out(const Problem& w, int64_t sms) {
   const auto whole = [](int64_t floats) { return (floats + 63) / 64 * 64; };
-  Layout l;
-  // All that are resident at once, but no more than there can be steps.
-  const int64_t steps = w.units() * (most_tiles(w) + kPagedUnitSteps);
+  Layout l = {};
   const int64_t full =
       sms * (w.d == 64 ? PagedConfig<64, false>::kCtas : PagedConfig<128, false>::kCtas);
+  const int64_t most = w.most_tiles();
+  if (!w.prefix_apart() && w.units() * 8 <= full && most <= 32 * 2) {
+    l.cluster = most > 8 && w.units() * 16 <= full ? 16 : 8;
+    if (most <= 4 * l.cluster) {
+      l.ctas = w.units() * l.cluster;
+      return l;
+    }
+    l.cluster = 0;
+  }
+  // All that are resident at once, but no more than there can be steps.
+  const int64_t steps = w.units() * (most + kPagedUnitSteps);
   l.ctas = steps < full ? steps : full;
-  const bool shared = w.prefix > 0;
+  const bool shared = w.prefix_apart();
   const int64_t slots = shared ? l.ctas + w.units() : 2 * l.ctas;
   const int64_t entries = shared ? w.units() : l.ctas;
   l.slots = 0;
   l.pieces = whole(slots * paged_slot_floats(static_cast<int>(w.slot_rows()), w.d));
   l.prefix_slots = l.pieces + whole(entries * static_cast<int64_t>(sizeof(PagedPieces)) / 4);
-  l.prefix_ctas = l.splits = 0;
   int64_t end = l.prefix_slots;
   if (shared) {
     const int nq = w.tiles_a_unit();
@@ -274,7 +299,7 @@ template <int D, bool kBF16>
 int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cudaStream_t stream) {
   using Cfg = PagedConfig<D, kBF16>;
   const Layout l = lay_out(w, dev.sms);
-  const bool shared = w.prefix > 0;
+  const bool shared = w.prefix_apart();
   CombineParams cp = {};
   int rc = MFA_OK;
   if (shared) {
@@ -302,11 +327,19 @@ int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cud
   p.window = static_cast<int>(w.window);
   p.sinks = static_cast<int>(w.sinks);
   p.pieces_only = shared ? 1 : 0;
+  p.prefix_pages = x.prefix_pages;
+  p.prefix = static_cast<int>(shared ? 0 : w.prefix);
+  p.prefix_tiles = static_cast<int>(w.prefix_tiles());
   p.scale_log2 = w.scale * 1.4426950408889634f;
   p.slots = x.workspace + l.slots;
   p.pieces = reinterpret_cast<PagedPieces*>(x.workspace + l.pieces);
   p.timeout_ns = dev.timeout_ns;
   p.status = dev.status;
+  if (l.cluster > 0) {
+    const cudaError_t ec = launch(&mfa_paged_cluster_kernel<D, kBF16>, l.ctas, Cfg::kThreads,
+                                  Cfg::kSmemBytes, stream, p, l.cluster);
+    return ec == cudaSuccess ? MFA_OK : host::fail_cuda(ec, "paged attention launch");
+  }
   cudaError_t e = launch(&mfa_paged_kernel<D, kBF16>, l.ctas, Cfg::kThreads, Cfg::kSmemBytes,
                          stream, p);
   if (e != cudaSuccess) return host::fail_cuda(e, "paged attention launch");
@@ -336,8 +369,8 @@ int attend(const Arrays& x, uint64_t workspace_bytes, Problem& w, void* stream) 
                           {a.prefix_pages, "prefix_pages", 4},
                           {a.block_table, "block_table", 4},
                           {a.lengths, "lengths", 4},
-                          {a.out, "out", 16},
-                          {a.workspace, "workspace", 256}};
+                          {a.out, "out", 16}};
+  const Pointer work[] = {{a.workspace, "workspace", 256}};
   if ((rc = check_pointers(ptrs, -1)) != MFA_OK) return rc;
   if (w.pages == 0) return invalid("the cache has no pages");
   host::Device dev;
@@ -346,6 +379,9 @@ int attend(const Arrays& x, uint64_t workspace_bytes, Problem& w, void* stream) 
   const int64_t need = lay_out(w, dev.sms).bytes;
   if (workspace_bytes < static_cast<uint64_t>(need))
     return invalid("the workspace must have " + std::to_string(need) + " bytes");
+  if (need > 0 && ((rc = check_pointers(work, -1)) != MFA_OK ||
+                   (rc = check_pointers(work, dev.index)) != MFA_OK))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = w.dtype == MFA_DTYPE_BF16;
   if (w.d == 64)

@@ -56,6 +56,10 @@ struct PagedParams {
   int pages;
   int window, sinks;       // window 0: everything is visible
   int pieces_only;         // every unit goes to slots (its result meets that of a prefix)
+  // A prefix that all requests share, in the pages prefix_pages, as the first tiles of every
+  // request (0: none, or one that the prefix kernel has; window is 0 with it).
+  const int* prefix_pages;
+  int prefix, prefix_tiles;
   float scale_log2;
   float* slots;            // of min(group, 16) rows each
   PagedPieces* pieces;     // [CTA], or [unit] if pieces_only
@@ -92,22 +96,31 @@ struct PagedConfig {
   static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
-// Tiles of a request of n tokens: those that hold sinks before the window, then the window's.
+// Tiles of a request of n tokens: those of the prefix, those that hold sinks before the window,
+// then the window's.
 struct PagedSpan {
   int n, tiles, sinks, skip;
   __device__ void set(const PagedParams& p, int length) {
     const int most = p.columns << p.page_shift;  // < 2^31 (checked by the launcher)
     n = length < 0 ? 0 : length < most ? length : most;
-    const int last = n > 0 ? (n - 1) >> 6 : 0;  // an empty request has one tile, which sees nothing
+    // a request that sees nothing has one tile, in which nothing is visible
+    const int own = n > 0 ? ((n - 1) >> 6) + 1 : p.prefix_tiles == 0;
     const int w0 = p.window > 0 && n > p.window ? (n - p.window) >> 6 : 0;
     const int sb = (p.sinks >> 6) + ((p.sinks & 63) != 0);
     sinks = sb < w0 ? sb : w0;
     skip = w0 - sinks;
-    tiles = last + 1 - skip;
+    tiles = p.prefix_tiles + own - skip;
   }
-  __device__ int tile(int t) const { return t < sinks ? t : t + skip; }
-  __device__ bool visible(const PagedParams& p, int key) const {
-    return key < n && (p.window == 0 || key >= n - p.window || key < p.sinks);
+  // Tile t: whether it is of the prefix, its first key there or among the request's own, and the
+  // first key behind the last of either.
+  __device__ bool shared(const PagedParams& p, int t) const { return t < p.prefix_tiles; }
+  __device__ int key0(const PagedParams& p, int t) const {
+    const int own = t - p.prefix_tiles;
+    return 64 * (own < 0 ? t : own < sinks ? own : own + skip);
+  }
+  __device__ int end(const PagedParams& p, int t) const { return shared(p, t) ? p.prefix : n; }
+  __device__ bool visible(const PagedParams& p, int key, int end) const {
+    return key < end && (p.window == 0 || key >= n - p.window || key < p.sinks);
   }
 };
 
@@ -158,6 +171,19 @@ struct PagedCursor {
     row0 = 16 * (unit - head * p.row_tiles);
     first = sh.begin - t;
     if (t >= span.tiles) next_unit(p);
+  }
+  // CTA `rank` of the `size` that share one unit.
+  __device__ void init_unit(const PagedParams& p, int unit, int rank, int size) {
+    const int per_request = p.kv_heads * p.row_tiles;
+    request = unit / per_request;
+    const int in = unit - request * per_request;
+    head = in / p.row_tiles;
+    row0 = 16 * (in - head * p.row_tiles);
+    ahead = p.lengths[request];
+    span.set(p, ahead);
+    first = 0;
+    t = span.tiles * rank / size;
+    left = span.tiles * (rank + 1) / size - t;
   }
   __device__ int segment() const { return span.tiles - t < left ? span.tiles - t : left; }
   // Past the unit's last tile (t >= tiles).
@@ -258,7 +284,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
 // Producer warp: the tiles of the share, a box for every page that holds a visible key. Lane i looks up the page of box i of a batch of tiles (32 boxes at most, of one
 // segment); the next batch's are on their way while this one's copies are issued.
 template <class Cfg>
-__device__ __forceinline__ void paged_load_role(const PagedParams& p, const PagedShare& sh,
+__device__ __forceinline__ void paged_load_role(const PagedParams& p, PagedCursor cur,
                                                 uint32_t smem, uint32_t bars,
                                                 const Watchdog& wd) {
   const int lane = threadIdx.x & 31;
@@ -266,8 +292,6 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
   const int box_shift = p.page_shift < 6 ? p.page_shift : 6;  // rows of a box
   const int tile_shift = 6 - box_shift;                       // boxes of a tile: 1, 2 or 4
   const uint32_t box_bytes = 128u << box_shift;
-  PagedCursor cur;
-  cur.init(p, sh);
   struct Batch {
     int count;     // tiles
     int page;      // this lane's page, as the table has it
@@ -277,15 +301,16 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
     Batch b;
     const int most = 32 >> tile_shift, seg = at.segment();
     b.count = seg < most ? seg : most;
-    const int i = lane >> tile_shift;
-    const int key0 = at.span.tile(at.t + i) * Cfg::kKeys +
-                     ((lane & ((1 << tile_shift) - 1)) << box_shift);
-    b.visible = i < b.count && key0 < at.span.n &&
+    const int i = lane >> tile_shift, t = at.t + i;
+    const int key0 = at.span.key0(p, t) + ((lane & ((1 << tile_shift) - 1)) << box_shift);
+    b.visible = i < b.count && key0 < at.span.end(p, t) &&
                 (p.window == 0 || key0 + (1 << box_shift) > at.span.n - p.window ||
                  key0 < p.sinks);
     b.page = 0;
-    if (b.visible)
-      b.page = p.block_table[static_cast<size_t>(at.request) * p.columns + (key0 >> p.page_shift)];
+    const int* table = at.span.shared(p, t)
+                           ? p.prefix_pages
+                           : p.block_table + static_cast<size_t>(at.request) * p.columns;
+    if (b.visible) b.page = table[key0 >> p.page_shift];
     return b;
   };
   Batch batch{0, 0, false};
@@ -312,7 +337,7 @@ __device__ __forceinline__ void paged_load_role(const PagedParams& p, const Page
         mbar_arrive_expect_tx(bar(Cfg::kBarFull + st),
                               2 * Cfg::kBoxes * box_bytes * __popc(here));
       __syncwarp();
-      const int row0 = (cur.span.tile(cur.t + i) * Cfg::kKeys) & ((1 << p.page_shift) - 1);
+      const int row0 = cur.span.key0(p, cur.t + i) & ((1 << p.page_shift) - 1);
       const uint32_t k_dst = smem + st * 2 * Cfg::kTileBytes, v_dst = k_dst + Cfg::kTileBytes;
       for (int j = 0; j < 1 << tile_shift; ++j) {
         const int pg = __shfl_sync(0xffffffffu, page, (i << tile_shift) + j);
@@ -372,10 +397,11 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
 // Consumer warp. Fragments: lane 4 g + q holds rows g and g + 8 of the 16 query rows and, of
 // every 8 keys (scores) or 8 columns (out), the two at 2 q. With at most 8 rows the upper eight
 // (g + 8) take part in the products only, as zeros, and are dropped.
-template <class Cfg>
-__device__ __forceinline__ void paged_consume_role(const PagedParams& p, const PagedShare& sh,
-                                                   uint8_t* smem_ptr, uint32_t bars,
-                                                   const Watchdog& wd) {
+// kCluster: the share is a part of one unit; its sums stay in shared memory, where the ring was.
+template <class Cfg, bool kCluster>
+__device__ __forceinline__ void paged_consume_role(const PagedParams& p, PagedCursor cur,
+                                                   const PagedShare& sh, uint8_t* smem_ptr,
+                                                   uint32_t bars, const Watchdog& wd) {
   constexpr int D = Cfg::kD;
   constexpr int kKSteps = D / 16;
   constexpr float kRescaleThreshold = 8.0f;  // as in the forward kernel
@@ -415,8 +441,6 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
     }
   };
 
-  PagedCursor cur;
-  cur.init(p, sh);
   if (cur.left > 0) {
     read_query(cur);
     // The share's queries are one run of memory. Its first 128 lines are brought to L2: from HBM,
@@ -459,16 +483,16 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
       }
       // Keys that are not visible, and rows of the tile that were never loaded: their scores
       // become -inf whatever they are, and their v rows 0 (0 * NaN would not be 0).
-      const int key0 = cur.span.tile(cur.t + i) * Cfg::kKeys;
+      const int key0 = cur.span.key0(p, cur.t + i), end = cur.span.end(p, cur.t + i);
       uint32_t keep[2] = {0xffffffffu, 0xffffffffu};  // v rows 2 q, 2 q + 1 (+ 8 for the second)
-      const bool edge = key0 + Cfg::kKeys > cur.span.n ||
+      const bool edge = key0 + Cfg::kKeys > end ||
                         (p.window > 0 && key0 < cur.span.n - p.window &&
                          key0 + Cfg::kKeys > p.sinks);
       if (edge) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int key = key0 + warp * 16 + 8 * h + 2 * q;
-          const bool a = cur.span.visible(p, key), b = cur.span.visible(p, key + 1);
+          const bool a = cur.span.visible(p, key, end), b = cur.span.visible(p, key + 1, end);
           keep[h] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
           if (!a) s[h][0] = s[h][2] = -INFINITY;
           if (!b) s[h][1] = s[h][3] = -INFINITY;
@@ -530,11 +554,13 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
     next.advance(p, seg);
     if (next.left > 0) read_query(next);
     const bool whole = cur.t == 0 && seg == cur.span.tiles;
-    const bool to_slot = p.pieces_only || !whole;
+    const bool to_slot = kCluster || p.pieces_only || !whole;
     const int unit = cur.unit(p);
     const int slot = p.pieces_only ? static_cast<int>(blockIdx.x) + unit
                                    : 2 * static_cast<int>(blockIdx.x) + (wrote ? 1 : 0);
-    float* slot_at = p.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
+    float* slot_at = kCluster
+                         ? reinterpret_cast<float*>(smem_ptr)
+                         : p.slots + static_cast<size_t>(slot) * paged_slot_floats(slot_rows, D);
     uint16_t* out_at = p.out + cur.query(p) * D;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -604,7 +630,7 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
         }
       }
     }
-    if (threadIdx.x == 0 && to_slot && cur.t == 0) {
+    if (!kCluster && threadIdx.x == 0 && to_slot && cur.t == 0) {
       // the unit starts here: its pieces run to the CTA of its last tile (said also when
       // unwinding: the combine kernel reads it in any case)
       const int last = cta_of_step(cur.first + cur.span.tiles - 1, sh.total, sh.ctas);
@@ -621,6 +647,20 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, const P
   }
 }
 
+// Barriers of a CTA, by one thread, before any of them is used.
+template <class Cfg>
+__device__ __forceinline__ void paged_set_up(const PagedParams& p, uint32_t bars,
+                                             volatile int* abort_flag) {
+  tma_prefetch_desc(&p.tm_k);
+  tma_prefetch_desc(&p.tm_v);
+  *abort_flag = 0;
+  for (int s = 0; s < Cfg::kStages; ++s) {
+    mbar_init(bars + 8 * (Cfg::kBarFull + s), 1);
+    mbar_init(bars + 8 * (Cfg::kBarEmpty + s), Cfg::kWarps);
+  }
+  mbar_init_fence();
+}
+
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D, kBF16>::kCtas)
     mfa_paged_kernel(const __grid_constant__ PagedParams p) {
@@ -630,32 +670,98 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const uint32_t bars = smem_addr(smem + Cfg::kBarOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kAbortOff);
-  // the combine kernel may be scheduled; it waits for this grid before it reads
-  if (threadIdx.x == 0) grid_dependents_launch();
   if (threadIdx.x == 0) {
-    tma_prefetch_desc(&p.tm_k);
-    tma_prefetch_desc(&p.tm_v);
-    *abort_flag = 0;
-    for (int s = 0; s < Cfg::kStages; ++s) {
-      mbar_init(bars + 8 * (Cfg::kBarFull + s), 1);
-      mbar_init(bars + 8 * (Cfg::kBarEmpty + s), Cfg::kWarps);
-    }
-    mbar_init_fence();
+    // the combine kernel may be scheduled; it waits for this grid before it reads
+    grid_dependents_launch();
+    paged_set_up<Cfg>(p, bars, abort_flag);
   }
-  // Nothing above touches global memory. Behind a prefix, the kernel before this one is the
-  // prefix's, whose results this one does not read, and it lets this one start only when all
-  // earlier work is done; so it waits for the prefix at its end instead (the combine kernel
-  // waits for this grid alone) and starts on every SM that the prefix has left.
+  // Nothing above touches global memory. Behind a prefix kernel, whose results this one does not
+  // read, and which lets this one start only when all earlier work is done, it waits at its
+  // end instead (the combine kernel waits for this grid alone) and starts on every SM that the
+  // prefix kernel has left.
   if (!p.pieces_only) grid_dependency_wait();
   const PagedShare sh = paged_share<Cfg>(p, reinterpret_cast<int*>(smem + Cfg::kScanOff));
   // no piece to combine, unless a consumer below says so (the same thread writes that)
   if (threadIdx.x == 0 && !p.pieces_only) p.pieces[blockIdx.x].count = 0;
   const Watchdog wd{abort_flag, p.status, p.timeout_ns};
+  PagedCursor cur;
+  cur.init(p, sh);
   if (threadIdx.x < 32 * Cfg::kWarps)
-    paged_consume_role<Cfg>(p, sh, smem, bars, wd);
+    paged_consume_role<Cfg, false>(p, cur, sh, smem, bars, wd);
   else
-    paged_load_role<Cfg>(p, sh, smem_addr(smem), bars, wd);
+    paged_load_role<Cfg>(p, cur, smem_addr(smem), bars, wd);
   if (p.pieces_only) grid_dependency_wait();
+}
+
+// Few units of few tiles: a cluster of CTAs a unit, which share its tiles and add their sums up in
+// one another's shared memory. One launch, no scan over the requests and no workspace; with
+// 16 CTAs a unit and one request of 1000 tokens (8 units of 16 tiles) @@ us against @@ for the
+// kernels above.
+template <int D, bool kBF16>
+__global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D, kBF16>::kCtas)
+    mfa_paged_cluster_kernel(const __grid_constant__ PagedParams p) {
+  using Cfg = PagedConfig<D, kBF16>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t bars = smem_addr(smem + Cfg::kBarOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Cfg::kAbortOff);
+  if (threadIdx.x == 0) {
+    grid_dependents_launch();
+    paged_set_up<Cfg>(p, bars, abort_flag);
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  const int size = cluster_size(), rank = cluster_rank();
+  const Watchdog wd{abort_flag, p.status, p.timeout_ns};
+  PagedCursor cur;
+  cur.init_unit(p, static_cast<int>(blockIdx.x) / size, rank, size);
+  const int slot_rows = p.group < Cfg::kRows ? p.group : Cfg::kRows;
+  float* sums = reinterpret_cast<float*>(smem);
+  float* tops = sums + slot_rows * D;
+  if (cur.left == 0) {  // no tile for this CTA
+    if (threadIdx.x < slot_rows) {
+      tops[threadIdx.x] = -INFINITY;
+      tops[slot_rows + threadIdx.x] = 0.0f;
+    }
+  } else if (threadIdx.x < 32 * Cfg::kWarps) {
+    paged_consume_role<Cfg, true>(p, cur, PagedShare{}, smem, bars, wd);
+  } else {
+    paged_load_role<Cfg>(p, cur, smem_addr(smem), bars, wd);
+  }
+  __syncwarp();
+  cluster_sync();
+  // The CTAs take the unit's float4s in turn. (A CTA that is unwinding takes part: its sums are
+  // not written, and the status word says so.)
+  const int rows = cur.rows(p);
+  const uint32_t base = smem_addr(sums), stats = smem_addr(tops);
+  for (int i = rank + size * static_cast<int>(threadIdx.x); i < rows * (D / 4);
+       i += size * Cfg::kThreads) {
+    const int row = i / (D / 4), col = 4 * (i % (D / 4));
+    float m = -INFINITY;
+    for (int c = 0; c < size; ++c) m = fmaxf(m, cluster_load(stats + 4 * row, c));
+    const float sub = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int c = 0; c < size; ++c) {
+      const float w = ex2_approx(cluster_load(stats + 4 * row, c) - sub);
+      const float pl = cluster_load(stats + 4 * (slot_rows + row), c);
+      const float4 x = cluster_load4(base + 4 * (row * D + col), c);
+      if (w > 0.0f) {
+        l = fmaf(pl, w, l);
+        acc.x = fmaf(x.x, w, acc.x);
+        acc.y = fmaf(x.y, w, acc.y);
+        acc.z = fmaf(x.z, w, acc.z);
+        acc.w = fmaf(x.w, w, acc.w);
+      }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    *reinterpret_cast<uint2*>(p.out + (cur.query(p) + row) * D + col) =
+        make_uint2(pack_pair<kBF16>(acc.x * inv, acc.y * inv),
+                   pack_pair<kBF16>(acc.z * inv, acc.w * inv));
+  }
+  cluster_sync();  // nobody leaves while its sums may be read
 }
 
 // ---------------------------------------------------------------- combine

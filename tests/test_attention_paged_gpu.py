@@ -32,12 +32,22 @@ LENGTHS = {
 }
 
 
+# A table for long requests goes to the kernels that cut the work into equal shares, a narrow one
+# and few requests to the one that gives a cluster of CTAs to a head of a request.
+WIDE = pytest.mark.parametrize("wide", [False, True], ids=["narrow", "wide"])
+
+
+def columns(lengths, page, wide):
+    return max(1, *(-(-n // page) for n in lengths), 5000 // page if wide else 1)
+
+
+@WIDE
 @pytest.mark.parametrize("lengths", LENGTHS.values(), ids=LENGTHS.keys())
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
-def test_decode(lengths, page, d, dtype):
-    cache = Cache(lengths, 2, d, page, dtype, seed=page + d)
+def test_decode(lengths, page, d, dtype, wide):
+    cache = Cache(lengths, 2, d, page, dtype, columns=columns(lengths, page, wide), seed=page + d)
     q = queries(len(lengths), 6, d, dtype)
     check(decode(cache, q), *cache.reference(q))
 
@@ -48,9 +58,11 @@ def test_decode(lengths, page, d, dtype):
                                           (900, 1000), (10000, 3), (63, 17)])
 @pytest.mark.parametrize("page,d,dtype", [(16, 64, torch.float16), (64, 128, torch.bfloat16),
                                           (256, 64, torch.bfloat16), (16, 128, torch.float16)])
-def test_decode_window(window, sinks, page, d, dtype):
+@WIDE
+def test_decode_window(window, sinks, page, d, dtype, wide):
     lengths = [1, 64, 100, 129, 0, 1000, 1537]
-    cache = Cache(lengths, 2, d, page, dtype, window=window, sinks=sinks, seed=window)
+    cache = Cache(lengths, 2, d, page, dtype, window=window, sinks=sinks, seed=window,
+                  columns=columns(lengths, page, wide))
     q = queries(len(lengths), 8, d, dtype)
     check(decode(cache, q, window, sinks), *cache.reference(q))
 
@@ -58,9 +70,11 @@ def test_decode_window(window, sinks, page, d, dtype):
 @pytest.mark.parametrize("kv_heads,group", [(1, 1), (8, 1), (3, 2), (1, 7), (2, 16), (1, 17), (2, 33),
                                             (1, 128)])
 @pytest.mark.parametrize("d", [64, 128])
-def test_decode_heads(kv_heads, group, d):
+@WIDE
+def test_decode_heads(kv_heads, group, d, wide):
     lengths = [200, 1, 333]
-    cache = Cache(lengths, kv_heads, d, 32, torch.bfloat16, seed=group)
+    cache = Cache(lengths, kv_heads, d, 32, torch.bfloat16, seed=group,
+                  columns=columns(lengths, 32, wide))
     q = queries(3, kv_heads * group, d, torch.bfloat16)
     check(decode(cache, q), *cache.reference(q))
 
@@ -106,17 +120,36 @@ def test_decode_large_scores_and_infinite_keys_out_of_sight():
 
 
 # --------------------------------------------------------------------------- shared prefix
-@pytest.mark.parametrize("prefix", [1, 16, 127, 128, 129, 1000])
+def behind_prefix(cache, q):
+    k, v, table, own = cache.tensors()
+    return mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), cache.prefix, table, own)
+
+
+# few bytes of prefix, which become each request's first tiles
+@WIDE
+@pytest.mark.parametrize("prefix", [1, 16, 63, 64, 65, 1000])
 @pytest.mark.parametrize("page", [16, 64, 256])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
-def test_prefix(prefix, page, d, dtype):
+def test_prefix(prefix, page, d, dtype, wide):
     lengths = [0, 1, 65, 200, 17]
-    cache = Cache(lengths, 2, d, page, dtype, prefix=prefix, seed=prefix)
+    cache = Cache(lengths, 2, d, page, dtype, prefix=prefix, seed=prefix,
+                  columns=columns(lengths, page, wide))
     q = queries(5, 6, d, dtype)
-    k, v, table, own = cache.tensors()
-    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), prefix, table, own)
-    check(out, *cache.reference(q))
+    check(behind_prefix(cache, q), *cache.reference(q))
+
+
+# more than 16 MB read by all requests together: the prefix has a kernel of its own
+@pytest.mark.parametrize("prefix,batch", [(17, 1100), (127, 140), (128, 140), (129, 140), (500, 140)])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
+def test_prefix_apart(prefix, batch, page, d, dtype):
+    batch = batch * 128 // d
+    lengths = [(7 * i) % 70 for i in range(batch)]
+    cache = Cache(lengths, 2, d, page, dtype, prefix=prefix, seed=prefix)
+    q = queries(batch, 6, d, dtype)
+    check(behind_prefix(cache, q), *cache.reference(q))
 
 
 # one tile of query rows, a tile and one row, several tiles, groups that do not divide a tile
@@ -124,13 +157,13 @@ def test_prefix(prefix, page, d, dtype):
                                                   (100, 1, 5), (3, 1, 128), (300, 2, 1),
                                                   (20, 1, 33)])
 @pytest.mark.parametrize("d", [64, 128])
-def test_prefix_rows(batch, kv_heads, group, d):
+@pytest.mark.parametrize("long", [False, True])
+def test_prefix_rows(batch, kv_heads, group, d, long):
     lengths = [(11 * i) % 30 for i in range(batch)]
-    cache = Cache(lengths, kv_heads, d, 32, torch.bfloat16, prefix=700, seed=batch)
+    prefix = 5_000_000 // (batch * kv_heads * d) + 100 if long else 70
+    cache = Cache(lengths, kv_heads, d, 32, torch.bfloat16, prefix=prefix, seed=batch)
     q = queries(batch, kv_heads * group, d, torch.bfloat16)
-    k, v, table, own = cache.tensors()
-    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), 700, table, own)
-    check(out, *cache.reference(q))
+    check(behind_prefix(cache, q), *cache.reference(q))
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -139,9 +172,7 @@ def test_prefix_several_units_a_cta(d):
     lengths = [(5 * i) % 50 for i in range(320)]
     cache = Cache(lengths, 4, d, 64, torch.bfloat16, prefix=1100)
     q = queries(320, 4 * 31, d, torch.bfloat16)
-    k, v, table, own = cache.tensors()
-    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), 1100, table, own)
-    check(out, *cache.reference(q))
+    check(behind_prefix(cache, q), *cache.reference(q))
 
 
 @pytest.mark.parametrize("batch,d,page", [(40, 128, 128), (150, 128, 16), (150, 64, 256)])
@@ -150,18 +181,14 @@ def test_prefix_past_the_l2(batch, d, page):
     prefix = 32768 * 128 // d - 5
     cache = Cache([i % 3 for i in range(batch)], 8, d, page, torch.float16, prefix=prefix)
     q = queries(batch, 64, d, torch.float16)
-    k, v, table, own = cache.tensors()
-    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), prefix, table, own)
-    check(out, *cache.reference(q))
+    check(behind_prefix(cache, q), *cache.reference(q))
 
 
 def test_prefix_long_and_none():
     lengths = [5, 300]
     cache = Cache(lengths, 8, 64, 64, torch.float16, prefix=20000)
     q = queries(2, 8, 64, torch.float16)
-    k, v, table, own = cache.tensors()
-    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), 20000, table, own)
-    check(out, *cache.reference(q))
+    check(behind_prefix(cache, q), *cache.reference(q))
     cache = Cache(lengths, 8, 64, 64, torch.float16)
     k, v, table, own = cache.tensors()
     out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), 0, table, own)
@@ -172,9 +199,10 @@ def test_prefix_long_and_none():
 def test_prefix_without_own_tokens():
     cache = Cache([0, 0, 0], 2, 64, 16, torch.bfloat16, prefix=333, columns=0)
     q = queries(3, 4, 64, torch.bfloat16)
-    k, v, table, own = cache.tensors()
-    out = mfa.shared_prefix_attention(q.cuda(), k, v, cache.pages(), 333, table, own)
-    check(out, *cache.reference(q))
+    check(behind_prefix(cache, q), *cache.reference(q))
+    cache = Cache([0] * 200, 2, 64, 16, torch.bfloat16, prefix=333, columns=0)
+    q = queries(200, 4, 64, torch.bfloat16)
+    check(behind_prefix(cache, q), *cache.reference(q))
 
 
 # ----------------------------------------------------------------------------- any caller
@@ -185,10 +213,17 @@ def test_same_result_again_on_streams_and_in_graphs():
     k, v, table, own = cache.tensors()
     pages = cache.pages()
 
+    wide = torch.cat((table, torch.full((4, 200), -1, dtype=torch.int32, device="cuda")), 1)
+    many = Cache([5] * 300, 2, 64, 16, torch.float16, prefix=500)  # its prefix has its own kernel
+    big, big_q = many.tensors(), queries(300, 8, 64, torch.float16).cuda()
+    big_pages = many.pages()
+
     def calls():
         return (mfa.paged_attention(q, k, v, table, own),
-                mfa.paged_attention(q, k, v, table, own, 1, 0),
-                mfa.shared_prefix_attention(q, k, v, pages, 500, table, own))
+                mfa.paged_attention(q, k, v, wide, own),
+                mfa.paged_attention(q, k, v, wide, own, 1, 0),
+                mfa.shared_prefix_attention(q, k, v, pages, 500, table, own),
+                mfa.shared_prefix_attention(big_q, *big[:2], big_pages, 500, *big[2:]))
 
     want = calls()
     assert all(torch.equal(a, b) for a, b in zip(want, calls()))
@@ -310,6 +345,8 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="D=64 and D=128"):
         mfa.paged_attention(x[0, :, :1], x, x, table[:1], own[:1])
     # the workspace of the C entry is checked
+    cache = Cache([40, 5], 2, 64, 16, torch.float16, columns=300)
+    k, v, table, own = cache.tensors()
     need = capi.paged_workspace_bytes(2, 4, 2, 64, 16, table.shape[1])
     work = torch.empty((need,), dtype=torch.uint8, device="cuda")
     out = torch.empty_like(q)
@@ -318,5 +355,13 @@ def test_refusals():
     with pytest.raises(capi.MfaError, match="the workspace must have"):
         capi.paged_attention(*ptrs, need - 1, *common)
     capi.paged_attention(*ptrs, need, *common, stream=torch.cuda.current_stream().cuda_stream)
-    cache.shared = [x[:0] for x in cache.shared]  # its reference without the prefix
+    torch.cuda.synchronize()
+    check(out, *cache.reference(q.cpu()))
+    # a call that takes none needs none
+    assert capi.paged_workspace_bytes(2, 4, 2, 64, 16, 3) == 0
+    ptrs[-1] = 0
+    narrow = table[:, :3].contiguous()
+    ptrs[3] = narrow.data_ptr()
+    capi.paged_attention(*ptrs, 0, 2, 4, 2, 64, k.shape[0], 16, 3, 0.125,
+                         stream=torch.cuda.current_stream().cuda_stream)
     check(out, *cache.reference(q.cpu()))
