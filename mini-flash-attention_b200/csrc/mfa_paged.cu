@@ -112,7 +112,7 @@ cudaError_t launch(void (*kernel)(P), int64_t grid, int threads, int smem, cudaS
   return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 
-constexpr int64_t kInlinePrefixBytes = 16 << 20;
+constexpr int64_t kInlinePrefixBytes = 64 << 20;
 
 // The arguments of the two attentions.
 struct Problem {
@@ -136,11 +136,14 @@ struct Problem {
   int64_t tile_batch() const { return 128 / group(); }
   int64_t tiles() const { return (batch + tile_batch() - 1) / tile_batch(); }
   int tiles_a_unit() const { return d == 128 || tiles() == 1 ? 1 : 2; }
-  // A prefix that costs less to read for every request (from L2) than the launches of its own
-  // kernel and of the joining of its pieces take: it becomes the first tiles of each request.
+  // A prefix that costs less to read for every request (from L2) than its own kernel and the
+  // joining of its pieces: it becomes the first tiles of each request. (Of 64 requests, 8 heads of
+  // 128: 67 MB 16.7 us either way, 134 MB 21.6 us inline and 17.2 apart; of 4 requests, 66 MB 13.3
+  // and 16.3, 16 MB 7.8 and 10.5; of 200 requests, 2 heads of 64: 52 MB 12.9 and 14.7, 102 MB 17.7
+  // and 15.7.)
   bool prefix_inline() const {
     return static_cast<double>(batch) * static_cast<double>(prefix) *
-               static_cast<double>(kv_heads * d * 4) <= kInlinePrefixBytes;
+               static_cast<double>(kv_heads * row_tiles() * d * 4) <= kInlinePrefixBytes;
   }
   bool prefix_apart() const { return prefix > 0 && !prefix_inline(); }
   int64_t prefix_tiles() const { return prefix_apart() ? 0 : (prefix + 63) / 64; }
@@ -200,13 +203,17 @@ Layout lay_out(const Problem& w, int64_t sms) {
   const int64_t full =
       sms * (w.d == 64 ? PagedConfig<64, false>::kCtas : PagedConfig<128, false>::kCtas);
   const int64_t most = w.most_tiles();
-  if (!w.prefix_apart() && w.units() * 8 <= full && most <= 32 * 2) {
-    l.cluster = most > 8 && w.units() * 16 <= full ? 16 : 8;
-    if (most <= 4 * l.cluster) {
-      l.ctas = w.units() * l.cluster;
+  if (!w.prefix_apart() && w.units() <= full) {
+    // CTAs a unit: as many as can be resident, up to 16, but two tiles each at least (at 16 tiles
+    // 8 CTAs measured 5.7 us and 16 6.0, at 2 tiles one 4.6 and two 4.9); if one would have
+    // more than eight tiles, the work is better cut evenly (see the cluster kernel).
+    int size = 1;
+    while (size < 16 && w.units() * size * 2 <= full && size * 4 <= most) size *= 2;
+    if (most <= 8 * size) {
+      l.cluster = size;
+      l.ctas = w.units() * size;
       return l;
     }
-    l.cluster = 0;
   }
   // All that are resident at once, but no more than there can be steps.
   const int64_t steps = w.units() * (most + kPagedUnitSteps);

@@ -91,7 +91,7 @@ struct PagedConfig {
   static constexpr int kBarOff = kStatsOff + 2 * kWarps * kRows * 4;
   static constexpr int kBarFull = 0, kBarEmpty = kStages;
   static constexpr int kScanOff = kBarOff + 2 * kStages * 8;  // warp sums, start
-  static constexpr int kAbortOff = kScanOff + 4 * (kWarps + 1 + 3);
+  static constexpr int kAbortOff = kScanOff + 4 * (kWarps + 1 + 3 + kWarps + 1);
   static constexpr int kSmemBytes = kAbortOff + 4 + 1024;
   static_assert(kCtas * (kSmemBytes + 1024) <= 228 * 1024, "shared memory of an SM");
 };
@@ -143,6 +143,7 @@ struct PagedShare {
   int request;  // of step `begin`
   int length;   // its tokens
   int before;   // steps of the requests before it
+  bool whole;   // CTA c has unit c instead, and nothing is cut
 };
 
 // The walk over a CTA's share, by segments (the tiles of one unit that it holds).
@@ -158,6 +159,10 @@ struct PagedCursor {
     ahead = p.lengths[request + 1 < p.batch ? request + 1 : request];
   }
   __device__ void init(const PagedParams& p, const PagedShare& sh) {
+    if (sh.whole && static_cast<int>(blockIdx.x) < sh.ctas) {
+      init_unit(p, static_cast<int>(blockIdx.x), 0, 1);
+      return;
+    }
     left = sh.end - sh.begin;
     request = sh.request;
     head = row0 = t = first = 0;
@@ -228,20 +233,26 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   const int per = (p.batch + Cfg::kThreads - 1) / Cfg::kThreads;
   const int r0 = tid * per < p.batch ? tid * per : p.batch;
   const int r1 = r0 + per < p.batch ? r0 + per : p.batch;
-  int mine = 0;
+  int mine = 0, most = 0;
   PagedSpan span;
 #pragma unroll 4
   for (int r = r0; r < r1; ++r) {
     span.set(p, p.lengths[r]);
     mine += span.tiles + kPagedUnitSteps;
+    most = max(most, span.tiles + kPagedUnitSteps);
   }
+  most = __reduce_max_sync(0xffffffffu, most);
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
-  if (lane == 31) scan[warp] = upto;
+  int* tops = scan + Cfg::kWarps + 4;
+  if (lane == 31) {
+    scan[warp] = upto;
+    tops[warp] = most;
+  }
   __syncthreads();
   int steps = 0, before = upto - mine;
 #pragma unroll
@@ -249,6 +260,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
     const int x = scan[w];
     if (w < warp) before += x;
     steps += x;
+    most = max(most, tops[w]);
   }
   const int heads = p.kv_heads * p.row_tiles;
   PagedShare sh;
@@ -256,6 +268,13 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   sh.ctas = static_cast<int>(gridDim.x) < sh.total ? static_cast<int>(gridDim.x) : sh.total;
   const int c = static_cast<int>(blockIdx.x);
   sh.begin = sh.end = 0;
+  // A CTA for each unit, if there are enough and the longest is no more than a quarter over an
+  // equal share: cutting nearly every unit in two costs more than that.
+  sh.whole = p.batch * heads <= sh.ctas && 4LL * most * sh.ctas <= 5LL * sh.total;
+  if (sh.whole) {
+    sh.ctas = p.batch * heads;
+    return sh;
+  }
   if (c < sh.ctas) {
     sh.begin = static_cast<int>(static_cast<long long>(c) * sh.total / sh.ctas);
     sh.end = static_cast<int>(static_cast<long long>(c + 1) * sh.total / sh.ctas);
@@ -633,7 +652,9 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, PagedCu
     if (!kCluster && threadIdx.x == 0 && to_slot && cur.t == 0) {
       // the unit starts here: its pieces run to the CTA of its last tile (said also when
       // unwinding: the combine kernel reads it in any case)
-      const int last = cta_of_step(cur.first + cur.span.tiles - 1, sh.total, sh.ctas);
+      const int last = sh.whole
+                           ? static_cast<int>(blockIdx.x)
+                           : cta_of_step(cur.first + cur.span.tiles - 1, sh.total, sh.ctas);
       PagedPieces out;
       out.count = last - static_cast<int>(blockIdx.x) + 1;
       out.first = slot;
@@ -693,10 +714,13 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D
   if (p.pieces_only) grid_dependency_wait();
 }
 
-// Few units of few tiles: a cluster of CTAs a unit, which share its tiles and add their sums up in
-// one another's shared memory. One launch, no scan over the requests and no workspace; with
-// 16 CTAs a unit and one request of 1000 tokens (8 units of 16 tiles) @@ us against @@ for the
-// kernels above.
+// Few units of few tiles: a cluster of CTAs (or one) a unit, which share its tiles and add their
+// sums up in one another's shared memory. One launch, no scan over the requests, no workspace. The
+// launcher takes it when all CTAs are resident at once and none has more than eight tiles; it
+// measured (this against the two kernels, 8 k / v heads of 128, equal lengths) 4.6 against 7.0 us
+// for 4 requests of 128 tokens (1 CTA a unit), 6.8 against 8.8 for 1000 and 11.5 against 12.9 for
+// 4000 (8 CTAs), 5.7 against 7.5 for one request of 1000, 11.1 against 12.7 for 8000 but 17.3
+// against 14.5 for 16000 (16 CTAs, 16 tiles each), and 9.9 against 13.9 for 32 of 512.
 template <int D, bool kBF16>
 __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D, kBF16>::kCtas)
     mfa_paged_cluster_kernel(const __grid_constant__ PagedParams p) {

@@ -38,7 +38,7 @@ WIDE = pytest.mark.parametrize("wide", [False, True], ids=["narrow", "wide"])
 
 
 def columns(lengths, page, wide):
-    return max(1, *(-(-n // page) for n in lengths), 5000 // page if wide else 1)
+    return max(1, *(-(-n // page) for n in lengths), 9000 // page if wide else 1)
 
 
 @WIDE
@@ -85,6 +85,17 @@ def test_decode_many_requests():
     cache = Cache(lengths, 1, 64, 16, torch.float16, columns=60)
     q = queries(500, 2, 64, torch.float16)
     check(decode(cache, q), *cache.reference(q))
+
+
+def test_decode_a_unit_a_cta():
+    # about as many units as CTAs, of about the same length, and a table for longer ones
+    lengths = [900 + 7 * i for i in range(30)]
+    cache = Cache(lengths, 8, 128, 32, torch.bfloat16, columns=100)
+    q = queries(30, 32, 128, torch.bfloat16)
+    check(decode(cache, q), *cache.reference(q))
+    cache = Cache(lengths, 8, 128, 32, torch.bfloat16, columns=100, prefix=1500)
+    q = queries(30, 32, 128, torch.bfloat16)
+    check(behind_prefix(cache, q), *cache.reference(q))
 
 
 def test_decode_very_many_requests():
@@ -139,8 +150,8 @@ def test_prefix(prefix, page, d, dtype, wide):
     check(behind_prefix(cache, q), *cache.reference(q))
 
 
-# more than 16 MB read by all requests together: the prefix has a kernel of its own
-@pytest.mark.parametrize("prefix,batch", [(17, 1100), (127, 140), (128, 140), (129, 140), (500, 140)])
+# more than 64 MB read by all requests together: the prefix has a kernel of its own
+@pytest.mark.parametrize("prefix,batch", [(127, 530), (128, 530), (129, 530), (1000, 140)])
 @pytest.mark.parametrize("page", [16, 64, 256])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
@@ -160,7 +171,7 @@ def test_prefix_apart(prefix, batch, page, d, dtype):
 @pytest.mark.parametrize("long", [False, True])
 def test_prefix_rows(batch, kv_heads, group, d, long):
     lengths = [(11 * i) % 30 for i in range(batch)]
-    prefix = 5_000_000 // (batch * kv_heads * d) + 100 if long else 70
+    prefix = 17_000_000 // (batch * kv_heads * d) + 100 if long else 70
     cache = Cache(lengths, kv_heads, d, 32, torch.bfloat16, prefix=prefix, seed=batch)
     q = queries(batch, kv_heads * group, d, torch.bfloat16)
     check(behind_prefix(cache, q), *cache.reference(q))
@@ -200,8 +211,8 @@ def test_prefix_without_own_tokens():
     cache = Cache([0, 0, 0], 2, 64, 16, torch.bfloat16, prefix=333, columns=0)
     q = queries(3, 4, 64, torch.bfloat16)
     check(behind_prefix(cache, q), *cache.reference(q))
-    cache = Cache([0] * 200, 2, 64, 16, torch.bfloat16, prefix=333, columns=0)
-    q = queries(200, 4, 64, torch.bfloat16)
+    cache = Cache([0] * 500, 2, 64, 16, torch.bfloat16, prefix=333, columns=0)
+    q = queries(500, 4, 64, torch.bfloat16)
     check(behind_prefix(cache, q), *cache.reference(q))
 
 
@@ -213,8 +224,8 @@ def test_same_result_again_on_streams_and_in_graphs():
     k, v, table, own = cache.tensors()
     pages = cache.pages()
 
-    wide = torch.cat((table, torch.full((4, 200), -1, dtype=torch.int32, device="cuda")), 1)
-    many = Cache([5] * 300, 2, 64, 16, torch.float16, prefix=500)  # its prefix has its own kernel
+    wide = torch.cat((table, torch.full((4, 600), -1, dtype=torch.int32, device="cuda")), 1)
+    many = Cache([5] * 300, 2, 64, 16, torch.float16, prefix=500)
     big, big_q = many.tensors(), queries(300, 8, 64, torch.float16).cuda()
     big_pages = many.pages()
 
@@ -223,7 +234,7 @@ def test_same_result_again_on_streams_and_in_graphs():
                 mfa.paged_attention(q, k, v, wide, own),
                 mfa.paged_attention(q, k, v, wide, own, 1, 0),
                 mfa.shared_prefix_attention(q, k, v, pages, 500, table, own),
-                mfa.shared_prefix_attention(big_q, *big[:2], big_pages, 500, *big[2:]))
+                mfa.shared_prefix_attention(big_q, *big[:2], big_pages, 500, *big[2:]))  # 77 MB
 
     want = calls()
     assert all(torch.equal(a, b) for a, b in zip(want, calls()))
@@ -345,7 +356,7 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="D=64 and D=128"):
         mfa.paged_attention(x[0, :, :1], x, x, table[:1], own[:1])
     # the workspace of the C entry is checked
-    cache = Cache([40, 5], 2, 64, 16, torch.float16, columns=300)
+    cache = Cache([40, 5], 2, 64, 16, torch.float16, columns=3000)
     k, v, table, own = cache.tensors()
     need = capi.paged_workspace_bytes(2, 4, 2, 64, 16, table.shape[1])
     work = torch.empty((need,), dtype=torch.uint8, device="cuda")
