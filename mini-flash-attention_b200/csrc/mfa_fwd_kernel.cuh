@@ -255,8 +255,11 @@ struct StepCursor {
 // past key 0 has kRowsPerUnit / 128 + ceil((window - 1) / 128) window blocks, the same for all of
 // them, so the blocks are dealt out without a split. The items are p.whole_units query blocks, then
 // the others' two 128-row tiles one by one: where whole blocks would leave half of the CTAs or more
-// idle in the last wave, single tiles, which take a CTA 0.57 times as long (it has no other
-// tile's products to do meanwhile), end sooner.
+// idle in the last wave, single tiles end sooner: a step of one tile takes a CTA 2200 cycles, one
+// of two 2600 (122 -> 119 us at 16 heads x 8192, window 2048; 12.6 -> 10.3 at 12 heads x 777).
+// Measured at the former, D = 64: 110 us, 558 TFLOP/s over the visible pairs (a tile computes 18
+// blocks where 16.5 are visible); the exponential unit is 58% busy, 69% inside a step, as without a
+// window, and the last wave of four is two thirds of one.
 template <int kRowsPerUnit>
 struct WindowCursor {
   int item;
@@ -661,7 +664,12 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
       issued_any = true;
       ++ts;
     }
-    if (leader) mma_commit(bar(Cfg::kBarKEmpty + st));
+    if (leader) {
+      if (!Cfg::kWindow || live)
+        mma_commit(bar(Cfg::kBarKEmpty + st));
+      else
+        mbar_arrive(bar(Cfg::kBarKEmpty + st));  // nothing of this tile reads the block
+    }
     __syncwarp();
     ++gs;
     cs.step(p);
@@ -734,7 +742,12 @@ __device__ __forceinline__ void mma_role(const FwdParams& p, uint8_t* smem, uint
         issued_any = true;
         ++tp;
       }
-      if (leader) mma_commit(bar(Cfg::kBarVEmpty + st));
+      if (leader) {
+        if (!Cfg::kWindow || live)
+          mma_commit(bar(Cfg::kBarVEmpty + st));
+        else
+          mbar_arrive(bar(Cfg::kBarVEmpty + st));
+      }
       __syncwarp();
       ++gp;
       cp.step(p);

@@ -18,6 +18,11 @@
 // steps. Tiles arrive by TMA, one box a page, in a ring of stages. In a tile each warp takes 16 keys with a running maximum of its own; at the end of a
 // unit the four warps' states meet in shared memory. What a CTA's share cuts off goes to a slot
 // of the workspace as unnormalised 32-bit sums, which the combine kernel joins in CTA order.
+//
+// Measured on a B200 (64 requests of 100 to 16384 tokens, 8 k / v heads of 128, 4 rows each, bf16):
+// 137 us, 6.3 TB/s of k and v, 96% of a copy's rate; DRAM reads equal the k and v bytes. Windows
+// (100 requests, 4 heads of 64, up to 17 tiles a unit): 17.8 us, of which 4 are start-up
+// (lengths, table, first copies) and a unit's merge takes as long as two tiles.
 #pragma once
 
 #include <cuda.h>
