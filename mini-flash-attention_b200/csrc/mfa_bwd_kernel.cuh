@@ -221,7 +221,6 @@ struct BwdCursor {
     const int bh = u / p.blocks;
     return {bh % p.heads, bh / p.heads};
   }
-  __device__ HeadBatch streamed(const BwdParams& p) const { return resident(p); }
   __device__ int block() const { return j; }
   __device__ size_t vec_row(const BwdParams& p) const { return static_cast<size_t>(u / p.blocks); }
   __device__ bool in_pieces() const { return false; }
@@ -362,10 +361,6 @@ struct BwdWindowCursor {
   __device__ HeadBatch resident(const BwdParams& p) const {
     return {row % p.heads, row / p.heads};  // heads: of the resident tensors
   }
-  __device__ HeadBatch streamed(const BwdParams& p) const {
-    const HeadBatch r = resident(p);
-    return {Cfg::kDKV ? r.h * p.group + g : r.h / p.group, r.b};
-  }
   __device__ int block() const { return Cfg::kDKV || j < sinks ? j : j + skip; }
   __device__ size_t vec_row(const BwdParams& p) const {  // query row of the L2 / D slices
     return static_cast<size_t>(row) * p.group + g;
@@ -389,9 +384,20 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
   cur.init(p, claims, BwdRole::kLoad);
   int g = 0;
   int res_loaded = 0, str_issued = 0;
+  HeadBatch res = {0, 0};              // of the resident tiles
+  [[maybe_unused]] int str_h = 0;      // window variant: first head that the unit streams
   while (cur.valid()) {
+    HeadBatch hb;  // of the streamed tiles; worked out before the waits
+    if constexpr (Cfg::kWindow) {
+      if (cur.first_step()) {
+        res = cur.resident(p);
+        str_h = Cfg::kDKV ? res.h * p.group : res.h / p.group;
+      }
+      hb = {str_h + (Cfg::kDKV ? cur.g : 0), res.b};
+    } else {
+      hb = res = cur.resident(p);
+    }
     if (cur.first_step()) {
-      const HeadBatch hb = cur.resident(p);
       const int s = cur.seg, b = s & 1;
       if (!wait_single(bar(Cfg::kBarResEmpty + b), (static_cast<uint32_t>(s >> 1) & 1u) ^ 1u, wd,
                        kSiteLoadQEmpty))
@@ -399,8 +405,8 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
       mbar_arrive_expect_tx(bar(Cfg::kBarResFull + b), 2 * Cfg::kTileBytes);
       const int row = cur.row_block(p) * Cfg::kRows;
       const uint32_t dst = sbase + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
-      tma_load_4d(dst, &p.tm_x, bar(Cfg::kBarResFull + b), 0, row, hb.h, hb.b);
-      tma_load_4d(dst + Cfg::kTileBytes, &p.tm_y, bar(Cfg::kBarResFull + b), 0, row, hb.h, hb.b);
+      tma_load_4d(dst, &p.tm_x, bar(Cfg::kBarResFull + b), 0, row, res.h, res.b);
+      tma_load_4d(dst + Cfg::kTileBytes, &p.tm_y, bar(Cfg::kBarResFull + b), 0, row, res.h, res.b);
       res_loaded = s + 1;
     }
     const int st = g % ST;
@@ -409,7 +415,6 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
       break;
     mbar_arrive_expect_tx(bar(Cfg::kBarStrFull + st),
                           2 * Cfg::kTileBytes + (Cfg::kDKV ? Cfg::kVecBytes : 0));
-    const HeadBatch hb = cur.streamed(p);
     const int row = cur.block() * Cfg::kCols;
     const uint32_t dst = sbase + Cfg::kStrOff + st * 2 * Cfg::kTileBytes;
     tma_load_4d_hint(dst, &p.tm_s0, bar(Cfg::kBarStrFull + st), 0, row, hb.h, hb.b, keep);
@@ -1082,19 +1087,19 @@ constexpr int bwd_smem_bytes() {
 // D_i = rowsum(dO ⊙ o) and L2_i = L_i * log2(e) for every row, into [bh][blocks * 128] arrays
 // padded past N with D = 0, L2 = +inf (so that padded queries get P = 0 in the dK/dV pass).
 // Eight threads per row (16 bytes each), grid-stride.
-template <bool kBF16>
+template <bool kBF16, bool kWindow = false>
 __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const void* dout,
                                                            const float* lse, float* lse2,
                                                            float* di, int bh, int n, int heads,
                                                            long long stride_b, long long stride_h,
                                                            long long stride_n, int blocks,
                                                            int* counters = nullptr) {
-  // window variant: a programmatic dependent, as is the kernel after it (neither does anything in
-  // a plain launch)
-  if (threadIdx.x == 0) grid_dependents_launch();
-  grid_dependency_wait();
-  // window variant: the two passes' unit counters start at zero
-  if (counters != nullptr && blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
+  if constexpr (kWindow) {
+    // a programmatic dependent, as is the kernel after it; the two passes' unit counters start at 0
+    if (threadIdx.x == 0) grid_dependents_launch();
+    grid_dependency_wait();
+    if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
+  }
   const long long rows = static_cast<long long>(bh) * blocks * 128;  // a multiple of 4
   const int sub = threadIdx.x & 7;
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);

@@ -282,7 +282,7 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
     const int64_t need = (static_cast<int64_t>(rows) / 4 + 7) / 8;
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
     // the three kernels wait for the stream's earlier work themselves and may be set up while it ends
-    e = launch(need < most ? need : most, 256, 0, stream, &mfa_bwd_prep_kernel<kBF16>, out, dout,
+    e = launch(need < most ? need : most, 256, 0, stream, &mfa_bwd_prep_kernel<kBF16, true>, out, dout,
                lse, lse2, di, static_cast<int>(bh), static_cast<int>(w.n),
                static_cast<int>(w.heads), static_cast<long long>(st.b),
                static_cast<long long>(st.h), static_cast<long long>(st.n),
