@@ -63,8 +63,8 @@ struct BwdParams {
   int pieces_sink;
   int chunk_rest;    // ... and of any other block's
   int pieces_rest;
-  int* claimed;      // units handed out so far
-  float* partials;   // dK/dV: [slot][dK, dV][128][64] of the units in pieces
+  int* claimed;      // units of this pass handed out so far
+  float* partials;   // dK/dV: [slot][dK, dV][128][D] of the units in pieces
 };
 
 template <class Cfg>
@@ -72,8 +72,17 @@ struct BwdCursor;
 template <class Cfg>
 struct BwdWindowCursor;
 
-template <bool kDKV_, bool kCausal_, bool kBF16_, bool kWindow_ = false>
+// What a pass over resident k and v computes. D = 64 does both at once; the two accumulators of
+// D = 128 and the P^T and dS^T operands do not fit in TMEM together, so it takes a pass for each.
+enum class BwdPart { kBoth, kDK, kDV };
+
+template <bool kDKV_, bool kCausal_, bool kBF16_, bool kWindow_ = false, int kD_ = 64,
+          BwdPart kPart_ = BwdPart::kBoth>
 struct BwdConfig {
+  static constexpr BwdPart kPart = kPart_;
+  static constexpr bool kBoth = kDKV_ && kPart_ == BwdPart::kBoth;
+  static constexpr bool kOnlyDV = kDKV_ && kPart_ == BwdPart::kDV;  // needs no dP, dS and v
+  static_assert(kD_ == 64 || (kWindow_ && !kBoth), "D = 128: window variant, a pass each");
   // sliding window with sink tokens and grouped k / v heads, as the forward's window variant
   static constexpr bool kWindow = kWindow_;
   static_assert(!kWindow_ || kCausal_, "the window variant is causal");
@@ -81,11 +90,22 @@ struct BwdConfig {
   static constexpr bool kDKV = kDKV_;  // dK/dV pass (k, v resident) or dQ pass (q, dO resident)
   static constexpr bool kCausal = kCausal_;
   static constexpr bool kBF16 = kBF16_;
-  static constexpr int kHeadDim = 64;
+  static constexpr int kHeadDim = kD_;
   static constexpr int kRows = 128;  // resident rows per unit (M of every MMA)
   static constexpr int kCols = 128;  // streamed rows per step
   static constexpr int kTileBytes = kRows * kHeadDim * 2;
-  static constexpr int STAGES = 3;
+  static constexpr int kBoxes = kHeadDim / 64;       // 64-column boxes of a tile
+  static constexpr int kBoxBytes = kRows * 64 * 2;
+  // two buffers for the resident tiles and three stages; D = 128, whose tiles are twice as
+  // large, one and two
+  static constexpr int STAGES = kD_ == 64 ? 3 : 2;
+  static constexpr int kResBuffers = kD_ == 64 ? 2 : 1;
+  static constexpr int kResTiles = kOnlyDV ? 1 : 2;
+  // buffer of a CTA's s-th unit, and the phase of its barriers
+  __host__ __device__ static constexpr int res_buffer(int s) { return kResBuffers == 1 ? 0 : s & 1; }
+  __host__ __device__ static constexpr uint32_t res_phase(int s) {
+    return static_cast<uint32_t>(kResBuffers == 1 ? s : s >> 1) & 1u;
+  }
   static constexpr int kSoftmaxWarps = 16;  // 16 rows x 64 columns each
   // Two MMA issuers: warp 16 the S and dP products (SS), warp 19 the accumulations (TS). One
   // thread issues a tcgen05.mma only every few tens of cycles, and a step has 24 products in
@@ -103,8 +123,8 @@ struct BwdConfig {
   static constexpr int kControlRegs = 64;
 
   // shared memory (1024-aligned base)
-  static constexpr int kResOff = 0;                                  // [2 buffers][x, y]
-  static constexpr int kStrOff = kResOff + 2 * 2 * kTileBytes;       // [STAGES][tile 0, tile 1]
+  static constexpr int kResOff = 0;                                  // [buffers][x, y]
+  static constexpr int kStrOff = kResOff + kResBuffers * 2 * kTileBytes;  // [STAGES][tile 0, tile 1]
   static constexpr int kVecBytes = 2 * kCols * 4;                    // L2 slice, D slice
   static constexpr int kVecOff = kStrOff + STAGES * 2 * kTileBytes;  // [STAGES] (dK/dV pass)
   static constexpr int kBarOff = kVecOff + (kDKV ? STAGES * kVecBytes : 0);
@@ -133,8 +153,10 @@ struct BwdConfig {
   static constexpr int kColDP = 128;
   static constexpr int kColOp0 = 256;  // dQ pass: dS; dK/dV pass: P^T
   static constexpr int kColOp1 = 320;  // dK/dV pass: dS^T
-  static constexpr int kColAcc0 = kDKV ? 384 : 320;  // dQ pass: dQ; dK/dV pass: dV
-  static constexpr int kColAcc1 = 448;               // dK/dV pass: dK
+  static constexpr int kColAcc0 = kBoth ? 384 : 320;  // dQ pass: dQ; dK/dV pass: dV; the one alone
+  static constexpr int kColAcc1 = 448;                // dK/dV pass: dK
+  static constexpr int kPieceFloats = (kBoth ? 2 : 1) * kRows * kHeadDim;  // of BwdParams::partials
+  static_assert(kColAcc0 + kHeadDim <= 512, "TMEM budget");
   static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
 
@@ -398,15 +420,20 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
       hb = res = cur.resident(p);
     }
     if (cur.first_step()) {
-      const int s = cur.seg, b = s & 1;
-      if (!wait_single(bar(Cfg::kBarResEmpty + b), (static_cast<uint32_t>(s >> 1) & 1u) ^ 1u, wd,
-                       kSiteLoadQEmpty))
+      const int s = cur.seg, b = Cfg::res_buffer(s);
+      if (!wait_single(bar(Cfg::kBarResEmpty + b), Cfg::res_phase(s) ^ 1u, wd, kSiteLoadQEmpty))
         break;
-      mbar_arrive_expect_tx(bar(Cfg::kBarResFull + b), 2 * Cfg::kTileBytes);
+      mbar_arrive_expect_tx(bar(Cfg::kBarResFull + b), Cfg::kResTiles * Cfg::kTileBytes);
       const int row = cur.row_block(p) * Cfg::kRows;
       const uint32_t dst = sbase + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
-      tma_load_4d(dst, &p.tm_x, bar(Cfg::kBarResFull + b), 0, row, res.h, res.b);
-      tma_load_4d(dst + Cfg::kTileBytes, &p.tm_y, bar(Cfg::kBarResFull + b), 0, row, res.h, res.b);
+#pragma unroll
+      for (int x = 0; x < Cfg::kBoxes; ++x) {
+        tma_load_4d(dst + x * Cfg::kBoxBytes, &p.tm_x, bar(Cfg::kBarResFull + b), 64 * x, row,
+                    res.h, res.b);
+        if (Cfg::kResTiles == 2)
+          tma_load_4d(dst + Cfg::kTileBytes + x * Cfg::kBoxBytes, &p.tm_y,
+                      bar(Cfg::kBarResFull + b), 64 * x, row, res.h, res.b);
+      }
       res_loaded = s + 1;
     }
     const int st = g % ST;
@@ -417,9 +444,13 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
                           2 * Cfg::kTileBytes + (Cfg::kDKV ? Cfg::kVecBytes : 0));
     const int row = cur.block() * Cfg::kCols;
     const uint32_t dst = sbase + Cfg::kStrOff + st * 2 * Cfg::kTileBytes;
-    tma_load_4d_hint(dst, &p.tm_s0, bar(Cfg::kBarStrFull + st), 0, row, hb.h, hb.b, keep);
-    tma_load_4d_hint(dst + Cfg::kTileBytes, &p.tm_s1, bar(Cfg::kBarStrFull + st), 0, row, hb.h,
-                     hb.b, keep);
+#pragma unroll
+    for (int x = 0; x < Cfg::kBoxes; ++x) {
+      tma_load_4d_hint(dst + x * Cfg::kBoxBytes, &p.tm_s0, bar(Cfg::kBarStrFull + st), 64 * x, row,
+                       hb.h, hb.b, keep);
+      tma_load_4d_hint(dst + Cfg::kTileBytes + x * Cfg::kBoxBytes, &p.tm_s1,
+                       bar(Cfg::kBarStrFull + st), 64 * x, row, hb.h, hb.b, keep);
+    }
     if (Cfg::kDKV) {
       // L2 and D of the 128 streamed queries (padded arrays: 512-byte aligned slices)
       const size_t off = cur.vec_row(p) * p.blocks * Cfg::kCols + row;
@@ -432,10 +463,10 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
     cur.step(p);
   }
   if (*wd.abort) {
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < Cfg::kResBuffers; ++b) {
       int last = -1;
-      for (int s = b; s < res_loaded; s += 2) last = s;
-      if (last >= 0) drain_wait(bar(Cfg::kBarResFull + b), static_cast<uint32_t>(last >> 1) & 1u);
+      for (int s = b; s < res_loaded; s += Cfg::kResBuffers) last = s;
+      if (last >= 0) drain_wait(bar(Cfg::kBarResFull + b), Cfg::res_phase(last));
     }
     for (int st = 0; st < ST; ++st) {
       int last = -1;
@@ -456,12 +487,18 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
   auto bar = [&](int idx) { return bars + 8u * static_cast<uint32_t>(idx); };
   const uint32_t sbase = smem_addr(smem);
   constexpr uint32_t kIdescSS = idesc_f16_f32(128, 128, false, Cfg::kBF16);
-  constexpr uint32_t kIdescTS = idesc_f16_f32(128, 64, true, Cfg::kBF16);
+  constexpr uint32_t kIdescTS = idesc_f16_f32(128, Cfg::kHeadDim, true, Cfg::kBF16);
   constexpr uint32_t kHi = smem_desc_hi(1024, kSwizzle128B);
   constexpr uint32_t kTile = Cfg::kTileBytes >> 4;
   const uint32_t res_lo = smem_desc_lo(sbase + Cfg::kResOff, 16);
   const uint32_t str_lo = smem_desc_lo(sbase + Cfg::kStrOff, 16);
-  const uint32_t str_mn_lo = smem_desc_lo(sbase + Cfg::kStrOff, Cfg::kTileBytes);
+  // MN-major (the streamed rows are the K of the accumulations): the leading offset goes from one
+  // 64-column box to the next (unused at D = 64)
+  const uint32_t str_mn_lo = smem_desc_lo(sbase + Cfg::kStrOff, Cfg::kBoxBytes);
+  // descriptor offset (16-byte units) of the kk-th 16 columns of a K-major tile
+  auto k_off = [](int kk) -> uint32_t {
+    return static_cast<uint32_t>((kk >> 2) * (Cfg::kBoxBytes >> 4) + (kk & 3) * 2);
+  };
   const bool leader = elect_one();
   bool issued_any = false;
 
@@ -470,10 +507,9 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
   int gs = 0, gp = 0;
   // S and dP of step gs once the softmax warps have read those of step gs - 1.
   auto issue_ss = [&]() -> bool {
-    const int b = cur.seg & 1;
+    const int b = Cfg::res_buffer(cur.seg);
     if (cur.first_step()) {
-      if (!wait_warp(bar(Cfg::kBarResFull + b), static_cast<uint32_t>(cur.seg >> 1) & 1u, wd,
-                     kSiteMmaQ))
+      if (!wait_warp(bar(Cfg::kBarResFull + b), Cfg::res_phase(cur.seg), wd, kSiteMmaQ))
         return false;
     }
     const int st = gs % ST;
@@ -488,13 +524,15 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
       const uint32_t xd = res_lo + b * 2 * kTile, yd = xd + kTile;
       const uint32_t s0 = str_lo + st * 2 * kTile, s1 = s0 + kTile;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)  // S = x s0^T
-        mma_ss(tmem + Cfg::kColS, desc_join(xd + 2 * kk, kHi), desc_join(s0 + 2 * kk, kHi),
+      for (int kk = 0; kk < Cfg::kHeadDim / 16; ++kk)  // S = x s0^T
+        mma_ss(tmem + Cfg::kColS, desc_join(xd + k_off(kk), kHi), desc_join(s0 + k_off(kk), kHi),
                kIdescSS, kk > 0 ? 1u : 0u);
+      if constexpr (!Cfg::kOnlyDV) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)  // dP = y s1^T
-        mma_ss(tmem + Cfg::kColDP, desc_join(yd + 2 * kk, kHi), desc_join(s1 + 2 * kk, kHi),
-               kIdescSS, kk > 0 ? 1u : 0u);
+        for (int kk = 0; kk < Cfg::kHeadDim / 16; ++kk)  // dP = y s1^T
+          mma_ss(tmem + Cfg::kColDP, desc_join(yd + k_off(kk), kHi), desc_join(s1 + k_off(kk), kHi),
+                 kIdescSS, kk > 0 ? 1u : 0u);
+      }
       mma_commit(bar(Cfg::kBarSSFull));
       mma_commit(bar(Cfg::kBarStrEmpty + st));
     }
@@ -522,7 +560,7 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
       if (leader) {
         const bool fresh = cur.first_step();
         const uint32_t s0 = str_mn_lo + st * 2 * kTile, s1 = s0 + kTile;
-        if (Cfg::kDKV) {
+        if (Cfg::kBoth) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO
             mma_ts(tmem + Cfg::kColAcc0, tmem + Cfg::kColOp0 + 8 * kk,
@@ -533,9 +571,10 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
                    desc_join(s0 + 128 * kk, kHi), kIdescTS, (!fresh || kk > 0) ? 1u : 0u);
         } else {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)  // dQ += dS k
+          for (int kk = 0; kk < 8; ++kk)  // dQ += dS k; dK += dS^T q or dV += P^T dO alone
             mma_ts(tmem + Cfg::kColAcc0, tmem + Cfg::kColOp0 + 8 * kk,
-                   desc_join(s0 + 128 * kk, kHi), kIdescTS, (!fresh || kk > 0) ? 1u : 0u);
+                   desc_join((Cfg::kOnlyDV ? s1 : s0) + 128 * kk, kHi), kIdescTS,
+                   (!fresh || kk > 0) ? 1u : 0u);
         }
         mma_commit(bar(Cfg::kBarAccDone));
         mma_commit(bar(Cfg::kBarStrEmpty + st));
@@ -580,8 +619,12 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
   tc_fence_after();
   // [4i + e]: row g + 8 (e / 2), column 64 * half + 8i + 2q + e % 2 (tS, tDP already point at
   // this warp's column half)
-  uint32_t sr[32], dp[32];
-  tmem_ld2_16x256b_sync(tS, sr, tDP, dp);
+  uint32_t sr[32];
+  [[maybe_unused]] uint32_t dp[32];
+  if constexpr (Cfg::kOnlyDV)
+    tmem_ld_16x256b_sync(tS, sr);
+  else
+    tmem_ld2_16x256b_sync(tS, sr, tDP, dp);
   tc_fence_before();
   __syncwarp();
   if (lane == 0) mbar_arrive(bar(Cfg::kBarSSFree));
@@ -628,9 +671,9 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
       if (j == p.blocks - 1) {
         const int valid = p.n - j * Cfg::kCols;
         if (valid < Cfg::kCols) {
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 8; ++i)
-  #pragma unroll
+#pragma unroll
             for (int e = 0; e < 4; ++e)
               if (8 * i + q2 + (e & 1) >= valid) sr[4 * i + e] = __float_as_uint(-INFINITY);
         }
@@ -638,9 +681,9 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
       if (Cfg::kCausal) {
         const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k > t0 (+8 for e >= 2)
         if (j * Cfg::kCols + Cfg::kCols - 1 > row0) {
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 8; ++i)
-  #pragma unroll
+#pragma unroll
             for (int e = 0; e < 4; ++e)
               if (8 * i + q2 + (e & 1) > t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
         }
@@ -648,16 +691,16 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
     } else if (Cfg::kCausal && j == blk) {
       // diagonal block: queries (columns) before the key row score -inf
       const int t0 = row0 + gq - j * Cfg::kCols;  // column k masked when k < t0 (+8 for e >= 2)
-  #pragma unroll
+#pragma unroll
       for (int i = 0; i < 8; ++i)
-  #pragma unroll
+#pragma unroll
         for (int e = 0; e < 4; ++e)
           if (8 * i + q2 + (e & 1) < t0 + 8 * (e >> 1)) sr[4 * i + e] = __float_as_uint(-INFINITY);
     }
   }
 
   const uint64_t c2 = f2_splat(p.scale_log2);
-  uint32_t pk[16], dk[16];  // [2i + r]: row g + 8r, columns 8i + q2, 8i + q2 + 1 (16x128b)
+  [[maybe_unused]] uint32_t pk[16], dk[16];  // [2i + r]: row g + 8r, columns 8i + q2, 8i + q2 + 1 (16x128b)
   const int st = g % Cfg::STAGES;
   const float* vec = reinterpret_cast<const float*>(smem + Cfg::kVecOff + st * Cfg::kVecBytes);
   if (Cfg::kDKV) {
@@ -684,12 +727,14 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
     float x0, x1;
     f2_unpack(x, x0, x1);
     const float e0 = ex2_approx(x0), e1 = ex2_approx(x1);
-    const uint64_t t = f2_add(f2_pack(f(dp[2 * k]), f(dp[2 * k + 1])), f2_neg(d2));
-    const uint64_t ds = f2_mul(f2_pack(e0, e1), t);
-    float ds0, ds1;
-    f2_unpack(ds, ds0, ds1);
+    if constexpr (!Cfg::kOnlyDV) {
+      const uint64_t t = f2_add(f2_pack(f(dp[2 * k]), f(dp[2 * k + 1])), f2_neg(d2));
+      const uint64_t ds = f2_mul(f2_pack(e0, e1), t);
+      float ds0, ds1;
+      f2_unpack(ds, ds0, ds1);
+      dk[k] = pack_pair<Cfg::kBF16>(ds0, ds1);
+    }
     pk[k] = pack_pair<Cfg::kBF16>(e0, e1);
-    dk[k] = pack_pair<Cfg::kBF16>(ds0, ds1);
   }
   // The operand columns are free once the previous step's TS MMAs have completed.
   if (g > 0) {
@@ -697,9 +742,11 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
       return false;
     tc_fence_after();
   }
-  if (Cfg::kDKV) {
+  if constexpr (Cfg::kBoth) {
     tmem_st_16x128b_x8(tOp0, pk);
     tmem_st_16x128b_x8(tOp1, dk);
+  } else if constexpr (Cfg::kOnlyDV) {
+    tmem_st_16x128b_x8(tOp0, pk);
   } else {
     tmem_st_16x128b_x8(tOp0, dk);
   }
@@ -743,7 +790,7 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
         drow[r] = p.di[idx];
       }
     }
-    const int b = cur.seg & 1;
+    const int b = Cfg::res_buffer(cur.seg);
     if constexpr (Cfg::kWindow) {
       do {
         if (!bwd_step<Cfg>(p, smem, bars, tS, tDP, tOp0, tOp1, lane, half, g, blk, cur.block(),
@@ -764,49 +811,61 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
       return;
     tc_fence_after();
     uint8_t* res = smem + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
-    // this warp's 32 of the 64 accumulator columns (its column half), 16-byte chunks
-    // 4 half .. 4 half + 3 of each of its rows in the 128B-swizzled staging tile
+    // This warp's half of the accumulator's columns, 32 at a time: `c0` on are 16-byte chunks
+    // c0 % 64 / 8 .. + 3 of each of its rows in box c0 / 64 of the 128B-swizzled staging tile.
     auto stage_acc = [&](uint32_t col, float mul, uint8_t* dst_tile) {
-      uint32_t a[16];
-      tmem_ld_16x256b_sync(tmem + lb + col + 32 * half, a);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = slice + gq + 8 * r;
+      for (int sub = 0; sub < Cfg::kBoxes; ++sub) {
+        const int c0 = Cfg::kHeadDim / 2 * half + 32 * sub;
+        uint32_t a[16];
+        tmem_ld_16x256b_sync(tmem + lb + col + c0, a);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w = pack_pair<Cfg::kBF16>(__uint_as_float(a[4 * i + 2 * r]) * mul,
-                                                   __uint_as_float(a[4 * i + 2 * r + 1]) * mul);
-          const int chunk = 4 * half + i;
-          const uint32_t dst =
-              smem_addr(dst_tile + row * 128 + ((chunk ^ (row & 7)) << 4) + 4 * q);
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
+        for (int r = 0; r < 2; ++r) {
+          const int row = slice + gq + 8 * r;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w = pack_pair<Cfg::kBF16>(__uint_as_float(a[4 * i + 2 * r]) * mul,
+                                                     __uint_as_float(a[4 * i + 2 * r + 1]) * mul);
+            const int chunk = (c0 & 63) / 8 + i;
+            const uint32_t dst = smem_addr(dst_tile + (c0 >> 6) * Cfg::kBoxBytes + row * 128 +
+                                           ((chunk ^ (row & 7)) << 4) + 4 * q);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
+          }
         }
       }
     };
     if (Cfg::kDKV && cur.in_pieces()) {
       // a piece's sums, unscaled, for the reduce kernel
-      float* part = p.partials + static_cast<size_t>(cur.slot()) *
-                                     (2 * Cfg::kRows * Cfg::kHeadDim);
+      float* part = p.partials + static_cast<size_t>(cur.slot()) * Cfg::kPieceFloats;
       auto keep_acc = [&](uint32_t col, float* dst) {
-        uint32_t a[16];
-        tmem_ld_16x256b_sync(tmem + lb + col + 32 * half, a);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float* at = dst + (slice + gq + 8 * r) * Cfg::kHeadDim + 32 * half + 2 * q;
+        for (int sub = 0; sub < Cfg::kBoxes; ++sub) {
+          const int c0 = Cfg::kHeadDim / 2 * half + 32 * sub;
+          uint32_t a[16];
+          tmem_ld_16x256b_sync(tmem + lb + col + c0, a);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<float2*>(at + 8 * i) =
-                make_float2(__uint_as_float(a[4 * i + 2 * r]),
-                            __uint_as_float(a[4 * i + 2 * r + 1]));
+          for (int r = 0; r < 2; ++r) {
+            float* at = dst + (slice + gq + 8 * r) * Cfg::kHeadDim + c0 + 2 * q;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<float2*>(at + 8 * i) =
+                  make_float2(__uint_as_float(a[4 * i + 2 * r]),
+                              __uint_as_float(a[4 * i + 2 * r + 1]));
+          }
         }
       };
-      keep_acc(Cfg::kColAcc1, part);
-      keep_acc(Cfg::kColAcc0, part + Cfg::kRows * Cfg::kHeadDim);
-    } else if (Cfg::kDKV) {
+      if constexpr (Cfg::kBoth) {
+        keep_acc(Cfg::kColAcc1, part);
+        keep_acc(Cfg::kColAcc0, part + Cfg::kRows * Cfg::kHeadDim);
+      } else {
+        keep_acc(Cfg::kColAcc0, part);
+      }
+    } else if constexpr (Cfg::kBoth) {
       stage_acc(Cfg::kColAcc1, p.scale, res);                    // dK over the k tile
       stage_acc(Cfg::kColAcc0, 1.0f, res + Cfg::kTileBytes);     // dV over the v tile
     } else {
-      stage_acc(Cfg::kColAcc0, p.scale, res);                    // dQ over the q tile
+      // dQ over the q tile; dK or dV over the k tile
+      stage_acc(Cfg::kColAcc0, Cfg::kOnlyDV ? 1.0f : p.scale, res);
     }
     tc_fence_before();
     fence_proxy_async_smem();
@@ -828,15 +887,17 @@ __device__ __forceinline__ void bwd_store_role(const BwdParams& p, uint8_t* smem
   cur.init(p, claims, BwdRole::kLane);
   int stores = 0;
   while (cur.valid()) {
-    const int b = cur.seg & 1;
+    const int b = Cfg::res_buffer(cur.seg);
     if (!wait_single(bar(Cfg::kBarStage), static_cast<uint32_t>(stores) & 1u, wd, kSiteSoftStage))
       break;
     uint8_t* res = smem + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
     if (!cur.in_pieces()) {
       const int r0 = cur.row_block(p) * Cfg::kRows;
       const HeadBatch hb = cur.resident(p);
-      tma_store_4d(&p.tm_o0, smem_addr(res), 0, r0, hb.h, hb.b);
-      if (Cfg::kDKV) tma_store_4d(&p.tm_o1, smem_addr(res + Cfg::kTileBytes), 0, r0, hb.h, hb.b);
+#pragma unroll
+      for (int x = 0; x < Cfg::kBoxes; ++x)
+        tma_store_4d(&p.tm_o0, smem_addr(res + x * Cfg::kBoxBytes), 64 * x, r0, hb.h, hb.b);
+      if (Cfg::kBoth) tma_store_4d(&p.tm_o1, smem_addr(res + Cfg::kTileBytes), 0, r0, hb.h, hb.b);
       tma_store_commit();
       tma_store_wait_read();
     }
@@ -848,7 +909,7 @@ __device__ __forceinline__ void bwd_store_role(const BwdParams& p, uint8_t* smem
   tma_store_wait_read();
 }
 
-// The barriers of a CTA, initialised by one thread (the indices are those of both passes).
+// The barriers of a CTA, initialised by one thread (the indices are those of all its passes).
 template <class Cfg>
 __device__ __forceinline__ void bwd_init_bars(uint32_t bars) {
   for (int b = 0; b < 2; ++b) {
@@ -875,23 +936,27 @@ __device__ __forceinline__ void bwd_init_bars(uint32_t bars) {
   mbar_init_fence();
 }
 
-// One CTA: the units of pass CA (params pa), then, if kTwo, those of pass CB (params pb). Between
-// the passes every role has finished (the MMA warp drains its commits, the store thread waits
-// for its stores' shared-memory reads), the CTA meets on named barrier 2 and the barriers
-// start afresh; TMEM stays allocated. The barriers live past both passes' shared-memory
+// One CTA: the units of pass CA (params pa), then, with kPasses > 1, those of pass CB (params pb),
+// then, with 3, those of CC (pc). Between the passes every role has finished (the MMA warps drain
+// their commits, the store thread waits for its stores' shared-memory reads), the CTA meets on
+// named barrier 2 and the barriers start afresh; TMEM stays allocated. The barriers live past all passes' shared-memory
 // layouts. Each role's calls stay inside its setmaxnreg branch, which is what lets the
 // register allocator give the softmax-side warps their 104 registers.
-template <class CA, class CB, bool kTwo>
-__device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb) {
+template <class CA, class CB, class CC, int kPasses>
+__device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb,
+                                        const BwdParams& pc) {
   static_assert(CA::kNumBars == CB::kNumBars && CA::kThreads == CB::kThreads &&
-                    CA::kTmemCols == CB::kTmemCols,
+                    CA::kTmemCols == CB::kTmemCols && CA::kNumBars == CC::kNumBars &&
+                    CA::kThreads == CC::kThreads && CA::kTmemCols == CC::kTmemCols,
                 "passes of one CTA share barriers, threads and TMEM");
-  constexpr int kBarOff = CA::kBarOff > CB::kBarOff ? CA::kBarOff : CB::kBarOff;
+  constexpr int kBarOff2 = CA::kBarOff > CB::kBarOff ? CA::kBarOff : CB::kBarOff;
+  constexpr int kBarOff = kBarOff2 > CC::kBarOff ? kBarOff2 : CC::kBarOff;
   constexpr int kTmemSlotOff = kBarOff + CA::kNumBars * 8;
   constexpr int kAbortOff = kTmemSlotOff + 4;
   constexpr int kRingBytes = CA::kWindow ? 4 * CA::kClaims : 0;
-  static_assert(kAbortOff + 4 + kRingBytes + 1024 <= (CA::kSmemBytes > CB::kSmemBytes ? CA::kSmemBytes
-                                                                         : CB::kSmemBytes),
+  constexpr int kSmem2 = CA::kSmemBytes > CB::kSmemBytes ? CA::kSmemBytes : CB::kSmemBytes;
+  static_assert(kAbortOff + 4 + kRingBytes + 1024 <=
+                    (kSmem2 > CC::kSmemBytes ? kSmem2 : CC::kSmemBytes),
                 "barriers inside the launch's shared memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -903,9 +968,9 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kAbortOff);
   volatile int* ring = reinterpret_cast<volatile int*>(smem + kAbortOff + 4);
   if (CA::kWindow && threadIdx.x == 0) grid_dependents_launch();  // the reduce kernel, which waits
-  // Between the passes: true if the second pass runs (the same verdict in every thread:
+  // Between the passes: true if the next pass runs (the same verdict in every thread:
   // nothing writes the flag between the two barriers).
-  auto next_pass = [&]() -> bool {
+  auto next_pass = [&](auto config) -> bool {
     __syncwarp();
     tc_fence_before();
     named_bar_sync(2, CA::kThreads);
@@ -913,7 +978,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     const bool go = *abort_flag == 0;
     if (go && warp == CA::kLoadWarp && lane == 0) {
       for (int i = 0; i < CA::kNumBars; ++i) mbar_inval(bars + 8 * i);
-      bwd_init_bars<CB>(bars);
+      bwd_init_bars<decltype(config)>(bars);
     }
     named_bar_sync(2, CA::kThreads);
     return go;
@@ -934,8 +999,12 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     const Watchdog wd{abort_flag, pa.status, pa.timeout_ns};
     const BwdClaims claims{ring, bars, &wd};
     if (lane == 0) bwd_load_role<CA>(pa, smem, bars, wd, claims);
-    if constexpr (kTwo) {
-      if (next_pass() && lane == 0) bwd_load_role<CB>(pb, smem, bars, wd, claims);
+    if constexpr (kPasses > 1) {
+      const bool go = next_pass(CB{});
+      if (go && lane == 0) bwd_load_role<CB>(pb, smem, bars, wd, claims);
+      if constexpr (kPasses > 2) {
+        if (go && next_pass(CC{}) && lane == 0) bwd_load_role<CC>(pc, smem, bars, wd, claims);
+      }
     }
   } else {
     if (warp == 0) {
@@ -954,8 +1023,13 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
     if (warp < CA::kSoftmaxWarps) {
       setmaxnreg_inc<CA::kSoftmaxRegs>();
       bwd_softmax_role<CA>(pa, smem, bars, tmem, wd, claims);
-      if constexpr (kTwo) {
-        if (next_pass()) bwd_softmax_role<CB>(pb, smem, bars, tmem, wd, claims);
+      if constexpr (kPasses > 1) {
+        if (next_pass(CB{})) {
+          bwd_softmax_role<CB>(pb, smem, bars, tmem, wd, claims);
+          if constexpr (kPasses > 2) {
+            if (next_pass(CC{})) bwd_softmax_role<CC>(pc, smem, bars, tmem, wd, claims);
+          }
+        }
       }
     } else {
       setmaxnreg_dec<CA::kControlRegs>();
@@ -966,14 +1040,25 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
       } else if (warp == CA::kStoreWarp) {
         if (lane == 0) bwd_store_role<CA>(pa, smem, bars, wd, claims);
       }
-      if constexpr (kTwo) {
-        if (next_pass()) {
+      if constexpr (kPasses > 1) {
+        if (next_pass(CB{})) {
           if (warp == CB::kMmaWarp) {
             bwd_mma_role<CB, false>(pb, smem, bars, tmem, wd, claims);
           } else if (warp == CB::kAccWarp) {
             bwd_mma_role<CB, true>(pb, smem, bars, tmem, wd, claims);
           } else if (warp == CB::kStoreWarp) {
             if (lane == 0) bwd_store_role<CB>(pb, smem, bars, wd, claims);
+          }
+          if constexpr (kPasses > 2) {
+            if (next_pass(CC{})) {
+              if (warp == CC::kMmaWarp) {
+                bwd_mma_role<CC, false>(pc, smem, bars, tmem, wd, claims);
+              } else if (warp == CC::kAccWarp) {
+                bwd_mma_role<CC, true>(pc, smem, bars, tmem, wd, claims);
+              } else if (warp == CC::kStoreWarp) {
+                if (lane == 0) bwd_store_role<CC>(pc, smem, bars, wd, claims);
+              }
+            }
           }
         }
       }
@@ -994,9 +1079,9 @@ __global__ void __launch_bounds__(BwdConfig<true, kCausal, kBF16>::kThreads, 1)
   using CQ = BwdConfig<false, kCausal, kBF16>;
   using CK = BwdConfig<true, kCausal, kBF16>;
   if (static_cast<int>(blockIdx.x) < pkv.cta0)
-    bwd_cta<CQ, CQ, false>(pq, pq);
+    bwd_cta<CQ, CQ, CQ, 1>(pq, pq, pq);
   else
-    bwd_cta<CK, CK, false>(pkv, pkv);
+    bwd_cta<CK, CK, CK, 1>(pkv, pkv, pkv);
 }
 
 // Both passes in one launch, every CTA on both: its dK/dV units first, then its dQ units,
@@ -1008,7 +1093,8 @@ template <bool kCausal, bool kBF16>
 __global__ void __launch_bounds__(BwdConfig<true, kCausal, kBF16>::kThreads, 1)
     mfa_bwd_mixed_kernel(const __grid_constant__ BwdParams pq,
                          const __grid_constant__ BwdParams pkv) {
-  bwd_cta<BwdConfig<true, kCausal, kBF16>, BwdConfig<false, kCausal, kBF16>, true>(pkv, pq);
+  using CQ = BwdConfig<false, kCausal, kBF16>;
+  bwd_cta<BwdConfig<true, kCausal, kBF16>, CQ, CQ, 2>(pkv, pq, pq);
 }
 
 // Window variant: every CTA on both passes, dK/dV units first (they are the longer ones), each
@@ -1017,21 +1103,39 @@ template <bool kBF16>
 __global__ void __launch_bounds__(BwdConfig<true, true, kBF16, true>::kThreads, 1)
     mfa_bwd_window_kernel(const __grid_constant__ BwdParams pq,
                           const __grid_constant__ BwdParams pkv) {
-  bwd_cta<BwdConfig<true, true, kBF16, true>, BwdConfig<false, true, kBF16, true>, true>(pkv, pq);
+  using CQ = BwdConfig<false, true, kBF16, true>;
+  bwd_cta<BwdConfig<true, true, kBF16, true>, CQ, CQ, 2>(pkv, pq, pq);
 }
 
-// dK and dV of the blocks whose units ran in pieces: the sum of the pieces in order, dK scaled.
-// One CTA per 16 rows of a (block, k / v head row) pair that may have pieces, sink blocks first; 16
-// threads per row, four columns each. The pieces are read four at a time (an L2 round trip each).
-// (16 heads x 8192, 16 sinks: 4 blocks of 4 pieces, 3 us behind the passes; one CTA a block took 9.)
+// D = 128: dK, dV and dQ in a pass each (the dV pass without dP).
 template <bool kBF16>
-__global__ void __launch_bounds__(256) mfa_bwd_reduce_kernel(const BwdParams p, uint16_t* dk,
-                                                             uint16_t* dv, long long stride_b,
-                                                             long long stride_h,
-                                                             long long stride_n) {
-  constexpr int kTile = 128 * 64;
+using BwdDK128 = BwdConfig<true, true, kBF16, true, 128, BwdPart::kDK>;
+template <bool kBF16>
+using BwdDV128 = BwdConfig<true, true, kBF16, true, 128, BwdPart::kDV>;
+template <bool kBF16>
+using BwdDQ128 = BwdConfig<false, true, kBF16, true, 128>;
+
+template <bool kBF16>
+__global__ void __launch_bounds__(BwdDQ128<kBF16>::kThreads, 1)
+    mfa_bwd_window128_kernel(const __grid_constant__ BwdParams pq,
+                             const __grid_constant__ BwdParams pk,
+                             const __grid_constant__ BwdParams pv) {
+  bwd_cta<BwdDK128<kBF16>, BwdDV128<kBF16>, BwdDQ128<kBF16>, 3>(pk, pv, pq);
+}
+
+// dK and dV of the blocks whose units ran in pieces: the sum of the pieces in order, dK scaled. The
+// pieces of slot i are at dk_sums and dv_sums + i * slot_floats. One CTA per 1024 / D rows of a
+// (block, k / v head row) pair that may have pieces, sink blocks first; D / 4 threads a row, four
+// columns each, of the tensors' `cols`. The pieces are read four at a time (an L2 round trip each). (16 heads x 8192, 16
+// sinks, D = 64: 4 blocks of 4 pieces, 3 us behind the passes; one CTA a block took 9.)
+template <bool kBF16, int kD>
+__global__ void __launch_bounds__(256)
+    mfa_bwd_reduce_kernel(const BwdParams p, const float* dk_sums, const float* dv_sums,
+                          long long slot_floats, int cols, uint16_t* dk, uint16_t* dv,
+                          long long stride_b, long long stride_h, long long stride_n) {
+  constexpr int kRows = 1024 / kD, kCtas = 128 / kRows;
   grid_dependency_wait();
-  const int pair = static_cast<int>(blockIdx.x) >> 3;
+  const int pair = static_cast<int>(blockIdx.x) / kCtas;
   const int blk = pair / p.bh, row = pair % p.bh;
   const bool sink = blk < p.sink_blocks;
   const int span = BwdWindowCursor<BwdConfig<true, true, kBF16, true>>::span(p, blk);
@@ -1045,16 +1149,15 @@ __global__ void __launch_bounds__(256) mfa_bwd_reduce_kernel(const BwdParams p, 
                  static_cast<long long>(blk - p.sink_blocks) * p.bh * p.pieces_rest + row;
   const long long base =
       static_cast<long long>(row / p.heads) * stride_b + (row % p.heads) * stride_h;
-  const int col = 4 * (threadIdx.x & 15);
-  const int r = (static_cast<int>(blockIdx.x) & 7) * 16 + (threadIdx.x >> 4);
-  if (blk * 128 + r < p.n) {
+  const int col = 4 * (threadIdx.x % (kD / 4));
+  const int r = static_cast<int>(blockIdx.x) % kCtas * kRows + threadIdx.x / (kD / 4);
+  if (blk * 128 + r < p.n && col < cols) {
     float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
 #pragma unroll 4
     for (int i = 0; i < count; ++i) {
-      const float* at = p.partials + (first + static_cast<long long>(i) * p.bh) * (2 * kTile) +
-                        r * 64 + col;
-      const float4 a = *reinterpret_cast<const float4*>(at);
-      const float4 b = *reinterpret_cast<const float4*>(at + kTile);
+      const long long at = (first + static_cast<long long>(i) * p.bh) * slot_floats + r * kD + col;
+      const float4 a = *reinterpret_cast<const float4*>(dk_sums + at);
+      const float4 b = *reinterpret_cast<const float4*>(dv_sums + at);
       k.x += a.x, k.y += a.y, k.z += a.z, k.w += a.w;
       v.x += b.x, v.y += b.y, v.z += b.z, v.w += b.w;
     }
@@ -1073,7 +1176,7 @@ template <bool kDKV, bool kCausal, bool kBF16>
 __global__ void __launch_bounds__(BwdConfig<kDKV, kCausal, kBF16>::kThreads, 1)
     mfa_bwd_pass_kernel(const __grid_constant__ BwdParams p) {
   using C = BwdConfig<kDKV, kCausal, kBF16>;
-  bwd_cta<C, C, false>(p, p);
+  bwd_cta<C, C, C, 1>(p, p, p);
 }
 
 // Dynamic shared memory of the two-pass launch.
@@ -1086,8 +1189,8 @@ constexpr int bwd_smem_bytes() {
 
 // D_i = rowsum(dO ⊙ o) and L2_i = L_i * log2(e) for every row, into [bh][blocks * 128] arrays
 // padded past N with D = 0, L2 = +inf (so that padded queries get P = 0 in the dK/dV pass).
-// Eight threads per row (16 bytes each), grid-stride.
-template <bool kBF16, bool kWindow = false>
+// D / 8 threads per row (16 bytes each), grid-stride.
+template <bool kBF16, bool kWindow = false, int kD = 64>
 __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const void* dout,
                                                            const float* lse, float* lse2,
                                                            float* di, int bh, int n, int heads,
@@ -1095,18 +1198,19 @@ __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const 
                                                            long long stride_n, int blocks,
                                                            int* counters = nullptr) {
   if constexpr (kWindow) {
-    // a programmatic dependent, as is the kernel after it; the two passes' unit counters start at 0
+    // a programmatic dependent, as is the kernel after it; the passes' unit counters start at 0
     if (threadIdx.x == 0) grid_dependents_launch();
     grid_dependency_wait();
-    if (blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x < 3) counters[threadIdx.x] = 0;
   }
-  const long long rows = static_cast<long long>(bh) * blocks * 128;  // a multiple of 4
-  const int sub = threadIdx.x & 7;
+  constexpr int kLanes = kD / 8, kRows = 32 / kLanes;  // threads of a row, rows of a warp
+  const long long rows = static_cast<long long>(bh) * blocks * 128;  // a multiple of kRows
+  const int sub = threadIdx.x & (kLanes - 1);
   const long long warps = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-  // four rows per warp and iteration; the trip count is the same for the whole warp
+  // kRows rows per warp and iteration; the trip count is the same for the whole warp
   for (long long w = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-       w * 4 < rows; w += warps) {
-    const long long r = w * 4 + ((threadIdx.x & 31) >> 3);
+       w * kRows < rows; w += warps) {
+    const long long r = w * kRows + (threadIdx.x & 31) / kLanes;
     const int h = static_cast<int>(r / (static_cast<long long>(blocks) * 128));
     const int row = static_cast<int>(r - static_cast<long long>(h) * blocks * 128);
     float acc = 0.0f;
@@ -1125,9 +1229,8 @@ __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const 
         acc = fmaf(a0, b0, fmaf(a1, b1, acc));
       }
     }
-    acc += __shfl_xor_sync(0xffffffffu, acc, 1);
-    acc += __shfl_xor_sync(0xffffffffu, acc, 2);
-    acc += __shfl_xor_sync(0xffffffffu, acc, 4);
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     if (sub == 0) {
       di[r] = row < n ? acc : 0.0f;
       lse2[r] = row < n ? lse[static_cast<long long>(h) * n + row] * 1.4426950408889634f

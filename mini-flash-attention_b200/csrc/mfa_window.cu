@@ -37,6 +37,14 @@ constexpr int window_bwd_smem() {
 }
 
 template <bool kBF16>
+constexpr int window_bwd128_smem() {
+  constexpr int kv = BwdDK128<kBF16>::kSmemBytes > BwdDV128<kBF16>::kSmemBytes
+                         ? BwdDK128<kBF16>::kSmemBytes
+                         : BwdDV128<kBF16>::kSmemBytes;
+  return kv > BwdDQ128<kBF16>::kSmemBytes ? kv : BwdDQ128<kBF16>::kSmemBytes;
+}
+
+template <bool kBF16>
 cudaError_t set_attributes() {
   const auto smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
   cudaError_t e = cudaFuncSetAttribute(window_kernel<Window<kBF16, 32>>(), smem,
@@ -49,6 +57,8 @@ cudaError_t set_attributes() {
                              Window<kBF16, 128>::kSmemBytes);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(mfa_bwd_window_kernel<kBF16>, smem, window_bwd_smem<kBF16>());
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(mfa_bwd_window128_kernel<kBF16>, smem, window_bwd128_smem<kBF16>());
   return e;
 }
 
@@ -168,15 +178,16 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
 }
 
 // How the dK/dV pass cuts its units into pieces (BwdWindowCursor). `span_steps` is the number of
-// (key block, query block) pairs of one head that hold a visible (key, query) pair: both passes
-// walk every one of them, the dK/dV pass at about 1.05 times a dQ step's cost.
+// (key block, query block) pairs of one head that hold a visible (key, query) pair: every pass
+// walks all of them; `passes` is what they cost together, in dQ steps (D = 64: the dK/dV step is
+// about 1.05 of one; D = 128: the dV step about 0.8).
 struct Pieces {
   int chunk_sink, pieces_sink, chunk_rest, pieces_rest;
 };
 
 Pieces plan_pieces(int64_t blocks, int64_t sink_blocks, int64_t span, int64_t span_steps,
-                   int64_t kv_rows, int64_t group, int64_t sms) {
-  const double share = 2.05 * static_cast<double>(span_steps) *
+                   int64_t kv_rows, int64_t group, int64_t sms, double passes) {
+  const double share = passes * static_cast<double>(span_steps) *
                        static_cast<double>(kv_rows * group) / static_cast<double>(sms);
   // A unit of `len` steps stays whole while it is not the longest thing a CTA does: up to
   // three quarters of a CTA's share of the work (units are claimed longest first). Longer ones
@@ -198,7 +209,29 @@ Pieces plan_pieces(int64_t blocks, int64_t sink_blocks, int64_t span, int64_t sp
   return out;
 }
 
+// The map of a tensor of the gradients: D = 32 runs as D = 64 with boxes that reach past its
+// columns, where loads read zeros, which change no sum, and stores write nothing.
+int encode_gradient(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
+                    int64_t d, int layout, bool bf16) {
+  if (d >= 64) return host::encode_heads(map, base, batch, heads, n, d, layout, bf16);
+  const host::Strides st = host::strides_of(layout, heads, n, d);
+  const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(n),
+                            static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(st.n) * 2, static_cast<uint64_t>(st.h) * 2,
+                               static_cast<uint64_t>(st.b) * 2};
+  const uint32_t box[4] = {64, 128, 1, 1};
+  return host::encode_map(map, base, 4, dims, strides, box, bf16);
+}
+
 template <bool kBF16>
+auto* prep_kernel(int32_t d) {
+  return d == 32   ? &mfa_bwd_prep_kernel<kBF16, true, 32>
+         : d == 64 ? &mfa_bwd_prep_kernel<kBF16, true, 64>
+                   : &mfa_bwd_prep_kernel<kBF16, true, 128>;
+}
+
+// D: the kernel's head dim, at least w.d
+template <bool kBF16, int D>
 int launch_backward(const void* q, const void* k, const void* v, const void* out,
                     const void* dout, const float* lse, void* dq, void* dk, void* dv,
                     const Problem& w, const host::Device& dev, cudaStream_t stream) {
@@ -211,16 +244,19 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
   const int64_t rest = blocks - sb, short_ones = reach < rest ? reach : rest;
   const int64_t span_steps = sb * blocks - sb * (sb - 1) / 2 + (rest - short_ones) * span +
                              short_ones * (short_ones + 1) / 2;
-  const Pieces pc = plan_pieces(blocks, sb, span, span_steps, bhk, group, dev.sms);
+  const Pieces pc = plan_pieces(blocks, sb, span, span_steps, bhk, group, dev.sms,
+                                D == 64 ? 2.05 : 2.85);
   const int64_t sink_units = bhk * sb * pc.pieces_sink;
   const int64_t kv_units = sink_units + bhk * rest * pc.pieces_rest, q_units = bh * blocks;
   if (kv_units > 0x3fff0000LL || blocks * group > 0x3fff0000LL)
     return host::fail(MFA_ERR_INVALID_ARGUMENT, "B * H * N is too large");
   const int64_t slots = pc.pieces_rest > 1 ? kv_units : pc.pieces_sink > 1 ? sink_units : 0;
 
-  // L2 and D of every row, the two counters, the pieces' sums (256-byte aligned)
+  // L2 and D of every row, the counters, the pieces' sums (256-byte aligned): at D = 64 a slot
+  // holds dK and dV, at D = 128 all slots of dK come first
+  constexpr int64_t kTile = 128 * D;
   const size_t rows = static_cast<size_t>(q_units) * 128;
-  const size_t floats = 2 * rows + 64 + static_cast<size_t>(slots) * 2 * 128 * 64;
+  const size_t floats = 2 * rows + 64 + static_cast<size_t>(slots * 2 * kTile);
   float* ws = nullptr;
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), floats * sizeof(float),
                                           dev.pool, stream);
@@ -228,6 +264,7 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
   float* lse2 = ws;
   float* di = ws + rows;
   int* counters = reinterpret_cast<int*>(ws + 2 * rows);
+  float* sums = ws + 2 * rows + 64;
 
   BwdParams pkv = {};
   pkv.n = static_cast<int>(w.n);
@@ -246,7 +283,7 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
   pkv.pieces_sink = pc.pieces_sink;
   pkv.chunk_rest = pc.chunk_rest;
   pkv.pieces_rest = pc.pieces_rest;
-  pkv.partials = ws + 2 * rows + 64;
+  pkv.partials = sums;
   BwdParams pq = pkv;
   pkv.heads = static_cast<int>(w.kv_heads);
   pkv.bh = static_cast<int>(bhk);
@@ -269,7 +306,7 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
                       {&pkv.tm_o1, dv, w.kv_heads}};
   int rc = MFA_OK;
   for (const Map& m : maps) {
-    rc = host::encode_heads(m.to, m.base, w.batch, m.heads, w.n, 64, w.layout, kBF16);
+    rc = encode_gradient(m.to, m.base, w.batch, m.heads, w.n, w.d, w.layout, kBF16);
     if (rc != MFA_OK) break;
   }
   pq.tm_o1 = pq.tm_o0;
@@ -278,23 +315,35 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
   pkv.tm_s0 = pq.tm_x;
   pkv.tm_s1 = pq.tm_y;
   if (rc == MFA_OK) {
-    const host::Strides st = host::strides_of(w.layout, w.heads, w.n, 64);
-    const int64_t need = (static_cast<int64_t>(rows) / 4 + 7) / 8;
+    const host::Strides st = host::strides_of(w.layout, w.heads, w.n, w.d);
+    const int64_t need = static_cast<int64_t>(rows) * w.d / 2048;  // 16 bytes a thread
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
-    // the three kernels wait for the stream's earlier work themselves and may be set up while it ends
-    e = launch(need < most ? need : most, 256, 0, stream, &mfa_bwd_prep_kernel<kBF16, true>, out, dout,
-               lse, lse2, di, static_cast<int>(bh), static_cast<int>(w.n),
-               static_cast<int>(w.heads), static_cast<long long>(st.b),
+    // the kernels wait for the stream's earlier work themselves and may be set up while it ends
+    e = launch(need < most ? need : most, 256, 0, stream, prep_kernel<kBF16>(w.d), out, dout, lse,
+               lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads), static_cast<long long>(st.b),
                static_cast<long long>(st.h), static_cast<long long>(st.n),
                static_cast<int>(blocks), counters);
     const int64_t units = kv_units > q_units ? kv_units : q_units;
-    if (e == cudaSuccess)
-      e = launch(units < dev.sms ? units : dev.sms, BwdConfig<true, true, kBF16, true>::kThreads,
-                 window_bwd_smem<kBF16>(), stream, &mfa_bwd_window_kernel<kBF16>, pq, pkv);
+    const int64_t ctas = units < dev.sms ? units : dev.sms;
+    if constexpr (D == 64) {
+      if (e == cudaSuccess)
+        e = launch(ctas, BwdConfig<true, true, kBF16, true>::kThreads, window_bwd_smem<kBF16>(),
+                   stream, &mfa_bwd_window_kernel<kBF16>, pq, pkv);
+    } else {
+      BwdParams pv = pkv;  // pkv: dK
+      pv.tm_o0 = pkv.tm_o1;
+      pv.claimed = counters + 2;
+      pv.partials = sums + slots * kTile;
+      if (e == cudaSuccess)
+        e = launch(ctas, BwdDQ128<kBF16>::kThreads, window_bwd128_smem<kBF16>(), stream,
+                   &mfa_bwd_window128_kernel<kBF16>, pq, pkv, pv);
+    }
     if (e == cudaSuccess && slots > 0) {
-      const host::Strides kv = host::strides_of(w.layout, w.kv_heads, w.n, 64);
+      const host::Strides kv = host::strides_of(w.layout, w.kv_heads, w.n, w.d);
       const int64_t pairs = bhk * (pc.pieces_rest > 1 ? blocks : sb);
-      e = launch(8 * pairs, 256, 0, stream, &mfa_bwd_reduce_kernel<kBF16>, pkv,
+      const long long slot_floats = D == 64 ? 2 * kTile : kTile;
+      e = launch(pairs * D / 8, 256, 0, stream, &mfa_bwd_reduce_kernel<kBF16, D>, pkv, sums,
+                 sums + (D == 64 ? kTile : slots * kTile), slot_floats, w.d,
                  static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv),
                  static_cast<long long>(kv.b), static_cast<long long>(kv.h),
                  static_cast<long long>(kv.n));
@@ -348,8 +397,6 @@ extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const
   Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale};
   int rc = check(w);
   if (rc != MFA_OK) return rc;
-  if (d != 64)
-    return host::fail(MFA_ERR_HEAD_DIM, "The backward pass supports only D=64");
   if (batch * heads == 0 || n == 0) return MFA_OK;
   const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv};
   const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv"};
@@ -362,7 +409,9 @@ extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const
   if ((rc = check_tensors(ptrs, names, 8, dev.index)) != MFA_OK) return rc;
   if ((rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MFA_DTYPE_BF16
-             ? launch_backward<true>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s)
-             : launch_backward<false>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s);
+  if (dtype == MFA_DTYPE_BF16)
+    return d <= 64 ? launch_backward<true, 64>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s)
+                   : launch_backward<true, 128>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s);
+  return d <= 64 ? launch_backward<false, 64>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s)
+                 : launch_backward<false, 128>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s);
 }

@@ -44,11 +44,6 @@ def test_refused(direction, change, code, text):
     assert e.value.code == code
 
 
-def test_backward_head_dim():
-    with pytest.raises(capi.MfaError, match="The backward pass supports only D=64"):
-        call("bwd", d=128)
-
-
 @pytest.mark.parametrize("direction", ["fwd", "bwd"])
 @pytest.mark.parametrize("change", [{"batch": 0}, {"n": 0}, {"heads": 0}])
 def test_nothing_to_do(direction, change):

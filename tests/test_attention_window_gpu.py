@@ -49,10 +49,11 @@ def test_forward(b, h, hk, n, window, sinks, dtype, d):
     assert torch.equal(out, mfa.forward_window(q, k, v, window, sinks))
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
 @TYPES
 @pytest.mark.parametrize("b,h,hk,n,window,sinks", SHAPES)
-def test_gradients(b, h, hk, n, window, sinks, dtype):
-    q, k, v, dout = inputs(b, h, hk, n, 64, dtype)
+def test_gradients(b, h, hk, n, window, sinks, dtype, d):
+    q, k, v, dout = inputs(b, h, hk, n, d, dtype)
     want = reference(q, k, v, window, sinks, dout)
     out, lse = mfa.forward_window_lse(q, k, v, window, sinks)
     for name, x in zip(("dq", "dk", "dv"),
@@ -63,12 +64,13 @@ def test_gradients(b, h, hk, n, window, sinks, dtype):
 
 # units in pieces: few heads and long reaches (every key block's unit is cut), and sink blocks
 # alone cut
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("b,h,hk,n,window,sinks", [
     (1, 1, 1, 4096, 4096, 0), (1, 8, 1, 2048, 2048, 0), (1, 4, 1, 3000, 128, 200),
     (1, 16, 2, 2500, 300, 4), (2, 2, 2, 4000, 1, 1),
 ])
-def test_gradients_in_pieces(b, h, hk, n, window, sinks):
-    q, k, v, dout = inputs(b, h, hk, n, 64, torch.bfloat16, seed=31)
+def test_gradients_in_pieces(b, h, hk, n, window, sinks, d):
+    q, k, v, dout = inputs(b, h, hk, n, d, torch.bfloat16, seed=31)
     want = reference(q, k, v, window, sinks, dout)
     out, lse = mfa.forward_window_lse(q, k, v, window, sinks)
     first = mfa.backward_window(q, k, v, out, lse, dout, window, sinks)
@@ -76,6 +78,53 @@ def test_gradients_in_pieces(b, h, hk, n, window, sinks):
         check(name, x, *want[name])
     again = mfa.backward_window(q, k, v, out, lse, dout, window, sinks)
     assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+# far more units than CTAs: every buffer and ring entry is used again, with and without pieces
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("b,h,hk,n,window,sinks", [
+    (16, 8, 8, 700, 130, 0), (3, 32, 8, 1100, 256, 4),
+])
+def test_gradients_many_units(b, h, hk, n, window, sinks, d):
+    q, k, v, dout = inputs(b, h, hk, n, d, torch.float16, seed=57)
+    out, lse = mfa.forward_window_lse(q, k, v, window, sinks)
+    got = mfa.backward_window(q, k, v, out, lse, dout, window, sinks)
+    for i in range(0, b, 2):
+        part = [x[i:i + 1] for x in (q, k, v)]
+        want = reference(*part, window, sinks, dout[i:i + 1])
+        for name, x in zip(("dq", "dk", "dv"), got):
+            check(name, x[i:i + 1], *want[name])
+
+
+# what lies before and behind a gradient stays as it was (a block's rows past the last token, the
+# columns past D = 32)
+@pytest.mark.parametrize("layout", [capi.LAYOUT_BHND, capi.LAYOUT_BNHD], ids=["bhnd", "bnhd"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("n,window,sinks", [(1, 1, 0), (77, 10, 3), (2050, 2050, 1)])
+def test_gradients_write_nothing_else(n, window, sinks, d, layout):
+    b, h, hk = 2, 4, 2
+    q, k, v, dout = inputs(b, h, hk, n, d, torch.float16, seed=91)
+    want = reference(q, k, v, window, sinks, dout)
+    turn = (lambda x: x) if layout == capi.LAYOUT_BHND else lambda x: x.transpose(1, 2).contiguous()
+    x = [turn(t) for t in (q, k, v, dout)]
+    room = 256 * d
+    buffers = [torch.full((t.numel() + 2 * room,), 7.0, device="cuda", dtype=torch.float16)
+               for t in (q, q, k, v)]
+    out, dq, dk, dv = [t[room:-room] for t in buffers]
+    lse = torch.empty((b, h, n), device="cuda")
+    common = dict(dtype=capi.DTYPE_FP16, layout=layout,
+                  stream=torch.cuda.current_stream().cuda_stream)
+    capi.fwd_window(*(t.data_ptr() for t in x[:3]), out.data_ptr(), lse.data_ptr(), b, h, hk, n, d,
+                    window, sinks, d ** -0.5, **common)
+    capi.bwd_window(*(t.data_ptr() for t in x[:3]), out.data_ptr(), x[3].data_ptr(),
+                    lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, h, hk, n, d,
+                    window, sinks, d ** -0.5, **common)
+    for name, got in zip(("out", "dq", "dk", "dv"), (out, dq, dk, dv)):
+        heads = h if name in ("out", "dq") else hk
+        shape = (b, heads, n, d) if layout == capi.LAYOUT_BHND else (b, n, heads, d)
+        check(name, turn(got.view(shape)), *want[name])
+    for t in buffers:
+        assert (t[:room] == 7).all() and (t[-room:] == 7).all()
 
 
 def test_whole_window_is_causal_attention():
@@ -100,8 +149,9 @@ def test_large_scores():
     assert torch.isfinite(lse).all()
 
 
-def test_autograd_and_differences():
-    q, k, v, dout = inputs(1, 4, 2, 200, 64, torch.float16)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_autograd_and_differences(d):
+    q, k, v, dout = inputs(1, 4, 2, 200, d, torch.float16)
     leaves = [x.requires_grad_() for x in (q, k, v)]
     out = mfa.window_attention(*leaves, 50, 2)
     grads = torch.autograd.grad(out, leaves, dout)
@@ -114,7 +164,8 @@ def test_autograd_and_differences():
     def loss(step):
         x, y, z = (t.detach().double() + step * w for t, w in zip(leaves, direction))
         y, z = (t.repeat_interleave(2, 1) for t in (y, z))
-        s = (x @ y.transpose(-1, -2) / 8).masked_fill(~visible(200, 50, 2, x.device), -torch.inf)
+        s = x @ y.transpose(-1, -2) * d ** -0.5
+        s = s.masked_fill(~visible(200, 50, 2, x.device), -torch.inf)
         return (torch.softmax(s, -1) @ z * dout.double()).sum()
 
     slope = ((loss(1e-5) - loss(-1e-5)) / 2e-5).item()
@@ -230,7 +281,5 @@ def test_refusals():
     x = randn((1, 2, 100, 48), 3)
     with pytest.raises(RuntimeError, match="D=32, D=64 and D=128"):
         mfa.forward_window(x, x, x, 5)
-    x = randn((1, 2, 100, 128), 3)
-    out, lse = mfa.forward_window_lse(x, x, x, 5)
-    with pytest.raises(RuntimeError, match="The backward pass supports only D=64"):
-        mfa.backward_window(x, x, x, out, lse, out, 5)
+    with pytest.raises(RuntimeError, match="D=32, D=64 and D=128"):
+        mfa.backward_window(x, x, x, x, randn((1, 2, 100), 4, torch.float32), x, 5)
