@@ -136,11 +136,10 @@ MFA_API int mfa_fwd_window(const void* q, const void* k, const void* v, void* ou
                            int32_t layout, void* stream);
 
 /*
- * Backward of mfa_fwd_window (D = 64; others: MFA_ERR_HEAD_DIM "The backward pass supports only
- * D=64"): dq, dk, dv from q, k, v, out, lse, dout. dk and dv of a shared head are the sum over its
- * query heads, in a fixed order. Takes 8 bytes per query row and up to a few hundred 64 KB
- * partial sums (of key blocks that many queries see) from the library's stream-ordered pool. No
- * counterpart in the reference.
+ * Backward of mfa_fwd_window, of the same types and head dims: dq, dk, dv from q, k, v, out, lse,
+ * dout. dk and dv of a shared head are the sum over its query heads, in a fixed order. Takes 8 bytes
+ * per query row and up to a few hundred partial sums of 64 KB (D = 128: 128 KB; of key blocks that
+ * many queries see) from the library's stream-ordered pool. No counterpart in the reference.
  */
 MFA_API int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
                            const void* dout, const float* lse, void* dq, void* dk, void* dv,

@@ -639,9 +639,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward_window", &flash_attn_forward_window,
         "Forward with a sliding window and sink tokens: [out] or, with_lse, [out, lse]");
   m.def("backward_window", &flash_attn_backward_window,
-        "Backward of forward_window: (dq, dk, dv) (D = 64)");
+        "Backward of forward_window: (dq, dk, dv)");
   m.def("window_attention", &window_attention,
-        "Differentiable forward_window (gradients for D = 64)");
+        "Differentiable forward_window");
   m.def("extend_block_tables", &extend_block_tables,
         "Pages and slots for new tokens of a paged cache: (slots, starts, used)");
   m.def("append_kv", &append_kv, "Rows of k and v to their slots of a paged cache");

@@ -65,6 +65,9 @@ struct BwdParams {
   int pieces_rest;
   int* claimed;      // units of this pass handed out so far
   float* partials;   // dK/dV: [slot][dK, dV][128][D] of the units in pieces
+  // D = 128: the pass's gradient and its strides
+  uint16_t* grad;
+  long long grad_b, grad_h, grad_n;
 };
 
 template <class Cfg>
@@ -96,10 +99,18 @@ struct BwdConfig {
   static constexpr int kTileBytes = kRows * kHeadDim * 2;
   static constexpr int kBoxes = kHeadDim / 64;       // 64-column boxes of a tile
   static constexpr int kBoxBytes = kRows * 64 * 2;
-  // two buffers for the resident tiles and three stages; D = 128, whose tiles are twice as
-  // large, one and two
-  static constexpr int STAGES = kD_ == 64 ? 3 : 2;
-  static constexpr int kResBuffers = kD_ == 64 ? 2 : 1;
+  // D = 64: two buffers for the resident tiles, three stages of a pair of streamed tiles.
+  // D = 128, whose tiles are twice as large (seven fit): one buffer, and a ring for each streamed
+  // tile of a step. The accumulation's operand (`late`: s0, in the dV pass s1) is held until
+  // the step's end and has three stages; the other (`early`) is free after the S and dP
+  // products and makes do with two (three in the dV pass, which has no second resident tile). With two stages of both tiles
+  // together a step waited for its 64 KB from L2: 576 us where this took 473 (16 heads x 8192,
+  // window 2048).
+  static constexpr bool kSplit = kD_ == 128;
+  static constexpr int STAGES = 3;
+  static constexpr int kEarly = kOnlyDV ? 3 : 2;
+  static constexpr int kVecSlots = kSplit ? 2 : STAGES;
+  static constexpr int kResBuffers = kSplit ? 1 : 2;
   static constexpr int kResTiles = kOnlyDV ? 1 : 2;
   // buffer of a CTA's s-th unit, and the phase of its barriers
   __host__ __device__ static constexpr int res_buffer(int s) { return kResBuffers == 1 ? 0 : s & 1; }
@@ -122,12 +133,20 @@ struct BwdConfig {
   static constexpr int kSoftmaxRegs = 104;
   static constexpr int kControlRegs = 64;
 
-  // shared memory (1024-aligned base)
-  static constexpr int kResOff = 0;                                  // [buffers][x, y]
-  static constexpr int kStrOff = kResOff + kResBuffers * 2 * kTileBytes;  // [STAGES][tile 0, tile 1]
-  static constexpr int kVecBytes = 2 * kCols * 4;                    // L2 slice, D slice
-  static constexpr int kVecOff = kStrOff + STAGES * 2 * kTileBytes;  // [STAGES] (dK/dV pass)
-  static constexpr int kBarOff = kVecOff + (kDKV ? STAGES * kVecBytes : 0);
+  // Shared memory (1024-aligned base). kSplit takes all of it: the slices and barriers lie in
+  // front of the tiles, and the base is aligned by its declaration. Else slices and barriers lie
+  // behind, with room for rounding the base up.
+  static constexpr int kVecBytes = 2 * kCols * 4;  // L2 slice, D slice
+  static constexpr int kHeaderBytes = kSplit ? 3 * 1024 : 0;
+  static constexpr int kResOff = kHeaderBytes;  // [buffers][x, y]
+  static constexpr int kStrOff = kResOff + kResBuffers * kResTiles * kTileBytes;
+                                                // [STAGES][tile 0, tile 1]; kSplit: [STAGES] late
+  static constexpr int kStageBytes = kSplit ? kTileBytes : 2 * kTileBytes;
+  static constexpr int kEarlyOff = kStrOff + STAGES * kStageBytes;  // kSplit: [kEarly]
+  static constexpr int kTilesEnd = kEarlyOff + (kSplit ? kEarly * kTileBytes : 0);
+  static constexpr int kVecOff = kSplit ? 0 : kTilesEnd;  // [kVecSlots] (dK/dV pass)
+  static constexpr int kBarOff = kSplit ? kVecSlots * kVecBytes
+                                        : kVecOff + (kDKV ? kVecSlots * kVecBytes : 0);
   static constexpr int kBarResFull = 0;   // [2]
   static constexpr int kBarResEmpty = 2;  // [2]
   static constexpr int kBarStrFull = 4;   // [STAGES]
@@ -142,11 +161,18 @@ struct BwdConfig {
   static constexpr int kClaims = 4;
   static constexpr int kBarClaimFull = kBarDrain + 2;  // [kClaims]
   static constexpr int kBarClaimEmpty = kBarClaimFull + (kWindow ? kClaims : 0);
-  static constexpr int kNumBars = kBarClaimEmpty + (kWindow ? kClaims : 0);
-  static constexpr int kClaimReaders = kSoftmaxWarps + 3;  // two MMA warps and the store thread
+  static constexpr int kBarEarlyFull = kBarClaimEmpty + (kWindow ? kClaims : 0);  // kSplit: [3]
+  static constexpr int kBarEarlyEmpty = kBarEarlyFull + (kSplit ? 3 : 0);         // [3]
+  static constexpr int kBarVecFull = kBarEarlyEmpty + (kSplit ? 3 : 0);           // [2]
+  static constexpr int kBarVecEmpty = kBarVecFull + (kSplit ? 2 : 0);             // [2]
+  static constexpr int kNumBars = kBarVecEmpty + (kSplit ? 2 : 0);
+  // two MMA warps and, if outputs are staged, the store thread
+  static constexpr int kClaimReaders = kSoftmaxWarps + (kSplit ? 2 : 3);
   static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
   static constexpr int kAbortOff = kTmemSlotOff + 4;
-  static constexpr int kSmemBytes = kAbortOff + 4 + (kWindow ? 4 * kClaims : 0) + 1024;
+  static constexpr int kSmemBytes =
+      kSplit ? kTilesEnd : kAbortOff + 4 + (kWindow ? 4 * kClaims : 0) + 1024;
+  static_assert(!kSplit || kAbortOff + 4 + 4 * kClaims <= kHeaderBytes, "header in front of the tiles");
 
   static constexpr int kTmemCols = 512;
   static constexpr int kColS = 0;
@@ -406,6 +432,7 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
   cur.init(p, claims, BwdRole::kLoad);
   int g = 0;
   int res_loaded = 0, str_issued = 0;
+  [[maybe_unused]] int early_issued = 0, vec_issued = 0;
   HeadBatch res = {0, 0};              // of the resident tiles
   [[maybe_unused]] int str_h = 0;      // window variant: first head that the unit streams
   while (cur.valid()) {
@@ -419,10 +446,10 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
     } else {
       hb = res = cur.resident(p);
     }
-    if (cur.first_step()) {
+    auto load_resident = [&]() -> bool {
       const int s = cur.seg, b = Cfg::res_buffer(s);
       if (!wait_single(bar(Cfg::kBarResEmpty + b), Cfg::res_phase(s) ^ 1u, wd, kSiteLoadQEmpty))
-        break;
+        return false;
       mbar_arrive_expect_tx(bar(Cfg::kBarResFull + b), Cfg::kResTiles * Cfg::kTileBytes);
       const int row = cur.row_block(p) * Cfg::kRows;
       const uint32_t dst = sbase + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
@@ -435,43 +462,80 @@ __device__ __forceinline__ void bwd_load_role(const BwdParams& p, uint8_t* smem,
                       bar(Cfg::kBarResFull + b), 64 * x, row, res.h, res.b);
       }
       res_loaded = s + 1;
+      return true;
+    };
+    if (!Cfg::kSplit && cur.first_step()) {
+      if (!load_resident()) break;
     }
     const int st = g % ST;
-    if (!wait_single(bar(Cfg::kBarStrEmpty + st), (static_cast<uint32_t>(g / ST) & 1u) ^ 1u, wd,
-                     kSiteLoadKEmpty))
-      break;
-    mbar_arrive_expect_tx(bar(Cfg::kBarStrFull + st),
-                          2 * Cfg::kTileBytes + (Cfg::kDKV ? Cfg::kVecBytes : 0));
     const int row = cur.block() * Cfg::kCols;
-    const uint32_t dst = sbase + Cfg::kStrOff + st * 2 * Cfg::kTileBytes;
-#pragma unroll
-    for (int x = 0; x < Cfg::kBoxes; ++x) {
-      tma_load_4d_hint(dst + x * Cfg::kBoxBytes, &p.tm_s0, bar(Cfg::kBarStrFull + st), 64 * x, row,
-                       hb.h, hb.b, keep);
-      tma_load_4d_hint(dst + Cfg::kTileBytes + x * Cfg::kBoxBytes, &p.tm_s1,
-                       bar(Cfg::kBarStrFull + st), 64 * x, row, hb.h, hb.b, keep);
-    }
-    if (Cfg::kDKV) {
-      // L2 and D of the 128 streamed queries (padded arrays: 512-byte aligned slices)
+    // L2 and D of the 128 streamed queries (padded arrays: 512-byte aligned slices)
+    auto load_vec = [&](int slot, uint32_t full) {
       const size_t off = cur.vec_row(p) * p.blocks * Cfg::kCols + row;
-      const uint32_t vdst = sbase + Cfg::kVecOff + st * Cfg::kVecBytes;
-      bulk_load(vdst, p.lse2 + off, Cfg::kCols * 4, bar(Cfg::kBarStrFull + st));
-      bulk_load(vdst + Cfg::kCols * 4, p.di + off, Cfg::kCols * 4, bar(Cfg::kBarStrFull + st));
+      const uint32_t vdst = sbase + Cfg::kVecOff + slot * Cfg::kVecBytes;
+      bulk_load(vdst, p.lse2 + off, Cfg::kCols * 4, full);
+      bulk_load(vdst + Cfg::kCols * 4, p.di + off, Cfg::kCols * 4, full);
+    };
+    if constexpr (Cfg::kSplit) {
+      auto load_tile = [&](uint32_t dst, const CUtensorMap* map, uint32_t full) {
+        mbar_arrive_expect_tx(full, Cfg::kTileBytes);
+#pragma unroll
+        for (int x = 0; x < Cfg::kBoxes; ++x)
+          tma_load_4d_hint(dst + x * Cfg::kBoxBytes, map, full, 64 * x, row, hb.h, hb.b, keep);
+      };
+      const int e = g % Cfg::kEarly;
+      if (!wait_single(bar(Cfg::kBarEarlyEmpty + e),
+                       (static_cast<uint32_t>(g / Cfg::kEarly) & 1u) ^ 1u, wd, kSiteLoadKEmpty))
+        break;
+      load_tile(sbase + Cfg::kEarlyOff + e * Cfg::kTileBytes, Cfg::kOnlyDV ? &p.tm_s0 : &p.tm_s1,
+                bar(Cfg::kBarEarlyFull + e));
+      early_issued = g + 1;
+      if (!wait_single(bar(Cfg::kBarStrEmpty + st), (static_cast<uint32_t>(g / ST) & 1u) ^ 1u, wd,
+                       kSiteLoadKEmpty))
+        break;
+      load_tile(sbase + Cfg::kStrOff + st * Cfg::kTileBytes, Cfg::kOnlyDV ? &p.tm_s1 : &p.tm_s0,
+                bar(Cfg::kBarStrFull + st));
+      str_issued = g + 1;
+      // behind the streamed tiles, whose stages are free before the last unit's resident ones
+      if (cur.first_step() && !load_resident()) break;
+      if constexpr (Cfg::kDKV) {
+        if (!wait_single(bar(Cfg::kBarVecEmpty + (g & 1)), (static_cast<uint32_t>(g >> 1) & 1u) ^ 1u,
+                         wd, kSiteLoadKEmpty))
+          break;
+        mbar_arrive_expect_tx(bar(Cfg::kBarVecFull + (g & 1)), Cfg::kVecBytes);
+        load_vec(g & 1, bar(Cfg::kBarVecFull + (g & 1)));
+        vec_issued = g + 1;
+      }
+    } else {
+      if (!wait_single(bar(Cfg::kBarStrEmpty + st), (static_cast<uint32_t>(g / ST) & 1u) ^ 1u, wd,
+                       kSiteLoadKEmpty))
+        break;
+      mbar_arrive_expect_tx(bar(Cfg::kBarStrFull + st),
+                            2 * Cfg::kTileBytes + (Cfg::kDKV ? Cfg::kVecBytes : 0));
+      const uint32_t dst = sbase + Cfg::kStrOff + st * 2 * Cfg::kTileBytes;
+      tma_load_4d_hint(dst, &p.tm_s0, bar(Cfg::kBarStrFull + st), 0, row, hb.h, hb.b, keep);
+      tma_load_4d_hint(dst + Cfg::kTileBytes, &p.tm_s1, bar(Cfg::kBarStrFull + st), 0, row, hb.h,
+                       hb.b, keep);
+      if (Cfg::kDKV) load_vec(st, bar(Cfg::kBarStrFull + st));
+      str_issued = g + 1;
     }
-    str_issued = g + 1;
     ++g;
     cur.step(p);
   }
   if (*wd.abort) {
-    for (int b = 0; b < Cfg::kResBuffers; ++b) {
-      int last = -1;
-      for (int s = b; s < res_loaded; s += Cfg::kResBuffers) last = s;
-      if (last >= 0) drain_wait(bar(Cfg::kBarResFull + b), Cfg::res_phase(last));
-    }
-    for (int st = 0; st < ST; ++st) {
-      int last = -1;
-      for (int x = st; x < str_issued; x += ST) last = x;
-      if (last >= 0) drain_wait(bar(Cfg::kBarStrFull + st), static_cast<uint32_t>(last / ST) & 1u);
+    // the last copies into each of a ring's `slots`, of `issued`
+    auto drain = [&](int full, int slots, int issued) {
+      for (int i = 0; i < slots; ++i) {
+        int last = -1;
+        for (int x = i; x < issued; x += slots) last = x;
+        if (last >= 0) drain_wait(bar(full + i), static_cast<uint32_t>(last / slots) & 1u);
+      }
+    };
+    drain(Cfg::kBarResFull, Cfg::kResBuffers, res_loaded);
+    drain(Cfg::kBarStrFull, ST, str_issued);
+    if constexpr (Cfg::kSplit) {
+      drain(Cfg::kBarEarlyFull, Cfg::kEarly, early_issued);
+      drain(Cfg::kBarVecFull, 2, vec_issued);
     }
   }
 }
@@ -495,6 +559,7 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
   // MN-major (the streamed rows are the K of the accumulations): the leading offset goes from one
   // 64-column box to the next (unused at D = 64)
   const uint32_t str_mn_lo = smem_desc_lo(sbase + Cfg::kStrOff, Cfg::kBoxBytes);
+  [[maybe_unused]] const uint32_t early_lo = smem_desc_lo(sbase + Cfg::kEarlyOff, 16);
   // descriptor offset (16-byte units) of the kk-th 16 columns of a K-major tile
   auto k_off = [](int kk) -> uint32_t {
     return static_cast<uint32_t>((kk >> 2) * (Cfg::kBoxBytes >> 4) + (kk & 3) * 2);
@@ -513,8 +578,17 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
         return false;
     }
     const int st = gs % ST;
-    if (!wait_warp(bar(Cfg::kBarStrFull + st), static_cast<uint32_t>(gs / ST) & 1u, wd, kSiteMmaK))
-      return false;
+    [[maybe_unused]] const int e = gs % Cfg::kEarly;
+    if constexpr (Cfg::kSplit) {
+      if (!wait_warp(bar(Cfg::kBarEarlyFull + e), static_cast<uint32_t>(gs / Cfg::kEarly) & 1u, wd,
+                     kSiteMmaK))
+        return false;
+    }
+    if (!Cfg::kOnlyDV) {
+      if (!wait_warp(bar(Cfg::kBarStrFull + st), static_cast<uint32_t>(gs / ST) & 1u, wd,
+                     kSiteMmaK))
+        return false;
+    }
     if (gs > 0) {
       if (!wait_warp(bar(Cfg::kBarSSFree), static_cast<uint32_t>(gs - 1) & 1u, wd, kSiteMmaSFree))
         return false;
@@ -522,7 +596,11 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
     tc_fence_after();
     if (leader) {
       const uint32_t xd = res_lo + b * 2 * kTile, yd = xd + kTile;
-      const uint32_t s0 = str_lo + st * 2 * kTile, s1 = s0 + kTile;
+      uint32_t s0 = str_lo + st * 2 * kTile, s1 = s0 + kTile;
+      if constexpr (Cfg::kSplit) {
+        s1 = early_lo + e * kTile;  // unused in the dV pass
+        s0 = Cfg::kOnlyDV ? s1 : str_lo + st * kTile;
+      }
 #pragma unroll
       for (int kk = 0; kk < Cfg::kHeadDim / 16; ++kk)  // S = x s0^T
         mma_ss(tmem + Cfg::kColS, desc_join(xd + k_off(kk), kHi), desc_join(s0 + k_off(kk), kHi),
@@ -534,7 +612,11 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
                  kIdescSS, kk > 0 ? 1u : 0u);
       }
       mma_commit(bar(Cfg::kBarSSFull));
-      mma_commit(bar(Cfg::kBarStrEmpty + st));
+      if constexpr (Cfg::kSplit) {
+        mma_commit(bar(Cfg::kBarEarlyEmpty + e));
+        if (cur.left == 0) mma_commit(bar(Cfg::kBarResEmpty));  // the unit's last products
+      }
+      if constexpr (!Cfg::kOnlyDV) mma_commit(bar(Cfg::kBarStrEmpty + st));
     }
     __syncwarp();
     issued_any = true;
@@ -559,7 +641,8 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
       tc_fence_after();
       if (leader) {
         const bool fresh = cur.first_step();
-        const uint32_t s0 = str_mn_lo + st * 2 * kTile, s1 = s0 + kTile;
+        const uint32_t s0 = str_mn_lo + st * (Cfg::kStageBytes >> 4);  // kSplit: the late tile
+        [[maybe_unused]] const uint32_t s1 = s0 + kTile;
         if (Cfg::kBoth) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // dV += P^T dO
@@ -573,11 +656,11 @@ __device__ __forceinline__ void bwd_mma_role(const BwdParams& p, uint8_t* smem, 
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // dQ += dS k; dK += dS^T q or dV += P^T dO alone
             mma_ts(tmem + Cfg::kColAcc0, tmem + Cfg::kColOp0 + 8 * kk,
-                   desc_join((Cfg::kOnlyDV ? s1 : s0) + 128 * kk, kHi), kIdescTS,
-                   (!fresh || kk > 0) ? 1u : 0u);
+                   desc_join(s0 + 128 * kk, kHi), kIdescTS, (!fresh || kk > 0) ? 1u : 0u);
         }
         mma_commit(bar(Cfg::kBarAccDone));
         mma_commit(bar(Cfg::kBarStrEmpty + st));
+        if constexpr (Cfg::kSplit && Cfg::kDKV) mma_commit(bar(Cfg::kBarVecEmpty + (gp & 1)));
       }
       __syncwarp();
       issued_any = true;
@@ -701,13 +784,13 @@ __device__ __forceinline__ bool bwd_step(const BwdParams& p, uint8_t* smem, uint
 
   const uint64_t c2 = f2_splat(p.scale_log2);
   [[maybe_unused]] uint32_t pk[16], dk[16];  // [2i + r]: row g + 8r, columns 8i + q2, 8i + q2 + 1 (16x128b)
-  const int st = g % Cfg::STAGES;
+  const int st = g % Cfg::kVecSlots;
   const float* vec = reinterpret_cast<const float*>(smem + Cfg::kVecOff + st * Cfg::kVecBytes);
   if (Cfg::kDKV) {
     // the L2 / D slices came by bulk copy: observe their completion before reading them (the
     // stage cannot be refilled before this step's OpFull)
-    if (!wait_warp(bar(Cfg::kBarStrFull + st), static_cast<uint32_t>(g / Cfg::STAGES) & 1u, wd,
-                   kSiteSoftStage))
+    if (!wait_warp(bar((Cfg::kSplit ? Cfg::kBarVecFull : Cfg::kBarStrFull) + st),
+                   static_cast<uint32_t>(g / Cfg::kVecSlots) & 1u, wd, kSiteSoftStage))
       return false;
   }
 #pragma unroll
@@ -810,10 +893,32 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
     if (!wait_warp(bar(Cfg::kBarAccDone), static_cast<uint32_t>(g - 1) & 1u, wd, kSiteSoftOFinal))
       return;
     tc_fence_after();
-    uint8_t* res = smem + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
-    // This warp's half of the accumulator's columns, 32 at a time: `c0` on are 16-byte chunks
-    // c0 % 64 / 8 .. + 3 of each of its rows in box c0 / 64 of the 128B-swizzled staging tile.
+    [[maybe_unused]] uint8_t* res = smem + Cfg::kResOff + b * 2 * Cfg::kTileBytes;
+    // This warp's 32 of the accumulator's columns: 16-byte chunks 4 * half .. 4 * half + 3 of each of
+    // its rows in the 128B-swizzled staging tile.
     auto stage_acc = [&](uint32_t col, float mul, uint8_t* dst_tile) {
+      uint32_t a[16];
+      tmem_ld_16x256b_sync(tmem + lb + col + 32 * half, a);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = slice + gq + 8 * r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = pack_pair<Cfg::kBF16>(__uint_as_float(a[4 * i + 2 * r]) * mul,
+                                                   __uint_as_float(a[4 * i + 2 * r + 1]) * mul);
+          const uint32_t dst =
+              smem_addr(dst_tile + row * 128 + (((4 * half + i) ^ (row & 7)) << 4) + 4 * q);
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
+        }
+      }
+    };
+    // kSplit: straight to global memory, 16 bytes a thread after a transposition inside each
+    // quad (64 bytes a row). The resident tiles are then free after the last products that read
+    // them, and the next unit's are loaded while this one ends. (Staged: 473 us where this takes
+    // 449, at 16 heads x 8192, window 2048; 244 and 223 at 4 x 16 x 2048, window 512.)
+    [[maybe_unused]] auto write_acc = [&](uint32_t col, float mul) {
+      const HeadBatch hb = cur.resident(p);
+      uint16_t* at = p.grad + hb.b * p.grad_b + hb.h * p.grad_h + (row0 + gq) * p.grad_n + 8 * q;
 #pragma unroll
       for (int sub = 0; sub < Cfg::kBoxes; ++sub) {
         const int c0 = Cfg::kHeadDim / 2 * half + 32 * sub;
@@ -821,16 +926,27 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
         tmem_ld_16x256b_sync(tmem + lb + col + c0, a);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int row = slice + gq + 8 * r;
+          uint32_t w[4];  // columns c0 + 8 i + 2 q, + 1
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = pack_pair<Cfg::kBF16>(__uint_as_float(a[4 * i + 2 * r]) * mul,
-                                                     __uint_as_float(a[4 * i + 2 * r + 1]) * mul);
-            const int chunk = (c0 & 63) / 8 + i;
-            const uint32_t dst = smem_addr(dst_tile + (c0 >> 6) * Cfg::kBoxBytes + row * 128 +
-                                           ((chunk ^ (row & 7)) << 4) + 4 * q);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
+          for (int i = 0; i < 4; ++i)
+            w[i] = pack_pair<Cfg::kBF16>(__uint_as_float(a[4 * i + 2 * r]) * mul,
+                                         __uint_as_float(a[4 * i + 2 * r + 1]) * mul);
+#pragma unroll
+          for (int bit = 1; bit <= 2; bit <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (i & bit) continue;
+              const uint32_t got =
+                  __shfl_xor_sync(0xffffffffu, (q & bit) ? w[i] : w[i + bit], bit);
+              if (q & bit)
+                w[i] = got;
+              else
+                w[i + bit] = got;
+            }
           }
+          if (row0 + gq + 8 * r < p.n)
+            *reinterpret_cast<uint4*>(at + 8 * r * p.grad_n + c0) =
+                make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
     };
@@ -863,15 +979,18 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
     } else if constexpr (Cfg::kBoth) {
       stage_acc(Cfg::kColAcc1, p.scale, res);                    // dK over the k tile
       stage_acc(Cfg::kColAcc0, 1.0f, res + Cfg::kTileBytes);     // dV over the v tile
+    } else if constexpr (Cfg::kSplit) {
+      write_acc(Cfg::kColAcc0, Cfg::kOnlyDV ? 1.0f : p.scale);
     } else {
-      // dQ over the q tile; dK or dV over the k tile
-      stage_acc(Cfg::kColAcc0, Cfg::kOnlyDV ? 1.0f : p.scale, res);
+      stage_acc(Cfg::kColAcc0, p.scale, res);                    // dQ over the q tile
     }
     tc_fence_before();
-    fence_proxy_async_smem();
-    __syncwarp();
-    // staging rows written: the store warp takes the unit from here (bwd_store_role)
-    if (lane == 0) mbar_arrive(bar(Cfg::kBarStage));
+    if constexpr (!Cfg::kSplit) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      // staging rows written: the store warp takes the unit from here (bwd_store_role)
+      if (lane == 0) mbar_arrive(bar(Cfg::kBarStage));
+    }
     cur.next_unit(p);
   }
 }
@@ -894,9 +1013,7 @@ __device__ __forceinline__ void bwd_store_role(const BwdParams& p, uint8_t* smem
     if (!cur.in_pieces()) {
       const int r0 = cur.row_block(p) * Cfg::kRows;
       const HeadBatch hb = cur.resident(p);
-#pragma unroll
-      for (int x = 0; x < Cfg::kBoxes; ++x)
-        tma_store_4d(&p.tm_o0, smem_addr(res + x * Cfg::kBoxBytes), 64 * x, r0, hb.h, hb.b);
+      tma_store_4d(&p.tm_o0, smem_addr(res), 0, r0, hb.h, hb.b);
       if (Cfg::kBoth) tma_store_4d(&p.tm_o1, smem_addr(res + Cfg::kTileBytes), 0, r0, hb.h, hb.b);
       tma_store_commit();
       tma_store_wait_read();
@@ -918,7 +1035,18 @@ __device__ __forceinline__ void bwd_init_bars(uint32_t bars) {
   }
   for (int s = 0; s < Cfg::STAGES; ++s) {
     mbar_init(bars + 8 * (Cfg::kBarStrFull + s), 1);
-    mbar_init(bars + 8 * (Cfg::kBarStrEmpty + s), 2);  // both MMA issuers read the stage
+    // both MMA issuers read the stage (the dV pass's late tile: the accumulation alone)
+    mbar_init(bars + 8 * (Cfg::kBarStrEmpty + s), Cfg::kOnlyDV ? 1 : 2);
+  }
+  if constexpr (Cfg::kSplit) {
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(bars + 8 * (Cfg::kBarEarlyFull + s), 1);
+      mbar_init(bars + 8 * (Cfg::kBarEarlyEmpty + s), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bars + 8 * (Cfg::kBarVecFull + s), 1);
+      mbar_init(bars + 8 * (Cfg::kBarVecEmpty + s), 1);
+    }
   }
   mbar_init(bars + 8 * Cfg::kBarSSFull, 1);
   mbar_init(bars + 8 * Cfg::kBarSSFree, Cfg::kSoftmaxWarps);
@@ -958,9 +1086,18 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
   static_assert(kAbortOff + 4 + kRingBytes + 1024 <=
                     (kSmem2 > CC::kSmemBytes ? kSmem2 : CC::kSmemBytes),
                 "barriers inside the launch's shared memory");
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  static_assert(CA::kSplit == CB::kSplit && CA::kSplit == CC::kSplit &&
+                    (!CA::kSplit || (CA::kBarOff == CB::kBarOff && CA::kBarOff == CC::kBarOff)),
+                "passes of one CTA share the header");
+  uint8_t* smem;
+  if constexpr (CA::kSplit) {
+    extern __shared__ __align__(1024) uint8_t smem_aligned[];
+    smem = smem_aligned;
+  } else {
+    extern __shared__ uint8_t smem_raw[];
+    smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                      ~static_cast<uintptr_t>(1023));
+  }
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t bars = smem_addr(smem + kBarOff);
@@ -1038,7 +1175,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
       } else if (warp == CA::kAccWarp) {
         bwd_mma_role<CA, true>(pa, smem, bars, tmem, wd, claims);
       } else if (warp == CA::kStoreWarp) {
-        if (lane == 0) bwd_store_role<CA>(pa, smem, bars, wd, claims);
+        if (!CA::kSplit && lane == 0) bwd_store_role<CA>(pa, smem, bars, wd, claims);
       }
       if constexpr (kPasses > 1) {
         if (next_pass(CB{})) {
@@ -1047,7 +1184,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
           } else if (warp == CB::kAccWarp) {
             bwd_mma_role<CB, true>(pb, smem, bars, tmem, wd, claims);
           } else if (warp == CB::kStoreWarp) {
-            if (lane == 0) bwd_store_role<CB>(pb, smem, bars, wd, claims);
+            if (!CB::kSplit && lane == 0) bwd_store_role<CB>(pb, smem, bars, wd, claims);
           }
           if constexpr (kPasses > 2) {
             if (next_pass(CC{})) {
@@ -1056,7 +1193,7 @@ __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb
               } else if (warp == CC::kAccWarp) {
                 bwd_mma_role<CC, true>(pc, smem, bars, tmem, wd, claims);
               } else if (warp == CC::kStoreWarp) {
-                if (lane == 0) bwd_store_role<CC>(pc, smem, bars, wd, claims);
+                if (!CC::kSplit && lane == 0) bwd_store_role<CC>(pc, smem, bars, wd, claims);
               }
             }
           }
@@ -1107,7 +1244,10 @@ __global__ void __launch_bounds__(BwdConfig<true, true, kBF16, true>::kThreads, 
   bwd_cta<BwdConfig<true, true, kBF16, true>, CQ, CQ, 2>(pkv, pq, pq);
 }
 
-// D = 128: dK, dV and dQ in a pass each (the dV pass without dP).
+// D = 128: dK, dV and dQ in a pass each (the dV pass without dP): eight products a step where five
+// would do, but S, dP, both operands and both accumulators of dK and dV are 640 columns of TMEM.
+// Measured at 16 query heads x 8192 over 4 k / v heads, window 2048, 16 sinks, bf16: 449 us, 1079
+// TFLOP/s over the eight products (674 over five); D = 64 278 us (545 over five).
 template <bool kBF16>
 using BwdDK128 = BwdConfig<true, true, kBF16, true, 128, BwdPart::kDK>;
 template <bool kBF16>

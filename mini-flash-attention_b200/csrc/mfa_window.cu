@@ -180,7 +180,7 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
 // How the dK/dV pass cuts its units into pieces (BwdWindowCursor). `span_steps` is the number of
 // (key block, query block) pairs of one head that hold a visible (key, query) pair: every pass
 // walks all of them; `passes` is what they cost together, in dQ steps (D = 64: the dK/dV step is
-// about 1.05 of one; D = 128: the dV step about 0.8).
+// about 1.05 of one; D = 128: the dV step, with two products for three, is taken as 0.85).
 struct Pieces {
   int chunk_sink, pieces_sink, chunk_rest, pieces_rest;
 };
@@ -330,8 +330,17 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
         e = launch(ctas, BwdConfig<true, true, kBF16, true>::kThreads, window_bwd_smem<kBF16>(),
                    stream, &mfa_bwd_window_kernel<kBF16>, pq, pkv);
     } else {
+      auto set_grad = [&](BwdParams& to, void* grad, int64_t heads) {
+        const host::Strides g = host::strides_of(w.layout, heads, w.n, w.d);
+        to.grad = static_cast<uint16_t*>(grad);
+        to.grad_b = g.b;
+        to.grad_h = g.h;
+        to.grad_n = g.n;
+      };
+      set_grad(pq, dq, w.heads);
       BwdParams pv = pkv;  // pkv: dK
-      pv.tm_o0 = pkv.tm_o1;
+      set_grad(pkv, dk, w.kv_heads);
+      set_grad(pv, dv, w.kv_heads);
       pv.claimed = counters + 2;
       pv.partials = sums + slots * kTile;
       if (e == cudaSuccess)

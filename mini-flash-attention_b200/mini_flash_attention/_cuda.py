@@ -99,8 +99,8 @@ def backward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
                     lse: torch.Tensor, dout: torch.Tensor, window: int,
                     sinks: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of forward_window for the output gradient dout, given its out and
-    lse (forward_window_lse); dk and dv of a shared head are summed over its query heads. D = 64,
-    fp16 or bf16."""
+    lse (forward_window_lse); dk and dv of a shared head are summed over its query heads.
+    The types and head dims of forward_window."""
     dq, dk, dv = _load_extension().backward_window(q, k, v, out, lse, dout.contiguous(),
                                                    int(window), int(sinks))
     return dq, dk, dv
@@ -108,8 +108,8 @@ def backward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
                      sinks: int = 0) -> torch.Tensor:
-    """Differentiable forward_window (D = 64 for gradients, which can be taken once: a gradient of a
-    gradient raises)."""
+    """Differentiable forward_window (gradients can be taken once: a gradient of a gradient
+    raises)."""
     return _load_extension().window_attention(q, k, v, int(window), int(sinks))
 
 
