@@ -282,7 +282,10 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     torch::autograd::variable_list d;
     {
       const at::NoGradGuard no_grad;
-      d = flash_attn_backward_window(s[0], s[1], s[2], s[3], s[4], grads[0].contiguous(),
+      // what follows the attention chooses this tensor: one that starts off 16 bytes is copied
+      auto dout = grads[0].contiguous();
+      if (reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 != 0) dout = dout.clone();
+      d = flash_attn_backward_window(s[0], s[1], s[2], s[3], s[4], dout,
                                      ctx->saved_data["window"].toInt(),
                                      ctx->saved_data["sinks"].toInt());
     }

@@ -103,9 +103,9 @@ struct BwdConfig {
   // D = 128, whose tiles are twice as large (seven fit): one buffer, and a ring for each streamed
   // tile of a step. The accumulation's operand (`late`: s0, in the dV pass s1) is held until
   // the step's end and has three stages; the other (`early`) is free after the S and dP
-  // products and makes do with two (three in the dV pass, which has no second resident tile). With two stages of both tiles
-  // together a step waited for its 64 KB from L2: 576 us where this took 473 (16 heads x 8192,
-  // window 2048).
+  // products and makes do with two (three in the dV pass, which has no second resident tile). With
+  // two stages of both tiles together a step waited for its 64 KB from L2: 576 us where this took
+  // 473 (16 heads x 8192, window 2048).
   static constexpr bool kSplit = kD_ == 128;
   static constexpr int STAGES = 3;
   static constexpr int kEarly = kOnlyDV ? 3 : 2;
@@ -1067,9 +1067,9 @@ __device__ __forceinline__ void bwd_init_bars(uint32_t bars) {
 // One CTA: the units of pass CA (params pa), then, with kPasses > 1, those of pass CB (params pb),
 // then, with 3, those of CC (pc). Between the passes every role has finished (the MMA warps drain
 // their commits, the store thread waits for its stores' shared-memory reads), the CTA meets on
-// named barrier 2 and the barriers start afresh; TMEM stays allocated. The barriers live past all passes' shared-memory
-// layouts. Each role's calls stay inside its setmaxnreg branch, which is what lets the
-// register allocator give the softmax-side warps their 104 registers.
+// named barrier 2 and the barriers start afresh; TMEM stays allocated. The barriers live past all
+// passes' shared-memory layouts. Each role's calls stay inside its setmaxnreg branch, which is what
+// lets the register allocator give the softmax-side warps their 104 registers.
 template <class CA, class CB, class CC, int kPasses>
 __device__ __forceinline__ void bwd_cta(const BwdParams& pa, const BwdParams& pb,
                                         const BwdParams& pc) {
@@ -1266,8 +1266,9 @@ __global__ void __launch_bounds__(BwdDQ128<kBF16>::kThreads, 1)
 // dK and dV of the blocks whose units ran in pieces: the sum of the pieces in order, dK scaled. The
 // pieces of slot i are at dk_sums and dv_sums + i * slot_floats. One CTA per 1024 / D rows of a
 // (block, k / v head row) pair that may have pieces, sink blocks first; D / 4 threads a row, four
-// columns each, of the tensors' `cols`. The pieces are read four at a time (an L2 round trip each). (16 heads x 8192, 16
-// sinks, D = 64: 4 blocks of 4 pieces, 3 us behind the passes; one CTA a block took 9.)
+// columns each, of the tensors' `cols`. The pieces are read four at a time (an L2 round trip each).
+// (16 heads x 8192, 16 sinks, D = 64: 4 blocks of 4 pieces, 3 us behind the passes; one CTA a block
+// took 9.)
 template <bool kBF16, int kD>
 __global__ void __launch_bounds__(256)
     mfa_bwd_reduce_kernel(const BwdParams p, const float* dk_sums, const float* dv_sums,

@@ -12,12 +12,13 @@
 // 390 operations a cycle are well inside what the warp-level tensor instruction gives; tcgen05
 // would pad the rows to 64 or 128 and bring the scores through tensor memory for nothing).
 //
-// Two or three CTAs per SM, each of four consumer warps and one producer warp, walk a common list of steps:
-// a step is one 64-key tile of one unit, a unit one (request, k / v head, 16 query rows). The
-// lengths are known to the GPU only, so every CTA sums them and takes an equal share of the
-// steps. Tiles arrive by TMA, one box a page, in a ring of stages. In a tile each warp takes 16 keys with a running maximum of its own; at the end of a
-// unit the four warps' states meet in shared memory. What a CTA's share cuts off goes to a slot
-// of the workspace as unnormalised 32-bit sums, which the combine kernel joins in CTA order.
+// Two or three CTAs per SM, each of four consumer warps and one producer warp, walk a common list
+// of steps: a step is one 64-key tile of one unit, a unit one (request, k / v head, 16 query rows).
+// The lengths are known to the GPU only, so every CTA sums them and takes an equal share of the
+// steps. Tiles arrive by TMA, one box a page, in a ring of stages. In a tile each warp takes 16
+// keys with a running maximum of its own; at the end of a unit the four warps' states meet in
+// shared memory. What a CTA's share cuts off goes to a slot of the workspace as unnormalised 32-bit
+// sums, which the combine kernel joins in CTA order.
 //
 // Measured on a B200 (64 requests of 100 to 16384 tokens, 8 k / v heads of 128, 4 rows each, bf16):
 // 137 us, 6.3 TB/s of k and v, 96% of a copy's rate; DRAM reads equal the k and v bytes. Windows
@@ -305,8 +306,9 @@ __device__ __forceinline__ PagedShare paged_share(const PagedParams& p, int* sca
   return sh;
 }
 
-// Producer warp: the tiles of the share, a box for every page that holds a visible key. Lane i looks up the page of box i of a batch of tiles (32 boxes at most, of one
-// segment); the next batch's are on their way while this one's copies are issued.
+// Producer warp: the tiles of the share, a box for every page that holds a visible key. Lane i
+// looks up the page of box i of a batch of tiles (32 boxes at most, of one segment); the next
+// batch's are on their way while this one's copies are issued.
 template <class Cfg>
 __device__ __forceinline__ void paged_load_role(const PagedParams& p, PagedCursor cur,
                                                 uint32_t smem, uint32_t bars,

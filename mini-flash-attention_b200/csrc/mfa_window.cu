@@ -320,7 +320,8 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
     // the kernels wait for the stream's earlier work themselves and may be set up while it ends
     e = launch(need < most ? need : most, 256, 0, stream, prep_kernel<kBF16>(w.d), out, dout, lse,
-               lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads), static_cast<long long>(st.b),
+               lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads),
+               static_cast<long long>(st.b),
                static_cast<long long>(st.h), static_cast<long long>(st.n),
                static_cast<int>(blocks), counters);
     const int64_t units = kv_units > q_units ? kv_units : q_units;

@@ -253,6 +253,18 @@ def test_capi_bnhd_layout():
     assert capi.device_status(torch.cuda.current_device()) == 0
 
 
+def test_autograd_unaligned_output_gradient():
+    q, k, v, dout = inputs(1, 4, 2, 150, 64, torch.bfloat16)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = mfa.window_attention(*leaves, 40, 2)
+    odd = torch.empty(dout.numel() + 1, device="cuda", dtype=dout.dtype)[1:].view_as(dout)
+    odd.copy_(dout)
+    grads = torch.autograd.grad(out, leaves, odd)
+    want = reference(*(x.detach() for x in leaves), 40, 2, dout)
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        check(name, x, *want[name])
+
+
 def test_empty():
     q = torch.empty((0, 4, 100, 64), device="cuda", dtype=torch.float16)
     k = torch.empty((0, 2, 100, 64), device="cuda", dtype=torch.float16)
