@@ -128,12 +128,15 @@ MFA_API int mfa_bwd(const void* q, const void* k, const void* v, const void* out
  * heads); d = 32, 64 or 128, any n, window >= 1 (at n or more: causal attention), sinks >= 0.
  * lse (may be NULL): the row log-sum-exp over the visible keys, fp32 [B*H, N]. Key blocks that
  * no row of a query block sees are neither read nor computed. k and v must be finite also where
- * they are masked, as for mfa_fwd. No counterpart in the reference.
+ * they are masked, as for mfa_fwd. `strides` (NULL: those of `layout`) are the element strides of
+ * q's, k's and v's batch, head and token dimension, nine values in that order: positive multiples
+ * of 8 (any value for a dimension of one element), as of the parts of a fused projection. The
+ * other tensors are contiguous in `layout`. No counterpart in the reference.
  */
 MFA_API int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
                            int64_t batch, int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
                            int64_t window, int64_t sinks, float scale, int32_t dtype,
-                           int32_t layout, void* stream);
+                           int32_t layout, const int64_t* strides, void* stream);
 
 /*
  * Backward of mfa_fwd_window, of the same types and head dims: dq, dk, dv from q, k, v, out, lse,
@@ -145,7 +148,7 @@ MFA_API int mfa_bwd_window(const void* q, const void* k, const void* v, const vo
                            const void* dout, const float* lse, void* dq, void* dk, void* dv,
                            int64_t batch, int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
                            int64_t window, int64_t sinks, float scale, int32_t dtype,
-                           int32_t layout, void* stream);
+                           int32_t layout, const int64_t* strides, void* stream);
 
 /*
  * Paged key / value cache. k_cache and v_cache are contiguous [pages, kv_heads, page_size, d]
@@ -180,7 +183,8 @@ MFA_API int mfa_append_kv(const void* k, const void* v, void* k_cache, void* v_c
                           int64_t v_head_stride, int64_t pages, int64_t page_size, void* stream);
 
 /*
- * Attention of one query token per request over the cache: q and out are [batch, heads, d], d =
+ * Attention of one query token per request over the cache: q and out are [batch, heads, d], q with
+ * element strides that are positive multiples of 8 (any value for a dimension of one element), d =
  * 64 or 128, heads a multiple of kv_heads (at most 128 query heads a k / v head), page_size 16, 32,
  * 64, 128 or 256. Request r has lengths[r] tokens (int32; clamped to [0, columns * page_size]), the
  * query's own among them; visible are all of them, or with window > 0 those in the newest
@@ -193,9 +197,10 @@ MFA_API int mfa_append_kv(const void* k, const void* v, void* k_cache, void* v_c
 MFA_API int mfa_paged_attention(const void* q, const void* k_cache, const void* v_cache,
                                 const int32_t* block_table, const int32_t* lengths, void* out,
                                 void* workspace, uint64_t workspace_bytes, int64_t batch,
-                                int64_t heads, int64_t kv_heads, int32_t d, int64_t pages,
-                                int64_t page_size, int64_t columns, int64_t window, int64_t sinks,
-                                float scale, int32_t dtype, void* stream);
+                                int64_t heads, int64_t kv_heads, int32_t d, int64_t q_batch_stride,
+                                int64_t q_head_stride, int64_t pages, int64_t page_size,
+                                int64_t columns, int64_t window, int64_t sinks, float scale,
+                                int32_t dtype, void* stream);
 
 /*
  * The same for requests that share their first prefix_length tokens, in the pages prefix_pages
@@ -207,6 +212,7 @@ MFA_API int mfa_shared_prefix_attention(const void* q, const void* k_cache, cons
                                         const int32_t* block_table, const int32_t* lengths,
                                         void* out, void* workspace, uint64_t workspace_bytes,
                                         int64_t batch, int64_t heads, int64_t kv_heads, int32_t d,
+                                        int64_t q_batch_stride, int64_t q_head_stride,
                                         int64_t pages, int64_t page_size, int64_t columns,
                                         float scale, int32_t dtype, void* stream);
 

@@ -177,7 +177,7 @@ std::vector<torch::Tensor> flash_attn_backward(torch::Tensor q, torch::Tensor k,
   return {dq, dk, dv};
 }
 
-// q [B, H, N, D] and k, v [B, Hkv, N, D] of the windowed attention.
+// q [B, H, N, D] and k, v [B, Hkv, N, D] of the windowed attention, with any strides but that of D.
 void check_window_inputs(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v) {
   TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   TORCH_CHECK(k.is_cuda(), "k must be a CUDA tensor");
@@ -188,15 +188,30 @@ void check_window_inputs(const torch::Tensor& q, const torch::Tensor& k, const t
   TORCH_CHECK(v.scalar_type() == q.scalar_type(), "v must have the same dtype as q");
   TORCH_CHECK(k.device() == q.device(), "k must be on the same device as q");
   TORCH_CHECK(v.device() == q.device(), "v must be on the same device as q");
-  TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
-  TORCH_CHECK(k.is_contiguous(), "k must be contiguous");
-  TORCH_CHECK(v.is_contiguous(), "v must be contiguous");
   TORCH_CHECK(q.dim() == 4, "q must have shape [B, H, N, D]");
   TORCH_CHECK(k.dim() == 4 && k.size(0) == q.size(0) && k.size(2) == q.size(2) &&
                   k.size(3) == q.size(3),
               "k must have shape [B, Hkv, N, D] with q's B, N and D");
   TORCH_CHECK(v.sizes() == k.sizes(), "v must have the same shape as k");
+  TORCH_CHECK(q.stride(3) == 1, "q must be contiguous in D");
+  TORCH_CHECK(k.stride(3) == 1, "k must be contiguous in D");
+  TORCH_CHECK(v.stride(3) == 1, "v must be contiguous in D");
 }
+
+// The layout of the outputs, out and the gradients: that of the memory of q.
+bool tokens_first(const torch::Tensor& q) {
+  return q.size(1) > 1 && q.size(2) > 1 && q.stride(1) < q.stride(2);
+}
+
+// The nine strides that mfa_fwd_window and mfa_bwd_window take.
+struct WindowStrides {
+  int64_t of[9];
+  WindowStrides(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v) {
+    int64_t* to = of;
+    for (const auto* x : {&q, &k, &v})
+      for (int i = 0; i < 3; ++i) *to++ = x->stride(i);
+  }
+};
 
 int dtype_of(const torch::Tensor& x) {
   return x.scalar_type() == torch::kBFloat16 ? MFA_DTYPE_BF16 : MFA_DTYPE_FP16;
@@ -206,6 +221,23 @@ int dtype_of(const torch::Tensor& x) {
 // a microsecond each, which a decoding step would notice).
 torch::Tensor new_empty(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
+// An uninitialised [B, H, N, D] tensor, contiguous as that or (bnhd) as [B, N, H, D].
+torch::Tensor new_heads(at::IntArrayRef sizes, bool bnhd, const torch::Tensor& like) {
+  if (!bnhd) return new_empty(sizes, like.scalar_type(), like);
+  const int64_t d = sizes[3], row = sizes[1] * d;
+  return at::detail::empty_strided_cuda(sizes, {sizes[2] * row, d, row, 1}, like.scalar_type(),
+                                        like.device());
+}
+
+// x, or a copy of it if it is not contiguous in that layout or starts off 16 bytes (an output
+// gradient is whatever the operation behind the attention made).
+torch::Tensor dense(const torch::Tensor& x, bool bnhd) {
+  auto y = bnhd ? x.transpose(1, 2).contiguous().transpose(1, 2) : x.contiguous();
+  if (reinterpret_cast<uintptr_t>(y.data_ptr()) % 16 == 0) return y;
+  auto z = new_heads(x.sizes(), bnhd, x);
+  return z.copy_(y);
 }
 
 void* current_stream() {
@@ -218,7 +250,9 @@ std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Ten
                                                      int64_t sinks, bool with_lse) {
   check_window_inputs(q, k, v);
   const c10::cuda::CUDAGuard device_guard(q.device());
-  auto out = new_empty(q.sizes(), q.scalar_type(), q);
+  const bool bnhd = tokens_first(q);
+  const WindowStrides strides(q, k, v);
+  auto out = new_heads(q.sizes(), bnhd, q);
   torch::Tensor lse;
   if (with_lse)
     lse = new_empty({q.size(0), q.size(1), q.size(2)}, torch::kFloat32, q);
@@ -226,8 +260,8 @@ std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Ten
   const int rc = mfa_fwd_window(
       q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
       with_lse ? lse.data_ptr<float>() : nullptr, q.size(0), q.size(1), k.size(1), q.size(2),
-      static_cast<int32_t>(q.size(3)), window, sinks, scale, dtype_of(q), MFA_LAYOUT_BHND,
-      current_stream());
+      static_cast<int32_t>(q.size(3)), window, sinks, scale, dtype_of(q),
+      bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of, current_stream());
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
   if (with_lse) return {out, lse};
   return {out};
@@ -246,21 +280,25 @@ std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Te
               "out and dout must have the same shape as q");
   TORCH_CHECK(out.scalar_type() == q.scalar_type() && dout.scalar_type() == q.scalar_type(),
               "out and dout must have q's dtype");
-  TORCH_CHECK(out.is_contiguous() && dout.is_contiguous() && lse.is_contiguous(),
-              "out, lse and dout must be contiguous");
+  TORCH_CHECK(lse.is_contiguous(), "lse must be contiguous");
   TORCH_CHECK(lse.scalar_type() == torch::kFloat32, "lse must be float32");
   TORCH_CHECK(lse.numel() == q.size(0) * q.size(1) * q.size(2),
               "lse must have one value per query row");
   const c10::cuda::CUDAGuard device_guard(q.device());
-  auto dq = new_empty(q.sizes(), q.scalar_type(), q);
-  auto dk = new_empty(k.sizes(), k.scalar_type(), k);
-  auto dv = new_empty(v.sizes(), v.scalar_type(), v);
+  const bool bnhd = tokens_first(q);
+  const WindowStrides strides(q, k, v);
+  out = dense(out, bnhd);
+  dout = dense(dout, bnhd);
+  auto dq = new_heads(q.sizes(), bnhd, q);
+  auto dk = new_heads(k.sizes(), bnhd, q);
+  auto dv = new_heads(v.sizes(), bnhd, q);
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
   const int rc = mfa_bwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                                 dout.data_ptr(), lse.data_ptr<float>(), dq.data_ptr(),
                                 dk.data_ptr(), dv.data_ptr(), q.size(0), q.size(1), k.size(1),
                                 q.size(2), static_cast<int32_t>(q.size(3)), window, sinks, scale,
-                                dtype_of(q), MFA_LAYOUT_BHND, current_stream());
+                                dtype_of(q), bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of,
+                                current_stream());
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
   return {dq, dk, dv};
 }
@@ -282,10 +320,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     torch::autograd::variable_list d;
     {
       const at::NoGradGuard no_grad;
-      // what follows the attention chooses this tensor: one that starts off 16 bytes is copied
-      auto dout = grads[0].contiguous();
-      if (reinterpret_cast<uintptr_t>(dout.data_ptr()) % 16 != 0) dout = dout.clone();
-      d = flash_attn_backward_window(s[0], s[1], s[2], s[3], s[4], dout,
+      d = flash_attn_backward_window(s[0], s[1], s[2], s[3], s[4], grads[0],
                                      ctx->saved_data["window"].toInt(),
                                      ctx->saved_data["sinks"].toInt());
     }
@@ -394,9 +429,9 @@ torch::Tensor attend_pages(const torch::Tensor& q, const torch::Tensor& k_cache,
   check_cache(k_cache, v_cache);
   TORCH_CHECK(q.device() == k_cache.device(), "k_cache must be on the same device as q");
   TORCH_CHECK(q.scalar_type() == k_cache.scalar_type(), "k_cache must have the same dtype as q");
-  TORCH_CHECK(q.is_contiguous(), "q must be contiguous");
   TORCH_CHECK(q.dim() == 3 && q.size(2) == k_cache.size(3),
               "q must have shape [B, H, D] with the cache's D");
+  TORCH_CHECK(q.stride(2) == 1, "q must be contiguous in D");
   check_index(block_table, "block_table", q);
   check_index(lengths, "lengths", q);
   const int64_t batch = q.size(0);
@@ -427,13 +462,13 @@ torch::Tensor attend_pages(const torch::Tensor& q, const torch::Tensor& k_cache,
                  q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                  prefix_pages->data_ptr<int>(), prefix_length, block_table.data_ptr<int>(),
                  lengths.data_ptr<int>(), out.data_ptr(), workspace.data_ptr(), bytes, batch,
-                 q.size(1), k_cache.size(1), d, k_cache.size(0), page_size, block_table.size(1),
-                 scale, dtype_of(q), current_stream())
+                 q.size(1), k_cache.size(1), d, q.stride(0), q.stride(1), k_cache.size(0),
+                 page_size, block_table.size(1), scale, dtype_of(q), current_stream())
            : mfa_paged_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                  block_table.data_ptr<int>(), lengths.data_ptr<int>(),
                                  out.data_ptr(), workspace.data_ptr(), bytes, batch, q.size(1),
-                                 k_cache.size(1), d, k_cache.size(0), page_size,
-                                 block_table.size(1), window, sinks, scale, dtype_of(q),
+                                 k_cache.size(1), d, q.stride(0), q.stride(1), k_cache.size(0),
+                                 page_size, block_table.size(1), window, sinks, scale, dtype_of(q),
                                  current_stream());
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
   return out;

@@ -201,15 +201,12 @@ Strides layout_strides(int layout, int64_t heads, int64_t n, int64_t d) {
 // 4-D TMA view {D, N, H, B} of one tensor, box {min(D, 64), 128, 1, 1}: 128-byte swizzle for
 // 64-column boxes, 64-byte swizzle for D = 32. The N extent keeps tiles inside their head:
 // rows past N read as zero and are not stored.
-// `rows` (default n) rows per head starting at `base`; the strides are those of an N = n tensor.
-int encode_tensor(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
-                  int64_t d, int layout, bool bf16, int64_t rows = -1) {
+int encode_strided(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t rows,
+                   int64_t d, const Strides& st, bool bf16) {
   std::string why;
   auto encode = tensor_map_encoder(&why);
   if (!encode) return fail(MFA_ERR_CUDA, why);
-  const Strides st = layout_strides(layout, heads, n, d);
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d),
-                              static_cast<cuuint64_t>(rows < 0 ? n : rows),
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(batch)};
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(st.n) * 2,
                                  static_cast<cuuint64_t>(st.h) * 2,
@@ -225,6 +222,13 @@ int encode_tensor(CUtensorMap* map, const void* base, int64_t batch, int64_t hea
   if (r != CUDA_SUCCESS)
     return fail(MFA_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
   return MFA_OK;
+}
+
+// `rows` (default n) rows per head starting at `base`; the strides are those of an N = n tensor.
+int encode_tensor(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
+                  int64_t d, int layout, bool bf16, int64_t rows = -1) {
+  return encode_strided(map, base, batch, heads, rows < 0 ? n : rows, d,
+                        layout_strides(layout, heads, n, d), bf16);
 }
 
 // Launches the split-mode merge as a programmatic dependent of the forward kernel just
@@ -588,8 +592,8 @@ int check_pointer(const void* p, const char* name, int dev) {
 }
 
 int encode_heads(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
-                 int64_t d, int layout, bool bf16) {
-  return encode_tensor(map, base, batch, heads, n, d, layout, bf16);
+                 int64_t d, const Strides& strides, bool bf16) {
+  return encode_strided(map, base, batch, heads, n, d, {strides.n, strides.h, strides.b}, bf16);
 }
 
 int encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,

@@ -28,19 +28,19 @@ int open_device(Device* out);
 // `p` must be memory that device `dev` addresses directly.
 int check_pointer(const void* p, const char* name, int dev);
 
-// 4-D map {D, N, H, B} of a contiguous tensor in `layout`, box of 128 rows and min(D, 64) columns.
-int encode_heads(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
-                 int64_t d, int layout, bool bf16);
-
-// A map of 16-bit elements with 64-column boxes in the 128-byte swizzle; rank - 1 strides.
-int encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-               const uint64_t* stride_bytes, const uint32_t* box, bool bf16);
-
 // Element strides of a contiguous tensor in `layout`.
 struct Strides {
   int64_t n, h, b;
 };
 Strides strides_of(int layout, int64_t heads, int64_t n, int64_t d);
+
+// 4-D map {D, N, H, B} of a tensor, box of 128 rows and min(D, 64) columns.
+int encode_heads(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
+                 int64_t d, const Strides& strides, bool bf16);
+
+// A map of 16-bit elements with 64-column boxes in the 128-byte swizzle; rank - 1 strides.
+int encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+               const uint64_t* stride_bytes, const uint32_t* box, bool bf16);
 
 }  // namespace host
 }  // namespace mfa

@@ -118,6 +118,7 @@ constexpr int64_t kInlinePrefixBytes = 64 << 20;
 struct Problem {
   int64_t batch, heads, kv_heads;
   int32_t d;
+  int64_t q_request, q_head;  // element strides of q
   int64_t pages, page_size, columns, window, sinks;
   int64_t prefix;  // tokens of the shared prefix
   float scale;
@@ -176,6 +177,12 @@ int check(Problem& w) {
   if (w.columns > kMost / w.page_size) return invalid("the block table has too many columns");
   if (w.prefix > kMost) return invalid("the prefix is too long");
   if (w.heads == 0 || w.batch == 0) return MFA_OK;
+  // a dimension of one element may have any stride
+  if (w.heads == 1) w.q_head = w.d;
+  if (w.batch == 1) w.q_request = w.d;
+  for (const int64_t s : {w.q_request, w.q_head})
+    if (s <= 0 || s % 8 != 0 || s >= int64_t{1} << 31)
+      return invalid("the strides of q must be positive multiples of 8 elements below 2^31");
   // steps of a launch are counted in 32 bits
   const double tiles = static_cast<double>(w.most_tiles() + kPagedUnitSteps);
   if (tiles * static_cast<double>(w.units()) > 0x7fffff00 ||
@@ -275,8 +282,8 @@ int launch_prefix(const Arrays& x, const Problem& w, const Layout& l, const host
   FwdParams p = {};
   const uint64_t dims[4] = {static_cast<uint64_t>(w.d), static_cast<uint64_t>(w.group()),
                             static_cast<uint64_t>(w.batch), static_cast<uint64_t>(w.kv_heads)};
-  const uint64_t row = static_cast<uint64_t>(w.d) * 2;
-  const uint64_t strides[3] = {row, row * static_cast<uint64_t>(w.heads), row * dims[1]};
+  const uint64_t row = static_cast<uint64_t>(w.q_head) * 2;
+  const uint64_t strides[3] = {row, static_cast<uint64_t>(w.q_request) * 2, row * dims[1]};
   const uint32_t box[4] = {64, static_cast<uint32_t>(w.group()),
                            static_cast<uint32_t>(w.tile_batch()), 1};
   int rc = host::encode_map(&p.tm_q, x.q, 4, dims, strides, box, Cfg::kBF16);
@@ -321,6 +328,8 @@ int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cud
       (rc = encode_cache(&p.tm_v, x.v_cache, w, 64)) != MFA_OK)
     return rc;
   p.q = static_cast<const uint16_t*>(x.q);
+  p.q_request = w.q_request;
+  p.q_head = w.q_head;
   p.out = static_cast<uint16_t*>(x.out);
   p.block_table = x.block_table;
   p.lengths = x.lengths;
@@ -503,10 +512,13 @@ extern "C" int mfa_append_kv(const void* k, const void* v, void* k_cache, void* 
 extern "C" int mfa_paged_attention(const void* q, const void* k_cache, const void* v_cache,
                                    const int32_t* block_table, const int32_t* lengths, void* out,
                                    void* workspace, uint64_t workspace_bytes, int64_t batch,
-                                   int64_t heads, int64_t kv_heads, int32_t d, int64_t pages,
+                                   int64_t heads, int64_t kv_heads, int32_t d,
+                                   int64_t q_batch_stride, int64_t q_head_stride, int64_t pages,
                                    int64_t page_size, int64_t columns, int64_t window,
                                    int64_t sinks, float scale, int32_t dtype, void* stream) {
-  Problem w{batch, heads, kv_heads, d, pages, page_size, columns, window, sinks, 0, scale, dtype};
+  Problem w{batch, heads,     kv_heads, d,      q_batch_stride, q_head_stride,
+            pages, page_size, columns,  window, sinks,          0,
+            scale, dtype};
   return attend({q, k_cache, v_cache, nullptr, block_table, lengths, out,
                  static_cast<float*>(workspace)},
                 workspace_bytes, w, stream);
@@ -517,11 +529,13 @@ extern "C" int mfa_shared_prefix_attention(const void* q, const void* k_cache, c
                                            const int32_t* block_table, const int32_t* lengths,
                                            void* out, void* workspace, uint64_t workspace_bytes,
                                            int64_t batch, int64_t heads, int64_t kv_heads,
-                                           int32_t d, int64_t pages, int64_t page_size,
-                                           int64_t columns, float scale, int32_t dtype,
-                                           void* stream) {
-  Problem w{batch, heads, kv_heads, d,     pages, page_size,
-            columns, 0,   0,        prefix_length, scale, dtype};
+                                           int32_t d, int64_t q_batch_stride,
+                                           int64_t q_head_stride, int64_t pages,
+                                           int64_t page_size, int64_t columns, float scale,
+                                           int32_t dtype, void* stream) {
+  Problem w{batch, heads,     kv_heads, d, q_batch_stride, q_head_stride,
+            pages, page_size, columns,  0, 0,              prefix_length,
+            scale, dtype};
   return attend({q, k_cache, v_cache, prefix_pages, block_table, lengths, out,
                  static_cast<float*>(workspace)},
                 workspace_bytes, w, stream);
@@ -532,8 +546,9 @@ extern "C" int mfa_paged_workspace_bytes(int64_t batch, int64_t heads, int64_t k
                                          int64_t prefix_length, uint64_t* bytes) {
   if (!bytes) return invalid("bytes must not be null");
   *bytes = 0;
-  Problem w{batch, heads, kv_heads, d, 1, page_size, columns, 0, 0, prefix_length, 1.0f,
-            MFA_DTYPE_FP16};
+  Problem w{batch, heads,     kv_heads, d, 8, 8,
+            1,     page_size, columns,  0, 0, prefix_length,
+            1.0f,  MFA_DTYPE_FP16};
   const int rc = check(w);
   if (rc != MFA_OK || batch == 0 || heads == 0) return rc;
   int dev = 0, sms = 0;

@@ -51,7 +51,8 @@ __host__ __device__ constexpr int paged_slot_floats(int rows, int d) {
 
 struct PagedParams {
   CUtensorMap tm_k, tm_v;  // {D, page_size, kv_heads, pages}, box {64, min(page_size, 64), 1, 1}
-  const uint16_t* q;       // [batch, kv_heads * group, D]
+  const uint16_t* q;       // [batch, kv_heads * group, D], its strides in elements:
+  long long q_request, q_head;
   uint16_t* out;
   const int* block_table;  // [batch, columns]
   const int* lengths;      // [batch]
@@ -223,7 +224,7 @@ struct PagedCursor {
     const int r = p.group - row0;
     return r < 16 ? r : 16;
   }
-  __device__ size_t query(const PagedParams& p) const {  // its first row in q and out
+  __device__ size_t query(const PagedParams& p) const {  // its first row in out
     return (static_cast<size_t>(request) * p.kv_heads + head) * p.group + row0;
   }
   __device__ int unit(const PagedParams& p) const {
@@ -454,10 +455,10 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, PagedCu
   uint32_t qf[kKSteps][4];
   auto read_query = [&](const PagedCursor& at) {
     const int rows = at.rows(p);
+    const uint16_t* first = p.q + at.request * p.q_request + (at.head * p.group + at.row0) * p.q_head;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const uint32_t* src =
-          reinterpret_cast<const uint32_t*>(p.q + (at.query(p) + gq + 8 * r) * D) + q;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(first + (gq + 8 * r) * p.q_head) + q;
       const bool here = gq + 8 * r < rows;
 #pragma unroll
       for (int kk = 0; kk < kKSteps; ++kk) {
@@ -469,13 +470,15 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, PagedCu
 
   if (cur.left > 0) {
     read_query(cur);
-    // The share's queries are one run of memory. Its first 128 lines are brought to L2: from HBM,
+    // The share's queries are a run of rows. Its first 128 lines are brought to L2: from HBM,
     // busy with keys, a unit's queries would take longer than the merge that hides them.
-    const size_t row = cur.query(p) * D;
-    const size_t end = static_cast<size_t>(p.batch) * p.kv_heads * p.group * D;
-    const size_t mine = row + 64 * threadIdx.x;
-    if (mine < end)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + mine));
+    const int heads = p.kv_heads * p.group;
+    const int head = cur.head * p.group + cur.row0 + static_cast<int>(threadIdx.x) / (D / 64);
+    const int request = cur.request + head / heads;
+    if (request < p.batch)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + request * p.q_request +
+                                                    head % heads * p.q_head +
+                                                    64 * (threadIdx.x % (D / 64))));
   }
   int g = 0;
   bool ok = true, wrote = false, merged = false;

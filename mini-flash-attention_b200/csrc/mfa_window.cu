@@ -77,7 +77,34 @@ struct Problem {
   int64_t batch, heads, kv_heads, n, window, sinks;
   int32_t d, dtype, layout;
   float scale;
+  host::Strides q, k, v;
 };
+
+// Strides of q, k and v: those of the layout, or the caller's {batch, head, token} of each.
+int set_strides(Problem& w, const int64_t* strides) {
+  const struct {
+    host::Strides* to;
+    int64_t heads;
+  } tensors[3] = {{&w.q, w.heads}, {&w.k, w.kv_heads}, {&w.v, w.kv_heads}};
+  for (int i = 0; i < 3; ++i) {
+    *tensors[i].to = host::strides_of(w.layout, tensors[i].heads, w.n, w.d);
+    if (!strides) continue;
+    const int64_t extents[3] = {w.batch, tensors[i].heads, w.n};
+    int64_t* const to[3] = {&tensors[i].to->b, &tensors[i].to->h, &tensors[i].to->n};
+    for (int x = 0; x < 3; ++x) {
+      const int64_t s = strides[3 * i + x];
+      if (extents[x] <= 1) {
+        *to[x] = w.d;  // a dimension of one element may have any stride
+      } else if (s <= 0 || s % 8 != 0 || s >= int64_t{1} << 38) {
+        return host::fail(MFA_ERR_INVALID_ARGUMENT,
+                          "the strides of q, k and v must be positive multiples of 8 elements");
+      } else {
+        *to[x] = s;
+      }
+    }
+  }
+  return MFA_OK;
+}
 
 int check(Problem& w) {
   if (w.batch < 0 || w.heads < 0 || w.kv_heads < 0 || w.n < 0)
@@ -147,13 +174,12 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
                    const Problem& w, const host::Device& dev, cudaStream_t stream) {
   FwdParams p = {};
   const bool bf16 = Cfg::kBF16;
-  int rc = host::encode_heads(&p.tm_q, q, w.batch, w.heads, w.n, w.d, w.layout, bf16);
+  int rc = host::encode_heads(&p.tm_q, q, w.batch, w.heads, w.n, w.d, w.q, bf16);
+  if (rc == MFA_OK) rc = host::encode_heads(&p.tm_k, k, w.batch, w.kv_heads, w.n, w.d, w.k, bf16);
+  if (rc == MFA_OK) rc = host::encode_heads(&p.tm_v, v, w.batch, w.kv_heads, w.n, w.d, w.v, bf16);
   if (rc == MFA_OK)
-    rc = host::encode_heads(&p.tm_k, k, w.batch, w.kv_heads, w.n, w.d, w.layout, bf16);
-  if (rc == MFA_OK)
-    rc = host::encode_heads(&p.tm_v, v, w.batch, w.kv_heads, w.n, w.d, w.layout, bf16);
-  if (rc == MFA_OK)
-    rc = host::encode_heads(&p.tm_o, out, w.batch, w.heads, w.n, w.d, w.layout, bf16);
+    rc = host::encode_heads(&p.tm_o, out, w.batch, w.heads, w.n, w.d,
+                            host::strides_of(w.layout, w.heads, w.n, w.d), bf16);
   if (rc != MFA_OK) return rc;
   p.n = p.nq = static_cast<int>(w.n);
   p.heads = static_cast<int>(w.heads);
@@ -212,9 +238,8 @@ Pieces plan_pieces(int64_t blocks, int64_t sink_blocks, int64_t span, int64_t sp
 // The map of a tensor of the gradients: D = 32 runs as D = 64 with boxes that reach past its
 // columns, where loads read zeros, which change no sum, and stores write nothing.
 int encode_gradient(CUtensorMap* map, const void* base, int64_t batch, int64_t heads, int64_t n,
-                    int64_t d, int layout, bool bf16) {
-  if (d >= 64) return host::encode_heads(map, base, batch, heads, n, d, layout, bf16);
-  const host::Strides st = host::strides_of(layout, heads, n, d);
+                    int64_t d, const host::Strides& st, bool bf16) {
+  if (d >= 64) return host::encode_heads(map, base, batch, heads, n, d, st, bf16);
   const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(n),
                             static_cast<uint64_t>(heads), static_cast<uint64_t>(batch)};
   const uint64_t strides[3] = {static_cast<uint64_t>(st.n) * 2, static_cast<uint64_t>(st.h) * 2,
@@ -298,15 +323,18 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
     CUtensorMap* to;
     const void* base;
     int64_t heads;
+    const host::Strides& strides;
   };
+  const host::Strides st = host::strides_of(w.layout, w.heads, w.n, w.d);  // out, dout, dq
+  const host::Strides kv = host::strides_of(w.layout, w.kv_heads, w.n, w.d);  // dk, dv
   // dQ: q, dO resident; k, v streamed. dK, dV: k, v resident; q, dO streamed.
-  const Map maps[] = {{&pq.tm_x, q, w.heads},        {&pq.tm_y, dout, w.heads},
-                      {&pq.tm_s0, k, w.kv_heads},    {&pq.tm_s1, v, w.kv_heads},
-                      {&pq.tm_o0, dq, w.heads},      {&pkv.tm_o0, dk, w.kv_heads},
-                      {&pkv.tm_o1, dv, w.kv_heads}};
+  const Map maps[] = {{&pq.tm_x, q, w.heads, w.q},      {&pq.tm_y, dout, w.heads, st},
+                      {&pq.tm_s0, k, w.kv_heads, w.k},  {&pq.tm_s1, v, w.kv_heads, w.v},
+                      {&pq.tm_o0, dq, w.heads, st},     {&pkv.tm_o0, dk, w.kv_heads, kv},
+                      {&pkv.tm_o1, dv, w.kv_heads, kv}};
   int rc = MFA_OK;
   for (const Map& m : maps) {
-    rc = encode_gradient(m.to, m.base, w.batch, m.heads, w.n, w.d, w.layout, kBF16);
+    rc = encode_gradient(m.to, m.base, w.batch, m.heads, w.n, w.d, m.strides, kBF16);
     if (rc != MFA_OK) break;
   }
   pq.tm_o1 = pq.tm_o0;
@@ -315,15 +343,13 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
   pkv.tm_s0 = pq.tm_x;
   pkv.tm_s1 = pq.tm_y;
   if (rc == MFA_OK) {
-    const host::Strides st = host::strides_of(w.layout, w.heads, w.n, w.d);
     const int64_t need = static_cast<int64_t>(rows) * w.d / 2048;  // 16 bytes a thread
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
     // the kernels wait for the stream's earlier work themselves and may be set up while it ends
     e = launch(need < most ? need : most, 256, 0, stream, prep_kernel<kBF16>(w.d), out, dout, lse,
                lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads),
-               static_cast<long long>(st.b),
-               static_cast<long long>(st.h), static_cast<long long>(st.n),
-               static_cast<int>(blocks), counters);
+               static_cast<long long>(st.b), static_cast<long long>(st.h),
+               static_cast<long long>(st.n), static_cast<int>(blocks), counters);
     const int64_t units = kv_units > q_units ? kv_units : q_units;
     const int64_t ctas = units < dev.sms ? units : dev.sms;
     if constexpr (D == 64) {
@@ -331,17 +357,16 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
         e = launch(ctas, BwdConfig<true, true, kBF16, true>::kThreads, window_bwd_smem<kBF16>(),
                    stream, &mfa_bwd_window_kernel<kBF16>, pq, pkv);
     } else {
-      auto set_grad = [&](BwdParams& to, void* grad, int64_t heads) {
-        const host::Strides g = host::strides_of(w.layout, heads, w.n, w.d);
+      auto set_grad = [](BwdParams& to, void* grad, const host::Strides& g) {
         to.grad = static_cast<uint16_t*>(grad);
         to.grad_b = g.b;
         to.grad_h = g.h;
         to.grad_n = g.n;
       };
-      set_grad(pq, dq, w.heads);
+      set_grad(pq, dq, st);
       BwdParams pv = pkv;  // pkv: dK
-      set_grad(pkv, dk, w.kv_heads);
-      set_grad(pv, dv, w.kv_heads);
+      set_grad(pkv, dk, kv);
+      set_grad(pv, dv, kv);
       pv.claimed = counters + 2;
       pv.partials = sums + slots * kTile;
       if (e == cudaSuccess)
@@ -349,7 +374,6 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
                    &mfa_bwd_window128_kernel<kBF16>, pq, pkv, pv);
     }
     if (e == cudaSuccess && slots > 0) {
-      const host::Strides kv = host::strides_of(w.layout, w.kv_heads, w.n, w.d);
       const int64_t pairs = bhk * (pc.pieces_rest > 1 ? blocks : sb);
       const long long slot_floats = D == 64 ? 2 * kTile : kTile;
       e = launch(pairs * D / 8, 256, 0, stream, &mfa_bwd_reduce_kernel<kBF16, D>, pkv, sums,
@@ -381,10 +405,11 @@ using namespace mfa;
 extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
                               int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
                               int32_t d, int64_t window, int64_t sinks, float scale,
-                              int32_t dtype, int32_t layout, void* stream) {
-  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale};
+                              int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
+  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
   int rc = check(w);
   if (rc != MFA_OK || batch * heads == 0 || n == 0) return rc;
+  if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
   const void* ptrs[] = {q, k, v, out};
   const char* names[] = {"q", "k", "v", "out"};
   if ((rc = check_tensors(ptrs, names, 4, -1)) != MFA_OK) return rc;
@@ -403,11 +428,12 @@ extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const
                               const void* dout, const float* lse, void* dq, void* dk, void* dv,
                               int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
                               int32_t d, int64_t window, int64_t sinks, float scale,
-                              int32_t dtype, int32_t layout, void* stream) {
-  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale};
+                              int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
+  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
   int rc = check(w);
   if (rc != MFA_OK) return rc;
   if (batch * heads == 0 || n == 0) return MFA_OK;
+  if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
   const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv};
   const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv"};
   if ((rc = check_tensors(ptrs, names, 8, -1)) != MFA_OK) return rc;

@@ -84,7 +84,11 @@ def forward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: in
     q is [B, H, N, D]; k and v are [B, Hkv, N, D], Hkv a divisor of H (query head h reads k / v
     head h // (H // Hkv)). fp16 or bf16, D = 32, 64 or 128, any N, scale 1/sqrt(D). Blocks of
     keys that no query of a block sees are skipped. A batch padded behind its sequences needs no
-    mask: no token sees a later one (the padding has to be finite)."""
+    mask: no token sees a later one (the padding has to be finite).
+
+    q, k and v may be views, as of a fused projection: contiguous in D, other strides multiples of
+    8. The output lies in memory as q does, [B, H, N, D] or (``x.view(B, N, H, D).transpose(1, 2)``)
+    [B, N, H, D], and the gradients with it."""
     return _load_extension().forward_window(q, k, v, int(window), int(sinks), False)[0]
 
 
@@ -100,9 +104,9 @@ def backward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
                     sinks: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients (dq, dk, dv) of forward_window for the output gradient dout, given its out and
     lse (forward_window_lse); dk and dv of a shared head are summed over its query heads.
-    The types and head dims of forward_window."""
-    dq, dk, dv = _load_extension().backward_window(q, k, v, out, lse, dout.contiguous(),
-                                                   int(window), int(sinks))
+    The types, head dims and views of forward_window; out and dout in another layout are copied."""
+    dq, dk, dv = _load_extension().backward_window(q, k, v, out, lse, dout, int(window),
+                                                   int(sinks))
     return dq, dk, dv
 
 
@@ -149,7 +153,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     sinks: int = 0) -> torch.Tensor:
     """Attention of one token per request over a paged cache (the decoding form of
     forward_window): q [B, H, D], caches [pages, Hkv, page_size, D], block_table int32 [B,
-    columns], lengths int32 [B], the query's own token among them. With ``window`` the ``window``
+    columns], lengths int32 [B], the query's own token among them; q's strides but that of D may be
+    those of a fused projection. With ``window`` the ``window``
     newest tokens and the ``sinks`` first are visible, otherwise all. fp16 or bf16, D = 64 or 128,
     page sizes 16 to 256 (powers of two), H a multiple of Hkv (up to 128 heads a k / v head),
     scale 1/sqrt(D). A request of length 0 gets 0. Lengths and table are read on the GPU: a

@@ -91,7 +91,7 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     lib.mfa_bwd.restype = ctypes.c_int
     window_args = [ctypes.c_int64] * 4 + [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
                                           ctypes.c_float, ctypes.c_int32, ctypes.c_int32,
-                                          ctypes.c_void_p]
+                                          ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p]
     lib.mfa_fwd_window.argtypes = [ctypes.c_void_p] * 5 + window_args
     lib.mfa_fwd_window.restype = ctypes.c_int
     lib.mfa_bwd_window.argtypes = [ctypes.c_void_p] * 9 + window_args
@@ -100,9 +100,9 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     lib.mfa_extend_block_tables.argtypes = [ptr] * 7 + [i64] * 5 + [ptr]
     lib.mfa_append_kv.argtypes = [ptr] * 5 + [i64] * 9 + [ptr]
     lib.mfa_paged_attention.argtypes = [ptr] * 7 + [ctypes.c_uint64] + [i64] * 3 + [
-        i32, *[i64] * 5, ctypes.c_float, i32, ptr]
+        i32, *[i64] * 7, ctypes.c_float, i32, ptr]
     lib.mfa_shared_prefix_attention.argtypes = [ptr] * 4 + [i64] + [ptr] * 4 + [
-        ctypes.c_uint64, *[i64] * 3, i32, *[i64] * 3, ctypes.c_float, i32, ptr]
+        ctypes.c_uint64, *[i64] * 3, i32, *[i64] * 5, ctypes.c_float, i32, ptr]
     lib.mfa_paged_workspace_bytes.argtypes = [i64] * 3 + [i32] + [i64] * 3 + [
         ctypes.POINTER(ctypes.c_uint64)]
     for name in ("mfa_extend_block_tables", "mfa_append_kv", "mfa_paged_attention",
@@ -178,22 +178,29 @@ def bwd(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_ptr: in
                           batch, heads, n, d, scale, int(causal), dtype, layout, stream))
 
 
+def _nine(strides):
+    return None if strides is None else (ctypes.c_int64 * 9)(*strides)
+
+
 def fwd_window(q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, lse_ptr: int, batch: int,
                heads: int, kv_heads: int, n: int, d: int, window: int, sinks: int, scale: float,
-               dtype: int = DTYPE_FP16, layout: int = LAYOUT_BHND, stream: int = 0) -> None:
-    """Launch mfa_fwd_window (lse_ptr 0: no log-sum-exp); raises MfaError."""
+               dtype: int = DTYPE_FP16, layout: int = LAYOUT_BHND, stream: int = 0,
+               strides: tuple[int, ...] | None = None) -> None:
+    """Launch mfa_fwd_window (lse_ptr 0: no log-sum-exp; strides: the nine (batch, head, token)
+    element strides of q, k and v); raises MfaError."""
     _check(load().mfa_fwd_window(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, batch, heads, kv_heads, n,
-                                 d, window, sinks, scale, dtype, layout, stream))
+                                 d, window, sinks, scale, dtype, layout, _nine(strides), stream))
 
 
 def bwd_window(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_ptr: int,
                dq_ptr: int, dk_ptr: int, dv_ptr: int, batch: int, heads: int, kv_heads: int,
                n: int, d: int, window: int, sinks: int, scale: float, dtype: int = DTYPE_FP16,
-               layout: int = LAYOUT_BHND, stream: int = 0) -> None:
-    """Launch mfa_bwd_window; raises MfaError."""
+               layout: int = LAYOUT_BHND, stream: int = 0,
+               strides: tuple[int, ...] | None = None) -> None:
+    """Launch mfa_bwd_window (strides as for fwd_window); raises MfaError."""
     _check(load().mfa_bwd_window(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, dq_ptr, dk_ptr,
                                  dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale, dtype,
-                                 layout, stream))
+                                 layout, _nine(strides), stream))
 
 
 def extend_block_tables(table_ptr: int, cached_ptr: int, added_ptr: int, free_ptr: int,
@@ -217,24 +224,27 @@ def paged_attention(q_ptr: int, k_cache_ptr: int, v_cache_ptr: int, table_ptr: i
                     lengths_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int,
                     batch: int, heads: int, kv_heads: int, d: int, pages: int, page_size: int,
                     columns: int, scale: float, window: int = 0, sinks: int = 0,
-                    dtype: int = DTYPE_FP16, stream: int = 0) -> None:
-    """Launch mfa_paged_attention; raises MfaError."""
+                    dtype: int = DTYPE_FP16, stream: int = 0,
+                    q_strides: tuple[int, int] | None = None) -> None:
+    """Launch mfa_paged_attention (q_strides: (batch, head) element strides of q, contiguous if
+    None); raises MfaError."""
     _check(load().mfa_paged_attention(q_ptr, k_cache_ptr, v_cache_ptr, table_ptr, lengths_ptr,
                                       out_ptr, workspace_ptr, workspace_bytes, batch, heads,
-                                      kv_heads, d, pages, page_size, columns, window, sinks,
-                                      scale, dtype, stream))
+                                      kv_heads, d, *(q_strides or (heads * d, d)), pages,
+                                      page_size, columns, window, sinks, scale, dtype, stream))
 
 
 def shared_prefix_attention(q_ptr: int, k_cache_ptr: int, v_cache_ptr: int, prefix_ptr: int,
                             prefix_length: int, table_ptr: int, lengths_ptr: int, out_ptr: int,
                             workspace_ptr: int, workspace_bytes: int, batch: int, heads: int,
                             kv_heads: int, d: int, pages: int, page_size: int, columns: int,
-                            scale: float, dtype: int = DTYPE_FP16, stream: int = 0) -> None:
-    """Launch mfa_shared_prefix_attention; raises MfaError."""
+                            scale: float, dtype: int = DTYPE_FP16, stream: int = 0,
+                            q_strides: tuple[int, int] | None = None) -> None:
+    """Launch mfa_shared_prefix_attention (q_strides as for paged_attention); raises MfaError."""
     _check(load().mfa_shared_prefix_attention(
         q_ptr, k_cache_ptr, v_cache_ptr, prefix_ptr, prefix_length, table_ptr, lengths_ptr,
-        out_ptr, workspace_ptr, workspace_bytes, batch, heads, kv_heads, d, pages, page_size,
-        columns, scale, dtype, stream))
+        out_ptr, workspace_ptr, workspace_bytes, batch, heads, kv_heads, d,
+        *(q_strides or (heads * d, d)), pages, page_size, columns, scale, dtype, stream))
 
 
 def paged_workspace_bytes(batch: int, heads: int, kv_heads: int, d: int, page_size: int,

@@ -13,14 +13,16 @@ INVALID = capi.MFA_ERR_INVALID_ARGUMENT
 
 def attend(shared=False, ptr=FAKE, out=None, batch=2, heads=8, kv_heads=2, d=64, pages=10,
            page_size=16, columns=4, window=0, sinks=0, prefix=50, scale=0.125,
-           dtype=capi.DTYPE_FP16):
+           dtype=capi.DTYPE_FP16, q_strides=None):
     out = ptr if out is None else out
     if shared:
         capi.shared_prefix_attention(ptr, ptr, ptr, ptr, prefix, ptr, ptr, out, ptr, 1 << 30, batch,
-                                     heads, kv_heads, d, pages, page_size, columns, scale, dtype)
+                                     heads, kv_heads, d, pages, page_size, columns, scale, dtype,
+                                     q_strides=q_strides)
     else:
         capi.paged_attention(ptr, ptr, ptr, ptr, ptr, out, ptr, 1 << 30, batch, heads, kv_heads, d,
-                             pages, page_size, columns, scale, window, sinks, dtype)
+                             pages, page_size, columns, scale, window, sinks, dtype,
+                             q_strides=q_strides)
 
 
 COMMON = [
@@ -38,6 +40,11 @@ COMMON = [
     ({"pages": 1 << 28}, INVALID, "too many tokens"),
     ({"columns": 1 << 28}, INVALID, "too many columns"),
     ({"batch": 1 << 20, "columns": 1 << 16}, INVALID, "batch \\* heads \\* tokens"),
+    ({"q_strides": (0, 64)}, INVALID, "strides of q must be positive multiples of 8"),
+    ({"q_strides": (512, -64)}, INVALID, "strides of q must be positive multiples of 8"),
+    ({"q_strides": (516, 64)}, INVALID, "strides of q must be positive multiples of 8"),
+    ({"q_strides": (1 << 31, 64)}, INVALID, "strides of q .* below 2\\^31"),
+    ({"q_strides": (3, 64), "batch": 1, "pages": 0}, INVALID, "the cache has no pages"),
     ({"pages": 0}, INVALID, "the cache has no pages"),
     ({"ptr": 0}, INVALID, "null q"),
     ({"ptr": FAKE + 4}, INVALID, "q must be 16-byte aligned"),

@@ -309,6 +309,34 @@ def test_bad_pages_are_reported():
         assert capi.device_status(device) == capi.STATUS_BAD_PAGE
 
 
+# q as a part of a fused projection, or with the heads outermost: bit for bit what a contiguous q
+# gives, in every form of the kernel (few units, equal shares, a prefix inside and apart)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("batch,group,prefix", [(3, 3, 0), (150, 4, 0), (9, 17, 0), (5, 2, 100),
+                                                (40, 5, 3000), (130, 1, 6000), (1, 2, 70), (4, 1, 0)])
+@WIDE
+def test_query_strides(batch, group, prefix, d, wide):
+    lengths = [(37 * i) % 200 for i in range(batch)]
+    cache = Cache(lengths, 2, d, 32, torch.bfloat16, prefix=prefix, seed=batch + prefix,
+                  columns=columns(lengths, 32, wide))
+    k, v, table, own = cache.tensors()
+    heads = 2 * group
+    q = queries(batch, heads, d, torch.bfloat16).cuda()
+    fused = torch.full((batch, (heads + 4) * d), float("nan"), device="cuda", dtype=q.dtype)
+    part = fused[:, 2 * d:(2 + heads) * d].view(batch, heads, d)
+    part.copy_(q)
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)
+    if prefix:
+        call = lambda x: mfa.shared_prefix_attention(  # noqa: E731
+            x, k, v, cache.pages(), prefix, table, own)
+    else:
+        call = lambda x: mfa.paged_attention(x, k, v, table, own, 60, 5)  # noqa: E731
+    want = call(q)
+    for x in (part, turned):
+        got = call(x)
+        assert got.is_contiguous() and torch.equal(got, want)
+
+
 def test_empty_batch():
     cache = Cache([5], 2, 64, 16, torch.float16)
     k, v, table, own = cache.tensors()
@@ -326,7 +354,12 @@ def test_refusals():
             ({"q": q.bfloat16()}, "same dtype"), ({"q": q.float()}, "same dtype"),
             ({"q": q[:, :3].contiguous()}, "multiple of the k / v heads"),
             ({"q": q[:, :, :32].contiguous()}, "q must have shape"),
-            ({"q": q.transpose(0, 1)}, "q must be contiguous"),
+            ({"q": q.repeat_interleave(2, 2)[:, :, ::2]}, "q must be contiguous in D"),
+            ({"q": q[:1].expand(2, 4, 64)}, "strides of q must be positive multiples of 8"),
+            ({"q": torch.zeros(2, 4, 68, device="cuda").half()[:, :, :64]},
+             "strides of q must be positive multiples of 8"),
+            ({"q": torch.zeros(2, 4, 72, device="cuda").half()[:, :, 4:68]},
+             "q must be 16-byte aligned"),
             ({"q": q.cpu()}, "CUDA tensor"),
             ({"k": k[:, :, ::2]}, "same shape"), ({"v": v[:-1]}, "same shape"),
             ({"k": k[:, :, :8].contiguous(), "v": v[:, :, :8].contiguous()}, "page size"),

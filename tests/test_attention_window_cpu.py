@@ -13,10 +13,11 @@ FAKE = 0x10000  # never dereferenced
 
 
 def call(direction="fwd", ptr=FAKE, batch=1, heads=4, kv_heads=2, n=256, d=64, window=16, sinks=0,
-         scale=0.125, dtype=capi.DTYPE_FP16, layout=capi.LAYOUT_BHND):
+         scale=0.125, dtype=capi.DTYPE_FP16, layout=capi.LAYOUT_BHND, strides=None):
     fn, count = (capi.fwd_window, 4) if direction == "fwd" else (capi.bwd_window, 9)
     more = (0,) if direction == "fwd" else ()
-    fn(*[ptr] * count, *more, batch, heads, kv_heads, n, d, window, sinks, scale, dtype, layout)
+    fn(*[ptr] * count, *more, batch, heads, kv_heads, n, d, window, sinks, scale, dtype, layout,
+       strides=strides)
 
 
 @pytest.mark.parametrize("direction", ["fwd", "bwd"])
@@ -35,6 +36,12 @@ def call(direction="fwd", ptr=FAKE, batch=1, heads=4, kv_heads=2, n=256, d=64, w
     ({"scale": float("nan")}, capi.MFA_ERR_INVALID_ARGUMENT, "scale must be positive"),
     ({"dtype": 7}, capi.MFA_ERR_INVALID_ARGUMENT, "dtype must be"),
     ({"layout": 7}, capi.MFA_ERR_INVALID_ARGUMENT, "layout must be"),
+    ({"strides": (1 << 16, 1 << 14, 0) * 3}, capi.MFA_ERR_INVALID_ARGUMENT, "strides of q, k"),
+    ({"strides": (1 << 16, -64, 64) * 3}, capi.MFA_ERR_INVALID_ARGUMENT, "strides of q, k"),
+    ({"batch": 2, "strides": (1 << 38, 64, 512) * 3}, capi.MFA_ERR_INVALID_ARGUMENT, "strides of"),
+    ({"strides": (1 << 16, 64, 512) * 2 + (1 << 16, 64, 516)}, capi.MFA_ERR_INVALID_ARGUMENT,
+     "strides of q, k"),
+    ({"strides": (-1, 64, 512) * 3, "ptr": 0}, capi.MFA_ERR_INVALID_ARGUMENT, "null q"),
     ({"ptr": 0}, capi.MFA_ERR_INVALID_ARGUMENT, "null q"),
     ({"ptr": FAKE + 8}, capi.MFA_ERR_INVALID_ARGUMENT, "16-byte aligned"),
 ])

@@ -253,6 +253,49 @@ def test_capi_bnhd_layout():
     assert capi.device_status(torch.cuda.current_device()) == 0
 
 
+# parts of a fused projection [B, N, (H + 2 Hkv) D], with one gradient for all of them
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("b,h,hk,n,window,sinks", [(2, 4, 2, 300, 70, 3), (1, 1, 1, 150, 40, 0),
+                                                   (3, 6, 1, 1, 5, 0), (1, 8, 8, 2100, 2100, 0)])
+def test_views_of_a_projection(b, h, hk, n, window, sinks, d):
+    q, k, v, dout = inputs(b, h, hk, n, d, torch.bfloat16, seed=11)
+    want = reference(q, k, v, window, sinks, dout)
+    fused = torch.cat([x.transpose(1, 2).reshape(b, n, -1) for x in (q, k, v)], 2)
+    fused.requires_grad_()
+    parts = [x.view(b, n, -1, d).transpose(1, 2) for x in fused.split((h * d, hk * d, hk * d), 2)]
+    out = mfa.window_attention(*parts, window, sinks)
+    check("out", out.detach(), *want["out"])
+    merged = out.transpose(1, 2)
+    assert merged.is_contiguous()  # ready for the next projection
+    merged.reshape(b, n, -1).backward(dout.transpose(1, 2).reshape(b, n, -1))
+    grads = fused.grad.split((h * d, hk * d, hk * d), 2)
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        check(name, x.view(b, n, -1, d).transpose(1, 2), *want[name])
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_mixed_layouts(d):
+    """Each tensor in another layout: bit for bit the results of contiguous ones."""
+    q, k, v, dout = inputs(2, 6, 3, 333, d, torch.float16, seed=5)
+    out, lse = mfa.forward_window_lse(q, k, v, 100, 2)
+    want = mfa.backward_window(q, k, v, out, lse, dout, 100, 2)
+    room = randn((2, 7, 400, d + 8), 3)
+    room[:, 2:5, 17:350, 8:] = v
+    for x in (q, q.transpose(1, 2).contiguous().transpose(1, 2),
+              q.permute(2, 1, 0, 3).contiguous().permute(2, 1, 0, 3)):
+        y = (x, k.transpose(1, 2).contiguous().transpose(1, 2), room[:, 2:5, 17:350, 8:])
+        o, s = mfa.forward_window_lse(*y, 100, 2)
+        assert torch.equal(o, out) and torch.equal(s, lse) and torch.equal(
+            mfa.forward_window(*y, 100, 2), out)
+        for other in (dout, dout.transpose(1, 2).contiguous().transpose(1, 2)):
+            got = mfa.backward_window(*y, o, s, other, 100, 2)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert all(a.is_contiguous() == x.is_contiguous() for a in got)
+    with pytest.raises(RuntimeError, match="lse must be contiguous"):
+        mfa.backward_window(q, k, v, out, lse.transpose(0, 1).contiguous().transpose(0, 1), dout,
+                            100, 2)
+
+
 def test_autograd_unaligned_output_gradient():
     q, k, v, dout = inputs(1, 4, 2, 150, 64, torch.bfloat16)
     leaves = [x.requires_grad_() for x in (q, k, v)]
@@ -286,7 +329,14 @@ def test_refusals():
             (lambda: mfa.forward_window(q, k, v[:, :1].contiguous(), 5), "same shape as k"),
             (lambda: mfa.forward_window(q, k.bfloat16(), v, 5), "same dtype"),
             (lambda: mfa.forward_window(q.float(), k, v, 5), "float16 or bfloat16"),
-            (lambda: mfa.forward_window(q.transpose(1, 2), k, v, 5), "contiguous"),
+            (lambda: mfa.forward_window(q.repeat_interleave(2, 3)[..., ::2], k, v, 5),
+             "q must be contiguous in D"),
+            (lambda: mfa.forward_window(q, k[:, :1].expand(1, 2, 100, 64), v, 5),
+             "strides of q, k and v must be positive multiples of 8"),
+            (lambda: mfa.forward_window(q, k, randn((1, 2, 100, 68), 9)[..., :64], 5),
+             "strides of q, k and v must be positive multiples of 8"),
+            (lambda: mfa.forward_window(q, k, randn((1, 2, 100, 72), 9)[..., 4:68], 5),
+             "v must be 16-byte aligned"),
             (lambda: mfa.forward_window(q, k.cpu(), v, 5), "CUDA tensor")):
         with pytest.raises(RuntimeError, match=match):
             call()
