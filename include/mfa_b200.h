@@ -185,7 +185,7 @@ MFA_API int mfa_append_kv(const void* k, const void* v, void* k_cache, void* v_c
 /*
  * Attention of one query token per request over the cache: q and out are [batch, heads, d], q with
  * element strides that are positive multiples of 8 (any value for a dimension of one element), d =
- * 64 or 128, heads a multiple of kv_heads (at most 128 query heads a k / v head), page_size 16, 32,
+ * 32, 64 or 128, heads a multiple of kv_heads (at most 128 query heads a k / v head), page_size 16, 32,
  * 64, 128 or 256. Request r has lengths[r] tokens (int32; clamped to [0, columns * page_size]), the
  * query's own among them; visible are all of them, or with window > 0 those in the newest
  * `window` positions and the first `sinks`. out is 0 for a request that sees nothing. Only pages

@@ -125,6 +125,7 @@ struct Problem {
   int32_t dtype;
 
   int64_t group() const { return heads / kv_heads; }
+  int kernel_d() const { return d == 128 ? 128 : 64; }  // see PagedConfig
   int64_t row_tiles() const { return (group() + 15) / 16; }
   int64_t units() const { return batch * kv_heads * row_tiles(); }
   int64_t slot_rows() const { return group() < 16 ? group() : 16; }
@@ -158,8 +159,8 @@ struct Problem {
 int check(Problem& w) {
   if (w.batch < 0 || w.heads < 0 || w.kv_heads < 0 || w.pages < 0 || w.columns < 0 || w.prefix < 0)
     return invalid("negative extent");
-  if (w.d != 64 && w.d != 128)
-    return host::fail(MFA_ERR_HEAD_DIM, "The paged attention supports only D=64 and D=128");
+  if (w.d != 32 && w.d != 64 && w.d != 128)
+    return host::fail(MFA_ERR_HEAD_DIM, "This kernel supports only D=32, D=64 and D=128");
   if (w.dtype != MFA_DTYPE_FP16 && w.dtype != MFA_DTYPE_BF16)
     return invalid("dtype must be MFA_DTYPE_FP16 or MFA_DTYPE_BF16");
   if (!(w.scale > 0.0f) || !std::isfinite(w.scale))
@@ -208,7 +209,7 @@ Layout lay_out(const Problem& w, int64_t sms) {
   const auto whole = [](int64_t floats) { return (floats + 63) / 64 * 64; };
   Layout l = {};
   const int64_t full =
-      sms * (w.d == 64 ? PagedConfig<64, false>::kCtas : PagedConfig<128, false>::kCtas);
+      sms * (w.kernel_d() == 64 ? PagedConfig<64, false>::kCtas : PagedConfig<128, false>::kCtas);
   const int64_t most = w.most_tiles();
   if (!w.prefix_apart() && w.units() <= full) {
     // CTAs a unit: as many as can be resident, up to 16, but two tiles each at least (at 16 tiles
@@ -229,7 +230,7 @@ Layout lay_out(const Problem& w, int64_t sms) {
   const int64_t slots = shared ? l.ctas + w.units() : 2 * l.ctas;
   const int64_t entries = shared ? w.units() : l.ctas;
   l.slots = 0;
-  l.pieces = whole(slots * paged_slot_floats(static_cast<int>(w.slot_rows()), w.d));
+  l.pieces = whole(slots * paged_slot_floats(static_cast<int>(w.slot_rows()), w.kernel_d()));
   l.prefix_slots = l.pieces + whole(entries * static_cast<int64_t>(sizeof(PagedPieces)) / 4);
   int64_t end = l.prefix_slots;
   if (shared) {
@@ -249,7 +250,7 @@ Layout lay_out(const Problem& w, int64_t sms) {
       }
     }
     l.prefix_ctas = units * l.splits < sms ? units * l.splits : sms;
-    end += units * l.splits * (128 * nq * (w.d + 2));
+    end += units * l.splits * (128 * nq * (w.kernel_d() + 2));
   }
   l.bytes = end * 4;
   return l;
@@ -330,6 +331,7 @@ int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cud
   p.q = static_cast<const uint16_t*>(x.q);
   p.q_request = w.q_request;
   p.q_head = w.q_head;
+  p.cols = w.d;
   p.out = static_cast<uint16_t*>(x.out);
   p.block_table = x.block_table;
   p.lengths = x.lengths;
@@ -365,6 +367,7 @@ int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cud
   cp.kv_heads = p.kv_heads;
   cp.group = p.group;
   cp.row_tiles = p.row_tiles;
+  cp.cols = p.cols;
   cp.pieces_only = p.pieces_only;
   e = shared ? launch(&mfa_paged_combine_kernel<D, kBF16, true>, w.units(), 128, 0, stream, cp)
              : launch(&mfa_paged_combine_kernel<D, kBF16, false>, l.ctas, 128, 0, stream, cp);
@@ -400,7 +403,7 @@ int attend(const Arrays& x, uint64_t workspace_bytes, Problem& w, void* stream) 
     return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = w.dtype == MFA_DTYPE_BF16;
-  if (w.d == 64)
+  if (w.kernel_d() == 64)
     return bf16 ? launch_paged<64, true>(a, w, dev, s) : launch_paged<64, false>(a, w, dev, s);
   return bf16 ? launch_paged<128, true>(a, w, dev, s) : launch_paged<128, false>(a, w, dev, s);
 }

@@ -155,7 +155,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     forward_window): q [B, H, D], caches [pages, Hkv, page_size, D], block_table int32 [B,
     columns], lengths int32 [B], the query's own token among them; q's strides but that of D may be
     those of a fused projection. With ``window`` the ``window``
-    newest tokens and the ``sinks`` first are visible, otherwise all. fp16 or bf16, D = 64 or 128,
+    newest tokens and the ``sinks`` first are visible, otherwise all. fp16 or bf16, D = 32, 64 or 128,
     page sizes 16 to 256 (powers of two), H a multiple of Hkv (up to 128 heads a k / v head),
     scale 1/sqrt(D). A request of length 0 gets 0. Lengths and table are read on the GPU: a
     captured call may be replayed with others of the same shape. Pages without visible tokens are

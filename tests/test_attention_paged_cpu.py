@@ -26,7 +26,7 @@ def attend(shared=False, ptr=FAKE, out=None, batch=2, heads=8, kv_heads=2, d=64,
 
 
 COMMON = [
-    ({"d": 32}, capi.MFA_ERR_HEAD_DIM, "D=64 and D=128"),
+    ({"d": 48}, capi.MFA_ERR_HEAD_DIM, "D=32, D=64 and D=128"),
     ({"dtype": 2}, INVALID, "dtype must be"),
     ({"scale": -1.0}, INVALID, "scale must be positive"),
     ({"page_size": 8}, INVALID, "page size"),

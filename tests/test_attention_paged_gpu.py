@@ -44,7 +44,7 @@ def columns(lengths, page, wide):
 @WIDE
 @pytest.mark.parametrize("lengths", LENGTHS.values(), ids=LENGTHS.keys())
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_decode(lengths, page, d, dtype, wide):
     cache = Cache(lengths, 2, d, page, dtype, columns=columns(lengths, page, wide), seed=page + d)
@@ -57,7 +57,8 @@ def test_decode(lengths, page, d, dtype, wide):
 @pytest.mark.parametrize("window,sinks", [(1, 0), (5, 1), (64, 4), (100, 65), (128, 64), (500, 130),
                                           (900, 1000), (10000, 3), (63, 17)])
 @pytest.mark.parametrize("page,d,dtype", [(16, 64, torch.float16), (64, 128, torch.bfloat16),
-                                          (256, 64, torch.bfloat16), (16, 128, torch.float16)])
+                                          (256, 64, torch.bfloat16), (16, 128, torch.float16),
+                                          (16, 32, torch.bfloat16), (128, 32, torch.float16)])
 @WIDE
 def test_decode_window(window, sinks, page, d, dtype, wide):
     lengths = [1, 64, 100, 129, 0, 1000, 1537]
@@ -69,7 +70,7 @@ def test_decode_window(window, sinks, page, d, dtype, wide):
 
 @pytest.mark.parametrize("kv_heads,group", [(1, 1), (8, 1), (3, 2), (1, 7), (2, 16), (1, 17), (2, 33),
                                             (1, 128)])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @WIDE
 def test_decode_heads(kv_heads, group, d, wide):
     lengths = [200, 1, 333]
@@ -140,7 +141,7 @@ def behind_prefix(cache, q):
 @WIDE
 @pytest.mark.parametrize("prefix", [1, 16, 63, 64, 65, 1000])
 @pytest.mark.parametrize("page", [16, 64, 256])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_prefix(prefix, page, d, dtype, wide):
     lengths = [0, 1, 65, 200, 17]
@@ -153,7 +154,7 @@ def test_prefix(prefix, page, d, dtype, wide):
 # more than 64 MB read by all requests together: the prefix has a kernel of its own
 @pytest.mark.parametrize("prefix,batch", [(127, 530), (128, 530), (129, 530), (1000, 140)])
 @pytest.mark.parametrize("page", [16, 64, 256])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("dtype", DTYPES.values(), ids=DTYPES.keys())
 def test_prefix_apart(prefix, batch, page, d, dtype):
     batch = batch * 128 // d
@@ -167,7 +168,7 @@ def test_prefix_apart(prefix, batch, page, d, dtype):
 @pytest.mark.parametrize("batch,kv_heads,group", [(1, 1, 1), (16, 2, 8), (17, 1, 8), (50, 2, 7),
                                                   (100, 1, 5), (3, 1, 128), (300, 2, 1),
                                                   (20, 1, 33)])
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("long", [False, True])
 def test_prefix_rows(batch, kv_heads, group, d, long):
     lengths = [(11 * i) % 30 for i in range(batch)]
@@ -177,7 +178,7 @@ def test_prefix_rows(batch, kv_heads, group, d, long):
     check(behind_prefix(cache, q), *cache.reference(q))
 
 
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 def test_prefix_several_units_a_cta(d):
     # more query tiles than CTAs: a CTA goes over several units
     lengths = [(5 * i) % 50 for i in range(320)]
@@ -186,7 +187,8 @@ def test_prefix_several_units_a_cta(d):
     check(behind_prefix(cache, q), *cache.reference(q))
 
 
-@pytest.mark.parametrize("batch,d,page", [(40, 128, 128), (150, 128, 16), (150, 64, 256)])
+@pytest.mark.parametrize("batch,d,page", [(40, 128, 128), (150, 128, 16), (150, 64, 256),
+                                           (50, 32, 64)])
 def test_prefix_past_the_l2(batch, d, page):
     # a prefix of more bytes than stay in L2: the units of a head read the same keys at the same time
     prefix = 32768 * 128 // d - 5
@@ -311,7 +313,7 @@ def test_bad_pages_are_reported():
 
 # q as a part of a fused projection, or with the heads outermost: bit for bit what a contiguous q
 # gives, in every form of the kernel (few units, equal shares, a prefix inside and apart)
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("batch,group,prefix", [(3, 3, 0), (150, 4, 0), (9, 17, 0), (5, 2, 100),
                                                 (40, 5, 3000), (130, 1, 6000), (1, 2, 70), (4, 1, 0)])
 @WIDE
@@ -385,8 +387,8 @@ def test_refusals():
             (lambda: mfa.shared_prefix_attention(q, k, v, pages.long(), 5, table, own), "int32")):
         with pytest.raises(RuntimeError, match=match):
             call()
-    x = torch.zeros((1, 1, 16, 32), device="cuda", dtype=torch.float16)
-    with pytest.raises(RuntimeError, match="D=64 and D=128"):
+    x = torch.zeros((1, 1, 16, 48), device="cuda", dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="D=32, D=64 and D=128"):
         mfa.paged_attention(x[0, :, :1], x, x, table[:1], own[:1])
     # the workspace of the C entry is checked
     cache = Cache([40, 5], 2, 64, 16, torch.float16, columns=3000)
