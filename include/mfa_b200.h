@@ -126,7 +126,8 @@ MFA_API int mfa_bwd(const void* q, const void* k, const void* v, const void* out
  * heads: query i sees key j if j <= i and (j > i - window or j < sinks); query head h reads k / v
  * head h / (heads / kv_heads). q and out have `heads` heads, k and v `kv_heads` (a divisor of
  * heads); d = 32, 64 or 128, any n, window >= 1 (at n or more: causal attention), sinks >= 0.
- * lse (may be NULL): the row log-sum-exp over the visible keys, fp32 [B*H, N]. Key blocks that
+ * lse (may be NULL): the row log-sum-exp over the visible keys, fp32 [B*H, N]. out_rest (may be
+ * NULL): what the rounding of out left, in its type and shape, for mfa_bwd_window. Key blocks that
  * no row of a query block sees are neither read nor computed. k and v must be finite also where
  * they are masked, as for mfa_fwd. `strides` (NULL: those of `layout`) are the element strides of
  * q's, k's and v's batch, head and token dimension, nine values in that order: positive multiples
@@ -134,21 +135,24 @@ MFA_API int mfa_bwd(const void* q, const void* k, const void* v, const void* out
  * other tensors are contiguous in `layout`. No counterpart in the reference.
  */
 MFA_API int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
-                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
-                           int64_t window, int64_t sinks, float scale, int32_t dtype,
-                           int32_t layout, const int64_t* strides, void* stream);
+                           void* out_rest, int64_t batch, int64_t heads, int64_t kv_heads,
+                           int64_t n, int32_t d, int64_t window, int64_t sinks, float scale,
+                           int32_t dtype, int32_t layout, const int64_t* strides, void* stream);
 
 /*
  * Backward of mfa_fwd_window, of the same types and head dims: dq, dk, dv from q, k, v, out, lse,
- * dout. dk and dv of a shared head are the sum over its query heads, in a fixed order. Takes 8 bytes
- * per query row and up to a few hundred partial sums of 64 KB (D = 128: 128 KB; of key blocks that
- * many queries see) from the library's stream-ordered pool. No counterpart in the reference.
+ * dout. dk and dv of a shared head are the sum over its query heads, in a fixed order. With out_rest
+ * (may be NULL) the rounding of out does not reach dq and dk; where rows see few keys it would be
+ * their largest error (without it 2.3 times that of their own rounding at two keys, 1.5 at fifty;
+ * with it 1.5 and 1.44). Takes 8 bytes per query row and up to a few hundred partial sums of 64 KB (D =
+ * 128: 128 KB; of key blocks that many queries see) from the library's stream-ordered pool. No
+ * counterpart in the reference.
  */
 MFA_API int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
-                           const void* dout, const float* lse, void* dq, void* dk, void* dv,
-                           int64_t batch, int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
-                           int64_t window, int64_t sinks, float scale, int32_t dtype,
-                           int32_t layout, const int64_t* strides, void* stream);
+                           const void* dout, const float* lse, const void* out_rest, void* dq,
+                           void* dk, void* dv, int64_t batch, int64_t heads, int64_t kv_heads,
+                           int64_t n, int32_t d, int64_t window, int64_t sinks, float scale,
+                           int32_t dtype, int32_t layout, const int64_t* strides, void* stream);
 
 /*
  * Paged key / value cache. k_cache and v_cache are contiguous [pages, kv_heads, page_size, d]

@@ -1034,6 +1034,27 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(Cfg::kBarStage + tile));
+      if constexpr (Cfg::kWindow && Cfg::kLSE) {
+        if (p.rest != nullptr) {
+          const HeadBatch ob = head_batch(p, cur.u);
+          uint16_t* at = p.rest + ob.b * p.rest_b + ob.h * p.rest_h + 2 * q;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int qrow = tile_row0<Cfg>(p, cur, tile) + slice + gq + 8 * r;
+            if (qrow >= p.nq) continue;
+            const float inv_l = 1.0f / l_row[r];
+            uint32_t* row = reinterpret_cast<uint32_t*>(at + qrow * p.rest_n);
+#pragma unroll
+            for (int i = 0; i < Cfg::kHeadDim / 8; ++i) {
+              const float x = __uint_as_float(o[4 * i + 2 * r]) * inv_l;
+              const float y = __uint_as_float(o[4 * i + 2 * r + 1]) * inv_l;
+              float x16, y16;
+              unpack_pair<Cfg::kBF16>(pack_pair<Cfg::kBF16>(x, y), x16, y16);
+              row[4 * i] = pack_pair<Cfg::kBF16>(x - x16, y - y16);
+            }
+          }
+        }
+      }
       if constexpr (!Cfg::kStoreRole) {
         // no store warp: the tile's first warp stores once all eight have written their
         // staging rows, then frees the Q buffer when the store has read it

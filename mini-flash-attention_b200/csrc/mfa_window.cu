@@ -171,15 +171,15 @@ cudaError_t launch(int64_t grid, int threads, int smem, cudaStream_t stream,
 
 template <class Cfg>
 int launch_forward(const void* q, const void* k, const void* v, void* out, float* lse,
-                   const Problem& w, const host::Device& dev, cudaStream_t stream) {
+                   void* rest, const Problem& w, const host::Device& dev, cudaStream_t stream) {
   FwdParams p = {};
   const bool bf16 = Cfg::kBF16;
+  const host::Strides st = host::strides_of(w.layout, w.heads, w.n, w.d);
   int rc = host::encode_heads(&p.tm_q, q, w.batch, w.heads, w.n, w.d, w.q, bf16);
   if (rc == MFA_OK) rc = host::encode_heads(&p.tm_k, k, w.batch, w.kv_heads, w.n, w.d, w.k, bf16);
   if (rc == MFA_OK) rc = host::encode_heads(&p.tm_v, v, w.batch, w.kv_heads, w.n, w.d, w.v, bf16);
   if (rc == MFA_OK)
-    rc = host::encode_heads(&p.tm_o, out, w.batch, w.heads, w.n, w.d,
-                            host::strides_of(w.layout, w.heads, w.n, w.d), bf16);
+    rc = host::encode_heads(&p.tm_o, out, w.batch, w.heads, w.n, w.d, st, bf16);
   if (rc != MFA_OK) return rc;
   p.n = p.nq = static_cast<int>(w.n);
   p.heads = static_cast<int>(w.heads);
@@ -188,6 +188,10 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
   p.timeout_ns = dev.timeout_ns;
   p.status = dev.status;
   p.lse = lse;
+  p.rest = static_cast<uint16_t*>(rest);
+  p.rest_b = st.b;
+  p.rest_h = st.h;
+  p.rest_n = st.n;
   p.window = static_cast<int>(w.window);
   p.sinks = static_cast<int>(w.sinks);
   p.sink_blocks = static_cast<int>((w.sinks + 127) / 128);
@@ -258,21 +262,21 @@ auto* prep_kernel(int32_t d) {
 // D: the kernel's head dim, at least w.d
 template <bool kBF16, int D>
 int launch_backward(const void* q, const void* k, const void* v, const void* out,
-                    const void* dout, const float* lse, void* dq, void* dk, void* dv,
-                    const Problem& w, const host::Device& dev, cudaStream_t stream) {
+                    const void* dout, const float* lse, const void* rest, void* dq, void* dk,
+                    void* dv, const Problem& w, const host::Device& dev, cudaStream_t stream) {
   const int64_t blocks = (w.n + 127) / 128, bh = w.batch * w.heads, bhk = w.batch * w.kv_heads;
   const int64_t group = w.heads / w.kv_heads, sb = (w.sinks + 127) / 128;
   // (key block, query block) pairs of one head: `reach` later query blocks see a key block
   // that holds no sinks, all later ones one that does
   const int64_t reach = (126 + w.window) >> 7;
   const int64_t span = reach + 1 < blocks ? reach + 1 : blocks;
-  const int64_t rest = blocks - sb, short_ones = reach < rest ? reach : rest;
-  const int64_t span_steps = sb * blocks - sb * (sb - 1) / 2 + (rest - short_ones) * span +
+  const int64_t others = blocks - sb, short_ones = reach < others ? reach : others;
+  const int64_t span_steps = sb * blocks - sb * (sb - 1) / 2 + (others - short_ones) * span +
                              short_ones * (short_ones + 1) / 2;
   const Pieces pc = plan_pieces(blocks, sb, span, span_steps, bhk, group, dev.sms,
                                 D == 64 ? 2.05 : 2.85);
   const int64_t sink_units = bhk * sb * pc.pieces_sink;
-  const int64_t kv_units = sink_units + bhk * rest * pc.pieces_rest, q_units = bh * blocks;
+  const int64_t kv_units = sink_units + bhk * others * pc.pieces_rest, q_units = bh * blocks;
   if (kv_units > 0x3fff0000LL || blocks * group > 0x3fff0000LL)
     return host::fail(MFA_ERR_INVALID_ARGUMENT, "B * H * N is too large");
   const int64_t slots = pc.pieces_rest > 1 ? kv_units : pc.pieces_sink > 1 ? sink_units : 0;
@@ -349,7 +353,7 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
     e = launch(need < most ? need : most, 256, 0, stream, prep_kernel<kBF16>(w.d), out, dout, lse,
                lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads),
                static_cast<long long>(st.b), static_cast<long long>(st.h),
-               static_cast<long long>(st.n), static_cast<int>(blocks), counters);
+               static_cast<long long>(st.n), static_cast<int>(blocks), counters, rest);
     const int64_t units = kv_units > q_units ? kv_units : q_units;
     const int64_t ctas = units < dev.sms ? units : dev.sms;
     if constexpr (D == 64) {
@@ -390,11 +394,11 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
 }
 
 template <bool kBF16>
-int forward_d(const void* q, const void* k, const void* v, void* out, float* lse,
+int forward_d(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
               const Problem& w, const host::Device& dev, cudaStream_t s) {
-  if (w.d == 32) return launch_forward<Window<kBF16, 32>>(q, k, v, out, lse, w, dev, s);
-  if (w.d == 64) return launch_forward<Window<kBF16, 64>>(q, k, v, out, lse, w, dev, s);
-  return launch_forward<Window<kBF16, 128>>(q, k, v, out, lse, w, dev, s);
+  if (w.d == 32) return launch_forward<Window<kBF16, 32>>(q, k, v, out, lse, rest, w, dev, s);
+  if (w.d == 64) return launch_forward<Window<kBF16, 64>>(q, k, v, out, lse, rest, w, dev, s);
+  return launch_forward<Window<kBF16, 128>>(q, k, v, out, lse, rest, w, dev, s);
 }
 
 }  // namespace
@@ -403,7 +407,7 @@ int forward_d(const void* q, const void* k, const void* v, void* out, float* lse
 using namespace mfa;
 
 extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
-                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
+                              void* rest, int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
                               int32_t d, int64_t window, int64_t sinks, float scale,
                               int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
   Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
@@ -412,21 +416,26 @@ extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void*
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
   const void* ptrs[] = {q, k, v, out};
   const char* names[] = {"q", "k", "v", "out"};
-  if ((rc = check_tensors(ptrs, names, 4, -1)) != MFA_OK) return rc;
+  const char* const rest_name = "out_rest";
+  if ((rc = check_tensors(ptrs, names, 4, -1)) != MFA_OK ||
+      (rest && (rc = check_tensors(&rest, &rest_name, 1, -1)) != MFA_OK))
+    return rc;
   if (reinterpret_cast<uintptr_t>(lse) & 3u)
     return host::fail(MFA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
   host::Device dev;
   if ((rc = host::open_device(&dev)) != MFA_OK || (rc = prepare(dev.index)) != MFA_OK) return rc;
-  if ((rc = check_tensors(ptrs, names, 4, dev.index)) != MFA_OK) return rc;
+  if ((rc = check_tensors(ptrs, names, 4, dev.index)) != MFA_OK ||
+      (rest && (rc = check_tensors(&rest, &rest_name, 1, dev.index)) != MFA_OK))
+    return rc;
   if (lse && (rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MFA_DTYPE_BF16 ? forward_d<true>(q, k, v, out, lse, w, dev, s)
-                                 : forward_d<false>(q, k, v, out, lse, w, dev, s);
+  return dtype == MFA_DTYPE_BF16 ? forward_d<true>(q, k, v, out, lse, rest, w, dev, s)
+                                 : forward_d<false>(q, k, v, out, lse, rest, w, dev, s);
 }
 
 extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
-                              const void* dout, const float* lse, void* dq, void* dk, void* dv,
-                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
+                              const void* dout, const float* lse, const void* rest, void* dq,
+                              void* dk, void* dv, int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
                               int32_t d, int64_t window, int64_t sinks, float scale,
                               int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
   Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
@@ -434,20 +443,21 @@ extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const
   if (rc != MFA_OK) return rc;
   if (batch * heads == 0 || n == 0) return MFA_OK;
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
-  const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv};
-  const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv"};
-  if ((rc = check_tensors(ptrs, names, 8, -1)) != MFA_OK) return rc;
+  const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv, rest};
+  const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv", "out_rest"};
+  const int count = rest ? 9 : 8;
+  if ((rc = check_tensors(ptrs, names, count, -1)) != MFA_OK) return rc;
   if (!lse) return host::fail(MFA_ERR_INVALID_ARGUMENT, "null lse pointer");
   if (reinterpret_cast<uintptr_t>(lse) & 3u)
     return host::fail(MFA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
   host::Device dev;
   if ((rc = host::open_device(&dev)) != MFA_OK || (rc = prepare(dev.index)) != MFA_OK) return rc;
-  if ((rc = check_tensors(ptrs, names, 8, dev.index)) != MFA_OK) return rc;
+  if ((rc = check_tensors(ptrs, names, count, dev.index)) != MFA_OK) return rc;
   if ((rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MFA_DTYPE_BF16)
-    return d <= 64 ? launch_backward<true, 64>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s)
-                   : launch_backward<true, 128>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s);
-  return d <= 64 ? launch_backward<false, 64>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s)
-                 : launch_backward<false, 128>(q, k, v, out, dout, lse, dq, dk, dv, w, dev, s);
+    return d <= 64 ? launch_backward<true, 64>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s)
+                   : launch_backward<true, 128>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s);
+  return d <= 64 ? launch_backward<false, 64>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s)
+                 : launch_backward<false, 128>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s);
 }

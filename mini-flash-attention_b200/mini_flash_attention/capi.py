@@ -92,9 +92,9 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     window_args = [ctypes.c_int64] * 4 + [ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
                                           ctypes.c_float, ctypes.c_int32, ctypes.c_int32,
                                           ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p]
-    lib.mfa_fwd_window.argtypes = [ctypes.c_void_p] * 5 + window_args
+    lib.mfa_fwd_window.argtypes = [ctypes.c_void_p] * 6 + window_args
     lib.mfa_fwd_window.restype = ctypes.c_int
-    lib.mfa_bwd_window.argtypes = [ctypes.c_void_p] * 9 + window_args
+    lib.mfa_bwd_window.argtypes = [ctypes.c_void_p] * 10 + window_args
     lib.mfa_bwd_window.restype = ctypes.c_int
     ptr, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
     lib.mfa_extend_block_tables.argtypes = [ptr] * 7 + [i64] * 5 + [ptr]
@@ -185,22 +185,23 @@ def _nine(strides):
 def fwd_window(q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, lse_ptr: int, batch: int,
                heads: int, kv_heads: int, n: int, d: int, window: int, sinks: int, scale: float,
                dtype: int = DTYPE_FP16, layout: int = LAYOUT_BHND, stream: int = 0,
-               strides: tuple[int, ...] | None = None) -> None:
-    """Launch mfa_fwd_window (lse_ptr 0: no log-sum-exp; strides: the nine (batch, head, token)
-    element strides of q, k and v); raises MfaError."""
-    _check(load().mfa_fwd_window(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, batch, heads, kv_heads, n,
-                                 d, window, sinks, scale, dtype, layout, _nine(strides), stream))
+               strides: tuple[int, ...] | None = None, rest_ptr: int = 0) -> None:
+    """Launch mfa_fwd_window (lse_ptr, rest_ptr 0: not written; strides: the nine (batch, head,
+    token) element strides of q, k and v); raises MfaError."""
+    _check(load().mfa_fwd_window(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, rest_ptr, batch, heads,
+                                 kv_heads, n, d, window, sinks, scale, dtype, layout,
+                                 _nine(strides), stream))
 
 
 def bwd_window(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_ptr: int,
                dq_ptr: int, dk_ptr: int, dv_ptr: int, batch: int, heads: int, kv_heads: int,
                n: int, d: int, window: int, sinks: int, scale: float, dtype: int = DTYPE_FP16,
                layout: int = LAYOUT_BHND, stream: int = 0,
-               strides: tuple[int, ...] | None = None) -> None:
-    """Launch mfa_bwd_window (strides as for fwd_window); raises MfaError."""
-    _check(load().mfa_bwd_window(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, dq_ptr, dk_ptr,
-                                 dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale, dtype,
-                                 layout, _nine(strides), stream))
+               strides: tuple[int, ...] | None = None, rest_ptr: int = 0) -> None:
+    """Launch mfa_bwd_window (strides as for fwd_window, rest_ptr 0: none); raises MfaError."""
+    _check(load().mfa_bwd_window(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, rest_ptr, dq_ptr,
+                                 dk_ptr, dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale,
+                                 dtype, layout, _nine(strides), stream))
 
 
 def extend_block_tables(table_ptr: int, cached_ptr: int, added_ptr: int, free_ptr: int,

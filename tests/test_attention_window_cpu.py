@@ -63,5 +63,6 @@ def test_cpu_tensors_refused_and_signatures():
         with pytest.raises(RuntimeError, match="q must be a CUDA tensor"):
             fn(q, q, q, 4)
         params = inspect.signature(fn).parameters
-        assert list(params) == ["q", "k", "v", "window", "sinks"]
-        assert params["sinks"].default == 0
+        more = ["rest"] if fn is mfa.forward_window_lse else []
+        assert list(params) == ["q", "k", "v", "window", "sinks", *more]
+        assert params["sinks"].default == 0 and all(not params[x].default for x in more)

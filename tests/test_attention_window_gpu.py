@@ -296,6 +296,54 @@ def test_mixed_layouts(d):
                             100, 2)
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@TYPES
+@pytest.mark.parametrize("b,h,hk,n,window,sinks", [(2, 2, 1, 1, 1, 0), (1, 4, 2, 300, 40, 3),
+                                                   (1, 3, 3, 1153, 200, 0), (2, 6, 2, 257, 257, 0)])
+def test_rest_of_the_output(b, h, hk, n, window, sinks, dtype, d):
+    q, k, v, dout = inputs(b, h, hk, n, d, dtype, seed=77)
+    want = reference(q, k, v, window, sinks, dout)
+    out, lse, rest = mfa.forward_window_lse(q, k, v, window, sinks, rest=True)
+    plain = mfa.forward_window_lse(q, k, v, window, sinks)
+    assert torch.equal(out, plain[0]) and torch.equal(lse, plain[1])
+    # the output's rounding is out of the bound, the rest's own in it: u |rest| <= u^2 |out| (1 + u),
+    # or half of fp16's smallest step
+    u = torch.finfo(dtype).eps / 2
+    value, bound = want["out"]
+    bound = bound - u * value.abs() + 1.01 * u * u * value.abs() + 2.0 ** -25
+    assert ((out.double() + rest.double() - value).abs() <= bound).all()
+    assert (rest.double().abs() <= 1.01 * u * out.double().abs() + 2.0 ** -24).all()
+    turned = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    got = mfa.backward_window(q, k, v, out, lse, dout, window, sinks, rest)
+    for name, x in zip(("dq", "dk", "dv"), got):
+        check(name, x, *want[name])
+    again = mfa.backward_window(q, k, v, out, lse, dout, window, sinks, turned(rest))
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+    views = [turned(x) for x in (q, k, v)]
+    same = mfa.forward_window_lse(*views, window, sinks, rest=True)
+    assert all(torch.equal(x, y) for x, y in zip(same, (out, lse, rest)))
+    for x in (rest[..., :16], rest.float(), rest.cpu()):
+        with pytest.raises(RuntimeError, match="rest must have"):
+            mfa.backward_window(q, k, v, out, lse, dout, window, sinks, x)
+
+
+@TYPES
+@pytest.mark.parametrize("window", [2, 3, 8])
+def test_few_visible_keys(window, dtype):
+    """dq and dk of rows that see few keys. Three roundings of about the same size make up their
+    error: their own, that of dS and, through the row sums, that of the forward's weights; so
+    it is at most 3 ** 0.5 times that of the first alone (and 1 in 100 for chance). The rounding of
+    the output, were it in the row sums, would make that 2.3 at two keys."""
+    q, k, v, dout = inputs(1, 4, 2, 1000, 64, dtype, seed=3)
+    want = reference(q, k, v, window, 0, dout)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(mfa.window_attention(*leaves, window), leaves, dout)
+    for name, x in zip(("dq", "dk"), grads):
+        value = want[name][0]
+        error = (x.double() - value).norm() / (value.to(dtype).double() - value).norm()
+        assert error <= 3 ** 0.5 * 1.01, (name, error.item())
+
+
 def test_autograd_unaligned_output_gradient():
     q, k, v, dout = inputs(1, 4, 2, 150, 64, torch.bfloat16)
     leaves = [x.requires_grad_() for x in (q, k, v)]
