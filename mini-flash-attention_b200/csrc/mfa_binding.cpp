@@ -261,9 +261,9 @@ std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Ten
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
   const int rc = mfa_fwd_window(
       q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-      with_lse ? lse.data_ptr<float>() : nullptr, with_rest ? rest.data_ptr() : nullptr, q.size(0), q.size(1), k.size(1), q.size(2),
-      static_cast<int32_t>(q.size(3)), window, sinks, scale, dtype_of(q),
-      bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of, current_stream());
+      with_lse ? lse.data_ptr<float>() : nullptr, with_rest ? rest.data_ptr() : nullptr, q.size(0),
+      q.size(1), k.size(1), q.size(2), static_cast<int32_t>(q.size(3)), window, sinks, scale,
+      dtype_of(q), bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of, current_stream());
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
   if (with_rest) return {out, lse, rest};
   if (with_lse) return {out, lse};
@@ -356,6 +356,10 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
 
 torch::Tensor window_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, int64_t window,
                                int64_t sinks) {
+  // nobody will ask for gradients: nothing is kept for them
+  if (!at::GradMode::is_enabled() ||
+      !(q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return flash_attn_forward_window(q, k, v, window, sinks, false, false)[0];
   return WindowAttention::apply(q, k, v, window, sinks);
 }
 

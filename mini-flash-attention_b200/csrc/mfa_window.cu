@@ -435,9 +435,10 @@ extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void*
 
 extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
                               const void* dout, const float* lse, const void* rest, void* dq,
-                              void* dk, void* dv, int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
-                              int32_t d, int64_t window, int64_t sinks, float scale,
-                              int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
+                              void* dk, void* dv, int64_t batch, int64_t heads,
+                              int64_t kv_heads, int64_t n, int32_t d, int64_t window,
+                              int64_t sinks, float scale, int32_t dtype, int32_t layout,
+                              const int64_t* strides, void* stream) {
   Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
   int rc = check(w);
   if (rc != MFA_OK) return rc;

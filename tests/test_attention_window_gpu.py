@@ -344,6 +344,22 @@ def test_few_visible_keys(window, dtype):
         assert error <= 3 ** 0.5 * 1.01, (name, error.item())
 
 
+def test_without_gradients():
+    q, k, v, _ = inputs(1, 4, 2, 150, 64, torch.float16)
+    want = mfa.forward_window(q, k, v, 40, 2)
+    assert torch.equal(mfa.window_attention(q, k, v, 40, 2), want)
+    k.requires_grad_()
+    with torch.no_grad():
+        out = mfa.window_attention(q, k, v, 40, 2)
+    assert torch.equal(out, want) and not out.requires_grad
+    del out
+    before = torch.cuda.memory_allocated()
+    out = mfa.window_attention(q, k, v, 40, 2)
+    assert torch.equal(out, want) and out.requires_grad
+    del out
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_autograd_unaligned_output_gradient():
     q, k, v, dout = inputs(1, 4, 2, 150, 64, torch.bfloat16)
     leaves = [x.requires_grad_() for x in (q, k, v)]
