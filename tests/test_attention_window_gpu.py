@@ -218,9 +218,10 @@ def test_other_stream_and_captured_step():
             assert all(torch.equal(a, b) for a, b in zip(want, result))
 
 
-def test_captured_autograd_step():
+@pytest.mark.parametrize("n,d", [(700, 64), (700, 128), (1300, 128), (1300, 32)])
+def test_captured_autograd_step(n, d):
     # the whole step in a graph (as for any operator, no eager graph of the leaves may live then)
-    q, k, v, dout = inputs(1, 4, 2, 700, 64, torch.float16)
+    q, k, v, dout = inputs(1, 4, 2, n, d, torch.float16)
     leaves = [x.requires_grad_() for x in (q, k, v)]
     want_out = mfa.window_attention(*leaves, 100, 3)
     want = torch.autograd.grad(want_out, leaves, dout)
@@ -231,6 +232,35 @@ def test_captured_autograd_step():
         got = torch.autograd.grad(out, leaves, dout)
     graph.replay()
     assert torch.equal(out, want_out) and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_two_graphs_and_two_streams(d):
+    """Steps of two layers captured apart and replayed together on two streams, again and again:
+    each has workspaces, counters and results of its own."""
+    steps = []
+    for seed, (h, hk, n, window, sinks) in enumerate(((8, 2, 2500, 300, 4), (4, 4, 1000, 1000, 0))):
+        q, k, v, dout = inputs(1, h, hk, n, d, torch.bfloat16, seed=20 * seed)
+        out, lse, rest = mfa.forward_window_lse(q, k, v, window, sinks, rest=True)
+        want = (out, lse, *mfa.backward_window(q, k, v, out, lse, dout, window, sinks, rest))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o, s, r = mfa.forward_window_lse(q, k, v, window, sinks, rest=True)
+            got = (o, s, *mfa.backward_window(q, k, v, o, s, dout, window, sinks, r))
+        steps.append((graph, got, want, torch.cuda.Stream(), (q, k, v, dout)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _, got, *_ in steps:
+            for x in got:
+                x.zero_()
+        torch.cuda.synchronize()
+        for graph, _, _, stream, _ in steps:
+            with torch.cuda.stream(stream):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, got, want, *_ in steps:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_capi_bnhd_layout():
