@@ -759,7 +759,9 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D
   const int slot_rows = p.group < Cfg::kRows ? p.group : Cfg::kRows;
   float* sums = reinterpret_cast<float*>(smem);
   float* tops = sums + slot_rows * D;
-  if (cur.left == 0) {  // no tile for this CTA
+  if (cur.left == 0) {  // no tile for this CTA: sums of nothing, which the others add as they are
+    for (int i = threadIdx.x; i < slot_rows * (D / 4); i += Cfg::kThreads)
+      reinterpret_cast<float4*>(sums)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (threadIdx.x < slot_rows) {
       tops[threadIdx.x] = -INFINITY;
       tops[slot_rows + threadIdx.x] = 0.0f;
@@ -789,13 +791,13 @@ __global__ void __launch_bounds__(PagedConfig<D, kBF16>::kThreads, PagedConfig<D
       const float w = ex2_approx(cluster_load(stats + 4 * row, c) - sub);
       const float pl = cluster_load(stats + 4 * (slot_rows + row), c);
       const float4 x = cluster_load4(base + 4 * (row * D + col), c);
-      if (w > 0.0f) {
-        l = fmaf(pl, w, l);
-        acc.x = fmaf(x.x, w, acc.x);
-        acc.y = fmaf(x.y, w, acc.y);
-        acc.z = fmaf(x.z, w, acc.z);
-        acc.w = fmaf(x.w, w, acc.w);
-      }
+      // (no weight is left out: of scores that are all NaN the maximum is -inf and the weight 0, of
+      // an infinite one inf and NaN, and the sums, NaN in both, have to reach the output)
+      l = fmaf(pl, w, l);
+      acc.x = fmaf(x.x, w, acc.x);
+      acc.y = fmaf(x.y, w, acc.y);
+      acc.z = fmaf(x.z, w, acc.z);
+      acc.w = fmaf(x.w, w, acc.w);
     }
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     *reinterpret_cast<uint2*>(p.out + (cur.query(p) + row) * p.cols + col) =
