@@ -46,7 +46,7 @@ __device__ __forceinline__ uint64_t f2_splat(float x) { return f2_pack(x, x); }
 __device__ __forceinline__ uint64_t f2_neg(uint64_t a) { return a ^ 0x8000000080000000ull; }
 
 // 2^x for a pair, on the FMA pipe. Inputs below -125 are clamped (the result is then
-// ~2^-125, i.e. zero for every consumer here); inputs are expected <= 2^22.
+// ~2^-125, i.e. zero for every consumer here), and so is NaN; inputs are expected <= 2^22.
 __device__ __forceinline__ void exp2_poly_pair(float x0, float x1, float& y0, float& y1) {
   constexpr float kC0 = 0.9999280571937561f;
   constexpr float kC1 = 0.6932609677314758f;

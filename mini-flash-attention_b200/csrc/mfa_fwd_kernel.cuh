@@ -44,6 +44,7 @@
 
 #include <cuda.h>
 #include <cuda_fp16.h>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -475,8 +476,8 @@ __device__ __forceinline__ void load_role(const FwdParams& p, uint8_t* smem, uin
 }
 
 // Load role of the prefix variant, executed by two whole warps: queries and k (kValue false), or v.
-// A query tile is tile_batch requests' group rows (its rows behind them are never written, and
-// their results never read); a key block is one box for each of its pages, of which those behind
+// A query tile is tile_batch requests' group rows (its rows behind them are 0, and their results
+// never read); a key block is one box for each of its pages, of which those behind
 // the prefix's end are left out. Lane i looks up box i of a batch of blocks (32 boxes); the next
 // batch's pages are on their way while this one's copies are issued.
 template <class Cfg, bool kValue>
@@ -497,6 +498,17 @@ __device__ __forceinline__ void prefix_load_role(const FwdParams& p, uint8_t* sm
   if (lane == 0) {
     if (!kValue) tma_prefetch_desc(&p.tm_q);
     tma_prefetch_desc(map);
+  }
+  if (!kValue && p.tile_rows < Cfg::kRows) {
+    // the rows behind tile_rows, which no copy writes, are 0: what lay there could be NaN and
+    // send the rows beside it through the path of a grown maximum in every step
+    constexpr int kChunks = Cfg::kRowBytes / 16;
+    for (int t = 0; t < Cfg::kQBuffers * Cfg::NQ * Cfg::kBoxes; ++t)
+      for (int c = p.tile_rows * kChunks + lane; c < Cfg::kRows * kChunks; c += 32)
+        *reinterpret_cast<uint4*>(smem + Cfg::kQOff + t * Cfg::kBoxBytes + 16 * c) =
+            make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+    __syncwarp();
   }
   auto look_up = [&](int block) -> int {  // this lane's page in the batch that starts at `block`
     const long long key = static_cast<long long>(block) * Cfg::kKeys + (lane << box_shift);
@@ -836,34 +848,40 @@ __device__ __forceinline__ bool softmax_step(const FwdParams& p, uint32_t bars, 
     }
   }
 
-  // This thread's row maxima: two 3-input max chains per row over its 32 scores.
+  // This thread's row maxima: two 3-input max chains per row over its 32 scores. A score of NaN
+  // makes the maximum NaN, which counts as grown below and makes every weight of the row NaN:
+  // the polynomial exponentials clamp their argument and would take NaN for a weight of 0.
   float mloc[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    float a = fmaxf(f(sr[2 * r]), f(sr[2 * r + 1]));
-    float b = fmaxf(f(sr[4 + 2 * r]), f(sr[5 + 2 * r]));
+    float a = max2_nan(f(sr[2 * r]), f(sr[2 * r + 1]));
+    float b = max2_nan(f(sr[4 + 2 * r]), f(sr[5 + 2 * r]));
 #pragma unroll
     for (int i = 2; i < 16; i += 2) {
-      a = max3(a, f(sr[4 * i + 2 * r]), f(sr[4 * i + 2 * r + 1]));
-      b = max3(b, f(sr[4 * i + 4 + 2 * r]), f(sr[4 * i + 5 + 2 * r]));
+      a = max3_nan(a, f(sr[4 * i + 2 * r]), f(sr[4 * i + 2 * r + 1]));
+      b = max3_nan(b, f(sr[4 * i + 4 + 2 * r]), f(sr[4 * i + 5 + 2 * r]));
     }
-    mloc[r] = fmaxf(a, b);
+    mloc[r] = max2_nan(a, b);
   }
   // The reference max is raised only when some row of the warp grew past the threshold. A
   // row grows iff one of its four threads holds a score past it (c > 0: scaling preserves
   // the order), so the vote runs on the thread maxima and the row maxima are combined by
   // shuffles only on that rare path; otherwise the reference max stays and alpha = 1.
-  const bool grow = __any_sync(0xffffffffu, mloc[0] * c > m_run[0] + Cfg::kRescaleThreshold ||
-                                                mloc[1] * c > m_run[1] + Cfg::kRescaleThreshold);
+  const bool grow =
+      __any_sync(0xffffffffu, !(mloc[0] * c <= m_run[0] + Cfg::kRescaleThreshold &&
+                                mloc[1] * c <= m_run[1] + Cfg::kRescaleThreshold));
   float alpha[2] = {1.0f, 1.0f};
   if (grow) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) mloc[r] = fmaxf(mloc[r], __shfl_xor_sync(0xffffffffu, mloc[r], 1));
+    for (int r = 0; r < 2; ++r)
+      mloc[r] = max2_nan(mloc[r], __shfl_xor_sync(0xffffffffu, mloc[r], 1));
 #pragma unroll
-    for (int r = 0; r < 2; ++r) mloc[r] = fmaxf(mloc[r], __shfl_xor_sync(0xffffffffu, mloc[r], 2));
+    for (int r = 0; r < 2; ++r)
+      mloc[r] = max2_nan(mloc[r], __shfl_xor_sync(0xffffffffu, mloc[r], 2));
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float m_use = fmaxf(m_run[r], mloc[r] * c);
+      float m_use = max2_nan(m_run[r], mloc[r] * c);
+      if (m_use == INFINITY) m_use = NAN;  // inf - inf: the row is NaN by the formula
       // 0 on a unit's first block (m_run = -inf); 1 while every key so far is masked
       // (causal, m_use = -inf), without an -inf - -inf
       if (!(Cfg::kCausal && m_use == -INFINITY)) alpha[r] = ex2_approx(m_run[r] - m_use);
