@@ -93,9 +93,7 @@ cudaError_t set_smem_attributes_d() {
 }
 
 struct DeviceState {
-  std::once_flag once;
-  int error = MFA_OK;
-  std::string message;
+  host::SetUp set_up;  // the fields below are valid once it is done
   int* status_ptr = nullptr;
   int num_sms = 0;
   cudaMemPool_t pool = nullptr;  // split-mode scratch; keeps its memory between calls
@@ -156,9 +154,10 @@ int check_architecture(int dev, int* num_sms, std::string* msg) {
 int prepare_device(int dev) {
   if (dev < 0 || dev >= kMaxDevices) return fail(MFA_ERR_DEVICE, "device index out of range");
   DeviceState& ds = g_devices[dev];
-  std::call_once(ds.once, [&ds, dev] {
-    ds.error = check_architecture(dev, &ds.num_sms, &ds.message);
-    if (ds.error != MFA_OK) return;
+  return ds.set_up([&ds, dev]() -> int {
+    std::string msg;
+    const int rc = check_architecture(dev, &ds.num_sms, &msg);
+    if (rc != MFA_OK) return fail(rc, msg);
     cudaError_t e = set_smem_attributes_d<32>();
     if (e == cudaSuccess) e = set_smem_attributes_d<64>();
     if (e == cudaSuccess) e = set_smem_attributes_d<128>();
@@ -166,7 +165,7 @@ int prepare_device(int dev) {
     if (e == cudaSuccess) e = set_smem_attribute<Simple<false>>();
     if (e == cudaSuccess) e = set_smem_attribute<Simple<true>>();
     if (e == cudaSuccess) e = cudaGetSymbolAddress(reinterpret_cast<void**>(&ds.status_ptr), g_device_status);
-    if (e == cudaSuccess) {
+    if (e == cudaSuccess && ds.pool == nullptr) {
       // A private stream-ordered pool for the split-mode partial results: the scratch is
       // allocated and freed on the caller's stream around each launch, and the pool keeps
       // the memory mapped so that later calls do not pay for mapping it again.
@@ -175,18 +174,13 @@ int prepare_device(int dev) {
       props.location.type = cudaMemLocationTypeDevice;
       props.location.id = dev;
       e = cudaMemPoolCreate(&ds.pool, &props);
-      if (e == cudaSuccess) {
-        uint64_t keep = UINT64_MAX;
-        e = cudaMemPoolSetAttribute(ds.pool, cudaMemPoolAttrReleaseThreshold, &keep);
-      }
     }
-    if (e != cudaSuccess) {
-      ds.error = MFA_ERR_CUDA;
-      ds.message = std::string("CUDA error: ") + cudaGetErrorString(e) + " (device set-up)";
+    if (e == cudaSuccess) {
+      uint64_t keep = UINT64_MAX;
+      e = cudaMemPoolSetAttribute(ds.pool, cudaMemPoolAttrReleaseThreshold, &keep);
     }
+    return e == cudaSuccess ? MFA_OK : fail_cuda(e, "device set-up");
   });
-  if (ds.error != MFA_OK) return fail(ds.error, ds.message);
-  return MFA_OK;
 }
 
 // Element strides (n, h, b) of a [B, H, N, D] (layout 0) or [B, N, H, D] (layout 1) tensor.

@@ -6,14 +6,43 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
+#include <mutex>
 #include <string>
+
+#include "../../include/mfa_b200.h"
 
 namespace mfa {
 namespace host {
 
 int fail(int code, const std::string& msg);
 int fail_cuda(cudaError_t e, const char* what);
+
+// A device's one-time set-up: `run` is called, by one thread at a time, until it has returned
+// MFA_OK. A failure is the calling entry's own, the next one tries again. The process's first
+// call may be one that is captured: nothing in a set-up belongs to the stream, so for its time the
+// thread may make the calls that a capture forbids by default (kernel attributes, symbol
+// addresses, a memory pool).
+class SetUp {
+ public:
+  template <class F>
+  int operator()(F&& run) {
+    if (done_.load(std::memory_order_acquire)) return MFA_OK;
+    const std::lock_guard<std::mutex> lock(mu_);
+    if (done_.load(std::memory_order_relaxed)) return MFA_OK;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    const int rc = run();
+    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+    if (rc == MFA_OK) done_.store(true, std::memory_order_release);
+    return rc;
+  }
+
+ private:
+  std::mutex mu_;
+  std::atomic<bool> done_{false};
+};
 
 // The current device after its one-time set-up.
 struct Device {

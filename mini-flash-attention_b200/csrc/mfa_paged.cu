@@ -5,7 +5,6 @@
 
 #include <cmath>
 #include <cstdint>
-#include <mutex>
 #include <string>
 
 #include "../../include/mfa_b200.h"
@@ -61,13 +60,12 @@ cudaError_t set_attributes() {
 }
 
 int prepare(int dev) {
-  static std::once_flag once[kMaxDevices];
-  static cudaError_t error[kMaxDevices];
-  std::call_once(once[dev], [dev] {
-    error[dev] = set_attributes<false>();
-    if (error[dev] == cudaSuccess) error[dev] = set_attributes<true>();
+  static host::SetUp set_up[kMaxDevices];
+  return set_up[dev]([]() -> int {
+    cudaError_t e = set_attributes<false>();
+    if (e == cudaSuccess) e = set_attributes<true>();
+    return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "paged kernel set-up");
   });
-  return error[dev] == cudaSuccess ? MFA_OK : host::fail_cuda(error[dev], "paged kernel set-up");
 }
 
 int invalid(const std::string& msg) { return host::fail(MFA_ERR_INVALID_ARGUMENT, msg); }

@@ -7,7 +7,6 @@
 
 #include <cmath>
 #include <cstdint>
-#include <mutex>
 #include <string>
 
 #include "../../include/mfa_b200.h"
@@ -63,13 +62,12 @@ cudaError_t set_attributes() {
 }
 
 int prepare(int dev) {
-  static std::once_flag once[kMaxDevices];
-  static cudaError_t error[kMaxDevices];
-  std::call_once(once[dev], [dev] {
-    error[dev] = set_attributes<false>();
-    if (error[dev] == cudaSuccess) error[dev] = set_attributes<true>();
+  static host::SetUp set_up[kMaxDevices];
+  return set_up[dev]([]() -> int {
+    cudaError_t e = set_attributes<false>();
+    if (e == cudaSuccess) e = set_attributes<true>();
+    return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "window kernel set-up");
   });
-  return error[dev] == cudaSuccess ? MFA_OK : host::fail_cuda(error[dev], "window kernel set-up");
 }
 
 // The arguments of both directions, checked.
