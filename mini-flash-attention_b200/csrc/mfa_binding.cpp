@@ -356,6 +356,10 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
 
 torch::Tensor window_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, int64_t window,
                                int64_t sinks) {
+  // a tangent (torch.autograd.forward_ad) needs no requires_grad; dropped, it would read as 0
+  for (const auto* x : {&q, &k, &v})
+    TORCH_CHECK(!x->_fw_grad(/*level=*/0).defined(),
+                "window_attention has no forward-mode derivative");
   // nobody will ask for gradients: nothing is kept for them
   if (!at::GradMode::is_enabled() ||
       !(q.requires_grad() || k.requires_grad() || v.requires_grad()))

@@ -119,8 +119,8 @@ def backward_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
                      sinks: int = 0) -> torch.Tensor:
     """Differentiable forward_window (gradients can be taken once: a gradient of a gradient
-    raises). It keeps q, k, v, the output and its log-sum-exp, and up to 1024 tokens or below a
-    window of 64 the output's rest (backward_window)."""
+    raises, and so does a forward-mode derivative). It keeps q, k, v, the output and its log-sum-exp,
+    and up to 1024 tokens or below a window of 64 the output's rest (backward_window)."""
     return _load_extension().window_attention(q, k, v, int(window), int(sinks))
 
 
