@@ -140,11 +140,22 @@ MFA_API int mfa_fwd_window(const void* q, const void* k, const void* v, void* ou
                            int32_t dtype, int32_t layout, const int64_t* strides, void* stream);
 
 /*
+ * mfa_fwd_window with an out_rest of the first rest_rows rows of every head only: its extents are
+ * [batch, heads, rest_rows, d], its memory order that of `layout`, 0 <= rest_rows <= n. The first rows of a
+ * sequence see few keys whatever its length. No counterpart in the reference.
+ */
+MFA_API int mfa_fwd_window_rest(const void* q, const void* k, const void* v, void* out, float* lse,
+                                void* out_rest, int64_t rest_rows, int64_t batch, int64_t heads,
+                                int64_t kv_heads, int64_t n, int32_t d, int64_t window,
+                                int64_t sinks, float scale, int32_t dtype, int32_t layout,
+                                const int64_t* strides, void* stream);
+
+/*
  * Backward of mfa_fwd_window, of the same types and head dims: dq, dk, dv from q, k, v, out, lse,
  * dout. dk and dv of a shared head are the sum over its query heads, in a fixed order. With out_rest
  * (may be NULL) the rounding of out does not reach dq and dk; where rows see few keys it would be
- * their largest error (without it 2.3 times that of their own rounding at two keys, 1.5 at fifty;
- * with it 1.5 and 1.44). Takes 8 bytes per query row and up to a few hundred partial sums of 64 KB (D =
+ * their largest error (without it 2.2 times that of their own rounding in rows that see two to four
+ * keys, 1.49 at 16 to 64, 1.45 from there on; with it 1.48, 1.45 and 1.44). Takes 8 bytes per query row and up to a few hundred partial sums of 64 KB (D =
  * 128: 128 KB; of key blocks that many queries see) from the library's stream-ordered pool. No
  * counterpart in the reference.
  */
@@ -153,6 +164,14 @@ MFA_API int mfa_bwd_window(const void* q, const void* k, const void* v, const vo
                            void* dk, void* dv, int64_t batch, int64_t heads, int64_t kv_heads,
                            int64_t n, int32_t d, int64_t window, int64_t sinks, float scale,
                            int32_t dtype, int32_t layout, const int64_t* strides, void* stream);
+
+/* mfa_bwd_window with the out_rest of mfa_fwd_window_rest. No counterpart in the reference. */
+MFA_API int mfa_bwd_window_rest(const void* q, const void* k, const void* v, const void* out,
+                                const void* dout, const float* lse, const void* out_rest,
+                                int64_t rest_rows, void* dq, void* dk, void* dv, int64_t batch,
+                                int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
+                                int64_t window, int64_t sinks, float scale, int32_t dtype,
+                                int32_t layout, const int64_t* strides, void* stream);
 
 /*
  * Paged key / value cache. k_cache and v_cache are contiguous [pages, kv_heads, page_size, d]

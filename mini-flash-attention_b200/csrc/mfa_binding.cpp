@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <limits>
@@ -244,12 +245,15 @@ void* current_stream() {
   return static_cast<void*>(at::cuda::getCurrentCUDAStream().stream());
 }
 
-// Windowed attention: out, then lse and the output's rest if asked for (the rest with lse only).
+// Windowed attention: out, then lse and the output's rest of the first rest_rows rows (-1: all) if
+// asked for (the rest with lse only).
 std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Tensor k,
                                                      torch::Tensor v, int64_t window,
                                                      int64_t sinks, bool with_lse,
-                                                     bool with_rest) {
+                                                     int64_t rest_rows) {
   check_window_inputs(q, k, v);
+  const bool with_rest = rest_rows != 0;
+  if (rest_rows < 0) rest_rows = q.size(2);
   const c10::cuda::CUDAGuard device_guard(q.device());
   const bool bnhd = tokens_first(q);
   const WindowStrides strides(q, k, v);
@@ -257,12 +261,12 @@ std::vector<torch::Tensor> flash_attn_forward_window(torch::Tensor q, torch::Ten
   torch::Tensor lse, rest;
   if (with_lse)
     lse = new_empty({q.size(0), q.size(1), q.size(2)}, torch::kFloat32, q);
-  if (with_rest) rest = new_heads(q.sizes(), bnhd, q);
+  if (with_rest) rest = new_heads({q.size(0), q.size(1), rest_rows, q.size(3)}, bnhd, q);
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
-  const int rc = mfa_fwd_window(
+  const int rc = mfa_fwd_window_rest(
       q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-      with_lse ? lse.data_ptr<float>() : nullptr, with_rest ? rest.data_ptr() : nullptr, q.size(0),
-      q.size(1), k.size(1), q.size(2), static_cast<int32_t>(q.size(3)), window, sinks, scale,
+      with_lse ? lse.data_ptr<float>() : nullptr, with_rest ? rest.data_ptr() : nullptr, rest_rows,
+      q.size(0), q.size(1), k.size(1), q.size(2), static_cast<int32_t>(q.size(3)), window, sinks, scale,
       dtype_of(q), bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of, current_stream());
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
   if (with_rest) return {out, lse, rest};
@@ -292,9 +296,11 @@ std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Te
   const bool bnhd = tokens_first(q);
   const WindowStrides strides(q, k, v);
   if (rest) {
-    TORCH_CHECK(rest->is_cuda() && rest->device() == q.device() && rest->sizes() == q.sizes() &&
+    TORCH_CHECK(rest->is_cuda() && rest->device() == q.device() && rest->dim() == 4 &&
+                    rest->size(0) == q.size(0) && rest->size(1) == q.size(1) &&
+                    rest->size(2) <= q.size(2) && rest->size(3) == q.size(3) &&
                     rest->scalar_type() == q.scalar_type(),
-                "rest must have q's device, shape and dtype");
+                "rest must have q's device, dtype and shape (or its first rows)");
     rest = dense(*rest, bnhd);
   }
   out = dense(out, bnhd);
@@ -303,13 +309,12 @@ std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Te
   auto dk = new_heads(k.sizes(), bnhd, q);
   auto dv = new_heads(v.sizes(), bnhd, q);
   const float scale = 1.0f / std::sqrt(static_cast<float>(q.size(3)));
-  const int rc = mfa_bwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                dout.data_ptr(), lse.data_ptr<float>(),
-                                rest ? rest->data_ptr() : nullptr, dq.data_ptr(), dk.data_ptr(),
-                                dv.data_ptr(), q.size(0), q.size(1), k.size(1), q.size(2),
-                                static_cast<int32_t>(q.size(3)), window, sinks, scale,
-                                dtype_of(q), bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of,
-                                current_stream());
+  const int rc = mfa_bwd_window_rest(
+      q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(),
+      lse.data_ptr<float>(), rest ? rest->data_ptr() : nullptr, rest ? rest->size(2) : 0,
+      dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), q.size(0), q.size(1), k.size(1), q.size(2),
+      static_cast<int32_t>(q.size(3)), window, sinks, scale, dtype_of(q),
+      bnhd ? MFA_LAYOUT_BNHD : MFA_LAYOUT_BHND, strides.of, current_stream());
   if (rc != MFA_OK) throw std::runtime_error(mfa_last_error_string());
   return {dq, dk, dv};
 }
@@ -319,12 +324,14 @@ std::vector<torch::Tensor> flash_attn_backward_window(torch::Tensor q, torch::Te
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor q,
                                torch::Tensor k, torch::Tensor v, int64_t window, int64_t sinks) {
-    // The rest of the output costs as much memory as the output, and is kept where it matters: with
-    // more than 1024 tokens of which 64 or more are seen, gradients are 1.48 times as far off as
-    // their own rounding without it and 1.44 times with it (mfa_bwd_prep_kernel has more).
-    const bool keep_rest = q.dim() == 4 && (q.size(2) <= 1024 || window < 64);
-    const auto r = flash_attn_forward_window(q, k, v, window, sinks, true, keep_rest);
-    if (keep_rest)
+    // The rest of the output is kept for the rows that see few keys: rows of 64 or more are 1.45 times
+    // as far off as their own rounding without it and 1.44 times with it, but those of fewer up to
+    // 2.2 times (mfa_bwd_prep_kernel has more). They are the first ones of a sequence of any length,
+    // and below a window of 64 all. (1024 rows, not 64: a short sequence has all of its rest.)
+    const int64_t n = q.dim() == 4 ? q.size(2) : 0;
+    const auto r = flash_attn_forward_window(q, k, v, window, sinks, true,
+                                             window < 64 ? n : std::min<int64_t>(n, 1024));
+    if (r.size() > 2)
       ctx->save_for_backward({q, k, v, r[0], r[1], r[2]});
     else
       ctx->save_for_backward({q, k, v, r[0], r[1]});

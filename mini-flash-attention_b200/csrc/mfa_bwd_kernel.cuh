@@ -1330,11 +1330,12 @@ constexpr int bwd_smem_bytes() {
 
 // D_i = rowsum(dO ⊙ o) and L2_i = L_i * log2(e) for every row, into [bh][blocks * 128] arrays
 // padded past N with D = 0, L2 = +inf (so that padded queries get P = 0 in the dK/dV pass).
-// D / 8 threads per row (16 bytes each), grid-stride. `rest`, if given, is what the rounding of o left:
-// dP - D is a difference, in which the rounding of o weighs most where few keys are visible. (Errors
-// of dq and dk over those of rounding them alone, normal inputs, without the rest and with it: 2.3 and
-// 1.5 at two visible keys, 1.6 and 1.46 at eight, 1.7 and 1.45 at causal 16, 1.5 and 1.46 at causal
-// 256. The rounding of dS alone makes 1.41, that of P for o most of what is left.)
+// D / 8 threads per row (16 bytes each), grid-stride. `rest` is what the rounding of o left, of the
+// first rest_rows (0: none) rows of every head: dP - D is a difference, in which the rounding of o
+// weighs most where few keys are visible. (Errors of dq over those of rounding it alone, normal
+// inputs, D = 64, without the rest and with it: 2.2 and 1.48 in rows that see two to four keys, 1.61 and
+// 1.46 up to 16, 1.49 and 1.45 up to 64, 1.45 and 1.44 beyond, at any length. The rounding of dS alone
+// makes 1.41, that of P for o most of what is left.)
 template <bool kBF16, bool kWindow = false, int kD = 64>
 __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const void* dout,
                                                            const float* lse, float* lse2,
@@ -1342,7 +1343,11 @@ __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const 
                                                            long long stride_b, long long stride_h,
                                                            long long stride_n, int blocks,
                                                            int* counters = nullptr,
-                                                           const void* rest = nullptr) {
+                                                           const void* rest = nullptr,
+                                                           int rest_rows = 0,
+                                                           long long rest_b = 0,
+                                                           long long rest_h = 0,
+                                                           long long rest_n = 0) {
   if constexpr (kWindow) {
     // a programmatic dependent, as is the kernel after it; the passes' unit counters start at 0
     if (threadIdx.x == 0) grid_dependents_launch();
@@ -1368,8 +1373,10 @@ __global__ void __launch_bounds__(256) mfa_bwd_prep_kernel(const void* o, const 
       const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(dout) + off);
       const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
       uint4 c = make_uint4(0u, 0u, 0u, 0u);
-      if (kWindow && rest != nullptr)
-        c = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(rest) + off);
+      if (kWindow && row < rest_rows)
+        c = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(rest) +
+                                            h / heads * rest_b + h % heads * rest_h +
+                                            row * rest_n + 8 * sub);
       [[maybe_unused]] const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {

@@ -43,9 +43,11 @@ struct FwdParams {
   int sink_blocks;
   int kv_group;
   int whole_units;  // query blocks done whole; the others tile by tile (WindowCursor)
-  // Optional (null: not written): the output less its rounding, in the type of the output and with
-  // these strides; the backward's row sums want the output itself (see mfa_bwd_prep_kernel).
+  // Optional (null: not written): the output less its rounding, of the first rest_rows rows of
+  // every head, in the type of the output and with these strides; the backward's row sums want
+  // the output itself (see mfa_bwd_prep_kernel).
   uint16_t* rest;
+  int rest_rows;
   long long rest_b, rest_h, rest_n;
   // Prefix variant: tm_q is {D, group, batch, kv_heads} with boxes of tile_batch requests (a
   // query tile has tile_rows = tile_batch * group rows), tm_k and tm_v are {D, page_size,

@@ -1059,7 +1059,7 @@ __device__ __forceinline__ void softmax_role(const FwdParams& p, uint8_t* smem, 
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int qrow = tile_row0<Cfg>(p, cur, tile) + slice + gq + 8 * r;
-            if (qrow >= p.nq) continue;
+            if (qrow >= p.rest_rows) continue;
             const float inv_l = 1.0f / l_row[r];
             uint32_t* row = reinterpret_cast<uint32_t*>(at + qrow * p.rest_n);
 #pragma unroll

@@ -75,6 +75,7 @@ struct Problem {
   int64_t batch, heads, kv_heads, n, window, sinks;
   int32_t d, dtype, layout;
   float scale;
+  int64_t rest_rows;  // of the output's rest, if it is given
   host::Strides q, k, v;
 };
 
@@ -134,6 +135,8 @@ int check(Problem& w) {
     w.sinks = 0;
   }
   if (w.sinks > w.n) w.sinks = w.n;
+  if (w.rest_rows < 0 || w.rest_rows > w.n)
+    return host::fail(MFA_ERR_INVALID_ARGUMENT, "rest_rows must be within [0, N]");
   return MFA_OK;
 }
 
@@ -186,10 +189,12 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
   p.timeout_ns = dev.timeout_ns;
   p.status = dev.status;
   p.lse = lse;
+  const host::Strides rs = host::strides_of(w.layout, w.heads, w.rest_rows, w.d);
   p.rest = static_cast<uint16_t*>(rest);
-  p.rest_b = st.b;
-  p.rest_h = st.h;
-  p.rest_n = st.n;
+  p.rest_rows = static_cast<int>(w.rest_rows);
+  p.rest_b = rs.b;
+  p.rest_h = rs.h;
+  p.rest_n = rs.n;
   p.window = static_cast<int>(w.window);
   p.sinks = static_cast<int>(w.sinks);
   p.sink_blocks = static_cast<int>((w.sinks + 127) / 128);
@@ -347,11 +352,14 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
   if (rc == MFA_OK) {
     const int64_t need = static_cast<int64_t>(rows) * w.d / 2048;  // 16 bytes a thread
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
+    const host::Strides rs = host::strides_of(w.layout, w.heads, w.rest_rows, w.d);
     // the kernels wait for the stream's earlier work themselves and may be set up while it ends
     e = launch(need < most ? need : most, 256, 0, stream, prep_kernel<kBF16>(w.d), out, dout, lse,
                lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads),
                static_cast<long long>(st.b), static_cast<long long>(st.h),
-               static_cast<long long>(st.n), static_cast<int>(blocks), counters, rest);
+               static_cast<long long>(st.n), static_cast<int>(blocks), counters, rest,
+               static_cast<int>(rest ? w.rest_rows : 0), static_cast<long long>(rs.b),
+               static_cast<long long>(rs.h), static_cast<long long>(rs.n));
     const int64_t units = kv_units > q_units ? kv_units : q_units;
     const int64_t ctas = units < dev.sms ? units : dev.sms;
     if constexpr (D == 64) {
@@ -399,18 +407,11 @@ int forward_d(const void* q, const void* k, const void* v, void* out, float* lse
   return launch_forward<Window<kBF16, 128>>(q, k, v, out, lse, rest, w, dev, s);
 }
 
-}  // namespace
-}  // namespace mfa
-
-using namespace mfa;
-
-extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
-                              void* rest, int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
-                              int32_t d, int64_t window, int64_t sinks, float scale,
-                              int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
-  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
+int forward(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
+            Problem& w, const int64_t* strides, void* stream) {
   int rc = check(w);
-  if (rc != MFA_OK || batch * heads == 0 || n == 0) return rc;
+  if (rc != MFA_OK || w.batch * w.heads == 0 || w.n == 0) return rc;
+  if (w.rest_rows == 0) rest = nullptr;
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
   const void* ptrs[] = {q, k, v, out};
   const char* names[] = {"q", "k", "v", "out"};
@@ -427,20 +428,16 @@ extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void*
     return rc;
   if (lse && (rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MFA_DTYPE_BF16 ? forward_d<true>(q, k, v, out, lse, rest, w, dev, s)
-                                 : forward_d<false>(q, k, v, out, lse, rest, w, dev, s);
+  return w.dtype == MFA_DTYPE_BF16 ? forward_d<true>(q, k, v, out, lse, rest, w, dev, s)
+                                   : forward_d<false>(q, k, v, out, lse, rest, w, dev, s);
 }
 
-extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
-                              const void* dout, const float* lse, const void* rest, void* dq,
-                              void* dk, void* dv, int64_t batch, int64_t heads,
-                              int64_t kv_heads, int64_t n, int32_t d, int64_t window,
-                              int64_t sinks, float scale, int32_t dtype, int32_t layout,
-                              const int64_t* strides, void* stream) {
-  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, {}, {}, {}};
+int backward(const void* q, const void* k, const void* v, const void* out, const void* dout,
+             const float* lse, const void* rest, void* dq, void* dk, void* dv, Problem& w,
+             const int64_t* strides, void* stream) {
   int rc = check(w);
-  if (rc != MFA_OK) return rc;
-  if (batch * heads == 0 || n == 0) return MFA_OK;
+  if (rc != MFA_OK || w.batch * w.heads == 0 || w.n == 0) return rc;
+  if (w.rest_rows == 0) rest = nullptr;
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
   const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv, rest};
   const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv", "out_rest"};
@@ -454,9 +451,53 @@ extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const
   if ((rc = check_tensors(ptrs, names, count, dev.index)) != MFA_OK) return rc;
   if ((rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == MFA_DTYPE_BF16)
-    return d <= 64 ? launch_backward<true, 64>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s)
-                   : launch_backward<true, 128>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s);
-  return d <= 64 ? launch_backward<false, 64>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s)
-                 : launch_backward<false, 128>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s);
+  if (w.dtype == MFA_DTYPE_BF16)
+    return w.d <= 64
+               ? launch_backward<true, 64>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s)
+               : launch_backward<true, 128>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s);
+  return w.d <= 64
+             ? launch_backward<false, 64>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s)
+             : launch_backward<false, 128>(q, k, v, out, dout, lse, rest, dq, dk, dv, w, dev, s);
+}
+
+}  // namespace
+}  // namespace mfa
+
+using namespace mfa;
+
+extern "C" int mfa_fwd_window(const void* q, const void* k, const void* v, void* out, float* lse,
+                              void* rest, int64_t batch, int64_t heads, int64_t kv_heads, int64_t n,
+                              int32_t d, int64_t window, int64_t sinks, float scale,
+                              int32_t dtype, int32_t layout, const int64_t* strides, void* stream) {
+  return mfa_fwd_window_rest(q, k, v, out, lse, rest, n > 0 ? n : 0, batch, heads, kv_heads, n, d,
+                             window, sinks, scale, dtype, layout, strides, stream);
+}
+
+extern "C" int mfa_fwd_window_rest(const void* q, const void* k, const void* v, void* out,
+                                   float* lse, void* rest, int64_t rest_rows, int64_t batch,
+                                   int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
+                                   int64_t window, int64_t sinks, float scale, int32_t dtype,
+                                   int32_t layout, const int64_t* strides, void* stream) {
+  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, rest_rows, {}, {}, {}};
+  return forward(q, k, v, out, lse, rest, w, strides, stream);
+}
+
+extern "C" int mfa_bwd_window(const void* q, const void* k, const void* v, const void* out,
+                              const void* dout, const float* lse, const void* rest, void* dq,
+                              void* dk, void* dv, int64_t batch, int64_t heads,
+                              int64_t kv_heads, int64_t n, int32_t d, int64_t window,
+                              int64_t sinks, float scale, int32_t dtype, int32_t layout,
+                              const int64_t* strides, void* stream) {
+  return mfa_bwd_window_rest(q, k, v, out, dout, lse, rest, n > 0 ? n : 0, dq, dk, dv, batch, heads,
+                             kv_heads, n, d, window, sinks, scale, dtype, layout, strides, stream);
+}
+
+extern "C" int mfa_bwd_window_rest(const void* q, const void* k, const void* v, const void* out,
+                                   const void* dout, const float* lse, const void* rest,
+                                   int64_t rest_rows, void* dq, void* dk, void* dv, int64_t batch,
+                                   int64_t heads, int64_t kv_heads, int64_t n, int32_t d,
+                                   int64_t window, int64_t sinks, float scale, int32_t dtype,
+                                   int32_t layout, const int64_t* strides, void* stream) {
+  Problem w{batch, heads, kv_heads, n, window, sinks, d, dtype, layout, scale, rest_rows, {}, {}, {}};
+  return backward(q, k, v, out, dout, lse, rest, dq, dk, dv, w, strides, stream);
 }

@@ -21,6 +21,8 @@ EXPORTED_SYMBOLS = (
     "mfa_bwd",
     "mfa_fwd_window",
     "mfa_bwd_window",
+    "mfa_fwd_window_rest",
+    "mfa_bwd_window_rest",
     "mfa_extend_block_tables",
     "mfa_append_kv",
     "mfa_paged_attention",
@@ -97,6 +99,10 @@ def load(path: str | Path | None = None) -> ctypes.CDLL:
     lib.mfa_bwd_window.argtypes = [ctypes.c_void_p] * 10 + window_args
     lib.mfa_bwd_window.restype = ctypes.c_int
     ptr, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+    lib.mfa_fwd_window_rest.argtypes = [ptr] * 6 + [i64] + window_args
+    lib.mfa_fwd_window_rest.restype = ctypes.c_int
+    lib.mfa_bwd_window_rest.argtypes = [ptr] * 7 + [i64] + [ptr] * 3 + window_args
+    lib.mfa_bwd_window_rest.restype = ctypes.c_int
     lib.mfa_extend_block_tables.argtypes = [ptr] * 7 + [i64] * 5 + [ptr]
     lib.mfa_append_kv.argtypes = [ptr] * 5 + [i64] * 9 + [ptr]
     lib.mfa_paged_attention.argtypes = [ptr] * 7 + [ctypes.c_uint64] + [i64] * 3 + [
@@ -185,23 +191,35 @@ def _nine(strides):
 def fwd_window(q_ptr: int, k_ptr: int, v_ptr: int, out_ptr: int, lse_ptr: int, batch: int,
                heads: int, kv_heads: int, n: int, d: int, window: int, sinks: int, scale: float,
                dtype: int = DTYPE_FP16, layout: int = LAYOUT_BHND, stream: int = 0,
-               strides: tuple[int, ...] | None = None, rest_ptr: int = 0) -> None:
+               strides: tuple[int, ...] | None = None, rest_ptr: int = 0,
+               rest_rows: int | None = None) -> None:
     """Launch mfa_fwd_window (lse_ptr, rest_ptr 0: not written; strides: the nine (batch, head,
-    token) element strides of q, k and v); raises MfaError."""
-    _check(load().mfa_fwd_window(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, rest_ptr, batch, heads,
-                                 kv_heads, n, d, window, sinks, scale, dtype, layout,
-                                 _nine(strides), stream))
+    token) element strides of q, k and v) or, with rest_rows, mfa_fwd_window_rest; raises
+    MfaError."""
+    tail = (batch, heads, kv_heads, n, d, window, sinks, scale, dtype, layout, _nine(strides),
+            stream)
+    if rest_rows is None:
+        _check(load().mfa_fwd_window(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, rest_ptr, *tail))
+    else:
+        _check(load().mfa_fwd_window_rest(q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, rest_ptr,
+                                          rest_rows, *tail))
 
 
 def bwd_window(q_ptr: int, k_ptr: int, v_ptr: int, o_ptr: int, do_ptr: int, lse_ptr: int,
                dq_ptr: int, dk_ptr: int, dv_ptr: int, batch: int, heads: int, kv_heads: int,
                n: int, d: int, window: int, sinks: int, scale: float, dtype: int = DTYPE_FP16,
                layout: int = LAYOUT_BHND, stream: int = 0,
-               strides: tuple[int, ...] | None = None, rest_ptr: int = 0) -> None:
-    """Launch mfa_bwd_window (strides as for fwd_window, rest_ptr 0: none); raises MfaError."""
-    _check(load().mfa_bwd_window(q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, rest_ptr, dq_ptr,
-                                 dk_ptr, dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale,
-                                 dtype, layout, _nine(strides), stream))
+               strides: tuple[int, ...] | None = None, rest_ptr: int = 0,
+               rest_rows: int | None = None) -> None:
+    """Launch mfa_bwd_window (strides as for fwd_window, rest_ptr 0: none) or, with rest_rows,
+    mfa_bwd_window_rest; raises MfaError."""
+    tail = (dq_ptr, dk_ptr, dv_ptr, batch, heads, kv_heads, n, d, window, sinks, scale, dtype,
+            layout, _nine(strides), stream)
+    head = (q_ptr, k_ptr, v_ptr, o_ptr, do_ptr, lse_ptr, rest_ptr)
+    if rest_rows is None:
+        _check(load().mfa_bwd_window(*head, *tail))
+    else:
+        _check(load().mfa_bwd_window_rest(*head, rest_rows, *tail))
 
 
 def extend_block_tables(table_ptr: int, cached_ptr: int, added_ptr: int, free_ptr: int,
