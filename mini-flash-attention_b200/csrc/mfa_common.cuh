@@ -43,6 +43,7 @@ struct FwdParams {
   int sink_blocks;
   int kv_group;
   int whole_units;  // query blocks done whole; the others tile by tile (WindowCursor)
+  float rescale_threshold;  // growth of the running maximum that raises it (log2 units)
   // Optional (null: not written): the output less its rounding, of the first rest_rows rows of
   // every head, in the type of the output and with these strides; the backward's row sums want
   // the output itself (see mfa_bwd_prep_kernel).

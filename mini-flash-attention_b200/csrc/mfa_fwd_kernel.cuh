@@ -867,9 +867,10 @@ __device__ __forceinline__ bool softmax_step(const FwdParams& p, uint32_t bars, 
   // row grows iff one of its four threads holds a score past it (c > 0: scaling preserves
   // the order), so the vote runs on the thread maxima and the row maxima are combined by
   // shuffles only on that rare path; otherwise the reference max stays and alpha = 1.
-  const bool grow =
-      __any_sync(0xffffffffu, !(mloc[0] * c <= m_run[0] + Cfg::kRescaleThreshold &&
-                                mloc[1] * c <= m_run[1] + Cfg::kRescaleThreshold));
+  float threshold = Cfg::kRescaleThreshold;
+  if constexpr (Cfg::kWindow) threshold = p.rescale_threshold;
+  const bool grow = __any_sync(0xffffffffu, !(mloc[0] * c <= m_run[0] + threshold &&
+                                              mloc[1] * c <= m_run[1] + threshold));
   float alpha[2] = {1.0f, 1.0f};
   if (grow) {
 #pragma unroll
