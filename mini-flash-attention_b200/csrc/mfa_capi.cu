@@ -24,7 +24,7 @@
 namespace mfa {
 namespace {
 
-constexpr int kMaxDevices = 64;
+using host::kMaxDevices;
 constexpr const char* kVersion = "mini-flash-attention-b200 0.1.0 (sm_100a)";
 
 thread_local std::string g_last_error;

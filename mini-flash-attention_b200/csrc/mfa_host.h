@@ -1,5 +1,5 @@
-// Host-side services shared by the translation units of libmfa_b200.so (defined in mfa_capi.cu):
-// errors, the per-device set-up, pointer checks and tensor maps. Every function that returns int
+// Host-side services shared by the translation units of libmfa_b200.so (those that are not here are
+// defined in mfa_capi.cu): errors, the per-device set-up, pointer checks, launches and tensor maps. Every function that returns int
 // returns an MFA_* code and leaves its message for mfa_last_error_string().
 #pragma once
 
@@ -18,6 +18,8 @@ namespace host {
 
 int fail(int code, const std::string& msg);
 int fail_cuda(cudaError_t e, const char* what);
+
+constexpr int kMaxDevices = 64;
 
 // A device's one-time set-up: `run` is called, by one thread at a time, until it has returned
 // MFA_OK. A failure is the calling entry's own, the next one tries again. The process's first
@@ -56,6 +58,51 @@ int open_device(Device* out);
 
 // `p` must be memory that device `dev` addresses directly.
 int check_pointer(const void* p, const char* name, int dev);
+
+// Null and misaligned pointers; with a device (dev >= 0), also those that are not its memory.
+struct Pointer {
+  const void* p;
+  const char* name;
+  uintptr_t align;
+};
+inline int check_pointers(const Pointer* ptrs, int count, int dev) {
+  for (int i = 0; i < count; ++i) {
+    const Pointer& x = ptrs[i];
+    if (!x.p) return fail(MFA_ERR_INVALID_ARGUMENT, std::string("null ") + x.name);
+    if (reinterpret_cast<uintptr_t>(x.p) & (x.align - 1))
+      return fail(MFA_ERR_INVALID_ARGUMENT, std::string(x.name) + " must be " +
+                                                std::to_string(x.align) + "-byte aligned");
+    const int rc = dev < 0 ? MFA_OK : check_pointer(x.p, x.name, dev);
+    if (rc != MFA_OK) return rc;
+  }
+  return MFA_OK;
+}
+
+// Launches a kernel that waits for the stream's earlier work itself (griddepcontrol.wait) and may be
+// set up while that work ends; in clusters of `cluster` CTAs.
+struct Grid {
+  int64_t ctas;
+  int threads, smem;
+  cudaStream_t stream;
+  int cluster = 1;
+};
+template <class... Params, class... Args>
+cudaError_t launch(const Grid& g, void (*kernel)(Params...), const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(g.ctas));
+  cfg.blockDim = dim3(static_cast<unsigned>(g.threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(g.smem);
+  cfg.stream = g.stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(g.cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = g.cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // Element strides of a contiguous tensor in `layout`.
 struct Strides {

@@ -16,7 +16,6 @@
 namespace mfa {
 namespace {
 
-constexpr int kMaxDevices = 64;
 constexpr int64_t kMost = 0x7fffff00LL;  // 32-bit counters with room for a tile
 
 // The prefix variant of the forward kernel. D = 64 has two query tiles a CTA as the forward does,
@@ -60,7 +59,7 @@ cudaError_t set_attributes() {
 }
 
 int prepare(int dev) {
-  static host::SetUp set_up[kMaxDevices];
+  static host::SetUp set_up[host::kMaxDevices];
   return set_up[dev]([]() -> int {
     cudaError_t e = set_attributes<false>();
     if (e == cudaSuccess) e = set_attributes<true>();
@@ -70,44 +69,10 @@ int prepare(int dev) {
 
 int invalid(const std::string& msg) { return host::fail(MFA_ERR_INVALID_ARGUMENT, msg); }
 
-struct Pointer {
-  const void* p;
-  const char* name;
-  uintptr_t align;
-};
-
-// Null and misaligned pointers; with a device, also those that are not its memory.
+using host::Pointer;
 template <int kCount>
 int check_pointers(const Pointer (&ptrs)[kCount], int dev) {
-  for (const Pointer& x : ptrs) {
-    if (!x.p) return invalid(std::string("null ") + x.name);
-    if (reinterpret_cast<uintptr_t>(x.p) & (x.align - 1))
-      return invalid(std::string(x.name) + " must be " + std::to_string(x.align) + "-byte aligned");
-    const int rc = dev < 0 ? MFA_OK : host::check_pointer(x.p, x.name, dev);
-    if (rc != MFA_OK) return rc;
-  }
-  return MFA_OK;
-}
-
-// A kernel that waits for the stream's earlier work itself (griddepcontrol.wait) and may be set up
-// while that work ends; in clusters of `cluster` CTAs.
-template <class P>
-cudaError_t launch(void (*kernel)(P), int64_t grid, int threads, int smem, cudaStream_t stream,
-                   const P& params, int cluster = 1) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, params);
+  return host::check_pointers(ptrs, kCount, dev);
 }
 
 constexpr int64_t kInlinePrefixBytes = 64 << 20;
@@ -303,8 +268,8 @@ int launch_prefix(const Arrays& x, const Problem& w, const Layout& l, const host
   p.page_shift = w.shift();
   p.pages = static_cast<int>(w.pages);
   *pp = {p.workspace, p.splits, p.sc.q_blocks, Cfg::kRowsPerUnit, p.tile_batch};
-  const cudaError_t e = launch(prefix_kernel<Cfg>(), l.prefix_ctas, Cfg::kThreads, Cfg::kSmemBytes,
-                               stream, p);
+  const cudaError_t e = host::launch({l.prefix_ctas, Cfg::kThreads, Cfg::kSmemBytes, stream},
+                                     prefix_kernel<Cfg>(), p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "prefix attention launch");
 }
 
@@ -352,12 +317,13 @@ int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cud
   p.timeout_ns = dev.timeout_ns;
   p.status = dev.status;
   if (l.cluster > 0) {
-    const cudaError_t ec = launch(&mfa_paged_cluster_kernel<D, kBF16>, l.ctas, Cfg::kThreads,
-                                  Cfg::kSmemBytes, stream, p, l.cluster);
+    const cudaError_t ec =
+        host::launch({l.ctas, Cfg::kThreads, Cfg::kSmemBytes, stream, l.cluster},
+                     &mfa_paged_cluster_kernel<D, kBF16>, p);
     return ec == cudaSuccess ? MFA_OK : host::fail_cuda(ec, "paged attention launch");
   }
-  cudaError_t e = launch(&mfa_paged_kernel<D, kBF16>, l.ctas, Cfg::kThreads, Cfg::kSmemBytes,
-                         stream, p);
+  cudaError_t e = host::launch({l.ctas, Cfg::kThreads, Cfg::kSmemBytes, stream},
+                               &mfa_paged_kernel<D, kBF16>, p);
   if (e != cudaSuccess) return host::fail_cuda(e, "paged attention launch");
   cp.pieces = p.pieces;
   cp.slots = p.slots;
@@ -367,8 +333,9 @@ int launch_paged(const Arrays& x, const Problem& w, const host::Device& dev, cud
   cp.row_tiles = p.row_tiles;
   cp.cols = p.cols;
   cp.pieces_only = p.pieces_only;
-  e = shared ? launch(&mfa_paged_combine_kernel<D, kBF16, true>, w.units(), 128, 0, stream, cp)
-             : launch(&mfa_paged_combine_kernel<D, kBF16, false>, l.ctas, 128, 0, stream, cp);
+  e = shared ? host::launch({w.units(), 128, 0, stream},
+                            &mfa_paged_combine_kernel<D, kBF16, true>, cp)
+             : host::launch({l.ctas, 128, 0, stream}, &mfa_paged_combine_kernel<D, kBF16, false>, cp);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "paged combine launch");
 }
 
@@ -451,8 +418,8 @@ extern "C" int mfa_extend_block_tables(int32_t* block_table, const int32_t* cach
   // a token a thread, two CTAs an SM at most (each scans all requests)
   const int64_t need = (capacity + kExtendThreads - 1) / kExtendThreads;
   const int64_t grid = need < 1 ? 1 : need < 2 * dev.sms ? need : 2 * dev.sms;
-  const cudaError_t e = launch(&mfa_extend_kernel, grid, kExtendThreads, 0,
-                               static_cast<cudaStream_t>(stream), p);
+  const cudaError_t e = host::launch({grid, kExtendThreads, 0, static_cast<cudaStream_t>(stream)},
+                                     &mfa_extend_kernel, p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "block table launch");
 }
 
@@ -505,8 +472,9 @@ extern "C" int mfa_append_kv(const void* k, const void* v, void* k_cache, void* 
   const int64_t spread = (tokens + 2 * dev.sms - 1) / (2 * dev.sms);
   if (per > spread) per = spread;
   p.tokens_a_block = static_cast<int>(per);
-  const cudaError_t e = launch(&mfa_append_kernel, (tokens + per - 1) / per, 256, 0,
-                               static_cast<cudaStream_t>(stream), p);
+  const cudaError_t e =
+      host::launch({(tokens + per - 1) / per, 256, 0, static_cast<cudaStream_t>(stream)},
+                   &mfa_append_kernel, p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "append launch");
 }
 

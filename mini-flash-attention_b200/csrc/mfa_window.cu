@@ -17,8 +17,6 @@
 namespace mfa {
 namespace {
 
-constexpr int kMaxDevices = 64;
-
 // The head dim's tile count and ring depth are the causal forward's.
 template <bool kBF16, int D>
 using Window = FwdConfig<D == 128 ? 1 : 2, D == 128 ? 2 : 3, true, kBF16, D, true, true>;
@@ -62,7 +60,7 @@ cudaError_t set_attributes() {
 }
 
 int prepare(int dev) {
-  static host::SetUp set_up[kMaxDevices];
+  static host::SetUp set_up[host::kMaxDevices];
   return set_up[dev]([]() -> int {
     cudaError_t e = set_attributes<false>();
     if (e == cudaSuccess) e = set_attributes<true>();
@@ -140,36 +138,6 @@ int check(Problem& w) {
   return MFA_OK;
 }
 
-int check_tensors(const void* const* ptrs, const char* const* names, int count, int dev) {
-  for (int i = 0; i < count; ++i) {
-    if (!ptrs[i]) return host::fail(MFA_ERR_INVALID_ARGUMENT, std::string("null ") + names[i]);
-    if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15u)
-      return host::fail(MFA_ERR_INVALID_ARGUMENT,
-                        std::string(names[i]) + " must be 16-byte aligned");
-    const int rc = dev < 0 ? MFA_OK : host::check_pointer(ptrs[i], names[i], dev);
-    if (rc != MFA_OK) return rc;
-  }
-  return MFA_OK;
-}
-
-// A programmatic dependent launch: the kernel waits for the stream's earlier work itself
-// (griddepcontrol.wait), and its set-up may overlap that work's end.
-template <class... Params, class... Args>
-cudaError_t launch(int64_t grid, int threads, int smem, cudaStream_t stream,
-                   void (*kernel)(Params...), const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <class Cfg>
 int launch_forward(const void* q, const void* k, const void* v, void* out, float* lse,
                    void* rest, const Problem& w, const host::Device& dev, cudaStream_t stream) {
@@ -213,8 +181,9 @@ int launch_forward(const void* q, const void* k, const void* v, void* out, float
   const int64_t whole = Cfg::NQ == 2 && 2 * over <= dev.sms ? units - over : units;
   const int64_t items = 2 * units - whole;
   p.whole_units = static_cast<int>(whole);
-  const cudaError_t e = launch(items < dev.sms ? items : dev.sms, Cfg::kThreads, Cfg::kSmemBytes,
-                               stream, window_kernel<Cfg>(), p);
+  const cudaError_t e =
+      host::launch({items < dev.sms ? items : dev.sms, Cfg::kThreads, Cfg::kSmemBytes, stream},
+                   window_kernel<Cfg>(), p);
   return e == cudaSuccess ? MFA_OK : host::fail_cuda(e, "window forward launch");
 }
 
@@ -362,18 +331,20 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
     const int64_t most = static_cast<int64_t>(dev.sms) * 16;
     const host::Strides rs = host::strides_of(w.layout, w.heads, w.rest_rows, w.d);
     // the kernels wait for the stream's earlier work themselves and may be set up while it ends
-    e = launch(need < most ? need : most, 256, 0, stream, prep_kernel<kBF16>(w.d), out, dout, lse,
-               lse2, di, static_cast<int>(bh), static_cast<int>(w.n), static_cast<int>(w.heads),
-               static_cast<long long>(st.b), static_cast<long long>(st.h),
-               static_cast<long long>(st.n), static_cast<int>(blocks), counters, rest,
-               static_cast<int>(rest ? w.rest_rows : 0), static_cast<long long>(rs.b),
-               static_cast<long long>(rs.h), static_cast<long long>(rs.n));
+    e = host::launch({need < most ? need : most, 256, 0, stream}, prep_kernel<kBF16>(w.d), out,
+                     dout, lse, lse2, di, static_cast<int>(bh), static_cast<int>(w.n),
+                     static_cast<int>(w.heads), static_cast<long long>(st.b),
+                     static_cast<long long>(st.h), static_cast<long long>(st.n),
+                     static_cast<int>(blocks), counters, rest,
+                     static_cast<int>(rest ? w.rest_rows : 0), static_cast<long long>(rs.b),
+                     static_cast<long long>(rs.h), static_cast<long long>(rs.n));
     const int64_t units = kv_units > q_units ? kv_units : q_units;
     const int64_t ctas = units < dev.sms ? units : dev.sms;
     if constexpr (D == 64) {
       if (e == cudaSuccess)
-        e = launch(ctas, BwdConfig<true, true, kBF16, true>::kThreads, window_bwd_smem<kBF16>(),
-                   stream, &mfa_bwd_window_kernel<kBF16>, pq, pkv);
+        e = host::launch({ctas, BwdConfig<true, true, kBF16, true>::kThreads,
+                          window_bwd_smem<kBF16>(), stream},
+                         &mfa_bwd_window_kernel<kBF16>, pq, pkv);
     } else {
       auto set_grad = [](BwdParams& to, void* grad, const host::Strides& g) {
         to.grad = static_cast<uint16_t*>(grad);
@@ -388,17 +359,17 @@ int launch_backward(const void* q, const void* k, const void* v, const void* out
       pv.claimed = counters + 2;
       pv.partials = sums + slots * kTile;
       if (e == cudaSuccess)
-        e = launch(ctas, BwdDQ128<kBF16>::kThreads, window_bwd128_smem<kBF16>(), stream,
-                   &mfa_bwd_window128_kernel<kBF16>, pq, pkv, pv);
+        e = host::launch({ctas, BwdDQ128<kBF16>::kThreads, window_bwd128_smem<kBF16>(), stream},
+                         &mfa_bwd_window128_kernel<kBF16>, pq, pkv, pv);
     }
     if (e == cudaSuccess && slots > 0) {
       const int64_t pairs = bhk * (pc.pieces_rest > 1 ? blocks : sb);
       const long long slot_floats = D == 64 ? 2 * kTile : kTile;
-      e = launch(pairs * D / 8, 256, 0, stream, &mfa_bwd_reduce_kernel<kBF16, D>, pkv, sums,
-                 sums + (D == 64 ? kTile : slots * kTile), slot_floats, w.d,
-                 static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv),
-                 static_cast<long long>(kv.b), static_cast<long long>(kv.h),
-                 static_cast<long long>(kv.n));
+      e = host::launch({pairs * D / 8, 256, 0, stream}, &mfa_bwd_reduce_kernel<kBF16, D>, pkv, sums,
+                       sums + (D == 64 ? kTile : slots * kTile), slot_floats, w.d,
+                       static_cast<uint16_t*>(dk), static_cast<uint16_t*>(dv),
+                       static_cast<long long>(kv.b), static_cast<long long>(kv.h),
+                       static_cast<long long>(kv.n));
     }
   }
   const cudaError_t ef = cudaFreeAsync(ws, stream);
@@ -421,20 +392,14 @@ int forward(const void* q, const void* k, const void* v, void* out, float* lse, 
   if (rc != MFA_OK || w.batch * w.heads == 0 || w.n == 0) return rc;
   if (w.rest_rows == 0) rest = nullptr;
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
-  const void* ptrs[] = {q, k, v, out};
-  const char* names[] = {"q", "k", "v", "out"};
-  const char* const rest_name = "out_rest";
-  if ((rc = check_tensors(ptrs, names, 4, -1)) != MFA_OK ||
-      (rest && (rc = check_tensors(&rest, &rest_name, 1, -1)) != MFA_OK))
-    return rc;
-  if (reinterpret_cast<uintptr_t>(lse) & 3u)
-    return host::fail(MFA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
+  host::Pointer ptrs[6] = {{q, "q", 16}, {k, "k", 16}, {v, "v", 16}, {out, "out", 16}};
+  int count = 4;
+  if (rest) ptrs[count++] = {rest, "out_rest", 16};
+  if (lse) ptrs[count++] = {lse, "lse", 4};
+  if ((rc = host::check_pointers(ptrs, count, -1)) != MFA_OK) return rc;
   host::Device dev;
   if ((rc = host::open_device(&dev)) != MFA_OK || (rc = prepare(dev.index)) != MFA_OK) return rc;
-  if ((rc = check_tensors(ptrs, names, 4, dev.index)) != MFA_OK ||
-      (rest && (rc = check_tensors(&rest, &rest_name, 1, dev.index)) != MFA_OK))
-    return rc;
-  if (lse && (rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
+  if ((rc = host::check_pointers(ptrs, count, dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return w.dtype == MFA_DTYPE_BF16 ? forward_d<true>(q, k, v, out, lse, rest, w, dev, s)
                                    : forward_d<false>(q, k, v, out, lse, rest, w, dev, s);
@@ -447,17 +412,14 @@ int backward(const void* q, const void* k, const void* v, const void* out, const
   if (rc != MFA_OK || w.batch * w.heads == 0 || w.n == 0) return rc;
   if (w.rest_rows == 0) rest = nullptr;
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
-  const void* ptrs[] = {q, k, v, out, dout, dq, dk, dv, rest};
-  const char* names[] = {"q", "k", "v", "out", "dout", "dq", "dk", "dv", "out_rest"};
-  const int count = rest ? 9 : 8;
-  if ((rc = check_tensors(ptrs, names, count, -1)) != MFA_OK) return rc;
-  if (!lse) return host::fail(MFA_ERR_INVALID_ARGUMENT, "null lse pointer");
-  if (reinterpret_cast<uintptr_t>(lse) & 3u)
-    return host::fail(MFA_ERR_INVALID_ARGUMENT, "lse must be 4-byte aligned");
+  const host::Pointer ptrs[] = {{q, "q", 16},   {k, "k", 16},   {v, "v", 16},     {out, "out", 16},
+                                {dout, "dout", 16}, {lse, "lse", 4}, {dq, "dq", 16}, {dk, "dk", 16},
+                                {dv, "dv", 16}, {rest, "out_rest", 16}};
+  const int count = rest ? 10 : 9;
+  if ((rc = host::check_pointers(ptrs, count, -1)) != MFA_OK) return rc;
   host::Device dev;
   if ((rc = host::open_device(&dev)) != MFA_OK || (rc = prepare(dev.index)) != MFA_OK) return rc;
-  if ((rc = check_tensors(ptrs, names, count, dev.index)) != MFA_OK) return rc;
-  if ((rc = host::check_pointer(lse, "lse", dev.index)) != MFA_OK) return rc;
+  if ((rc = host::check_pointers(ptrs, count, dev.index)) != MFA_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (w.dtype == MFA_DTYPE_BF16)
     return w.d <= 64
