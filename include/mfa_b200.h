@@ -129,7 +129,7 @@ MFA_API int mfa_bwd(const void* q, const void* k, const void* v, const void* out
  * lse (may be NULL): the row log-sum-exp over the visible keys, fp32 [B*H, N]. out_rest (may be
  * NULL): what the rounding of out left, in its type and shape, for mfa_bwd_window. Key blocks that
  * no row of a query block sees are neither read nor computed. k and v must be finite also where
- * they are masked, as for mfa_fwd. `strides` (NULL: those of `layout`) are the element strides of
+ * they are masked, as for mfa_fwd; a visible score of NaN or +inf makes its row NaN. `strides` (NULL: those of `layout`) are the element strides of
  * q's, k's and v's batch, head and token dimension, nine values in that order: positive multiples
  * of 8 (any value for a dimension of one element), as of the parts of a fused projection. The
  * other tensors are contiguous in `layout`. No counterpart in the reference.
@@ -198,7 +198,7 @@ MFA_API int mfa_extend_block_tables(int32_t* block_table, const int32_t* cached,
  * Copies token t's rows of k and v ([tokens, kv_heads, d]; token and head strides in elements,
  * multiples of 8; d a multiple of 8) to slot slots[t]; tokens whose slot is outside the cache are
  * skipped. A slot may occur once in a call: of two tokens with one slot either may stay, also
- * in parts.
+ * in parts. k and v must not overlap the caches.
  */
 MFA_API int mfa_append_kv(const void* k, const void* v, void* k_cache, void* v_cache,
                           const int32_t* slots, int64_t tokens, int64_t kv_heads, int64_t d,
@@ -214,7 +214,9 @@ MFA_API int mfa_append_kv(const void* k, const void* v, void* k_cache, void* v_c
  * `window` positions and the first `sinks`. out is 0 for a request that sees nothing. Only pages
  * with visible tokens are looked up and read, and what else their rows hold (NaN too) does not
  * matter. A looked-up page outside the cache reads as zeros and sets the device status word
- * (mfa_device_status) to 0x200. The workspace (256-byte aligned, mfa_paged_workspace_bytes) must
+ * (mfa_device_status) to 0x200. A visible score of NaN or +inf makes its row of out NaN. `columns`
+ * selects the kernel: few requests of a narrow table take one launch and no workspace, the same
+ * requests with a wide table two launches. The workspace (256-byte aligned, mfa_paged_workspace_bytes) must
  * not be shared by calls that may overlap; nothing in it has to be kept between calls.
  */
 MFA_API int mfa_paged_attention(const void* q, const void* k_cache, const void* v_cache,

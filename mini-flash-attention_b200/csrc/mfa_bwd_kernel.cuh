@@ -1,23 +1,35 @@
-// FlashAttention backward for sm_100a (D = 64, fp16 or bf16, optional causal mask): the last
-// "next" item of the reference's README (backward pass, README.md:125). Not a translation: the
-// reference has no backward.
+// FlashAttention backward for sm_100a, fp16 or bf16: the last "next" item of the reference's README
+// (backward pass, README.md:125). Not a translation: the reference has no backward. Two variants:
+//   dense : D = 64, optional causal mask, as many k / v heads as query heads (mfa_bwd);
+//   window: causal with a sliding window and sink tokens, k / v heads shared by groups of query
+//           heads (mfa_bwd_window); D = 64, D = 32 as D = 64 with boxes that reach past the columns,
+//           and D = 128.
 //
 // Given q, k, v, o, dO and the forward's row log-sum-exp L (natural log), with
-// P = exp(scale * q k^T - L) and D_i = rowsum(dO ⊙ o):
+// P = exp(scale * q k^T - L) and D_i = rowsum(dO ⊙ o) (mfa_bwd_prep_kernel):
 //   dV = P^T dO,   dS = P ⊙ (dO v^T - D),   dQ = scale * dS k,   dK = scale * dS^T q.
-// Two passes of one persistent kernel, no atomics (dQ gets its own pass, which recomputes S
+// Passes of one persistent kernel, no atomics on sums (dQ gets its own pass, which recomputes S
 // and dP, instead of accumulating across CTAs):
 //   dQ pass  : a CTA keeps a 128-row block of q and dO resident and streams the k, v blocks;
 //              S = q k^T and dP = dO v^T (tcgen05 SS MMAs into TMEM), dS in registers (fp16
 //              or bf16 into TMEM), dQ += dS k (TS MMA; k read MN-major, no transpose).
 //   dK/dV pass: a CTA keeps a 128-row block of k and v resident and streams the q, dO blocks
 //              with their L and D slices; S^T = k q^T and dP^T = v dO^T, P^T and dS^T in TMEM,
-//              dV += P^T dO and dK += dS^T q.
-// TMEM (columns): S or S^T [0,128), dP or dP^T [128,256), P^T / dS [256,320), dS^T [320,384),
-// accumulators dQ [320,384) or dV [384,448) and dK [448,512).
+//              dV += P^T dO and dK += dS^T q. At D = 128 a pass each for dK and dV (BwdPart); the
+//              dV pass needs neither v nor dP.
+// Dense units are dealt out by index (BwdCursor), the window's claimed from a counter, the longest
+// of its dK/dV units in pieces whose 32-bit sums mfa_bwd_reduce_kernel adds (BwdWindowCursor).
+// P and dS are operands of tensor-core products and therefore rounded to the type of q; everything
+// else (S, dP, L, D, P before it is used, all sums) is held in 32 bits. The rounding of dS makes dQ and
+// dK about 1.41 times as far off as their own, that of P dV.
+// TMEM (columns): S or S^T [0,128), dP or dP^T [128,256) (not in the dV pass), the first operand
+// [256,320): dS in the dQ pass, P^T in the dK/dV and dV passes, dS^T in the dK pass; dK/dV pass:
+// dS^T [320,384), accumulators dV [384,448) and dK [448,512); the others: their one accumulator
+// [320,384), at D = 128 [320,448).
 // Warp roles as in the forward kernel (csrc/mfa_fwd_kernel.cuh): 16 softmax-side warps on
 // 16x256b TMEM fragments (lane 4g + q: rows g and g + 8 of a 16-row slice, columns 2q, 2q + 1
-// of every 8), one MMA warp (one elected lane issues), one TMA warp; every wait is bounded.
+// of every 8), two MMA warps (S and dP, accumulations; one elected lane issues), one TMA warp, one
+// store thread (not at D = 128); every wait is bounded.
 // The backward needs no row reductions (L and D come precomputed), so the 128 columns of a
 // block are split between two warps per 16-row slice: warp w takes TMEM lane quadrant w % 4,
 // slice half (w / 4) % 2 and column half w / 8, which doubles the warps that hide each other's
@@ -889,7 +901,9 @@ __device__ __forceinline__ void bwd_softmax_role(const BwdParams& p, uint8_t* sm
           return;
       }
     }
-    // ---- unit epilogue: accumulators -> (scaled) fp16 / bf16 -> staging -> TMA
+    // ---- unit epilogue. A unit in pieces: 32-bit sums to its slot of `partials`. Else the scaled
+    // accumulators, rounded, go to the staging tiles and the store thread's TMA (D = 64), or
+    // straight to global memory (D = 128).
     if (!wait_warp(bar(Cfg::kBarAccDone), static_cast<uint32_t>(g - 1) & 1u, wd, kSiteSoftOFinal))
       return;
     tc_fence_after();

@@ -1,7 +1,9 @@
-// FlashAttention forward for sm_100a: fp16 Q/K/V in [BH, N, 64], fp32 online softmax,
-// fp16 output. Persistent: one CTA per SM walks a contiguous range of work units
-// (head, query block of 128*NQ rows, key block of 128 keys) and streams K/V through a TMA +
-// mbarrier ring that runs across unit boundaries.
+// FlashAttention forward for sm_100a: fp16 or bf16 Q/K/V with D = 32, 64 or 128, fp32 online softmax,
+// output in the inputs' type. Persistent: one CTA per SM walks work units (head, query block of
+// 128*NQ rows) over their key blocks of 128 keys and streams K/V through a TMA + mbarrier ring
+// that runs across unit boundaries. Variants: dense, with an optional causal mask (StepCursor);
+// causal with a sliding window, sink tokens and grouped k / v heads (WindowCursor); the queries of
+// many requests against the paged prefix that they share (PrefixCursor).
 //
 // Reference semantics (lavawolfiee/mini-flash-attention):
 //   src/mini_flash_attention/flash_attn_cuda.cu:190-368   FlashAttnCuteKernel (per Q tile
@@ -34,7 +36,9 @@
 // TMEM columns: S_i at 128*i, P_i (fp16 pairs) at 128*NQ + 64*i, O_i at 192*NQ + 64*i.
 // exp is exp2 with scale*log2(e) folded into one FMA; 1 of every 8 pairs uses an FMA-pipe
 // polynomial instead of MUFU. The running max is only raised when it grows by more than
-// kRescaleThreshold (log2 units), so O is rescaled in TMEM rarely.
+// kRescaleThreshold (log2 units; windows below 64: by anything), so O is rescaled in TMEM rarely.
+// P is an operand of the P.V product and therefore rounded to the inputs' type; S, the maxima, the
+// row sums (of P before it is rounded) and O are held in 32 bits.
 // Work split: see FwdParams::split. A unit range that covers a whole query block ends with
 // O / l stored as fp16 by TMA; a piece of a query block leaves fp32 partial results in the
 // workspace for mfa_merge_kernel.

@@ -33,15 +33,21 @@ class SetUp {
     if (done_.load(std::memory_order_acquire)) return MFA_OK;
     const std::lock_guard<std::mutex> lock(mu_);
     if (done_.load(std::memory_order_relaxed)) return MFA_OK;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    const Relaxed relaxed;
     const int rc = run();
-    if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
     if (rc == MFA_OK) done_.store(true, std::memory_order_release);
     return rc;
   }
 
  private:
+  // The thread's capture mode, relaxed while this lives.
+  struct Relaxed {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    const bool changed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
+    ~Relaxed() {
+      if (changed) cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+  };
   std::mutex mu_;
   std::atomic<bool> done_{false};
 };

@@ -557,7 +557,9 @@ __device__ __forceinline__ void paged_consume_role(const PagedParams& p, PagedCu
           }
         }
       }
-      uint32_t pf[4] = {0u, 0u, 0u, 0u};  // P: rows g, g + 8 by keys 2 q, then by keys 2 q + 8
+      // P: rows g, g + 8 by keys 2 q, then by keys 2 q + 8. Rounded to the type of v, as an operand of
+      // the product with it; maxima, sums (of p before it is rounded) and outputs are 32-bit.
+      uint32_t pf[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         if (r == 1 && !upper) break;
