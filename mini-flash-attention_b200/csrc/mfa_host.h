@@ -1,6 +1,7 @@
 // Host-side services shared by the translation units of libmfa_b200.so (those that are not here are
-// defined in mfa_capi.cu): errors, the per-device set-up, pointer checks, launches and tensor maps. Every function that returns int
-// returns an MFA_* code and leaves its message for mfa_last_error_string().
+// defined in mfa_capi.cu): errors, the per-device set-up, pointer checks, launches and tensor maps.
+// Every function that returns int returns an MFA_* code and leaves its message for
+// mfa_last_error_string().
 #pragma once
 
 #include <cuda.h>

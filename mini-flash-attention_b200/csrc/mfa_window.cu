@@ -412,9 +412,10 @@ int backward(const void* q, const void* k, const void* v, const void* out, const
   if (rc != MFA_OK || w.batch * w.heads == 0 || w.n == 0) return rc;
   if (w.rest_rows == 0) rest = nullptr;
   if ((rc = set_strides(w, strides)) != MFA_OK) return rc;
-  const host::Pointer ptrs[] = {{q, "q", 16},   {k, "k", 16},   {v, "v", 16},     {out, "out", 16},
-                                {dout, "dout", 16}, {lse, "lse", 4}, {dq, "dq", 16}, {dk, "dk", 16},
-                                {dv, "dv", 16}, {rest, "out_rest", 16}};
+  const host::Pointer ptrs[] = {{q, "q", 16}, {k, "k", 16}, {v, "v", 16},
+                                {out, "out", 16}, {dout, "dout", 16}, {lse, "lse", 4},
+                                {dq, "dq", 16}, {dk, "dk", 16}, {dv, "dv", 16},
+                                {rest, "out_rest", 16}};
   const int count = rest ? 10 : 9;
   if ((rc = host::check_pointers(ptrs, count, -1)) != MFA_OK) return rc;
   host::Device dev;
